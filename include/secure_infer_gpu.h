@@ -586,6 +586,155 @@ int secure_infer_d2h_swap(hipStream_t stream, si_session* session, const void* d
                           uint32_t n, uint32_t kind, uint32_t layer, uint32_t codec_bits,
                           uint32_t heads, uint32_t head_dim);
 
+/* ------------------------------------------------------------------ */
+/* 4. Operators on the paged cache (no reference counterpart: the reference
+ *    leaves attention and block management to vLLM).  They work on the caches
+ *    the layer calls above fill and drain: `nslots` pages of `page_tokens`
+ *    tokens per tensor, page s at base + s * slot_bytes, [page_tokens, kv
+ *    heads, head dim] of 16-bit values inside it.  tables[b * table_stride +
+ *    j] is the slot of sequence b's page j; an entry outside [0, nslots) is no
+ *    page.  What the device reads (tables, lengths, row lists) cannot be
+ *    checked before the work is queued, so it is bounded there: nothing
+ *    outside the tensors is touched, and rows that cannot be served are
+ *    counted in *fail_count.  Every call is asynchronous on `stream`,
+ *    allocates nothing, and may be captured into a graph.  0, or -1 on
+ *    an invalid argument (nothing queued) or a refused launch.             */
+
+enum {
+    SI_DTYPE_BF16 = 0,
+    SI_DTYPE_FP16 = 1,
+};
+
+/* Attention of new tokens over their sequences' pages.  Sequence b has
+ * kv_lens[b] tokens in its pages (clamped to [0, table_pages * page_tokens]),
+ * the last n_b of them the new ones: q rows [q_starts[b], q_starts[b + 1])
+ * (clamped to [0, tokens]; NULL: row b alone).  New token i stands at p =
+ * kv_lens[b] - n_b + i and sees key j iff j's page is held, j < kv_lens[b],
+ * j <= p (causal) and j > p - window (window > 0).
+ *   out = sum_j softmax_j(scale * q.k_j) v_j;  lse = log sum_j exp(scale * q.k_j)
+ * over the seen keys; none: out = 0, lse = -inf.  Query head h reads KV head
+ * h / (q_heads / kv_heads).  Keys that a token does not see have no influence
+ * on it, whatever bits they hold.  Scores, statistics and sums are float. */
+typedef struct si_paged_attention_desc {
+    const void* q;            /* rows of q_heads x head_dim, dim contiguous    */
+    uint64_t q_token_stride;  /* in elements, as q_head_stride: multiples of 8 */
+    uint64_t q_head_stride;
+    void* out;
+    uint64_t out_token_stride;
+    uint64_t out_head_stride;
+    float* lse;               /* [tokens][q_heads], or NULL                    */
+    const void* cache_k;
+    const void* cache_v;
+    uint64_t slot_bytes;      /* multiple of 16                                */
+    uint64_t nslots;
+    const int64_t* tables;
+    uint64_t table_stride;    /* entries from one sequence's row to the next   */
+    const int64_t* kv_lens;
+    const int64_t* q_starts;  /* seqs + 1, ascending; NULL: tokens == seqs     */
+    uint32_t table_pages;     /* entries of a row; table_pages * page_tokens < 2^31 */
+    uint32_t tokens;          /* rows of q: tokens * q_heads < 2^31            */
+    uint32_t seqs;
+    uint32_t q_heads;         /* a multiple of kv_heads                        */
+    uint32_t kv_heads;
+    uint32_t head_dim;        /* a multiple of 8, at most 256                  */
+    uint32_t page_tokens;     /* a power of two, 8 .. 32768                    */
+    uint32_t dtype;           /* SI_DTYPE_* of q, out and the caches           */
+    uint32_t causal;
+    uint32_t window;          /* 0: no window                                  */
+    float scale;
+    void* workspace;          /* device, secure_infer_gpu_paged_attention_workspace bytes */
+    uint64_t workspace_bytes;
+} si_paged_attention_desc;
+
+int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attention_desc* desc);
+/* Workspace bytes the call needs (its contents are scratch: no two calls that
+ * may overlap share one); 0 is a valid answer.  UINT64_MAX if the call would
+ * refuse the descriptor. */
+uint64_t secure_infer_gpu_paged_attention_workspace(const si_paged_attention_desc* desc);
+
+/* New tokens' K and V rows into their pages: token i of sequence b (positions
+ * and q_starts as above) goes to row p % page_tokens of page p /
+ * page_tokens.  A token at p < 0, past the table or without a page is dropped
+ * and counted. */
+typedef struct si_paged_append_desc {
+    const void* k;            /* rows of kv_heads x head_dim, dim contiguous   */
+    const void* v;
+    uint64_t k_token_stride;  /* in elements, multiples of 8                   */
+    uint64_t k_head_stride;
+    uint64_t v_token_stride;
+    uint64_t v_head_stride;
+    void* cache_k;
+    void* cache_v;
+    uint64_t slot_bytes;
+    uint64_t nslots;
+    const int64_t* tables;
+    uint64_t table_stride;
+    const int64_t* kv_lens;
+    const int64_t* q_starts;
+    uint32_t table_pages;
+    uint32_t tokens;
+    uint32_t seqs;
+    uint32_t kv_heads;
+    uint32_t head_dim;        /* a multiple of 8                               */
+    uint32_t page_tokens;     /* a power of two, 8 .. 32768                    */
+    uint32_t* fail_count;     /* += tokens dropped; NULL ok                    */
+} si_paged_append_desc;
+
+int secure_infer_gpu_paged_append(hipStream_t stream, const si_paged_append_desc* desc);
+
+/* Page management over every layer's caches at once.  refs[s] counts the
+ * sequences that hold slot s (0: free).  The calls read tables, kv_lens and
+ * refs and write tables_out, kv_lens_out and refs_out whole; each output may be
+ * its input (in place), and must not overlap anything else. */
+typedef struct si_pages_desc {
+    void* const* caches;      /* host array: device base of each tensor        */
+    uint32_t ncaches;
+    uint32_t page_tokens;     /* a power of two                                */
+    uint64_t slot_bytes;      /* from one page to the next, a multiple of 16   */
+    uint64_t page_bytes;      /* of one page, a multiple of 16                 */
+    uint64_t nslots;          /* < 2^31                                        */
+    const int64_t* tables;    /* [rows][table_pages]                           */
+    const int64_t* kv_lens;   /* [rows] (unused by compact)                    */
+    const int32_t* refs;      /* [nslots]                                      */
+    int64_t* tables_out;
+    int64_t* kv_lens_out;
+    int32_t* refs_out;
+    uint32_t rows;
+    uint32_t table_pages;
+    const int64_t* list;      /* fork: [n][2] (parent row, child row); free: [n] rows;
+                                 reserve: [rows] tokens to come; compact: NULL */
+    uint32_t n;
+    uint32_t scrub;           /* free: zero the freed pages; compact: zero the pages moved from */
+    uint32_t* fail_count;     /* NULL ok                                       */
+    void* workspace;
+    uint64_t workspace_bytes;
+} si_pages_desc;
+
+/* Each child row becomes its parent: whole pages are shared (refs + 1), a
+ * partly filled last page is copied in every tensor into a free slot (the
+ * lowest ones, in the list's order).  A child must be an empty row (length 0,
+ * no pages) and not be named before; parents are read as they were before the
+ * call.  A pair that cannot be served (rows out of range, no free slot) leaves
+ * its child as it was and is counted. */
+int secure_infer_gpu_pages_fork(hipStream_t stream, const si_pages_desc* desc);
+/* The rows named (each once, however often it is named) give up their pages
+ * (refs - 1) and become empty; a slot nobody holds any more is free, and with
+ * `scrub` its page is zeroed in every tensor.  Rows out of range, and holds
+ * beyond a slot's count, are counted. */
+int secure_infer_gpu_pages_free(hipStream_t stream, const si_pages_desc* desc);
+/* With L slots held, the held slots >= L move to the free slots < L, both
+ * ascending, in every tensor; tables and refs follow. */
+int secure_infer_gpu_pages_compact(hipStream_t stream, const si_pages_desc* desc);
+/* Row b grows by list[b] tokens: kv_lens_out = kv_lens + list[b], and the pages
+ * it then lacks are taken from the free slots, the lowest first, rows in
+ * order.  A row is served whole or not at all: not if it outgrows the table, or
+ * if it and the rows before it that fit theirs need more slots than are free.
+ * A row not served still has its new length (its tokens without a page are then
+ * dropped by append and unseen by attention) and is counted. */
+int secure_infer_gpu_pages_reserve(hipStream_t stream, const si_pages_desc* desc);
+/* Workspace bytes of any of the four, from nslots, rows and n. */
+uint64_t secure_infer_gpu_pages_workspace(const si_pages_desc* desc);
+
 /* Library build / device information. */
 const char* secure_infer_gpu_version(void);
 /* Tuning: minimum rows (of 256 blocks) of one workgroup's share of a layer's

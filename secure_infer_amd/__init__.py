@@ -14,3 +14,5 @@ from .gcm import (  # noqa: F401
     reference_ticket_order, register_host_range, replay_reserve, retire_transfer_prefetches,
     set_chunk_rows, set_job_id, set_straddle_rows, transfer_prefetch_stats, wait_job_authentication,
     wire_stride, wire_tag_offset)
+from .paged import (  # noqa: F401
+    compact_pages, fork_pages, free_pages, paged_append, paged_attention, paged_attention_workspace, reserve_pages)

@@ -36,6 +36,39 @@ class SiWritebackDesc(ct.Structure):
     ]
 
 
+class SiPagedAttentionDesc(ct.Structure):
+    """si_paged_attention_desc (include/secure_infer_gpu.h)."""
+    _fields_ = [
+        ("q", _v), ("q_token_stride", _u64), ("q_head_stride", _u64), ("out", _v), ("out_token_stride", _u64),
+        ("out_head_stride", _u64), ("lse", _v), ("cache_k", _v), ("cache_v", _v), ("slot_bytes", _u64),
+        ("nslots", _u64), ("tables", _v), ("table_stride", _u64), ("kv_lens", _v), ("q_starts", _v),
+        ("table_pages", _u32), ("tokens", _u32), ("seqs", _u32), ("q_heads", _u32), ("kv_heads", _u32),
+        ("head_dim", _u32), ("page_tokens", _u32), ("dtype", _u32), ("causal", _u32), ("window", _u32),
+        ("scale", ct.c_float), ("workspace", _v), ("workspace_bytes", _u64),
+    ]
+
+
+class SiPagedAppendDesc(ct.Structure):
+    """si_paged_append_desc (include/secure_infer_gpu.h)."""
+    _fields_ = [
+        ("k", _v), ("v", _v), ("k_token_stride", _u64), ("k_head_stride", _u64), ("v_token_stride", _u64),
+        ("v_head_stride", _u64), ("cache_k", _v), ("cache_v", _v), ("slot_bytes", _u64), ("nslots", _u64),
+        ("tables", _v), ("table_stride", _u64), ("kv_lens", _v), ("q_starts", _v), ("table_pages", _u32),
+        ("tokens", _u32), ("seqs", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("page_tokens", _u32),
+        ("fail_count", _v),
+    ]
+
+
+class SiPagesDesc(ct.Structure):
+    """si_pages_desc (include/secure_infer_gpu.h)."""
+    _fields_ = [
+        ("caches", ct.POINTER(_v)), ("ncaches", _u32), ("page_tokens", _u32), ("slot_bytes", _u64),
+        ("page_bytes", _u64), ("nslots", _u64), ("tables", _v), ("kv_lens", _v), ("refs", _v), ("tables_out", _v),
+        ("kv_lens_out", _v), ("refs_out", _v), ("rows", _u32), ("table_pages", _u32), ("list", _v), ("n", _u32),
+        ("scrub", _u32), ("fail_count", _v), ("workspace", _v), ("workspace_bytes", _u64),
+    ]
+
+
 # name -> (argtypes, restype); every symbol declared in include/secure_infer_gpu.h
 SIGNATURES = {
     "secure_infer_gpu_gcm_decrypt_verify_do": ([_v] * 7 + [_u64] + [_u32] * 4, _i),
@@ -62,6 +95,14 @@ SIGNATURES = {
     "secure_infer_gpu_reload_layer": ([_v, _v, ct.POINTER(SiReloadDesc)], _i),
     "secure_infer_gpu_reload_layer_noalloc": ([_v, _v, ct.POINTER(SiReloadDesc)], _i),
     "secure_infer_gpu_writeback_layer": ([_v, _v, ct.POINTER(SiWritebackDesc)], _i),
+    "secure_infer_gpu_paged_attention": ([_v, ct.POINTER(SiPagedAttentionDesc)], _i),
+    "secure_infer_gpu_paged_attention_workspace": ([ct.POINTER(SiPagedAttentionDesc)], _u64),
+    "secure_infer_gpu_paged_append": ([_v, ct.POINTER(SiPagedAppendDesc)], _i),
+    "secure_infer_gpu_pages_fork": ([_v, ct.POINTER(SiPagesDesc)], _i),
+    "secure_infer_gpu_pages_free": ([_v, ct.POINTER(SiPagesDesc)], _i),
+    "secure_infer_gpu_pages_compact": ([_v, ct.POINTER(SiPagesDesc)], _i),
+    "secure_infer_gpu_pages_reserve": ([_v, ct.POINTER(SiPagesDesc)], _i),
+    "secure_infer_gpu_pages_workspace": ([ct.POINTER(SiPagesDesc)], _u64),
     "secure_infer_gpu_time_next_layer": ([_v, _v], _i),
     "secure_infer_gpu_clock_next_layers": ([_v, _u64, _u32], _i),
     "secure_infer_gpu_clock_layers_used": ([_v, _u32], _i),

@@ -1,0 +1,375 @@
+"""Operators on the paged KV cache the transfers fill and drain.
+
+* ``paged_append`` writes new tokens' K and V rows into their pages.
+* ``paged_attention`` attends from new tokens (one per sequence, or a chunk
+  of each) over their sequences' pages.
+* ``fork_pages`` / ``free_pages`` / ``compact_pages`` / ``reserve_pages`` manage
+  the pages of every layer at once.
+
+Caches are the transfers' paged caches: [slots, page tokens, kv heads, head
+dim] of 16-bit values.  ``tables`` [sequences, pages] int64 holds the slot of each page (an entry
+outside [0, slots) is no page) and ``kv_lens`` [sequences] int64 the
+tokens in a sequence's pages, the new ones included.  ``q_starts`` [sequences +
+1] int64 says which rows are a sequence's new tokens (None: row b is
+sequence b's one new token).  What lives on the device is not read back: the
+kernels stay inside the tensors whatever it holds, and count what they cannot
+serve in ``fail_count`` (an int32 tensor they add to), as the reload calls
+do.  Every call is asynchronous on the given (default: current) stream, and
+may be captured into a graph.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as ct
+import math
+
+import torch
+
+from . import _lib
+from .gcm import _check, lib
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_REFUSED = (1 << 64) - 1
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch_stream(stream, device):
+    """The torch stream of a call (a torch stream, a raw handle, or None for
+    the device's current stream)."""
+    if stream is None:
+        return torch.cuda.current_stream(device)
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    raw = stream.value if isinstance(stream, ct.c_void_p) else int(stream)
+    return torch.cuda.ExternalStream(raw or 0, device=device)
+
+
+@contextlib.contextmanager
+def _on(stream, device, tensors):
+    """What the call allocates belongs to its stream, and the caller's tensors
+    are not reused before that stream is done with them."""
+    current = torch.cuda.current_stream(device)
+    s = _launch_stream(stream, device)
+    if s == current:
+        yield ct.c_void_p(s.cuda_stream)
+        return
+    with torch.cuda.stream(s):
+        yield ct.c_void_p(s.cuda_stream)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(s)
+
+
+def _index(t, name: str, ndim: int, device, dtype=torch.int64) -> None:
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise ValueError(f"{name} must be a tensor on {device}")
+    if t.dtype != dtype or t.ndim != ndim or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {ndim}-d {dtype} tensor")
+
+
+def _fail_count(t, device) -> None:
+    if t is not None and (t.device != device or t.dtype != torch.int32 or t.numel() != 1):
+        raise ValueError(f"fail_count must be one int32 on {device}")
+
+
+def _paged_cache(t, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.ndim != 4 or t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be [slots, page tokens, kv heads, head dim] in bfloat16 or float16")
+    slots, ps, heads, dim = t.shape
+    if 0 in t.shape:
+        raise ValueError(f"{name} is empty")
+    if t.stride()[1:] != (heads * dim, dim, 1) or (slots > 1 and t.stride(0) < ps * heads * dim):
+        raise ValueError(f"a page of {name} must be contiguous")
+    if ps & (ps - 1) or not 8 <= ps <= 32768:
+        raise ValueError(f"{name} has pages of {ps} tokens: must be a power of two from 8 to 32768")
+    if dim % 8:
+        raise ValueError(f"{name} has head dim {dim}: must be a multiple of 8")
+    _aligned(t, name)
+
+
+def _aligned(t, name: str) -> None:
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name} must start on a 16-byte boundary")
+
+
+def _slot_stride(t) -> int:
+    """Elements from one page to the next (a cache of one slot: a page)."""
+    return t.stride(0) if t.shape[0] > 1 else t[0].numel()
+
+
+def _cache_pair(cache_k, cache_v) -> None:
+    _paged_cache(cache_k, "cache_k")
+    _paged_cache(cache_v, "cache_v")
+    if (cache_k.shape != cache_v.shape or cache_k.dtype != cache_v.dtype or cache_k.device != cache_v.device
+            or _slot_stride(cache_k) != _slot_stride(cache_v)):
+        raise ValueError("cache_k and cache_v must have one shape, dtype, slot stride and device")
+    if _slot_stride(cache_k) % 8:
+        raise ValueError("the caches' slot stride must be a multiple of 16 bytes")
+
+
+def _rows(t, name: str, heads: int, dim: int, cache) -> tuple[int, int]:
+    """(token stride, head stride) of [tokens, heads, dim] rows."""
+    if not isinstance(t, torch.Tensor) or t.device != cache.device or t.dtype != cache.dtype:
+        raise ValueError(f"{name} must be a {cache.dtype} tensor on {cache.device}")
+    if t.ndim != 3 or t.shape[1:] != (heads, dim):
+        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(t.shape)}")
+    # the stride of a single token or head is never used
+    token = t.stride(0) if t.shape[0] > 1 else heads * dim
+    head = t.stride(1) if heads > 1 else dim
+    if (dim > 1 and t.stride(2) != 1) or token % 8 or head % 8:
+        raise ValueError(f"{name} needs a contiguous head dim and token / head strides that are multiples of 8")
+    _aligned(t, name)
+    return token, head
+
+
+def _sequences(tables, kv_lens, q_starts, tokens: int, cache) -> None:
+    if not isinstance(tables, torch.Tensor) or tables.device != cache.device:
+        raise ValueError(f"tables must be a tensor on {cache.device}")
+    if tables.dtype != torch.int64 or tables.ndim != 2 or (tables.shape[1] > 1 and tables.stride(1) != 1):
+        raise ValueError("tables must be a 2-d torch.int64 tensor with contiguous rows")
+    _index(kv_lens, "kv_lens", 1, cache.device)
+    if kv_lens.shape[0] != tables.shape[0]:
+        raise ValueError("kv_lens needs one entry per row of tables")
+    if q_starts is None:
+        if tokens != tables.shape[0]:
+            raise ValueError("without q_starts there is one row per sequence")
+    else:
+        _index(q_starts, "q_starts", 1, cache.device)
+        if q_starts.shape[0] != tables.shape[0] + 1:
+            raise ValueError("q_starts needs one entry more than tables has rows")
+    if tables.shape[1] * cache.shape[1] >= 1 << 31:
+        raise ValueError("a table row may span at most 2**31 - 1 tokens")
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor,
+                 tables: torch.Tensor, kv_lens: torch.Tensor, q_starts: torch.Tensor | None = None,
+                 fail_count: torch.Tensor | None = None, stream=None) -> None:
+    """New tokens' K and V rows ([tokens, kv heads, head dim], any token and
+    head stride in multiples of 8) into their pages.  Token i of a sequence with n new
+    ones goes to position kv_len - n + i; a token whose position is
+    negative, past the table or on no page is dropped and counted."""
+    _cache_pair(cache_k, cache_v)
+    slots, ps, heads, dim = cache_k.shape
+    kt, kh = _rows(k, "k", heads, dim, cache_k)
+    vt, vh = _rows(v, "v", heads, dim, cache_k)
+    if k.shape[0] != v.shape[0]:
+        raise ValueError("k and v must have the same tokens")
+    _sequences(tables, kv_lens, q_starts, k.shape[0], cache_k)
+    _fail_count(fail_count, cache_k.device)
+    if k.shape[0] == 0 or tables.shape[0] == 0:
+        return
+    if tables.shape[1] == 0:
+        raise ValueError("tables has no pages")
+    with _on(stream, cache_k.device, (k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count)) as s:
+        d = _lib.SiPagedAppendDesc(
+            k=k.data_ptr(), v=v.data_ptr(), k_token_stride=kt, k_head_stride=kh, v_token_stride=vt, v_head_stride=vh,
+            cache_k=cache_k.data_ptr(), cache_v=cache_v.data_ptr(), slot_bytes=2 * _slot_stride(cache_k), nslots=slots,
+            tables=tables.data_ptr(), table_stride=tables.stride(0), kv_lens=kv_lens.data_ptr(), q_starts=_ptr(q_starts),
+            table_pages=tables.shape[1], tokens=k.shape[0], seqs=tables.shape[0], kv_heads=heads, head_dim=dim,
+            page_tokens=ps, fail_count=_ptr(fail_count))
+        _check(lib().secure_infer_gpu_paged_append(s, ct.byref(d)), "paged_append")
+
+
+def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, tables: torch.Tensor,
+                    kv_lens: torch.Tensor, q_starts: torch.Tensor | None = None, scale: float | None = None,
+                    causal: bool = True, window: int = 0, out: torch.Tensor | None = None,
+                    lse: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                    stream=None) -> torch.Tensor:
+    """Attention of q [tokens, query heads, head dim] over the pages:
+    softmax(scale q k^T) v per token and query head (head h reads KV head
+    h // (query heads / kv heads)).  Token i of a sequence with n new ones stands at p = kv_len
+    - n + i; it sees the keys on held pages below kv_len, up to p
+    (``causal``) and after p - window (``window`` > 0).  Without a key to see
+    its output is 0.  ``scale`` defaults to head_dim ** -0.5.  ``lse`` [tokens, query heads]
+    float32, if given, receives the log-sum-exp of the scaled scores (-inf
+    without a key), with which two parts' outputs can be joined.  ``workspace`` (uint8, at least
+    ``paged_attention_workspace`` bytes) saves an allocation per call.  Returns ``out``."""
+    d, keep = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse)
+    if d is None:
+        return keep
+    device = q.device
+    with _on(stream, device, (q, cache_k, cache_v, tables, kv_lens, q_starts, out, lse, workspace)) as s:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            d.out, d.out_token_stride, d.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
+        need = int(lib().secure_infer_gpu_paged_attention_workspace(ct.byref(d)))
+        if need == _REFUSED:
+            raise ValueError("paged_attention refuses these arguments")
+        if need:
+            if workspace is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            elif workspace.device != device or not workspace.is_contiguous():
+                raise ValueError(f"workspace must be contiguous on {device}")
+            elif workspace.numel() * workspace.element_size() < need:
+                raise ValueError(f"workspace needs {need} bytes")
+            _aligned(workspace, "workspace")
+            d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _check(lib().secure_infer_gpu_paged_attention(s, ct.byref(d)), "paged_attention")
+    return out
+
+
+def paged_attention_workspace(q, cache_k, cache_v, tables, kv_lens, q_starts=None, causal: bool = True,
+                              window: int = 0) -> int:
+    """Workspace bytes of a paged_attention call with these arguments."""
+    d, _ = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, None, causal, window, q, None)
+    return 0 if d is None else int(lib().secure_infer_gpu_paged_attention_workspace(ct.byref(d)))
+
+
+def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse):
+    """The checked descriptor (without an output if ``out`` is None), or
+    (None, the answer) where there is nothing to compute."""
+    _cache_pair(cache_k, cache_v)
+    slots, ps, heads, dim = cache_k.shape
+    if dim > 256:
+        raise ValueError(f"head dim {dim} is over 256")
+    if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.shape[1] == 0 or q.shape[1] % heads:
+        raise ValueError(f"q must be [tokens, query heads, {dim}] with a multiple of {heads} query heads")
+    tokens, q_heads = q.shape[:2]
+    qt, qh = _rows(q, "q", q_heads, dim, cache_k)
+    if tokens * q_heads >= 1 << 31:
+        raise ValueError("q has too many rows")
+    _sequences(tables, kv_lens, q_starts, tokens, cache_k)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not 0 <= int(window) < 1 << 31:
+        raise ValueError("window must be 0 (none) or a positive number of keys")
+    ot = oh = 0
+    if out is not None:
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+        ot, oh = _rows(out, "out", q_heads, dim, cache_k)
+        if min(ot, oh) < dim or max(ot, oh) < min(ot, oh) * (q_heads if ot > oh else tokens):
+            raise ValueError("out's rows must not overlap")
+    if lse is not None and (lse.device != q.device or lse.dtype != torch.float32 or lse.shape != q.shape[:2]
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous float32 [tokens, query heads] tensor on {q.device}")
+    if tokens == 0:
+        return None, torch.empty_like(q) if out is None else out
+    if tables.shape[0] == 0 or tables.shape[1] == 0:
+        raise ValueError("tables has no pages")
+    return _lib.SiPagedAttentionDesc(
+        q=q.data_ptr(), q_token_stride=qt, q_head_stride=qh, out=q.data_ptr() if out is None else out.data_ptr(),
+        out_token_stride=ot, out_head_stride=oh, lse=_ptr(lse), cache_k=cache_k.data_ptr(),
+        cache_v=cache_v.data_ptr(), slot_bytes=2 * _slot_stride(cache_k), nslots=slots, tables=tables.data_ptr(),
+        table_stride=tables.stride(0), kv_lens=kv_lens.data_ptr(), q_starts=_ptr(q_starts),
+        table_pages=tables.shape[1], tokens=tokens, seqs=tables.shape[0], q_heads=q_heads, kv_heads=heads,
+        head_dim=dim, page_tokens=ps, dtype=_DTYPES[q.dtype], causal=int(bool(causal)), window=int(window),
+        scale=scale), None
+
+
+# ------------------------------------------------------------------ pages
+
+def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, list_ndim, scrub, fail_count, out,
+                stream):
+    device = refs.device if isinstance(refs, torch.Tensor) else None
+    if device is None or not refs.is_cuda:
+        raise ValueError("refs must be a device tensor")
+    caches = list(caches)
+    for c in caches:
+        _paged_cache(c, "a cache")
+        if c.device != device or c.shape != caches[0].shape or _slot_stride(c) != _slot_stride(caches[0]):
+            raise ValueError("the caches must have one shape and slot stride, on refs' device")
+        if c.shape[0] != refs.shape[0]:
+            raise ValueError("refs needs one entry per slot")
+    if caches and _slot_stride(caches[0]) % 8:
+        raise ValueError("the caches' slot stride must be a multiple of 16 bytes")
+    _index(refs, "refs", 1, device, torch.int32)
+    _index(tables, "tables", 2, device)
+    if kv_lens is not None:
+        _index(kv_lens, "kv_lens", 1, device)
+        if kv_lens.shape[0] != tables.shape[0]:
+            raise ValueError("kv_lens needs one entry per row of tables")
+    if page_tokens < 1 or page_tokens & (page_tokens - 1):
+        raise ValueError("page_tokens must be a power of two")
+    if tables.shape[1] * page_tokens >= 1 << 31:
+        raise ValueError("a table row may span at most 2**31 - 1 tokens")
+    if rows_list is not None:
+        _index(rows_list, "the row list", list_ndim, device)
+    _fail_count(fail_count, device)
+    state = (tables, refs) if kv_lens is None else (tables, kv_lens, refs)
+    if out is not None:
+        if len(out) != len(state):
+            raise ValueError(f"out needs {len(state)} tensors")
+        for o, i in zip(out, state):
+            if o.shape != i.shape or o.dtype != i.dtype or o.device != device or not o.is_contiguous():
+                raise ValueError("out must match the inputs in shape, dtype and device, and be contiguous")
+    if 0 in tables.shape or refs.shape[0] == 0:
+        raise ValueError("tables and refs must not be empty")
+    with _on(stream, device, (*caches, *state, rows_list, fail_count, *(out or ()))) as s:
+        if out is None:
+            out = tuple(torch.empty_like(t) for t in state)
+        page = caches[0][0].numel() * 2 if caches else 0
+        d = _lib.SiPagesDesc(
+            caches=(ct.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches]), ncaches=len(caches),
+            page_tokens=page_tokens, slot_bytes=2 * _slot_stride(caches[0]) if caches else 0, page_bytes=page,
+            nslots=refs.shape[0], tables=tables.data_ptr(), kv_lens=_ptr(kv_lens), refs=refs.data_ptr(),
+            tables_out=out[0].data_ptr(), kv_lens_out=None if kv_lens is None else out[1].data_ptr(),
+            refs_out=out[-1].data_ptr(), rows=tables.shape[0], table_pages=tables.shape[1], list=_ptr(rows_list),
+            n=0 if rows_list is None else rows_list.shape[0], scrub=int(bool(scrub)), fail_count=_ptr(fail_count))
+        need = int(lib().secure_infer_gpu_pages_workspace(ct.byref(d)))
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        d.workspace, d.workspace_bytes = workspace.data_ptr(), need
+        _check(getattr(lib(), fn_name)(s, ct.byref(d)), fn_name.removeprefix("secure_infer_gpu_"))
+    return tuple(out)
+
+
+def _page_tokens(caches) -> int:
+    caches = list(caches)
+    if not caches:
+        raise ValueError("no caches given")
+    _paged_cache(caches[0], "a cache")
+    return caches[0].shape[1]
+
+
+def fork_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, pairs: torch.Tensor,
+               fail_count: torch.Tensor | None = None, out=None, stream=None):
+    """Each pair (parent row, child row) of ``pairs`` [n, 2] int64 makes the child
+    the parent's copy: whole pages are shared (refs + 1), a partly filled last page is
+    copied in every tensor of ``caches`` into the lowest free slots, in the list's
+    order.  A child must be an empty row named once; a pair that cannot be served (a
+    row out of range, no free slot) leaves its child empty and is counted.
+    Returns (tables, kv_lens, refs), new or written to ``out`` (which may be the
+    inputs).  ``refs`` [slots] int32 counts the rows that hold a slot."""
+    if not isinstance(pairs, torch.Tensor) or pairs.ndim != 2 or pairs.shape[1] != 2:
+        raise ValueError("pairs must be [n, 2]")
+    return _pages_call("secure_infer_gpu_pages_fork", caches, tables, kv_lens, refs, _page_tokens(caches), pairs, 2,
+                       False, fail_count, out, stream)
+
+
+def free_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor,
+               scrub: bool = True, fail_count: torch.Tensor | None = None, out=None, stream=None):
+    """The rows named in ``rows`` [n] int64 give up their pages (refs - 1) and become
+    empty; with ``scrub`` a page nobody holds any more is zeroed in every tensor
+    of ``caches``, so a freed slot keeps no plaintext.  Returns (tables, kv_lens,
+    refs) as fork_pages does."""
+    return _pages_call("secure_infer_gpu_pages_free", caches, tables, kv_lens, refs, _page_tokens(caches), rows, 1,
+                       scrub, fail_count, out, stream)
+
+
+def compact_pages(caches, tables: torch.Tensor, refs: torch.Tensor, scrub: bool = False, out=None, stream=None):
+    """With L slots held, the held slots >= L move to the free slots < L (both
+    ascending) in every tensor of ``caches``; ``scrub`` zeroes the pages moved
+    from.  Returns (tables, refs), new or written to ``out``."""
+    return _pages_call("secure_infer_gpu_pages_compact", caches, tables, None, refs, _page_tokens(caches), None, 0,
+                       scrub, None, out, stream)
+
+
+def reserve_pages(tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, counts: torch.Tensor,
+                  page_tokens: int, fail_count: torch.Tensor | None = None, out=None, stream=None):
+    """Row b grows by counts[b] tokens (negative: by none) and takes the pages it
+    then lacks from the free slots, the lowest first, rows in order.  A row
+    that outgrows its table, or that needs more slots than are left, takes none
+    and is counted; its new length stands, so its tokens without a page are
+    dropped by paged_append and unseen by paged_attention.  Returns (tables,
+    kv_lens, refs) as fork_pages does."""
+    if not isinstance(counts, torch.Tensor) or not isinstance(tables, torch.Tensor) \
+            or counts.shape != tables.shape[:1]:
+        raise ValueError("counts needs one entry per row of tables")
+    return _pages_call("secure_infer_gpu_pages_reserve", (), tables, kv_lens, refs, int(page_tokens), counts, 1,
+                       False, fail_count, out, stream)
