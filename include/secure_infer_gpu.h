@@ -631,7 +631,7 @@ typedef struct si_paged_attention_desc {
     uint64_t table_stride;    /* entries from one sequence's row to the next   */
     const int64_t* kv_lens;
     const int64_t* q_starts;  /* seqs + 1, ascending; NULL: tokens == seqs     */
-    uint32_t table_pages;     /* entries of a row; table_pages * page_tokens < 2^31 */
+    uint32_t table_pages;     /* entries of a row; table_pages * page_tokens <= 2^30 */
     uint32_t tokens;          /* rows of q: tokens * q_heads < 2^31            */
     uint32_t seqs;
     uint32_t q_heads;         /* a multiple of kv_heads                        */

@@ -1,4 +1,13 @@
 // Attention of new tokens over a paged KV cache.
+//
+// Both kernels compute the transposed scores S^T = K Q^T with matrix
+// instructions, so a query is a column: a lane holds one query's scores of
+// several keys, the softmax statistics are per lane, and the weights already
+// lie where the second product O^T = V^T P^T takes them (its contraction runs
+// over keys, whose order within an instruction is free as long as V's rows
+// come in the same order).  V^T comes out of LDS through transposing reads.
+// The rows of one KV head are (token, query head) pairs of its group, so K and V
+// are read once for all heads that share them.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -25,9 +34,39 @@ struct AttendArgs {
     uint64_t table_stride;
     const int64_t* kv_lens;
     const int64_t* q_starts;
-    uint32_t pages, tokens, seqs, q_heads, kv_heads, dim, page_shift, causal, window;
-    float scale_log2;  // scale * log2(e): weights are powers of two
+    uint32_t pages, tokens, seqs, q_heads, kv_heads, group, dim, page_shift, causal, window;
+    uint32_t negate;   // the scale is negative: q's sign is flipped instead
+    float scale_log2;  // |scale| * log2(e): weights are powers of two
+    // Sequences of at most few_rows rows (tokens * group) belong to the few-row
+    // kernel, the others to the tile kernel.
+    uint32_t few_rows, few_split, tile_split, tiles;
+    // Parts of split sequences: numerators (dim floats a row) and (m, l).
+    float* few_o;
+    float2* few_ml;
+    float* tile_o;
+    float2* tile_ml;
 };
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// The tile kernel's keys per step, and the fewest keys a split is made for.
+constexpr uint32_t kTileKeys = 64;
+constexpr uint32_t kTileWaves = 4;
+constexpr uint32_t kTileRows = 32 * kTileWaves;
+constexpr uint32_t kTileSplitMin = 512;
+// The few-row kernel's keys per wave and step; a workgroup's step.
+constexpr uint32_t kFewKeys = 32;
+constexpr uint32_t kFewWaves = 4;
+constexpr uint32_t kFewStep = kFewKeys * kFewWaves;
+constexpr uint32_t kMaxSplit = 64;
 
 __device__ __forceinline__ bool held(int64_t e, int64_t nslots) { return e >= 0 && e < nslots; }
 
@@ -45,86 +84,801 @@ __device__ __forceinline__ uint16_t from_f32(float x)
     else return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
 }
 
-// One wave per (token, query head): 64 keys at a time, one key a lane for the
-// scores, the head's dims over the lanes for the sum over the values.
 template <bool kBf16>
-__global__ __launch_bounds__(64) void attend_plain_kernel(AttendArgs a)
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c)
 {
-    __shared__ float qs[256];
-    const uint32_t lane = threadIdx.x;
-    const uint32_t t = blockIdx.x / a.q_heads, h = blockIdx.x - t * a.q_heads;
-    const uint32_t kvh = h / (a.q_heads / a.kv_heads);
-    uint32_t b = t;
-    int64_t back = 1;  // tokens from here to the sequence's end
-    bool owned = true;
+    if constexpr (kBf16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
+{
+    if constexpr (kBf16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+}
+
+// Eight floats rounded to nearest even: the weights' one rounding, to the
+// type the matrix instruction takes (relative 2^-9 / 2^-12 a weight; the sum
+// they are divided by is that of the unrounded ones, in float).
+template <bool kBf16>
+__device__ __forceinline__ u32x4 pack8(f32x8 x)
+{
+    if constexpr (kBf16) return __builtin_bit_cast(u32x4, __builtin_convertvector(x, bf16x8));
+    else return __builtin_bit_cast(u32x4, __builtin_convertvector(x, f16x8));
+}
+
+// Four rows of a 16-bit matrix in LDS, transposed: each 16 lanes read 4 rows x
+// 16 columns (lane i: row i / 4, columns 4 (i % 4) ..) and lane i receives column
+// i of the 4 rows.
+__device__ __forceinline__ u32x2 read_tr(const uint16_t* p)
+{
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+}
+
+// max / sum over lanes l, l ^ 32 and (kQuarters) l ^ 16: the lanes that hold
+// the same query.
+template <bool kQuarters, class F>
+__device__ __forceinline__ float across(float x, F f)
+{
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    if constexpr (kQuarters) {
+        const uint32_t v = __float_as_uint(x);
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        x = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    }
+    return x;
+}
+
+__device__ __forceinline__ float fmax2(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float fadd2(float a, float b) { return a + b; }
+
+template <bool kBf16>
+__device__ __forceinline__ bool nonfinite(uint32_t x)
+{
+    constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
+    return (x & e) == e;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ bool any_nonfinite(u32x4 x)
+{
+    bool r = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r = r || nonfinite<kBf16>(x[i]) || nonfinite<kBf16>(x[i] >> 16);
+    return r;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ u32x4 zero_nonfinite(u32x4 x)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (nonfinite<kBf16>(x[i])) x[i] &= 0xffff0000u;
+        if (nonfinite<kBf16>(x[i] >> 16)) x[i] &= 0x0000ffffu;
+    }
+    return x;
+}
+
+// One sequence's rows of q and positions.
+struct Seq {
+    uint32_t b;
+    uint32_t q0, n_new;  // rows [q0, q0 + n_new) of q
+    int32_t len;         // keys
+    int32_t base;        // position of its first new token (may be negative)
+};
+
+__device__ __forceinline__ uint32_t start_of(const AttendArgs& a, uint32_t b)
+{
+    const int64_t s = a.q_starts[b];
+    return uint32_t(s < 0 ? 0 : s > int64_t(a.tokens) ? int64_t(a.tokens) : s);
+}
+
+__device__ __forceinline__ Seq seq_of(const AttendArgs& a, uint32_t b)
+{
+    Seq s;
+    s.b = b;
+    s.q0 = b;
+    s.n_new = 1;
     if (a.q_starts) {
-        uint32_t at_or_before = 0;
-        for (uint32_t s0 = 0; s0 <= a.seqs; s0 += 64) {
-            const bool le = s0 + lane <= a.seqs && a.q_starts[s0 + lane] <= int64_t(t);
-            at_or_before += __popcll(__ballot(le));
-        }
-        owned = at_or_before != 0 && at_or_before <= a.seqs;
-        if (owned) {
-            b = at_or_before - 1;
-            const int64_t end = a.q_starts[b + 1];
-            back = (end < a.tokens ? end : a.tokens) - t;
-        }
+        s.q0 = start_of(a, b);
+        const uint32_t end = start_of(a, b + 1);
+        s.n_new = end > s.q0 ? end - s.q0 : 0;
     }
     const int64_t most = int64_t(a.pages) << a.page_shift;
-    int64_t n = owned ? a.kv_lens[b] : 0;
-    n = n < 0 ? 0 : n > most ? most : n;
-    const int64_t p = n - back;
-    const int64_t hi = a.causal ? p + 1 : n;
-    int64_t lo = a.window && p - int64_t(a.window) + 1 > 0 ? p - int64_t(a.window) + 1 : 0;
-    for (uint32_t d = lane; d < a.dim; d += 64)
-        qs[d] = to_f32<kBf16>(a.q[t * a.q_token + h * a.q_head + d]) * a.scale_log2;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, acc[4] = {0, 0, 0, 0};
-    for (int64_t j0 = lo; j0 < hi; j0 += 64) {
-        const int64_t j = j0 + lane;
-        int64_t slot = -1;
-        if (j < hi) slot = a.tables[b * a.table_stride + uint64_t(j >> a.page_shift)];
-        const bool seen = held(slot, a.nslots);
-        const uint64_t o = seen ? uint64_t(slot) * a.slot_bytes +
-                                      (uint64_t(j & ((1ll << a.page_shift) - 1)) * a.kv_heads + kvh) * a.dim * 2
-                                : 0;
-        float s = -INFINITY;
-        if (seen) {
-            const uint16_t* k = reinterpret_cast<const uint16_t*>(a.cache_k + o);
-            s = 0.0f;
-            for (uint32_t d = 0; d < a.dim; ++d) s = __builtin_fmaf(qs[d], to_f32<kBf16>(k[d]), s);
-        }
-        float top = s;
+    const int64_t n = a.kv_lens[b];
+    s.len = int32_t(n < 0 ? 0 : n > most ? most : n);
+    s.base = s.len - int32_t(s.n_new);
+    return s;
+}
+
+// How a sequence's keys are cut: parts of `per` keys from `lo`.
+struct Cut {
+    int32_t lo, per;
+    uint32_t parts;
+};
+
+__device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Seq& s, uint32_t split, int32_t step, int32_t least)
+{
+    Cut c;
+    c.lo = 0;
+    if (a.window && s.base - int32_t(a.window) + 1 > 0) c.lo = (s.base - int32_t(a.window) + 1) & ~63;
+    const int32_t span = s.len > c.lo ? s.len - c.lo : 0;
+    int32_t per = (span + int32_t(split) - 1) / int32_t(split);
+    per = per < least ? least : per;
+    c.per = (per + step - 1) / step * step;
+    c.parts = uint32_t((span + c.per - 1) / c.per);
+    return c;
+}
+
+// Rows of q before the first sequence and after the last: nothing to see.
+template <bool kBf16>
+__device__ void zero_unowned(const AttendArgs& a)
+{
+    const uint32_t first = start_of(a, 0), end = start_of(a, a.seqs);
+    const uint32_t n = first + (end < a.tokens ? a.tokens - end : 0);
+    for (uint32_t i = threadIdx.x; i < n * a.q_heads; i += blockDim.x) {
+        const uint32_t x = i / a.q_heads, h = i - x * a.q_heads;
+        const uint32_t t = x < first ? x : end + (x - first);
+        for (uint32_t d = 0; d < a.dim; d += 8)
+            *reinterpret_cast<u32x4*>(a.out + t * a.out_token + h * a.out_head + d) = u32x4{0, 0, 0, 0};
+        if (a.lse) a.lse[uint64_t(t) * a.q_heads + h] = -INFINITY;
+    }
+}
+
+// The slots of `kKeys` consecutive keys from k0 (lane j: key k0 + j % kKeys),
+// and which of them may be read: held pages, lo <= key < hi.
+template <int kKeys>
+struct Keys {
+    int64_t slot;   // per lane; with pages of at least kKeys tokens, the tile's
+    uint64_t ok;    // bit j: key k0 + j
+
+    __device__ __forceinline__ void find(const AttendArgs& a, const int64_t* table, int32_t k0, int32_t lo, int32_t hi)
+    {
+        const uint32_t lane = threadIdx.x & 63u;
+        const int32_t k = k0 + int32_t(lane & (kKeys - 1));
+        slot = -1;
+        if (k >= lo && k < hi) slot = table[k >> a.page_shift];
+        ok = __ballot(held(slot, a.nslots));
+        if constexpr (kKeys < 64) ok &= (1ull << kKeys) - 1ull;
+    }
+    // Byte offset of key k0 + j's row of KV head kvh in its cache (j: this
+    // lane's choice; every lane calls it).
+    __device__ __forceinline__ uint64_t row(const AttendArgs& a, int32_t k0, uint32_t j, uint32_t kvh) const
+    {
+        const int64_t s = __shfl(slot, int(j));
+        return uint64_t(s) * a.slot_bytes +
+               (uint64_t((uint32_t(k0) + j) & ((1u << a.page_shift) - 1u)) * a.kv_heads + kvh) * (a.dim * 2u);
+    }
+};
+
+// Bits j of the keys k0 + j a query at position p sees among the `ok` ones.
+__device__ __forceinline__ uint64_t seen_bits(const AttendArgs& a, uint64_t ok, int32_t k0, int32_t p)
+{
+    if (a.causal) {
+        const int32_t last = p - k0;  // keys up to bit `last`
+        ok &= last < 0 ? 0ull : last >= 63 ? ~0ull : (2ull << last) - 1ull;
+    }
+    if (a.window) {
+        const int32_t first = p - int32_t(a.window) + 1 - k0;
+        ok &= first <= 0 ? ~0ull : first > 63 ? 0ull : ~0ull << first;
+    }
+    return ok;
+}
+
+// Four dims of one row: the numerators divided by the weights' sum.  l = 0: no
+// key had a weight.
+template <bool kBf16>
+__device__ __forceinline__ void store_out(const AttendArgs& a, uint32_t t, uint32_t h, uint32_t d, f32x4 acc, float l,
+                                          float shift)
+{
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    u32x2 v;
 #pragma unroll
-        for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-        const float mn = fmaxf(m, top);
-        if (mn == -INFINITY) continue;
-        const float w = seen ? exp2f(s - mn) : 0.0f;
-        const float keep = exp2f(m - mn);
-        m = mn;
-        float sum = w;
+    for (int i = 0; i < 2; ++i)
+        v[i] = uint32_t(from_f32<kBf16>(acc[2 * i] * inv)) | uint32_t(from_f32<kBf16>(acc[2 * i + 1] * inv)) << 16;
+    *reinterpret_cast<u32x2*>(a.out + t * a.out_token + h * a.out_head + d) = v;
+    if (a.lse && d == 0)
+        a.lse[uint64_t(t) * a.q_heads + h] = l == 0.0f ? -INFINITY : (shift + log2f(l)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------- few rows
+
+// One workgroup per (sequence, KV head, part of the keys): at most 16 * kBlocks
+// rows.  Each wave takes every fourth step of 32 keys: K straight into the
+// registers of S^T = K Q^T, V through the wave's own LDS.  Memory bounds
+// it: the next step's K and V are in flight while a step is computed, with no
+// barrier until the waves' results are joined at the end.
+template <bool kBf16, int kDim, int kBlocks>
+__global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few_kernel(AttendArgs a)
+{
+    constexpr int kSteps = kDim / 32;       // contraction steps of K Q^T
+    constexpr int kOut = kDim / 16;         // 16-wide blocks of the output
+    constexpr int kChunks = kDim / 8;       // 16-byte chunks of a row
+    constexpr int kPitch = kDim + 16;       // LDS row of V: 32 bytes of padding spread the rows over the banks
+    constexpr int kLoads = kChunks / 2;     // 16-byte loads a lane makes for 32 rows
+    constexpr int kOPitch = kDim + 4;
+    constexpr int kV = kFewKeys * kPitch * 2;
+    constexpr int kO = 16 * kOPitch * 4;
+    constexpr int kWaveBytes = kV > kO ? kV : kO;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves * kWaveBytes];
+    __shared__ float2 ml[kFewWaves][16];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t col = lane & 15u, quad = lane >> 4;
+    if (a.q_starts && blockIdx.x == 0 && blockIdx.y == 0) zero_unowned<kBf16>(a);
+    const uint32_t kvh = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads, part = blockIdx.y;
+    const Seq s = seq_of(a, b);
+    const uint32_t rows = s.n_new * a.group;
+    if (rows == 0 || rows > 16 * kBlocks) return;
+    const Cut cut = cut_of(a, s, a.few_split, kFewStep, kFewStep);
+    if (part > 0 && part >= cut.parts) return;
+    const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
+
+    // Positions: row r is token r / group; the last row's token sees most.
+    int32_t pos[kBlocks];
+    u32x4 q[kBlocks][kSteps];
 #pragma unroll
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-        l = __builtin_fmaf(l, keep, sum);
+    for (int x = 0; x < kBlocks; ++x) {
+        const uint32_t r = 16 * x + col;
+        const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
+        pos[x] = s.base + int32_t(tok);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= keep;
-        const uint64_t mask = __ballot(seen);
-        for (int kk = 0; kk < 64; ++kk) {
-            if (!(mask >> kk & 1)) continue;
-            const float wk = __shfl(w, kk);
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(a.cache_v + __shfl(o, kk));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + 64 * i < a.dim) acc[i] = __builtin_fmaf(wk, to_f32<kBf16>(v[lane + 64 * i]), acc[i]);
+        for (int k = 0; k < kSteps; ++k) {
+            const uint32_t d = 32 * k + 8 * quad;
+            u32x4 v{0, 0, 0, 0};
+            if (r < rows && d < a.dim)
+                v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
+            q[x][k] = v ^ (a.negate ? 0x80008000u : 0u);
         }
     }
-    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    const int32_t p_last = s.base + int32_t(s.n_new) - 1;
+    const int32_t hi0 = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
+    const int32_t hi = hi0 < cut.lo + int32_t(part + 1) * cut.per ? hi0 : cut.lo + int32_t(part + 1) * cut.per;
+    const int32_t k_first = cut.lo + int32_t(part) * cut.per;
+    // keys below lo are behind every row's window
+    const int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
+
+    uint16_t* const vs = reinterpret_cast<uint16_t*>(lds + wave * kWaveBytes);
+    float m[kBlocks], l[kBlocks];
+    f32x4 o[kBlocks][kOut];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < a.dim)
-            a.out[t * a.out_token + h * a.out_head + lane + 64 * i] = from_f32<kBf16>(acc[i] * inv);
-    if (a.lse && lane == 0)
-        a.lse[uint64_t(t) * a.q_heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    for (int x = 0; x < kBlocks; ++x) {
+        m[x] = -INFINITY;
+        l[x] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) o[x][i] = f32x4{0, 0, 0, 0};
+    }
+
+    u32x4 kr[2][kSteps], vr[kLoads];
+    Keys<kFewKeys> keys;
+    const auto load_k = [&](int32_t k0) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const uint32_t j = 16 * y + col;
+            const uint64_t off = keys.row(a, k0, j, kvh);
+            const bool ok = keys.ok >> j & 1;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const uint32_t d = 32 * k + 8 * quad;
+                kr[y][k] = u32x4{0, 0, 0, 0};
+                if (ok && d < a.dim) kr[y][k] = *reinterpret_cast<const u32x4*>(a.cache_k + off + d * 2);
+            }
+        }
+    };
+    const auto load_v = [&](int32_t k0) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t c = 64 * i + lane, j = c / kChunks, d = (c % kChunks) * 8;
+            const uint64_t off = keys.row(a, k0, j, kvh);
+            vr[i] = u32x4{0, 0, 0, 0};
+            if ((keys.ok >> j & 1) && d < a.dim) vr[i] = *reinterpret_cast<const u32x4*>(a.cache_v + off + d * 2);
+        }
+    };
+    int32_t k0 = k_first + int32_t(wave * kFewKeys);
+    if (k0 < hi) {
+        keys.find(a, table, k0, lo, hi);
+        load_k(k0);
+        load_v(k0);
+    }
+    for (; k0 < hi; k0 += int32_t(kFewStep)) {
+        const uint64_t ok = keys.ok;
+        const int32_t next = k0 + int32_t(kFewStep);
+        if (next < hi) keys.find(a, table, next, lo, hi);
+        f32x4 st[kBlocks][2];
+#pragma unroll
+        for (int x = 0; x < kBlocks; ++x) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                st[x][y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) st[x][y] = mfma16<kBf16>(kr[y][k], q[x][k], st[x][y]);
+            }
+        }
+        if (next < hi) load_k(next);
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t c = 64 * i + lane;
+            *reinterpret_cast<u32x4*>(vs + (c / kChunks) * kPitch + (c % kChunks) * 8) = vr[i];
+        }
+        // A key that some rows see and others do not: 0 x inf and 0 x NaN in
+        // the matrix product would reach the rows that do not.
+        const bool partial =
+            s.n_new > 1 && ((a.causal && k0 + int32_t(kFewKeys) - 1 > s.base) ||
+                            (a.window && k0 <= p_last - int32_t(a.window)));
+        if (partial) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) odd |= any_nonfinite<kBf16>(vr[i]);
+        }
+        if (next < hi) load_v(next);
+
+        u32x4 pw[kBlocks];
+        uint32_t seen[kBlocks];
+#pragma unroll
+        for (int x = 0; x < kBlocks; ++x) {
+            seen[x] = uint32_t(partial ? seen_bits(a, ok, k0, pos[x]) : ok);
+            const uint32_t mine = seen[x] >> (4 * quad);
+            float top = -INFINITY;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!(mine >> (16 * y + i) & 1)) st[x][y][i] = -INFINITY;
+                    top = fmaxf(top, st[x][y][i]);
+                }
+            top = across<true>(top, fmax2);
+            const float mn = fmaxf(m[x], top);
+            const float safe = mn == -INFINITY ? 0.0f : mn;
+            const float keep = __builtin_amdgcn_exp2f((m[x] - safe) * a.scale_log2);
+            const float shift = safe * a.scale_log2;
+            m[x] = mn;
+            f32x8 w;
+            float sum = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[4 * y + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][y][i], a.scale_log2, -shift));
+                    sum += w[4 * y + i];
+                }
+            l[x] = __builtin_fmaf(l[x], keep, sum);
+            pw[x] = pack8<kBf16>(w);
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) o[x][i] *= keep;
+        }
+        if (partial && __ballot(odd) != 0) {
+            // Rows that see a key with an infinity or NaN take it itself (a
+            // weight is positive); then it is cleared for the product.
+            for (uint32_t j = 0; j < kFewKeys; ++j) {
+#pragma unroll
+                for (int i = 0; i < kOut; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t v = vs[j * kPitch + 16 * i + 4 * quad + e];
+                        if (nonfinite<kBf16>(v)) {
+#pragma unroll
+                            for (int x = 0; x < kBlocks; ++x)
+                                if (seen[x] >> j & 1) o[x][i][e] += to_f32<kBf16>(v);
+                        }
+                    }
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t c = 64 * i + lane;
+                u32x4* v = reinterpret_cast<u32x4*>(vs + (c / kChunks) * kPitch + (c % kChunks) * 8);
+                *v = zero_nonfinite<kBf16>(*v);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+            // keys 4 quad + 0..3 and 16 + 4 quad + 0..3 of 16 columns
+            const uint16_t* v = vs + (4 * quad + (col >> 2)) * kPitch + 16 * i + 4 * (col & 3u);
+            const u32x2 v0 = read_tr(v), v1 = read_tr(v + 16 * kPitch);
+            const u32x4 vt{v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+            for (int x = 0; x < kBlocks; ++x) o[x][i] = mfma16<kBf16>(vt, pw[x], o[x][i]);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // Join the waves, 16 rows at a time.
+#pragma unroll
+    for (int x = 0; x < kBlocks; ++x) {
+        if (16 * x >= int(rows)) break;
+        __syncthreads();
+        const float lw = across<true>(l[x], fadd2);
+        if (quad == 0) ml[wave][col] = float2{m[x], lw};
+        float* ow = reinterpret_cast<float*>(lds + wave * kWaveBytes);
+#pragma unroll
+        for (int i = 0; i < kOut; ++i)
+            *reinterpret_cast<f32x4*>(ow + col * kOPitch + 16 * i + 4 * quad) = o[x][i];
+        __syncthreads();
+        const uint32_t quads = a.dim / 4;
+        for (uint32_t e = threadIdx.x; e < 16 * quads; e += 64 * kFewWaves) {
+            const uint32_t rr = e / quads, d = (e - rr * quads) * 4, r = 16 * x + rr;
+            if (r >= rows) break;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < int(kFewWaves); ++w) top = fmaxf(top, ml[w][rr].x);
+            const float safe = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+            f32x4 acc{0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < int(kFewWaves); ++w) {
+                const float2 v = ml[w][rr];
+                const float f = __builtin_amdgcn_exp2f((v.x - safe) * a.scale_log2);
+                sum = __builtin_fmaf(v.y, f, sum);
+                acc += *reinterpret_cast<const f32x4*>(lds + w * kWaveBytes + (rr * kOPitch + d) * 4) * f;
+            }
+            const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group), t = s.q0 + tok;
+            if (cut.parts > 1) {
+                const uint64_t row = (uint64_t(part) * a.seqs * a.kv_heads + uint64_t(b) * a.kv_heads + kvh) * a.few_rows + r;
+                *reinterpret_cast<f32x4*>(a.few_o + row * a.dim + d) = acc;
+                if (d == 0) a.few_ml[row] = float2{safe * a.scale_log2, sum};
+            } else {
+                store_out<kBf16>(a, t, h, d, acc, sum, safe * a.scale_log2);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- tiles of rows
+
+// One workgroup per (128 rows of a sequence and KV head, part of the keys):
+// each of the 4 waves holds 32 rows, all of them share the K and V of 64 keys
+// at a time, staged through registers into two LDS buffers (one barrier a
+// step).  Rows of LDS are 16-byte chunks in an order permuted by the row
+// (a power of two of them), so that the 8 rows of a read fall on different banks.
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_tile_kernel(AttendArgs a)
+{
+    constexpr int kChunks = kDim <= 64 ? 8 : kDim <= 128 ? 16 : 32;  // chunks of an LDS row
+    constexpr int kPitch = kChunks * 8;
+    constexpr int kThreads = 64 * int(kTileWaves);
+    constexpr int kLoads = int(kTileKeys) * kChunks / kThreads;
+    constexpr int kRowStep = kThreads / kChunks;
+    constexpr int kSteps = kDim / 16;
+    constexpr int kOut = kDim / 32;
+    __shared__ __attribute__((aligned(16))) uint16_t ks[2][kTileKeys * kPitch];
+    __shared__ __attribute__((aligned(16))) uint16_t vs[2][kTileKeys * kPitch];
+    __shared__ uint32_t odd_flag[2];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t col = lane & 31u, half = lane >> 5;
+    if (a.q_starts && a.few_rows == 0 && blockIdx.x == 0) zero_unowned<kBf16>(a);
+
+    // Workgroups in groups of one KV head's part; consecutive ones go to the
+    // same XCD (workgroup i runs on XCD i % 8), whose L2 then holds their K and V.
+    const uint32_t total = gridDim.x;
+    const uint32_t x8 = total / 8, r8 = total % 8;
+    const uint32_t xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+    const uint32_t w = xcd * x8 + (xcd < r8 ? xcd : r8) + nth;
+    const uint32_t tile = a.tiles - 1 - w % a.tiles;  // the last tiles see most keys: first
+    const uint32_t rest = w / a.tiles;
+    const uint32_t part = rest % a.tile_split, kvh = rest / a.tile_split;
+
+    // Sequence b's tiles start at floor(q_starts[b] * group / rows) + b, which
+    // leaves it at least the tiles it needs.
+    uint32_t b = tile;
+    uint32_t first_tile = tile;
+    if (a.q_starts) {
+        uint32_t at_or_before = 0;
+        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
+            const uint32_t s = s0 + lane;
+            const uint32_t f = s < a.seqs ? uint32_t(uint64_t(start_of(a, s)) * a.group / kTileRows) + s : 0;
+            const uint64_t le = __ballot(s < a.seqs && f <= tile);
+            at_or_before += __popcll(le);
+            if (le) first_tile = __builtin_amdgcn_readfirstlane(__shfl(f, 63 - __clzll(le)));
+        }
+        if (at_or_before == 0) return;
+        b = at_or_before - 1;
+    } else {
+        b = tile / ((a.group + kTileRows - 1) / kTileRows);
+        first_tile = b * ((a.group + kTileRows - 1) / kTileRows);
+    }
+    const Seq s = seq_of(a, b);
+    const uint32_t rows = s.n_new * a.group;
+    const uint32_t r0 = (tile - first_tile) * kTileRows;
+    if (rows <= a.few_rows || r0 >= rows) return;
+    const Cut cut = cut_of(a, s, a.tile_split, kTileKeys, kTileSplitMin);
+    if (part > 0 && part >= cut.parts) return;
+    const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
+
+    const uint32_t r_last = (r0 + kTileRows < rows ? r0 + kTileRows : rows) - 1;
+    const int32_t p_first = s.base + int32_t(r0 / a.group), p_last = s.base + int32_t(r_last / a.group);
+    const uint32_t r = r0 + wave * 32 + col;
+    const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
+    const int32_t pos = s.base + int32_t(tok);
+    u32x4 q[kSteps];
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        const uint32_t d = 16 * k + 8 * half;
+        u32x4 v{0, 0, 0, 0};
+        if (r < rows && d < a.dim)
+            v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
+        q[k] = v ^ (a.negate ? 0x80008000u : 0u);
+    }
+    const int32_t part_end = cut.lo + int32_t(part + 1) * cut.per;
+    int32_t hi = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
+    hi = hi < part_end ? hi : part_end;
+    const int32_t lo = a.window ? p_first - int32_t(a.window) + 1 : 0;  // behind every row's window below
+    int32_t k0 = cut.lo + int32_t(part) * cut.per;
+    if (a.window && lo > k0) k0 = lo & ~int32_t(kTileKeys - 1);
+
+    f32x16 o[kOut];
+#pragma unroll
+    for (int i = 0; i < kOut; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    u32x4 kr[kLoads], vr[kLoads];
+    const uint32_t chunk = threadIdx.x % kChunks, row0 = threadIdx.x / kChunks;
+    const uint32_t kv_row = a.kv_heads * a.dim * 2u;
+    Keys<kTileKeys> keys;
+    const auto load = [&](int32_t kb) {
+        if ((1u << a.page_shift) >= kTileKeys) {
+            // one page holds the tile
+            int64_t slot = -1;
+            if (keys.ok) slot = __shfl(keys.slot, __builtin_ctzll(keys.ok));
+            slot = (int64_t(__builtin_amdgcn_readfirstlane(int(slot >> 32))) << 32) |
+                   uint32_t(__builtin_amdgcn_readfirstlane(int(slot)));
+            const uint64_t at = uint64_t(slot) * a.slot_bytes +
+                                uint64_t(uint32_t(kb) & ((1u << a.page_shift) - 1u)) * kv_row + kvh * a.dim * 2u;
+            const uint8_t* kp = a.cache_k + at;
+            const uint8_t* vp = a.cache_v + at;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t j = row0 + i * kRowStep;
+                kr[i] = vr[i] = u32x4{0, 0, 0, 0};
+                if ((keys.ok >> j & 1) && chunk * 8 < a.dim) {
+                    kr[i] = *reinterpret_cast<const u32x4*>(kp + j * kv_row + chunk * 16);
+                    vr[i] = *reinterpret_cast<const u32x4*>(vp + j * kv_row + chunk * 16);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t j = row0 + i * kRowStep;
+                const uint64_t off = keys.row(a, kb, j, kvh) + chunk * 16;
+                kr[i] = vr[i] = u32x4{0, 0, 0, 0};
+                if ((keys.ok >> j & 1) && chunk * 8 < a.dim) {
+                    kr[i] = *reinterpret_cast<const u32x4*>(a.cache_k + off);
+                    vr[i] = *reinterpret_cast<const u32x4*>(a.cache_v + off);
+                }
+            }
+        }
+    };
+    // Chunk orders: K is read a chunk of 32 rows at a time (8 lanes a
+    // clock: rows of different r % 8), V two chunks of 4 rows.
+    const auto k_at = [](uint32_t row, uint32_t c) { return row * kPitch + ((c ^ (row & (kChunks - 1))) * 8); };
+    const auto v_at = [](uint32_t row, uint32_t c) {
+        return row * kPitch + ((c ^ ((row << 1) & (kChunks - 1) & 14)) * 8);
+    };
+    const auto stage = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t j = row0 + i * kRowStep;
+            *reinterpret_cast<u32x4*>(&ks[buf][k_at(j, chunk)]) = kr[i];
+            *reinterpret_cast<u32x4*>(&vs[buf][v_at(j, chunk)]) = vr[i];
+        }
+    };
+    // Keys that some of the tile's rows see and others do not.
+    const auto is_partial = [&](int32_t kb) {
+        return (a.causal && kb + int32_t(kTileKeys) - 1 > p_first) || (a.window && kb <= p_last - int32_t(a.window));
+    };
+    // Before the barrier that makes a buffer visible: does it hold an infinity
+    // or NaN in V that not every row sees?
+    const auto flag_odd = [&](int buf, int32_t kb) {
+        if (!is_partial(kb)) return;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) odd |= any_nonfinite<kBf16>(vr[i]);
+        if (__ballot(odd) && lane == 0) odd_flag[buf] = 1;
+    };
+
+    if (threadIdx.x < 2) odd_flag[threadIdx.x] = 0;
+    uint64_t ok = 0;
+    if (k0 < hi) {
+        keys.find(a, table, k0, lo, hi);
+        load(k0);
+        ok = keys.ok;
+    }
+    __syncthreads();
+    if (k0 < hi) {
+        stage(0);
+        flag_odd(0, k0);
+        if (k0 + int32_t(kTileKeys) < hi) {
+            keys.find(a, table, k0 + int32_t(kTileKeys), lo, hi);
+            load(k0 + int32_t(kTileKeys));
+        }
+    }
+    __syncthreads();
+    int buf = 0;
+    for (; k0 < hi; k0 += int32_t(kTileKeys)) {
+        const int32_t next = k0 + int32_t(kTileKeys);
+        f32x16 st[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[y][e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(&ks[buf][k_at(32 * y + col, 2 * k + half)]);
+                st[y] = mfma32<kBf16>(kf, q[k], st[y]);
+            }
+        }
+        const bool partial = is_partial(k0);
+        uint64_t seen = ok;
+        if (partial) seen = seen_bits(a, ok, k0, pos);
+        if (partial || ok != ~0ull) {
+            const uint64_t mine = seen >> (4 * half);
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(mine >> (32 * y + 8 * (e / 4) + e % 4) & 1)) st[y][e] = -INFINITY;
+        }
+        float top = st[0][0];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, st[y][e]);
+        top = across<false>(top, fmax2);
+        const float mn = fmaxf(m, top);
+        const float safe = mn == -INFINITY ? 0.0f : mn;
+        if (__ballot(mn != m)) {
+            const float keep = __builtin_amdgcn_exp2f((m - safe) * a.scale_log2);
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) o[i] *= keep;
+        }
+        m = mn;
+        const float shift = safe * a.scale_log2;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                st[y][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][e], a.scale_log2, -shift));
+                l += st[y][e];
+            }
+        if (partial && odd_flag[buf]) {
+            // Rows that see a key with an infinity or NaN take it itself (a
+            // weight is positive); then it is cleared for the product.
+            for (uint32_t j = 0; j < kTileKeys; ++j) {
+#pragma unroll
+                for (int i = 0; i < kOut; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const uint32_t d = 32 * i + 8 * (e / 4) + 4 * half + e % 4;
+                        const uint16_t v = vs[buf][v_at(j, d / 8) + d % 8];
+                        if (nonfinite<kBf16>(v) && (seen >> j & 1)) o[i][e] += to_f32<kBf16>(v);
+                    }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                u32x4* v = reinterpret_cast<u32x4*>(&vs[buf][v_at(row0 + i * kRowStep, chunk)]);
+                *v = zero_nonfinite<kBf16>(*v);
+            }
+            if (threadIdx.x == 0) odd_flag[buf] = 0;
+            __syncthreads();
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            f32x8 w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = st[y / 2][8 * (y % 2) + e];
+            const u32x4 pw = pack8<kBf16>(w);
+            const uint32_t row = 16 * y + 4 * half + ((lane & 15u) >> 2);
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {
+                const uint32_t d = 32 * i + (lane & 16u) + 4 * (lane & 3u);
+                const u32x2 v0 = read_tr(&vs[buf][v_at(row, d / 8) + d % 8]);
+                const u32x2 v1 = read_tr(&vs[buf][v_at(row + 8, d / 8) + d % 8]);
+                o[i] = mfma32<kBf16>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pw, o[i]);
+            }
+        }
+        buf ^= 1;
+        if (next < hi) {
+            stage(buf);
+            flag_odd(buf, next);
+            ok = keys.ok;
+            if (next + int32_t(kTileKeys) < hi) {
+                keys.find(a, table, next + int32_t(kTileKeys), lo, hi);
+                load(next + int32_t(kTileKeys));
+            }
+        }
+        __syncthreads();
+    }
+
+    l = across<false>(l, fadd2);
+    if (r >= rows) return;
+    const uint32_t t = s.q0 + tok;
+    const float shift = m == -INFINITY ? 0.0f : m * a.scale_log2;
+    if (cut.parts > 1) {
+        const uint64_t row = (uint64_t(part) * a.tokens + t) * a.q_heads + h;
+        if (half == 0) a.tile_ml[row] = float2{shift, l};
+#pragma unroll
+        for (int i = 0; i < kOut; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const uint32_t d = 32 * i + 2 * e + 4 * half;
+                if (d < a.dim)
+                    *reinterpret_cast<f32x4*>(a.tile_o + row * a.dim + d) =
+                        f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kOut; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const uint32_t d = 32 * i + 2 * e + 4 * half;
+                if (d < a.dim)
+                    store_out<kBf16>(a, t, h, d, f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]}, l, shift);
+            }
+    }
+}
+
+// ---------------------------------------------------------------- parts joined
+
+// One wave per (token, query head) of a split sequence: the parts' (m, l) one
+// a lane, then the numerators, 4 dims a lane, in the order of the parts.
+template <bool kBf16>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t th = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (th >= a.tokens * a.q_heads) return;
+    const uint32_t t = th / a.q_heads, h = th - t * a.q_heads;
+    uint32_t b = t;
+    if (a.q_starts) {
+        uint32_t at_or_before = 0;
+        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64)
+            at_or_before += __popcll(__ballot(s0 + lane < a.seqs && start_of(a, s0 + lane) <= t));
+        if (at_or_before == 0) return;
+        b = at_or_before - 1;
+    }
+    const Seq s = seq_of(a, b);
+    if (t < s.q0 || t >= s.q0 + s.n_new) return;
+    const bool few = s.n_new * a.group <= a.few_rows;
+    const Cut cut = few ? cut_of(a, s, a.few_split, kFewStep, kFewStep)
+                        : cut_of(a, s, a.tile_split, kTileKeys, kTileSplitMin);
+    if (cut.parts <= 1) return;
+    const uint32_t kvh = h / a.group;
+    const uint64_t row = few ? (uint64_t(b) * a.kv_heads + kvh) * a.few_rows + (t - s.q0) * a.group + (h - kvh * a.group)
+                             : uint64_t(t) * a.q_heads + h;
+    const uint64_t step = few ? uint64_t(a.seqs) * a.kv_heads * a.few_rows : uint64_t(a.tokens) * a.q_heads;
+    const float2* mls = (few ? a.few_ml : a.tile_ml) + row;
+    const float* os = (few ? a.few_o : a.tile_o) + row * a.dim;
+    float2 v{0.0f, 0.0f};
+    if (lane < cut.parts) v = mls[lane * step];
+    float top = v.y == 0.0f ? -INFINITY : v.x;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (top == -INFINITY) top = 0.0f;
+    const float f = v.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);
+    float sum = v.y * f;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    const uint32_t d = lane * 4;
+    f32x4 acc{0, 0, 0, 0};
+    for (uint32_t p = 0; p < cut.parts; ++p) {
+        const float fp = __shfl(f, int(p));
+        if (fp != 0.0f && d < a.dim) acc += *reinterpret_cast<const f32x4*>(os + p * step * a.dim + d) * fp;
+    }
+    if (d < a.dim) store_out<kBf16>(a, t, h, d, acc, sum, top);
 }
 
 bool aligned(const void* p, uint64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -137,7 +891,7 @@ bool attend_ok(const si_paged_attention_desc& d)
     if (uint64_t(d.tokens) * d.q_heads >= (1ull << 31) || d.seqs >= (1u << 31)) return false;
     if (!d.head_dim || d.head_dim % 8 || d.head_dim > 256 || d.dtype > SI_DTYPE_FP16) return false;
     if (d.page_tokens < 8 || d.page_tokens > 32768 || (d.page_tokens & (d.page_tokens - 1))) return false;
-    if (uint64_t(d.table_pages) * d.page_tokens >= (1ull << 31)) return false;
+    if (uint64_t(d.table_pages) * d.page_tokens > (1ull << 30)) return false;
     if (!d.nslots || d.nslots >= (1ull << 31)) return false;
     const uint64_t row = 2ull * d.kv_heads * d.head_dim;
     if (row >= (1ull << 30) || d.slot_bytes % 16 || d.slot_bytes < row * d.page_tokens) return false;
@@ -148,7 +902,89 @@ bool attend_ok(const si_paged_attention_desc& d)
     return true;
 }
 
-uint64_t attend_workspace(const si_paged_attention_desc&) { return 0; }
+// How a call is launched.  The device's lengths are not known here: the table's
+// width bounds them, and a sequence is cut into fewer parts on the device where
+// it is shorter.
+struct Plan {
+    uint32_t few_rows = 0, few_split = 1, tile_split = 1, tiles = 0;
+    bool few = false, tile = false;
+    uint64_t few_o = 0, few_ml = 0, tile_o = 0, tile_ml = 0, bytes = 0;
+};
+
+// Workgroups a launch should have: two for each of the 256 CUs.
+constexpr uint64_t kTarget = 512;
+
+uint32_t splits(uint64_t groups, uint64_t keys, uint64_t least)
+{
+    uint64_t n = (kTarget + groups - 1) / groups;
+    const uint64_t most = (keys + least - 1) / least;
+    n = n < most ? n : most;
+    n = n < kMaxSplit ? n : kMaxSplit;
+    return uint32_t(n ? n : 1);
+}
+
+Plan attend_plan(const si_paged_attention_desc& d)
+{
+    Plan p;
+    const uint64_t group = d.q_heads / d.kv_heads, keys = uint64_t(d.table_pages) * d.page_tokens;
+    const uint64_t rows = d.tokens * group;
+    // One token each: one kernel.  Any mix of lengths: both, unless no
+    // sequence can be long or the only one is.
+    p.few = group <= 32 && (!d.q_starts || d.seqs > 1 || rows <= 32);
+    if (p.few) p.few_rows = group <= 16 ? 16 : 32;
+    p.tile = d.q_starts ? rows > p.few_rows : !p.few;
+    const uint64_t pairs = uint64_t(d.seqs) * d.kv_heads;
+    if (p.few) p.few_split = splits(pairs, keys, kFewStep);
+    if (p.tile) {
+        p.tiles = uint32_t(d.q_starts ? rows / kTileRows + d.seqs
+                                      : uint64_t(d.seqs) * ((group + kTileRows - 1) / kTileRows));
+        p.tile_split = splits(uint64_t(p.tiles) * d.kv_heads, keys, kTileSplitMin);
+    }
+    const auto take = [&](uint64_t n) {
+        const uint64_t at = p.bytes;
+        p.bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    if (p.few_split > 1) {
+        const uint64_t n = p.few_split * pairs * p.few_rows;
+        p.few_o = take(n * d.head_dim * 4);
+        p.few_ml = take(n * 8);
+    }
+    if (p.tile_split > 1) {
+        const uint64_t n = uint64_t(p.tile_split) * d.tokens * d.q_heads;
+        p.tile_o = take(n * d.head_dim * 4);
+        p.tile_ml = take(n * 8);
+    }
+    return p;
+}
+
+uint64_t attend_workspace(const si_paged_attention_desc& d) { return attend_plan(d).bytes; }
+
+template <bool kBf16, int kDim>
+hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
+{
+    hipError_t e = hipSuccess;
+    if (p.few) {
+        const dim3 grid(a.seqs * a.kv_heads, p.few_split);
+        e = p.few_rows <= 16 ? launch(attend_few_kernel<kBf16, kDim, 1>, grid, dim3(64 * kFewWaves), stream, a)
+                             : launch(attend_few_kernel<kBf16, kDim, 2>, grid, dim3(64 * kFewWaves), stream, a);
+    }
+    if (e == hipSuccess && p.tile)
+        e = launch(attend_tile_kernel<kBf16, kDim>, dim3(p.tiles * a.kv_heads * p.tile_split), dim3(64 * kTileWaves),
+                   stream, a);
+    if (e == hipSuccess && (p.few_split > 1 || p.tile_split > 1))
+        e = launch(attend_join_kernel<kBf16>, dim3((a.tokens * a.q_heads + 3) / 4), dim3(256), stream, a);
+    return e;
+}
+
+template <bool kBf16>
+hipError_t attend_by_dim(hipStream_t stream, const AttendArgs& a, const Plan& p)
+{
+    if (a.dim <= 64) return attend_launch<kBf16, 64>(stream, a, p);
+    if (a.dim <= 96) return attend_launch<kBf16, 96>(stream, a, p);
+    if (a.dim <= 128) return attend_launch<kBf16, 128>(stream, a, p);
+    return attend_launch<kBf16, 256>(stream, a, p);
+}
 
 }  // namespace
 
@@ -165,8 +1001,8 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
 {
     using namespace si;
     if (!d || !attend_ok(*d)) return -1;
-    const uint64_t need = attend_workspace(*d);
-    if (need && (!d->workspace || d->workspace_bytes < need || !aligned(d->workspace, 16))) return -1;
+    const Plan p = attend_plan(*d);
+    if (p.bytes && (!d->workspace || d->workspace_bytes < p.bytes || !aligned(d->workspace, 16))) return -1;
     AttendArgs a{};
     a.q = static_cast<const uint16_t*>(d->q);
     a.q_token = d->q_token_stride;
@@ -192,10 +1028,22 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     a.page_shift = uint32_t(__builtin_ctz(d->page_tokens));
     a.causal = d->causal;
     a.window = d->window;
-    a.scale_log2 = d->scale * 1.44269504088896341f;
-    const dim3 grid(d->tokens * d->q_heads);
-    const hipError_t e = d->dtype == SI_DTYPE_BF16 ? launch(attend_plain_kernel<true>, grid, dim3(64), stream, a)
-                                                   : launch(attend_plain_kernel<false>, grid, dim3(64), stream, a);
+    a.group = d->q_heads / d->kv_heads;
+    a.negate = d->scale < 0.0f;
+    // A scale of 0 (every seen key weighs the same) stays positive, so that a
+    // masked score's -inf times it is still -inf.
+    a.scale_log2 = fmaxf(std::fabs(d->scale) * 1.44269504088896341f, 1e-30f);
+    a.few_rows = p.few_rows;
+    a.few_split = p.few_split;
+    a.tile_split = p.tile_split;
+    a.tiles = p.tiles;
+    uint8_t* const ws = static_cast<uint8_t*>(d->workspace);
+    a.few_o = reinterpret_cast<float*>(ws + p.few_o);
+    a.few_ml = reinterpret_cast<float2*>(ws + p.few_ml);
+    a.tile_o = reinterpret_cast<float*>(ws + p.tile_o);
+    a.tile_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
+    const hipError_t e = d->dtype == SI_DTYPE_BF16 ? attend_by_dim<true>(stream, a, p)
+                                                   : attend_by_dim<false>(stream, a, p);
     return e == hipSuccess ? 0 : -1;
 }
 

@@ -498,7 +498,7 @@ bool pages_ok(const si_pages_desc& d, PageOp op)
     if (!d.tables || !d.refs || !d.tables_out || !d.refs_out || !d.workspace) return false;
     if (d.nslots == 0 || d.nslots >= (1ull << 31) || d.rows == 0 || d.rows >= (1u << 31) || d.table_pages == 0)
         return false;
-    if (!power_of_two(d.page_tokens) || (uint64_t(d.table_pages) << log2_of(d.page_tokens)) >= (1ull << 31)) return false;
+    if (!power_of_two(d.page_tokens) || (uint64_t(d.table_pages) << log2_of(d.page_tokens)) > (1ull << 30)) return false;
     if (op != OP_COMPACT && (!d.kv_lens || !d.kv_lens_out)) return false;
     if (op == OP_RESERVE ? !d.list : op != OP_COMPACT && d.n && !d.list) return false;
     if (d.n >= (1u << 29)) return false;

@@ -142,8 +142,8 @@ def _sequences(tables, kv_lens, q_starts, tokens: int, cache) -> None:
         _index(q_starts, "q_starts", 1, cache.device)
         if q_starts.shape[0] != tables.shape[0] + 1:
             raise ValueError("q_starts needs one entry more than tables has rows")
-    if tables.shape[1] * cache.shape[1] >= 1 << 31:
-        raise ValueError("a table row may span at most 2**31 - 1 tokens")
+    if tables.shape[1] * cache.shape[1] > 1 << 30:
+        raise ValueError("a table row may span at most 2**30 tokens")
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor,
@@ -287,8 +287,8 @@ def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, 
             raise ValueError("kv_lens needs one entry per row of tables")
     if page_tokens < 1 or page_tokens & (page_tokens - 1):
         raise ValueError("page_tokens must be a power of two")
-    if tables.shape[1] * page_tokens >= 1 << 31:
-        raise ValueError("a table row may span at most 2**31 - 1 tokens")
+    if tables.shape[1] * page_tokens > 1 << 30:
+        raise ValueError("a table row may span at most 2**30 tokens")
     if rows_list is not None:
         _index(rows_list, "the row list", list_ndim, device)
     _fail_count(fail_count, device)
