@@ -39,7 +39,7 @@ struct AttendArgs {
     float scale_log2;  // |scale| * log2(e): weights are powers of two
     // Sequences of at most few_rows rows (tokens * group) belong to the few-row
     // kernel, the others to the tile kernel.
-    uint32_t few_rows, few_split, tile_split, tiles;
+    uint32_t few_rows, few_per, tile_per, tile_split, tiles;
     // Parts of split sequences: numerators (dim floats a row) and (m, l).
     float* few_o;
     float2* few_ml;
@@ -67,6 +67,11 @@ constexpr uint32_t kFewKeys = 32;
 constexpr uint32_t kFewWaves = 4;
 constexpr uint32_t kFewStep = kFewKeys * kFewWaves;
 constexpr uint32_t kMaxSplit = 64;
+// Workgroups a launch is cut into, at the longest lengths the tables allow.
+constexpr uint64_t kFewTarget = 4096;
+constexpr uint64_t kTileTarget = 1024;
+// Rows up to which a whole workgroup joins one row's parts.
+constexpr uint32_t kJoinWide = 2048;
 
 __device__ __forceinline__ bool held(int64_t e, int64_t nslots) { return e >= 0 && e < nslots; }
 
@@ -202,22 +207,21 @@ __device__ __forceinline__ Seq seq_of(const AttendArgs& a, uint32_t b)
     return s;
 }
 
-// How a sequence's keys are cut: parts of `per` keys from `lo`.
+// How a sequence's keys are cut: parts of `per` keys from `lo` (a multiple of
+// 64, behind every row's window).  All sequences' parts have one length, which
+// keeps workgroups of ragged batches alike.
 struct Cut {
-    int32_t lo, per;
+    int32_t lo;
     uint32_t parts;
 };
 
-__device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Seq& s, uint32_t split, int32_t step, int32_t least)
+__device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Seq& s, uint32_t per)
 {
     Cut c;
     c.lo = 0;
     if (a.window && s.base - int32_t(a.window) + 1 > 0) c.lo = (s.base - int32_t(a.window) + 1) & ~63;
-    const int32_t span = s.len > c.lo ? s.len - c.lo : 0;
-    int32_t per = (span + int32_t(split) - 1) / int32_t(split);
-    per = per < least ? least : per;
-    c.per = (per + step - 1) / step * step;
-    c.parts = uint32_t((span + c.per - 1) / c.per);
+    const uint32_t span = s.len > c.lo ? uint32_t(s.len - c.lo) : 0;
+    c.parts = (span + per - 1) / per;
     return c;
 }
 
@@ -236,29 +240,40 @@ __device__ void zero_unowned(const AttendArgs& a)
     }
 }
 
-// The slots of `kKeys` consecutive keys from k0 (lane j: key k0 + j % kKeys),
-// and which of them may be read: held pages, lo <= key < hi.
+// The pages of `kKeys` consecutive keys from k0 (lane j: key k0 + j % kKeys):
+// fetch() reads the table, a step before resolve() needs it to say which keys
+// may be read (held pages, lo <= key < hi) and where they are.
 template <int kKeys>
 struct Keys {
-    int64_t slot;   // per lane; with pages of at least kKeys tokens, the tile's
+    int64_t entry;  // of the step fetched
+    int32_t slot;
     uint64_t ok;    // bit j: key k0 + j
 
-    __device__ __forceinline__ void find(const AttendArgs& a, const int64_t* table, int32_t k0, int32_t lo, int32_t hi)
+    __device__ __forceinline__ void fetch(const AttendArgs& a, const int64_t* table, int32_t k0, int32_t lo, int32_t hi)
     {
-        const uint32_t lane = threadIdx.x & 63u;
-        const int32_t k = k0 + int32_t(lane & (kKeys - 1));
-        slot = -1;
-        if (k >= lo && k < hi) slot = table[k >> a.page_shift];
-        ok = __ballot(held(slot, a.nslots));
+        const int32_t k = k0 + int32_t(threadIdx.x & (kKeys - 1));
+        entry = -1;
+        if (k >= lo && k < hi) entry = table[k >> a.page_shift];
+    }
+    __device__ __forceinline__ void resolve(const AttendArgs& a)
+    {
+        const bool h = held(entry, a.nslots);
+        slot = int32_t(entry);
+        ok = __ballot(h);
         if constexpr (kKeys < 64) ok &= (1ull << kKeys) - 1ull;
     }
     // Byte offset of key k0 + j's row of KV head kvh in its cache (j: this
     // lane's choice; every lane calls it).
     __device__ __forceinline__ uint64_t row(const AttendArgs& a, int32_t k0, uint32_t j, uint32_t kvh) const
     {
-        const int64_t s = __shfl(slot, int(j));
+        const uint32_t s = uint32_t(__shfl(slot, int(j)));
         return uint64_t(s) * a.slot_bytes +
                (uint64_t((uint32_t(k0) + j) & ((1u << a.page_shift) - 1u)) * a.kv_heads + kvh) * (a.dim * 2u);
+    }
+    // The one slot of a step that lies in one page (where any key is ok).
+    __device__ __forceinline__ uint32_t page_slot() const
+    {
+        return uint32_t(__builtin_amdgcn_readlane(slot, ok ? __builtin_ctzll(ok) : 0));
     }
 };
 
@@ -320,7 +335,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
     const Seq s = seq_of(a, b);
     const uint32_t rows = s.n_new * a.group;
     if (rows == 0 || rows > 16 * kBlocks) return;
-    const Cut cut = cut_of(a, s, a.few_split, kFewStep, kFewStep);
+    const Cut cut = cut_of(a, s, a.few_per);
     if (part > 0 && part >= cut.parts) return;
     const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
 
@@ -343,8 +358,8 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
     }
     const int32_t p_last = s.base + int32_t(s.n_new) - 1;
     const int32_t hi0 = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
-    const int32_t hi = hi0 < cut.lo + int32_t(part + 1) * cut.per ? hi0 : cut.lo + int32_t(part + 1) * cut.per;
-    const int32_t k_first = cut.lo + int32_t(part) * cut.per;
+    const int32_t k_first = cut.lo + int32_t(part * a.few_per);
+    const int32_t hi = hi0 < k_first + int32_t(a.few_per) ? hi0 : k_first + int32_t(a.few_per);
     // keys below lo are behind every row's window
     const int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
 
@@ -386,14 +401,19 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
     };
     int32_t k0 = k_first + int32_t(wave * kFewKeys);
     if (k0 < hi) {
-        keys.find(a, table, k0, lo, hi);
+        keys.fetch(a, table, k0, lo, hi);
+        keys.resolve(a);
+        keys.fetch(a, table, k0 + int32_t(kFewStep), lo, hi);
         load_k(k0);
         load_v(k0);
     }
     for (; k0 < hi; k0 += int32_t(kFewStep)) {
         const uint64_t ok = keys.ok;
         const int32_t next = k0 + int32_t(kFewStep);
-        if (next < hi) keys.find(a, table, next, lo, hi);
+        if (next < hi) {
+            keys.resolve(a);
+            keys.fetch(a, table, next + int32_t(kFewStep), lo, hi);
+        }
         f32x4 st[kBlocks][2];
 #pragma unroll
         for (int x = 0; x < kBlocks; ++x) {
@@ -591,7 +611,7 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
     const uint32_t rows = s.n_new * a.group;
     const uint32_t r0 = (tile - first_tile) * kTileRows;
     if (rows <= a.few_rows || r0 >= rows) return;
-    const Cut cut = cut_of(a, s, a.tile_split, kTileKeys, kTileSplitMin);
+    const Cut cut = cut_of(a, s, a.tile_per);
     if (part > 0 && part >= cut.parts) return;
     const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
 
@@ -609,11 +629,10 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
             v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
         q[k] = v ^ (a.negate ? 0x80008000u : 0u);
     }
-    const int32_t part_end = cut.lo + int32_t(part + 1) * cut.per;
     int32_t hi = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
-    hi = hi < part_end ? hi : part_end;
+    int32_t k0 = cut.lo + int32_t(part * a.tile_per);
+    hi = hi < k0 + int32_t(a.tile_per) ? hi : k0 + int32_t(a.tile_per);
     const int32_t lo = a.window ? p_first - int32_t(a.window) + 1 : 0;  // behind every row's window below
-    int32_t k0 = cut.lo + int32_t(part) * cut.per;
     if (a.window && lo > k0) k0 = lo & ~int32_t(kTileKeys - 1);
 
     f32x16 o[kOut];
@@ -629,12 +648,8 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
     Keys<kTileKeys> keys;
     const auto load = [&](int32_t kb) {
         if ((1u << a.page_shift) >= kTileKeys) {
-            // one page holds the tile
-            int64_t slot = -1;
-            if (keys.ok) slot = __shfl(keys.slot, __builtin_ctzll(keys.ok));
-            slot = (int64_t(__builtin_amdgcn_readfirstlane(int(slot >> 32))) << 32) |
-                   uint32_t(__builtin_amdgcn_readfirstlane(int(slot)));
-            const uint64_t at = uint64_t(slot) * a.slot_bytes +
+            // one page holds the step's keys
+            const uint64_t at = uint64_t(keys.page_slot()) * a.slot_bytes +
                                 uint64_t(uint32_t(kb) & ((1u << a.page_shift) - 1u)) * kv_row + kvh * a.dim * 2u;
             const uint8_t* kp = a.cache_k + at;
             const uint8_t* vp = a.cache_v + at;
@@ -691,7 +706,9 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
     if (threadIdx.x < 2) odd_flag[threadIdx.x] = 0;
     uint64_t ok = 0;
     if (k0 < hi) {
-        keys.find(a, table, k0, lo, hi);
+        keys.fetch(a, table, k0, lo, hi);
+        keys.resolve(a);
+        keys.fetch(a, table, k0 + int32_t(kTileKeys), lo, hi);
         load(k0);
         ok = keys.ok;
     }
@@ -699,10 +716,9 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
     if (k0 < hi) {
         stage(0);
         flag_odd(0, k0);
-        if (k0 + int32_t(kTileKeys) < hi) {
-            keys.find(a, table, k0 + int32_t(kTileKeys), lo, hi);
-            load(k0 + int32_t(kTileKeys));
-        }
+        keys.resolve(a);
+        keys.fetch(a, table, k0 + 2 * int32_t(kTileKeys), lo, hi);
+        if (k0 + int32_t(kTileKeys) < hi) load(k0 + int32_t(kTileKeys));
     }
     __syncthreads();
     int buf = 0;
@@ -795,10 +811,9 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
             stage(buf);
             flag_odd(buf, next);
             ok = keys.ok;
-            if (next + int32_t(kTileKeys) < hi) {
-                keys.find(a, table, next + int32_t(kTileKeys), lo, hi);
-                load(next + int32_t(kTileKeys));
-            }
+            keys.resolve(a);
+            keys.fetch(a, table, next + 2 * int32_t(kTileKeys), lo, hi);
+            if (next + int32_t(kTileKeys) < hi) load(next + int32_t(kTileKeys));
         }
         __syncthreads();
     }
@@ -833,13 +848,19 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
 
 // ---------------------------------------------------------------- parts joined
 
-// One wave per (token, query head) of a split sequence: the parts' (m, l) one
-// a lane, then the numerators, 4 dims a lane, in the order of the parts.
-template <bool kBf16>
+// kWaves waves per (token, query head) of a split sequence: every wave reads
+// the parts' (m, l), one a lane; the numerators, 4 dims a lane, are summed by
+// groups of lanes that take every kStride-th part each, then over the groups in
+// their order.
+template <bool kBf16, int kDim, int kWaves>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
 {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t th = blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr uint32_t kLanes = kDim / 4 > 64 ? 64 : kDim / 4 > 32 ? 64 : kDim / 4 > 16 ? 32 : 16;  // of one row
+    constexpr uint32_t kStride = 64 * kWaves / kLanes;
+    constexpr uint32_t kRows = 4 / kWaves;
+    __shared__ f32x4 sums[kWaves == 1 ? 1 : 4][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t th = blockIdx.x * kRows + wave / kWaves;
     if (th >= a.tokens * a.q_heads) return;
     const uint32_t t = th / a.q_heads, h = th - t * a.q_heads;
     uint32_t b = t;
@@ -853,8 +874,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
     const Seq s = seq_of(a, b);
     if (t < s.q0 || t >= s.q0 + s.n_new) return;
     const bool few = s.n_new * a.group <= a.few_rows;
-    const Cut cut = few ? cut_of(a, s, a.few_split, kFewStep, kFewStep)
-                        : cut_of(a, s, a.tile_split, kTileKeys, kTileSplitMin);
+    const Cut cut = cut_of(a, s, few ? a.few_per : a.tile_per);
     if (cut.parts <= 1) return;
     const uint32_t kvh = h / a.group;
     const uint64_t row = few ? (uint64_t(b) * a.kv_heads + kvh) * a.few_rows + (t - s.q0) * a.group + (h - kvh * a.group)
@@ -864,21 +884,50 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
     const float* os = (few ? a.few_o : a.tile_o) + row * a.dim;
     float2 v{0.0f, 0.0f};
     if (lane < cut.parts) v = mls[lane * step];
+    const uint32_t which = kWaves == 1 ? lane / kLanes : threadIdx.x / kLanes, d = lane % kLanes * 4;
+    f32x4 acc{0, 0, 0, 0};
+    constexpr uint32_t kAhead = kMaxSplit / kStride < 8 ? kMaxSplit / kStride : 8;
+    f32x4 part[kAhead];
+    const auto load = [&](uint32_t p0) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t p = p0 + which + i * kStride;
+            part[i] = f32x4{0, 0, 0, 0};
+            if (p < cut.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(os + p * step * a.dim + d);
+        }
+    };
+    load(0);
     float top = v.y == 0.0f ? -INFINITY : v.x;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     if (top == -INFINITY) top = 0.0f;
     const float f = v.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);
     float sum = v.y * f;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    const uint32_t d = lane * 4;
-    f32x4 acc{0, 0, 0, 0};
-    for (uint32_t p = 0; p < cut.parts; ++p) {
-        const float fp = __shfl(f, int(p));
-        if (fp != 0.0f && d < a.dim) acc += *reinterpret_cast<const f32x4*>(os + p * step * a.dim + d) * fp;
+    for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+    for (uint32_t p0 = 0;;) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const float fp = __shfl(f, int((p0 + which + i * kStride) & 63u));
+            if (fp != 0.0f) acc += part[i] * fp;
+        }
+        p0 += kAhead * kStride;
+        if (p0 >= cut.parts) break;
+        load(p0);
     }
-    if (d < a.dim) store_out<kBf16>(a, t, h, d, acc, sum, top);
+#pragma unroll
+    for (uint32_t x = kLanes; x < 64; x <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], int(x));
+    if constexpr (kWaves > 1) {
+        sums[wave][lane] = acc;
+        __syncthreads();
+        if (wave != 0) return;
+        acc = sums[0][lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) acc += sums[w][lane];
+    }
+    if (lane < kLanes && d < a.dim) store_out<kBf16>(a, t, h, d, acc, sum, top);
 }
 
 bool aligned(const void* p, uint64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -906,21 +955,22 @@ bool attend_ok(const si_paged_attention_desc& d)
 // width bounds them, and a sequence is cut into fewer parts on the device where
 // it is shorter.
 struct Plan {
-    uint32_t few_rows = 0, few_split = 1, tile_split = 1, tiles = 0;
+    uint32_t few_rows = 0, few_per = 0, few_split = 1, tile_per = 0, tile_split = 1, tiles = 0;
     bool few = false, tile = false;
     uint64_t few_o = 0, few_ml = 0, tile_o = 0, tile_ml = 0, bytes = 0;
 };
 
-// Workgroups a launch should have: two for each of the 256 CUs.
-constexpr uint64_t kTarget = 512;
-
-uint32_t splits(uint64_t groups, uint64_t keys, uint64_t least)
+// Keys of a part, so that `groups` sequences of `keys` keys make about `target`
+// workgroups, and the parts of the longest sequence.
+uint32_t part_keys(uint64_t groups, uint64_t keys, uint64_t least, uint64_t step, uint64_t target, uint32_t* parts)
 {
-    uint64_t n = (kTarget + groups - 1) / groups;
-    const uint64_t most = (keys + least - 1) / least;
-    n = n < most ? n : most;
-    n = n < kMaxSplit ? n : kMaxSplit;
-    return uint32_t(n ? n : 1);
+    uint64_t per = groups * keys / target;
+    const uint64_t fewest = (keys + kMaxSplit - 1) / kMaxSplit;
+    per = per > least ? per : least;
+    per = per > fewest ? per : fewest;
+    per = (per + step - 1) / step * step;
+    *parts = uint32_t((keys + per - 1) / per);
+    return uint32_t(per);
 }
 
 Plan attend_plan(const si_paged_attention_desc& d)
@@ -934,11 +984,11 @@ Plan attend_plan(const si_paged_attention_desc& d)
     if (p.few) p.few_rows = group <= 16 ? 16 : 32;
     p.tile = d.q_starts ? rows > p.few_rows : !p.few;
     const uint64_t pairs = uint64_t(d.seqs) * d.kv_heads;
-    if (p.few) p.few_split = splits(pairs, keys, kFewStep);
+    if (p.few) p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &p.few_split);
     if (p.tile) {
         p.tiles = uint32_t(d.q_starts ? rows / kTileRows + d.seqs
                                       : uint64_t(d.seqs) * ((group + kTileRows - 1) / kTileRows));
-        p.tile_split = splits(uint64_t(p.tiles) * d.kv_heads, keys, kTileSplitMin);
+        p.tile_per = part_keys(uint64_t(p.tiles) * d.kv_heads, keys, kTileSplitMin, kTileKeys, kTileTarget, &p.tile_split);
     }
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
@@ -972,8 +1022,11 @@ hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
     if (e == hipSuccess && p.tile)
         e = launch(attend_tile_kernel<kBf16, kDim>, dim3(p.tiles * a.kv_heads * p.tile_split), dim3(64 * kTileWaves),
                    stream, a);
-    if (e == hipSuccess && (p.few_split > 1 || p.tile_split > 1))
-        e = launch(attend_join_kernel<kBf16>, dim3((a.tokens * a.q_heads + 3) / 4), dim3(256), stream, a);
+    if (e == hipSuccess && (p.few_split > 1 || p.tile_split > 1)) {
+        const uint32_t rows = a.tokens * a.q_heads;
+        e = rows <= kJoinWide ? launch(attend_join_kernel<kBf16, kDim, 4>, dim3(rows), dim3(256), stream, a)
+                              : launch(attend_join_kernel<kBf16, kDim, 1>, dim3((rows + 3) / 4), dim3(256), stream, a);
+    }
     return e;
 }
 
@@ -1034,7 +1087,8 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     // masked score's -inf times it is still -inf.
     a.scale_log2 = fmaxf(std::fabs(d->scale) * 1.44269504088896341f, 1e-30f);
     a.few_rows = p.few_rows;
-    a.few_split = p.few_split;
+    a.few_per = p.few_per;
+    a.tile_per = p.tile_per;
     a.tile_split = p.tile_split;
     a.tiles = p.tiles;
     uint8_t* const ws = static_cast<uint8_t*>(d->workspace);

@@ -19,7 +19,6 @@ may be captured into a graph.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as ct
 import math
 
@@ -36,60 +35,50 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _launch_stream(stream, device):
-    """The torch stream of a call (a torch stream, a raw handle, or None for
-    the device's current stream)."""
+def _stream_of(stream, device: int):
+    """(raw handle, the torch stream if it is not the device's current one) of
+    a call's stream: a torch stream, a raw handle, or None for the current."""
+    current = torch._C._cuda_getCurrentRawStream(device)
     if stream is None:
-        return torch.cuda.current_stream(device)
+        return current, None
     if isinstance(stream, torch.cuda.Stream):
-        return stream
-    raw = stream.value if isinstance(stream, ct.c_void_p) else int(stream)
-    return torch.cuda.ExternalStream(raw or 0, device=device)
+        raw = stream.cuda_stream
+    else:
+        raw = stream.value or 0 if isinstance(stream, ct.c_void_p) else int(stream)
+        stream = None
+    if raw == current:
+        return raw, None
+    return raw, torch.cuda.ExternalStream(raw, device=torch.device("cuda", device)) if stream is None else stream
 
 
-@contextlib.contextmanager
-def _on(stream, device, tensors):
-    """What the call allocates belongs to its stream, and the caller's tensors
-    are not reused before that stream is done with them."""
-    current = torch.cuda.current_stream(device)
-    s = _launch_stream(stream, device)
-    if s == current:
-        yield ct.c_void_p(s.cuda_stream)
-        return
-    with torch.cuda.stream(s):
-        yield ct.c_void_p(s.cuda_stream)
-    for t in tensors:
-        if t is not None:
-            t.record_stream(s)
+def _kept_by(other, tensors) -> None:
+    """Tensors used on a stream other than the one they were made on are not
+    reused before that stream is done with them."""
+    if other is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(other)
 
 
-def _index(t, name: str, ndim: int, device, dtype=torch.int64) -> None:
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise ValueError(f"{name} must be a tensor on {device}")
+def _empty(other, shape, dtype, device: int):
+    """A tensor that belongs to the call's stream."""
+    where = torch.device("cuda", device)
+    if other is None:
+        return torch.empty(shape, dtype=dtype, device=where)
+    with torch.cuda.stream(other):
+        return torch.empty(shape, dtype=dtype, device=where)
+
+
+def _index(t, name: str, ndim: int, device: int, dtype=torch.int64) -> None:
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        raise ValueError(f"{name} must be a tensor on cuda:{device}")
     if t.dtype != dtype or t.ndim != ndim or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {ndim}-d {dtype} tensor")
 
 
-def _fail_count(t, device) -> None:
-    if t is not None and (t.device != device or t.dtype != torch.int32 or t.numel() != 1):
-        raise ValueError(f"fail_count must be one int32 on {device}")
-
-
-def _paged_cache(t, name: str) -> None:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a device tensor")
-    if t.ndim != 4 or t.dtype not in _DTYPES:
-        raise ValueError(f"{name} must be [slots, page tokens, kv heads, head dim] in bfloat16 or float16")
-    slots, ps, heads, dim = t.shape
-    if 0 in t.shape:
-        raise ValueError(f"{name} is empty")
-    if t.stride()[1:] != (heads * dim, dim, 1) or (slots > 1 and t.stride(0) < ps * heads * dim):
-        raise ValueError(f"a page of {name} must be contiguous")
-    if ps & (ps - 1) or not 8 <= ps <= 32768:
-        raise ValueError(f"{name} has pages of {ps} tokens: must be a power of two from 8 to 32768")
-    if dim % 8:
-        raise ValueError(f"{name} has head dim {dim}: must be a multiple of 8")
-    _aligned(t, name)
+def _fail_count(t, device: int) -> None:
+    if t is not None and (t.get_device() != device or t.dtype != torch.int32 or t.numel() != 1):
+        raise ValueError(f"fail_count must be one int32 on cuda:{device}")
 
 
 def _aligned(t, name: str) -> None:
@@ -97,53 +86,80 @@ def _aligned(t, name: str) -> None:
         raise ValueError(f"{name} must start on a 16-byte boundary")
 
 
-def _slot_stride(t) -> int:
-    """Elements from one page to the next (a cache of one slot: a page)."""
-    return t.stride(0) if t.shape[0] > 1 else t[0].numel()
+def _paged_cache(t, name: str):
+    """(device, dtype, slots, page tokens, heads, dim, elements from one page to the next)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    dtype = t.dtype
+    if t.ndim != 4 or dtype not in _DTYPES:
+        raise ValueError(f"{name} must be [slots, page tokens, kv heads, head dim] in bfloat16 or float16")
+    slots, ps, heads, dim = t.shape
+    page = ps * heads * dim
+    if slots * page == 0:
+        raise ValueError(f"{name} is empty")
+    stride = t.stride()
+    step = stride[0] if slots > 1 else page  # the stride of a single page is never used
+    if stride[1:] != (heads * dim, dim, 1) or step < page:
+        raise ValueError(f"a page of {name} must be contiguous")
+    if ps & (ps - 1) or not 8 <= ps <= 32768:
+        raise ValueError(f"{name} has pages of {ps} tokens: must be a power of two from 8 to 32768")
+    if dim % 8:
+        raise ValueError(f"{name} has head dim {dim}: must be a multiple of 8")
+    if step % 8:
+        raise ValueError(f"{name}'s slot stride must be a multiple of 16 bytes")
+    _aligned(t, name)
+    return t.get_device(), dtype, slots, ps, heads, dim, step
 
 
-def _cache_pair(cache_k, cache_v) -> None:
-    _paged_cache(cache_k, "cache_k")
-    _paged_cache(cache_v, "cache_v")
-    if (cache_k.shape != cache_v.shape or cache_k.dtype != cache_v.dtype or cache_k.device != cache_v.device
-            or _slot_stride(cache_k) != _slot_stride(cache_v)):
+def _cache_pair(cache_k, cache_v):
+    geometry = _paged_cache(cache_k, "cache_k")
+    if geometry != _paged_cache(cache_v, "cache_v"):
         raise ValueError("cache_k and cache_v must have one shape, dtype, slot stride and device")
-    if _slot_stride(cache_k) % 8:
-        raise ValueError("the caches' slot stride must be a multiple of 16 bytes")
+    return geometry
 
 
-def _rows(t, name: str, heads: int, dim: int, cache) -> tuple[int, int]:
-    """(token stride, head stride) of [tokens, heads, dim] rows."""
-    if not isinstance(t, torch.Tensor) or t.device != cache.device or t.dtype != cache.dtype:
-        raise ValueError(f"{name} must be a {cache.dtype} tensor on {cache.device}")
+def _rows(t, name: str, heads: int, dim: int, dtype, device: int) -> tuple[int, int, int]:
+    """(tokens, token stride, head stride) of [tokens, heads, dim] rows."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor on cuda:{device}")
     if t.ndim != 3 or t.shape[1:] != (heads, dim):
         raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(t.shape)}")
+    token, head, one = t.stride()
+    tokens = t.shape[0]
     # the stride of a single token or head is never used
-    token = t.stride(0) if t.shape[0] > 1 else heads * dim
-    head = t.stride(1) if heads > 1 else dim
-    if (dim > 1 and t.stride(2) != 1) or token % 8 or head % 8:
+    if tokens <= 1:
+        token = heads * dim
+    if heads == 1:
+        head = dim
+    if (dim > 1 and one != 1) or token % 8 or head % 8:
         raise ValueError(f"{name} needs a contiguous head dim and token / head strides that are multiples of 8")
     _aligned(t, name)
-    return token, head
+    return tokens, token, head
 
 
-def _sequences(tables, kv_lens, q_starts, tokens: int, cache) -> None:
-    if not isinstance(tables, torch.Tensor) or tables.device != cache.device:
-        raise ValueError(f"tables must be a tensor on {cache.device}")
-    if tables.dtype != torch.int64 or tables.ndim != 2 or (tables.shape[1] > 1 and tables.stride(1) != 1):
+def _sequences(tables, kv_lens, q_starts, tokens: int, ps: int, device: int):
+    """(sequences, pages of a row, row stride) of the tables."""
+    if not isinstance(tables, torch.Tensor) or tables.get_device() != device:
+        raise ValueError(f"tables must be a tensor on cuda:{device}")
+    if tables.dtype != torch.int64 or tables.ndim != 2:
         raise ValueError("tables must be a 2-d torch.int64 tensor with contiguous rows")
-    _index(kv_lens, "kv_lens", 1, cache.device)
-    if kv_lens.shape[0] != tables.shape[0]:
+    seqs, pages = tables.shape
+    row, one = tables.stride()
+    if pages > 1 and one != 1:
+        raise ValueError("tables must be a 2-d torch.int64 tensor with contiguous rows")
+    _index(kv_lens, "kv_lens", 1, device)
+    if kv_lens.shape[0] != seqs:
         raise ValueError("kv_lens needs one entry per row of tables")
     if q_starts is None:
-        if tokens != tables.shape[0]:
+        if tokens != seqs:
             raise ValueError("without q_starts there is one row per sequence")
     else:
-        _index(q_starts, "q_starts", 1, cache.device)
-        if q_starts.shape[0] != tables.shape[0] + 1:
+        _index(q_starts, "q_starts", 1, device)
+        if q_starts.shape[0] != seqs + 1:
             raise ValueError("q_starts needs one entry more than tables has rows")
-    if tables.shape[1] * cache.shape[1] > 1 << 30:
+    if pages * ps > 1 << 30:
         raise ValueError("a table row may span at most 2**30 tokens")
+    return seqs, pages, row
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor,
@@ -153,26 +169,26 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_
     head stride in multiples of 8) into their pages.  Token i of a sequence with n new
     ones goes to position kv_len - n + i; a token whose position is
     negative, past the table or on no page is dropped and counted."""
-    _cache_pair(cache_k, cache_v)
-    slots, ps, heads, dim = cache_k.shape
-    kt, kh = _rows(k, "k", heads, dim, cache_k)
-    vt, vh = _rows(v, "v", heads, dim, cache_k)
-    if k.shape[0] != v.shape[0]:
+    device, dtype, slots, ps, heads, dim, step = _cache_pair(cache_k, cache_v)
+    tokens, kt, kh = _rows(k, "k", heads, dim, dtype, device)
+    v_tokens, vt, vh = _rows(v, "v", heads, dim, dtype, device)
+    if tokens != v_tokens:
         raise ValueError("k and v must have the same tokens")
-    _sequences(tables, kv_lens, q_starts, k.shape[0], cache_k)
-    _fail_count(fail_count, cache_k.device)
-    if k.shape[0] == 0 or tables.shape[0] == 0:
+    seqs, pages, row = _sequences(tables, kv_lens, q_starts, tokens, ps, device)
+    _fail_count(fail_count, device)
+    if tokens == 0 or seqs == 0:
         return
-    if tables.shape[1] == 0:
+    if pages == 0:
         raise ValueError("tables has no pages")
-    with _on(stream, cache_k.device, (k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count)) as s:
-        d = _lib.SiPagedAppendDesc(
-            k=k.data_ptr(), v=v.data_ptr(), k_token_stride=kt, k_head_stride=kh, v_token_stride=vt, v_head_stride=vh,
-            cache_k=cache_k.data_ptr(), cache_v=cache_v.data_ptr(), slot_bytes=2 * _slot_stride(cache_k), nslots=slots,
-            tables=tables.data_ptr(), table_stride=tables.stride(0), kv_lens=kv_lens.data_ptr(), q_starts=_ptr(q_starts),
-            table_pages=tables.shape[1], tokens=k.shape[0], seqs=tables.shape[0], kv_heads=heads, head_dim=dim,
-            page_tokens=ps, fail_count=_ptr(fail_count))
-        _check(lib().secure_infer_gpu_paged_append(s, ct.byref(d)), "paged_append")
+    raw, other = _stream_of(stream, device)
+    d = _lib.SiPagedAppendDesc(
+        k=k.data_ptr(), v=v.data_ptr(), k_token_stride=kt, k_head_stride=kh, v_token_stride=vt, v_head_stride=vh,
+        cache_k=cache_k.data_ptr(), cache_v=cache_v.data_ptr(), slot_bytes=2 * step, nslots=slots,
+        tables=tables.data_ptr(), table_stride=row, kv_lens=kv_lens.data_ptr(), q_starts=_ptr(q_starts),
+        table_pages=pages, tokens=tokens, seqs=seqs, kv_heads=heads, head_dim=dim, page_tokens=ps,
+        fail_count=_ptr(fail_count))
+    _check(lib().secure_infer_gpu_paged_append(raw, ct.byref(d)), "paged_append")
+    _kept_by(other, (k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count))
 
 
 def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, tables: torch.Tensor,
@@ -189,27 +205,28 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     float32, if given, receives the log-sum-exp of the scaled scores (-inf
     without a key), with which two parts' outputs can be joined.  ``workspace`` (uint8, at least
     ``paged_attention_workspace`` bytes) saves an allocation per call.  Returns ``out``."""
-    d, keep = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse)
+    d, device = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse)
     if d is None:
-        return keep
-    device = q.device
-    with _on(stream, device, (q, cache_k, cache_v, tables, kv_lens, q_starts, out, lse, workspace)) as s:
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-            d.out, d.out_token_stride, d.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
-        need = int(lib().secure_infer_gpu_paged_attention_workspace(ct.byref(d)))
-        if need == _REFUSED:
-            raise ValueError("paged_attention refuses these arguments")
-        if need:
-            if workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            elif workspace.device != device or not workspace.is_contiguous():
-                raise ValueError(f"workspace must be contiguous on {device}")
-            elif workspace.numel() * workspace.element_size() < need:
-                raise ValueError(f"workspace needs {need} bytes")
-            _aligned(workspace, "workspace")
-            d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        _check(lib().secure_infer_gpu_paged_attention(s, ct.byref(d)), "paged_attention")
+        return torch.empty_like(q) if out is None else out
+    raw, other = _stream_of(stream, device)
+    if out is None:
+        out = _empty(other, q.shape, q.dtype, device)
+        d.out, d.out_token_stride, d.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
+    L = lib()
+    need = L.secure_infer_gpu_paged_attention_workspace(ct.byref(d))
+    if need == _REFUSED:
+        raise ValueError("paged_attention refuses these arguments")
+    if need:
+        if workspace is None:
+            workspace = _empty(other, (need,), torch.uint8, device)
+        elif workspace.get_device() != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be contiguous on cuda:{device}")
+        elif workspace.numel() * workspace.element_size() < need:
+            raise ValueError(f"workspace needs {need} bytes")
+        _aligned(workspace, "workspace")
+        d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _check(L.secure_infer_gpu_paged_attention(raw, ct.byref(d)), "paged_attention")
+    _kept_by(other, (q, cache_k, cache_v, tables, kv_lens, q_starts, out, lse, workspace))
     return out
 
 
@@ -221,19 +238,18 @@ def paged_attention_workspace(q, cache_k, cache_v, tables, kv_lens, q_starts=Non
 
 
 def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse):
-    """The checked descriptor (without an output if ``out`` is None), or
-    (None, the answer) where there is nothing to compute."""
-    _cache_pair(cache_k, cache_v)
-    slots, ps, heads, dim = cache_k.shape
+    """(the checked descriptor, without an output if ``out`` is None; the
+    device), or (None, the device) where there is nothing to compute."""
+    device, dtype, slots, ps, heads, dim, step = _cache_pair(cache_k, cache_v)
     if dim > 256:
         raise ValueError(f"head dim {dim} is over 256")
     if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.shape[1] == 0 or q.shape[1] % heads:
         raise ValueError(f"q must be [tokens, query heads, {dim}] with a multiple of {heads} query heads")
-    tokens, q_heads = q.shape[:2]
-    qt, qh = _rows(q, "q", q_heads, dim, cache_k)
+    q_heads = q.shape[1]
+    tokens, qt, qh = _rows(q, "q", q_heads, dim, dtype, device)
     if tokens * q_heads >= 1 << 31:
         raise ValueError("q has too many rows")
-    _sequences(tables, kv_lens, q_starts, tokens, cache_k)
+    seqs, pages, row = _sequences(tables, kv_lens, q_starts, tokens, ps, device)
     scale = dim ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
@@ -243,88 +259,102 @@ def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causa
     if out is not None:
         if out.shape != q.shape:
             raise ValueError("out must have q's shape")
-        ot, oh = _rows(out, "out", q_heads, dim, cache_k)
+        _, ot, oh = _rows(out, "out", q_heads, dim, dtype, device)
         if min(ot, oh) < dim or max(ot, oh) < min(ot, oh) * (q_heads if ot > oh else tokens):
             raise ValueError("out's rows must not overlap")
-    if lse is not None and (lse.device != q.device or lse.dtype != torch.float32 or lse.shape != q.shape[:2]
+    if lse is not None and (lse.get_device() != device or lse.dtype != torch.float32 or lse.shape != q.shape[:2]
                             or not lse.is_contiguous()):
-        raise ValueError(f"lse must be a contiguous float32 [tokens, query heads] tensor on {q.device}")
+        raise ValueError(f"lse must be a contiguous float32 [tokens, query heads] tensor on cuda:{device}")
     if tokens == 0:
-        return None, torch.empty_like(q) if out is None else out
-    if tables.shape[0] == 0 or tables.shape[1] == 0:
+        return None, device
+    if seqs == 0 or pages == 0:
         raise ValueError("tables has no pages")
     return _lib.SiPagedAttentionDesc(
         q=q.data_ptr(), q_token_stride=qt, q_head_stride=qh, out=q.data_ptr() if out is None else out.data_ptr(),
         out_token_stride=ot, out_head_stride=oh, lse=_ptr(lse), cache_k=cache_k.data_ptr(),
-        cache_v=cache_v.data_ptr(), slot_bytes=2 * _slot_stride(cache_k), nslots=slots, tables=tables.data_ptr(),
-        table_stride=tables.stride(0), kv_lens=kv_lens.data_ptr(), q_starts=_ptr(q_starts),
-        table_pages=tables.shape[1], tokens=tokens, seqs=tables.shape[0], q_heads=q_heads, kv_heads=heads,
-        head_dim=dim, page_tokens=ps, dtype=_DTYPES[q.dtype], causal=int(bool(causal)), window=int(window),
-        scale=scale), None
+        cache_v=cache_v.data_ptr(), slot_bytes=2 * step, nslots=slots, tables=tables.data_ptr(), table_stride=row,
+        kv_lens=kv_lens.data_ptr(), q_starts=_ptr(q_starts), table_pages=pages, tokens=tokens, seqs=seqs,
+        q_heads=q_heads, kv_heads=heads, head_dim=dim, page_tokens=ps, dtype=_DTYPES[dtype],
+        causal=1 if causal else 0, window=int(window), scale=scale), device
 
 
 # ------------------------------------------------------------------ pages
 
+def _same_layout(caches):
+    """(device, dtype, slots, page tokens, heads, dim, slot stride) of caches
+    that share it, and their addresses.  (A set per property: a check of each tensor in
+    Python costs 1 us a tensor, which for 160 tensors is many times the copies.)"""
+    if not caches:
+        raise ValueError("no caches given")
+    geometry = _paged_cache(caches[0], "a cache")
+    T = torch.Tensor
+    if len(caches) > 1:
+        if not all([isinstance(c, T) for c in caches]):
+            raise ValueError("a cache must be a device tensor")
+        if (len(set(map(T.size, caches))) > 1 or len({c.dtype for c in caches}) > 1
+                or len(set(map(T.get_device, caches))) > 1
+                or (len(set(map(T.stride, caches))) > 1 and any(_paged_cache(c, "a cache") != geometry for c in caches))):
+            raise ValueError("the caches must have one shape, dtype, slot stride and device")
+    addresses = list(map(T.data_ptr, caches))
+    if any([p & 15 for p in addresses]):
+        raise ValueError("a cache must start on a 16-byte boundary")
+    return geometry, addresses
+
+
 def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, list_ndim, scrub, fail_count, out,
                 stream):
-    device = refs.device if isinstance(refs, torch.Tensor) else None
-    if device is None or not refs.is_cuda:
+    if not isinstance(refs, torch.Tensor) or not refs.is_cuda:
         raise ValueError("refs must be a device tensor")
-    caches = list(caches)
-    for c in caches:
-        _paged_cache(c, "a cache")
-        if c.device != device or c.shape != caches[0].shape or _slot_stride(c) != _slot_stride(caches[0]):
-            raise ValueError("the caches must have one shape and slot stride, on refs' device")
-        if c.shape[0] != refs.shape[0]:
-            raise ValueError("refs needs one entry per slot")
-    if caches and _slot_stride(caches[0]) % 8:
-        raise ValueError("the caches' slot stride must be a multiple of 16 bytes")
+    device = refs.get_device()
     _index(refs, "refs", 1, device, torch.int32)
+    nslots = refs.shape[0]
+    addresses, slot_bytes, page_bytes = (), 0, 0
+    if caches is not None:
+        caches = list(caches)
+        (where, _, slots, page_tokens, heads, dim, step), addresses = _same_layout(caches)
+        if where != device:
+            raise ValueError("the caches must be on refs' device")
+        if slots != nslots:
+            raise ValueError("refs needs one entry per slot")
+        slot_bytes, page_bytes = 2 * step, 2 * page_tokens * heads * dim
     _index(tables, "tables", 2, device)
+    rows, pages = tables.shape
     if kv_lens is not None:
         _index(kv_lens, "kv_lens", 1, device)
-        if kv_lens.shape[0] != tables.shape[0]:
+        if kv_lens.shape[0] != rows:
             raise ValueError("kv_lens needs one entry per row of tables")
     if page_tokens < 1 or page_tokens & (page_tokens - 1):
         raise ValueError("page_tokens must be a power of two")
-    if tables.shape[1] * page_tokens > 1 << 30:
+    if pages * page_tokens > 1 << 30:
         raise ValueError("a table row may span at most 2**30 tokens")
     if rows_list is not None:
         _index(rows_list, "the row list", list_ndim, device)
     _fail_count(fail_count, device)
+    if rows * pages * nslots == 0:
+        raise ValueError("tables and refs must not be empty")
     state = (tables, refs) if kv_lens is None else (tables, kv_lens, refs)
-    if out is not None:
+    raw, other = _stream_of(stream, device)
+    if out is None:
+        out = tuple([_empty(other, t.shape, t.dtype, device) for t in state])
+    else:
         if len(out) != len(state):
             raise ValueError(f"out needs {len(state)} tensors")
         for o, i in zip(out, state):
-            if o.shape != i.shape or o.dtype != i.dtype or o.device != device or not o.is_contiguous():
+            if o.shape != i.shape or o.dtype != i.dtype or o.get_device() != device or not o.is_contiguous():
                 raise ValueError("out must match the inputs in shape, dtype and device, and be contiguous")
-    if 0 in tables.shape or refs.shape[0] == 0:
-        raise ValueError("tables and refs must not be empty")
-    with _on(stream, device, (*caches, *state, rows_list, fail_count, *(out or ()))) as s:
-        if out is None:
-            out = tuple(torch.empty_like(t) for t in state)
-        page = caches[0][0].numel() * 2 if caches else 0
-        d = _lib.SiPagesDesc(
-            caches=(ct.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches]), ncaches=len(caches),
-            page_tokens=page_tokens, slot_bytes=2 * _slot_stride(caches[0]) if caches else 0, page_bytes=page,
-            nslots=refs.shape[0], tables=tables.data_ptr(), kv_lens=_ptr(kv_lens), refs=refs.data_ptr(),
-            tables_out=out[0].data_ptr(), kv_lens_out=None if kv_lens is None else out[1].data_ptr(),
-            refs_out=out[-1].data_ptr(), rows=tables.shape[0], table_pages=tables.shape[1], list=_ptr(rows_list),
-            n=0 if rows_list is None else rows_list.shape[0], scrub=int(bool(scrub)), fail_count=_ptr(fail_count))
-        need = int(lib().secure_infer_gpu_pages_workspace(ct.byref(d)))
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        d.workspace, d.workspace_bytes = workspace.data_ptr(), need
-        _check(getattr(lib(), fn_name)(s, ct.byref(d)), fn_name.removeprefix("secure_infer_gpu_"))
+    d = _lib.SiPagesDesc(
+        caches=(ct.c_void_p * max(1, len(addresses)))(*addresses), ncaches=len(addresses), page_tokens=page_tokens,
+        slot_bytes=slot_bytes, page_bytes=page_bytes, nslots=nslots, tables=tables.data_ptr(), kv_lens=_ptr(kv_lens),
+        refs=refs.data_ptr(), tables_out=out[0].data_ptr(), kv_lens_out=None if kv_lens is None else out[1].data_ptr(),
+        refs_out=out[-1].data_ptr(), rows=rows, table_pages=pages, list=_ptr(rows_list),
+        n=0 if rows_list is None else rows_list.shape[0], scrub=1 if scrub else 0, fail_count=_ptr(fail_count))
+    L = lib()
+    workspace = _empty(other, (L.secure_infer_gpu_pages_workspace(ct.byref(d)),), torch.uint8, device)
+    d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _check(getattr(L, fn_name)(raw, ct.byref(d)), fn_name.removeprefix("secure_infer_gpu_"))
+    if other is not None:
+        _kept_by(other, (*(caches or ()), *state, rows_list, fail_count, *out))
     return tuple(out)
-
-
-def _page_tokens(caches) -> int:
-    caches = list(caches)
-    if not caches:
-        raise ValueError("no caches given")
-    _paged_cache(caches[0], "a cache")
-    return caches[0].shape[1]
 
 
 def fork_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, pairs: torch.Tensor,
@@ -338,7 +368,7 @@ def fork_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
     inputs).  ``refs`` [slots] int32 counts the rows that hold a slot."""
     if not isinstance(pairs, torch.Tensor) or pairs.ndim != 2 or pairs.shape[1] != 2:
         raise ValueError("pairs must be [n, 2]")
-    return _pages_call("secure_infer_gpu_pages_fork", caches, tables, kv_lens, refs, _page_tokens(caches), pairs, 2,
+    return _pages_call("secure_infer_gpu_pages_fork", caches, tables, kv_lens, refs, 0, pairs, 2,
                        False, fail_count, out, stream)
 
 
@@ -348,7 +378,7 @@ def free_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
     empty; with ``scrub`` a page nobody holds any more is zeroed in every tensor
     of ``caches``, so a freed slot keeps no plaintext.  Returns (tables, kv_lens,
     refs) as fork_pages does."""
-    return _pages_call("secure_infer_gpu_pages_free", caches, tables, kv_lens, refs, _page_tokens(caches), rows, 1,
+    return _pages_call("secure_infer_gpu_pages_free", caches, tables, kv_lens, refs, 0, rows, 1,
                        scrub, fail_count, out, stream)
 
 
@@ -356,7 +386,7 @@ def compact_pages(caches, tables: torch.Tensor, refs: torch.Tensor, scrub: bool 
     """With L slots held, the held slots >= L move to the free slots < L (both
     ascending) in every tensor of ``caches``; ``scrub`` zeroes the pages moved
     from.  Returns (tables, refs), new or written to ``out``."""
-    return _pages_call("secure_infer_gpu_pages_compact", caches, tables, None, refs, _page_tokens(caches), None, 0,
+    return _pages_call("secure_infer_gpu_pages_compact", caches, tables, None, refs, 0, None, 0,
                        scrub, None, out, stream)
 
 
@@ -371,5 +401,5 @@ def reserve_pages(tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tenso
     if not isinstance(counts, torch.Tensor) or not isinstance(tables, torch.Tensor) \
             or counts.shape != tables.shape[:1]:
         raise ValueError("counts needs one entry per row of tables")
-    return _pages_call("secure_infer_gpu_pages_reserve", (), tables, kv_lens, refs, int(page_tokens), counts, 1,
+    return _pages_call("secure_infer_gpu_pages_reserve", None, tables, kv_lens, refs, int(page_tokens), counts, 1,
                        False, fail_count, out, stream)
