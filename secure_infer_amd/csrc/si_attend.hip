@@ -653,6 +653,15 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
                                 uint64_t(uint32_t(kb) & ((1u << a.page_shift) - 1u)) * kv_row + kvh * a.dim * 2u;
             const uint8_t* kp = a.cache_k + at;
             const uint8_t* vp = a.cache_v + at;
+            if (keys.ok == ~0ull && a.dim == kChunks * 8u) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const uint32_t j = row0 + i * kRowStep;
+                    kr[i] = *reinterpret_cast<const u32x4*>(kp + j * kv_row + chunk * 16);
+                    vr[i] = *reinterpret_cast<const u32x4*>(vp + j * kv_row + chunk * 16);
+                }
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const uint32_t j = row0 + i * kRowStep;
@@ -679,7 +688,7 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
     // clock: rows of different r % 8), V two chunks of 4 rows.
     const auto k_at = [](uint32_t row, uint32_t c) { return row * kPitch + ((c ^ (row & (kChunks - 1))) * 8); };
     const auto v_at = [](uint32_t row, uint32_t c) {
-        return row * kPitch + ((c ^ ((row << 1) & (kChunks - 1) & 14)) * 8);
+        return row * kPitch + ((c ^ ((row << 2) & (kChunks - 1) & 12)) * 8);
     };
     const auto stage = [&](int buf) {
 #pragma unroll
@@ -724,17 +733,22 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
     int buf = 0;
     for (; k0 < hi; k0 += int32_t(kTileKeys)) {
         const int32_t next = k0 + int32_t(kTileKeys);
+        // The matrix instructions go first where two workgroups' waves meet on
+        // a SIMD, so that one's weights are formed during the other's products.
+        __builtin_amdgcn_s_setprio(1);
         f32x16 st[2];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
             for (int e = 0; e < 16; ++e) st[y][e] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
                 const u32x4 kf = *reinterpret_cast<const u32x4*>(&ks[buf][k_at(32 * y + col, 2 * k + half)]);
                 st[y] = mfma32<kBf16>(kf, q[k], st[y]);
             }
-        }
+        __builtin_amdgcn_s_setprio(0);
         const bool partial = is_partial(k0);
         uint64_t seen = ok;
         if (partial) seen = seen_bits(a, ok, k0, pos);
@@ -752,23 +766,27 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, st[y][e]);
         top = across<false>(top, fmax2);
-        const float mn = fmaxf(m, top);
-        const float safe = mn == -INFINITY ? 0.0f : mn;
-        if (__ballot(mn != m)) {
-            const float keep = __builtin_amdgcn_exp2f((m - safe) * a.scale_log2);
+        // m follows the maximum only where a weight would pass 2^8 (float sums
+        // and rounded weights keep their relative error), so that the
+        // numerators are seldom rescaled.
+        if (__ballot((top - m) * a.scale_log2 > 8.0f)) {
+            const float mn = fmaxf(m, top);
+            const float keep = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
             l *= keep;
 #pragma unroll
             for (int i = 0; i < kOut; ++i) o[i] *= keep;
+            m = mn;
         }
-        m = mn;
-        const float shift = safe * a.scale_log2;
+        const float shift = m == -INFINITY ? 0.0f : m * a.scale_log2;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int y = 0; y < 2; ++y)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 st[y][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][e], a.scale_log2, -shift));
-                l += st[y][e];
+                sum[e % 4] += st[y][e];
             }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (partial && odd_flag[buf]) {
             // Rows that see a key with an infinity or NaN take it itself (a
             // weight is positive); then it is cleared for the product.
@@ -791,6 +809,7 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
             if (threadIdx.x == 0) odd_flag[buf] = 0;
             __syncthreads();
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
             f32x8 w;
@@ -806,6 +825,7 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
                 o[i] = mfma32<kBf16>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pw, o[i]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         buf ^= 1;
         if (next < hi) {
             stage(buf);
