@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <cmath>
+#include <numeric>
 
 #include "secure_infer_gpu.h"
 #include "si_launch.h"
@@ -61,7 +62,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr uint32_t kTileKeys = 64;
 constexpr uint32_t kTileWaves = 4;
 constexpr uint32_t kTileRows = 32 * kTileWaves;
-constexpr uint32_t kTileSplitMin = 512;
+constexpr uint32_t kTileSplitMin = 256;
 // The few-row kernel's keys per wave and step; a workgroup's step.
 constexpr uint32_t kFewKeys = 32;
 constexpr uint32_t kFewWaves = 4;
@@ -69,9 +70,10 @@ constexpr uint32_t kFewStep = kFewKeys * kFewWaves;
 constexpr uint32_t kMaxSplit = 64;
 // Workgroups a launch is cut into, at the longest lengths the tables allow.
 constexpr uint64_t kFewTarget = 4096;
-constexpr uint64_t kTileTarget = 1024;
+constexpr uint64_t kTileTarget = 1280;
+constexpr uint64_t kTileFew = 384;
 // Rows up to which a whole workgroup joins one row's parts.
-constexpr uint32_t kJoinWide = 2048;
+constexpr uint32_t kJoinRows = 2048;
 
 __device__ __forceinline__ bool held(int64_t e, int64_t nslots) { return e >= 0 && e < nslots; }
 
@@ -121,12 +123,45 @@ __device__ __forceinline__ u32x4 pack8(f32x8 x)
     else return __builtin_bit_cast(u32x4, __builtin_convertvector(x, f16x8));
 }
 
+// LDS is addressed by byte offsets where instructions without a pointer form
+// read or fill it.
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ u32x4 read_lds(uint32_t at)
+{
+    return *reinterpret_cast<__attribute__((address_space(3))) const u32x4*>(at);
+}
+
+// 16 bytes a lane from memory to LDS (a wave's 1 KiB at `to`), without passing
+// through registers.  Written as instructions because the compiler, which cannot tell the
+// two buffers apart, would wait for them at the next read of LDS; a wait_loads() and a
+// barrier stand before their data is read.
+__device__ __forceinline__ void to_lds(const uint8_t* p, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory");
+}
+__device__ __forceinline__ void to_lds(const uint8_t* base, uint32_t offset, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
+                 : "memory");
+}
+
+// Everything this wave has asked memory for has arrived.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// A pointer that is the same in every lane, as one.
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p)
+{
+    const uint64_t x = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const uint8_t*>(uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x >> 32)))) << 32 |
+                                            uint32_t(__builtin_amdgcn_readfirstlane(int(x))));
+}
+
 // Four rows of a 16-bit matrix in LDS, transposed: each 16 lanes read 4 rows x
 // 16 columns (lane i: row i / 4, columns 4 (i % 4) ..) and lane i receives column
 // i of the 4 rows.
-__device__ __forceinline__ u32x2 read_tr(const uint16_t* p)
+__device__ __forceinline__ u32x2 read_tr(uint32_t at)
 {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at)));
 }
 
 // max / sum over lanes l, l ^ 32 and (kQuarters) l ^ 16: the lanes that hold
@@ -148,31 +183,13 @@ __device__ __forceinline__ float across(float x, F f)
 __device__ __forceinline__ float fmax2(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float fadd2(float a, float b) { return a + b; }
 
+// Bits 15 and 31 of the result mark infinities and NaN among eight values: an
+// exponent of ones carries into the sign's place.
 template <bool kBf16>
-__device__ __forceinline__ bool nonfinite(uint32_t x)
+__device__ __forceinline__ uint32_t nonfinite_marks(u32x4 x)
 {
-    constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
-    return (x & e) == e;
-}
-
-template <bool kBf16>
-__device__ __forceinline__ bool any_nonfinite(u32x4 x)
-{
-    bool r = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r = r || nonfinite<kBf16>(x[i]) || nonfinite<kBf16>(x[i] >> 16);
-    return r;
-}
-
-template <bool kBf16>
-__device__ __forceinline__ u32x4 zero_nonfinite(u32x4 x)
-{
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (nonfinite<kBf16>(x[i])) x[i] &= 0xffff0000u;
-        if (nonfinite<kBf16>(x[i] >> 16)) x[i] &= 0x0000ffffu;
-    }
-    return x;
+    constexpr uint32_t e = kBf16 ? 0x7f807f80u : 0x7c007c00u, one = kBf16 ? 0x00800080u : 0x04000400u;
+    return ((x[0] & e) + one) | ((x[1] & e) + one) | ((x[2] & e) + one) | ((x[3] & e) + one);
 }
 
 // One sequence's rows of q and positions.
@@ -277,6 +294,37 @@ struct Keys {
     }
 };
 
+// The slots of 64 pages of a sequence, one a lane (-1: not held), from a
+// multiple of 64 on, and of the 64 after them, read ahead.
+struct Window {
+    int32_t now;
+    int64_t ahead;
+    uint32_t base;
+
+    __device__ __forceinline__ int64_t entry(const AttendArgs& a, const int64_t* table, uint32_t from, int32_t hi)
+    {
+        const uint32_t page = from + (threadIdx.x & 63u);
+        return int64_t(page) << a.page_shift < hi ? table[page] : -1;
+    }
+    __device__ __forceinline__ void start(const AttendArgs& a, const int64_t* table, int32_t k0, int32_t hi)
+    {
+        base = (uint32_t(k0) >> a.page_shift) & ~63u;
+        const int64_t e = entry(a, table, base, hi);
+        now = held(e, a.nslots) ? int32_t(e) : -1;
+        ahead = entry(a, table, base + 64, hi);
+    }
+    // Moves on to the page of key k (at most 64 pages).
+    __device__ __forceinline__ void reach(const AttendArgs& a, const int64_t* table, int32_t k, int32_t hi)
+    {
+        if ((uint32_t(k) >> a.page_shift) - base < 64) return;
+        base += 64;
+        now = held(ahead, a.nslots) ? int32_t(ahead) : -1;
+        ahead = entry(a, table, base + 64, hi);
+    }
+    __device__ __forceinline__ int32_t slot(uint32_t page) const { return __builtin_amdgcn_readlane(now, int(page - base)); }
+    __device__ __forceinline__ int32_t slot_of(uint32_t page) const { return __shfl(now, int(page - base) & 63); }
+};
+
 // Bits j of the keys k0 + j a query at position p sees among the `ok` ones.
 __device__ __forceinline__ uint64_t seen_bits(const AttendArgs& a, uint64_t ok, int32_t k0, int32_t p)
 {
@@ -307,6 +355,73 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, uint32_t t, uint3
         a.lse[uint64_t(t) * a.q_heads + h] = l == 0.0f ? -INFINITY : (shift + log2f(l)) * 0.69314718055994531f;
 }
 
+// One row by one wave, key by key: the keys in [from, to) that token t (at pos)
+// sees, one a lane for the scores, the head's dims over the lanes for the sum
+// over the values.  No key that is not seen takes part in anything: the way
+// out where V holds an infinity or NaN among keys that not every row of a
+// workgroup sees, which the matrix product would multiply by 0.
+template <bool kBf16>
+__device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t, uint32_t h, uint32_t kvh, int32_t pos,
+                          int32_t from, int32_t to, bool split, float* part_o, float2* part_ml)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    if (a.causal && to > pos + 1) to = pos + 1;
+    if (a.window && from < pos - int32_t(a.window) + 1) from = pos - int32_t(a.window) + 1;
+    const uint16_t* q = a.q + t * a.q_token + h * a.q_head;
+    const float c = a.negate ? -a.scale_log2 : a.scale_log2;
+    float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int32_t j0 = from; j0 < to; j0 += 64) {
+        const int32_t j = j0 + int32_t(lane);
+        int64_t slot = -1;
+        if (j < to) slot = table[j >> a.page_shift];
+        const bool seen = held(slot, a.nslots);
+        const uint64_t at = seen ? uint64_t(slot) * a.slot_bytes +
+                                       (uint64_t(uint32_t(j) & ((1u << a.page_shift) - 1u)) * a.kv_heads + kvh) * a.dim * 2
+                                 : 0;
+        float s = -INFINITY;
+        if (seen) {
+            const uint16_t* k = reinterpret_cast<const uint16_t*>(a.cache_k + at);
+            float dot = 0.0f;
+            for (uint32_t d = 0; d < a.dim; ++d) dot = __builtin_fmaf(to_f32<kBf16>(q[d]), to_f32<kBf16>(k[d]), dot);
+            s = dot * c;
+        }
+        float top = s;
+#pragma unroll
+        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float mn = fmaxf(m, top);
+        if (mn == -INFINITY) continue;
+        const float w = seen ? __builtin_amdgcn_exp2f(s - mn) : 0.0f;
+        const float keep = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        float sum = w;
+#pragma unroll
+        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+        l = __builtin_fmaf(l, keep, sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= keep;
+        const uint64_t mask = __ballot(seen);
+        for (int x = 0; x < 64; ++x) {
+            if (!(mask >> x & 1)) continue;
+            const float wx = __shfl(w, x);
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(a.cache_v + __shfl(at, x));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (lane + 64 * i < a.dim) acc[i] = __builtin_fmaf(wx, to_f32<kBf16>(v[lane + 64 * i]), acc[i]);
+        }
+    }
+    const float shift = m == -INFINITY ? 0.0f : m, inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t d = lane + 64 * i;
+        if (d >= a.dim) continue;
+        if (split) part_o[d] = acc[i];
+        else a.out[t * a.out_token + h * a.out_head + d] = from_f32<kBf16>(acc[i] * inv);
+    }
+    if (lane != 0) return;
+    if (split) *part_ml = float2{shift, l};
+    else if (a.lse) a.lse[uint64_t(t) * a.q_heads + h] = l == 0.0f ? -INFINITY : (shift + log2f(l)) * 0.69314718055994531f;
+}
+
 // ---------------------------------------------------------------- few rows
 
 // One workgroup per (sequence, KV head, part of the keys): at most 16 * kBlocks
@@ -314,8 +429,20 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, uint32_t t, uint3
 // registers of S^T = K Q^T, V through the wave's own LDS.  Memory bounds
 // it: the next step's K and V are in flight while a step is computed, with no
 // barrier until the waves' results are joined at the end.
+template <int kDim>
+constexpr int few_wave_bytes()
+{
+    const int v = int(kFewKeys) * (kDim + 16) * 2, o = 16 * (kDim + 4) * 4;
+    return v > o ? v : o;
+}
+template <int kDim>
+constexpr int few_lds_bytes()
+{
+    return int(kFewWaves) * (few_wave_bytes<kDim>() + 16 * 8 + 16);
+}
+
 template <bool kBf16, int kDim, int kBlocks>
-__global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few_kernel(AttendArgs a)
+__device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, uint32_t group, uint32_t part)
 {
     constexpr int kSteps = kDim / 32;       // contraction steps of K Q^T
     constexpr int kOut = kDim / 16;         // 16-wide blocks of the output
@@ -323,15 +450,13 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
     constexpr int kPitch = kDim + 16;       // LDS row of V: 32 bytes of padding spread the rows over the banks
     constexpr int kLoads = kChunks / 2;     // 16-byte loads a lane makes for 32 rows
     constexpr int kOPitch = kDim + 4;
-    constexpr int kV = kFewKeys * kPitch * 2;
-    constexpr int kO = 16 * kOPitch * 4;
-    constexpr int kWaveBytes = kV > kO ? kV : kO;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves * kWaveBytes];
-    __shared__ float2 ml[kFewWaves][16];
+    constexpr int kWaveBytes = few_wave_bytes<kDim>();
+    float2(*const ml)[16] = reinterpret_cast<float2(*)[16]>(lds + kFewWaves * kWaveBytes);
+    uint32_t* const odd = reinterpret_cast<uint32_t*>(lds + kFewWaves * (kWaveBytes + 16 * 8));
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = lane & 15u, quad = lane >> 4;
-    if (a.q_starts && blockIdx.x == 0 && blockIdx.y == 0) zero_unowned<kBf16>(a);
-    const uint32_t kvh = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads, part = blockIdx.y;
+    if (a.q_starts && group == 0 && part == 0) zero_unowned<kBf16>(a);
+    const uint32_t kvh = group % a.kv_heads, b = group / a.kv_heads;
     const Seq s = seq_of(a, b);
     const uint32_t rows = s.n_new * a.group;
     if (rows == 0 || rows > 16 * kBlocks) return;
@@ -364,6 +489,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
     const int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
 
     uint16_t* const vs = reinterpret_cast<uint16_t*>(lds + wave * kWaveBytes);
+    const uint32_t vs_at = uint32_t(reinterpret_cast<uintptr_t>((lds_void*)lds)) + wave * kWaveBytes;
     float m[kBlocks], l[kBlocks];
     f32x4 o[kBlocks][kOut];
 #pragma unroll
@@ -374,6 +500,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
         for (int i = 0; i < kOut; ++i) o[x][i] = f32x4{0, 0, 0, 0};
     }
 
+    uint32_t marks = 0;  // of V that not every row sees
     u32x4 kr[2][kSteps], vr[kLoads];
     Keys<kFewKeys> keys;
     const auto load_k = [&](int32_t k0) {
@@ -425,29 +552,26 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
             }
         }
         if (next < hi) load_k(next);
-        bool odd = false;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t c = 64 * i + lane;
             *reinterpret_cast<u32x4*>(vs + (c / kChunks) * kPitch + (c % kChunks) * 8) = vr[i];
         }
-        // A key that some rows see and others do not: 0 x inf and 0 x NaN in
-        // the matrix product would reach the rows that do not.
+        // Keys that some rows see and others do not: an infinity or NaN in their
+        // V would meet a weight of 0.
         const bool partial =
             s.n_new > 1 && ((a.causal && k0 + int32_t(kFewKeys) - 1 > s.base) ||
                             (a.window && k0 <= p_last - int32_t(a.window)));
         if (partial) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) odd |= any_nonfinite<kBf16>(vr[i]);
+            for (int i = 0; i < kLoads; ++i) marks |= nonfinite_marks<kBf16>(vr[i]);
         }
         if (next < hi) load_v(next);
 
         u32x4 pw[kBlocks];
-        uint32_t seen[kBlocks];
 #pragma unroll
         for (int x = 0; x < kBlocks; ++x) {
-            seen[x] = uint32_t(partial ? seen_bits(a, ok, k0, pos[x]) : ok);
-            const uint32_t mine = seen[x] >> (4 * quad);
+            const uint32_t mine = uint32_t(partial ? seen_bits(a, ok, k0, pos[x]) : ok) >> (4 * quad);
             float top = -INFINITY;
 #pragma unroll
             for (int y = 0; y < 2; ++y)
@@ -476,36 +600,12 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
 #pragma unroll
             for (int i = 0; i < kOut; ++i) o[x][i] *= keep;
         }
-        if (partial && __ballot(odd) != 0) {
-            // Rows that see a key with an infinity or NaN take it itself (a
-            // weight is positive); then it is cleared for the product.
-            for (uint32_t j = 0; j < kFewKeys; ++j) {
-#pragma unroll
-                for (int i = 0; i < kOut; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint16_t v = vs[j * kPitch + 16 * i + 4 * quad + e];
-                        if (nonfinite<kBf16>(v)) {
-#pragma unroll
-                            for (int x = 0; x < kBlocks; ++x)
-                                if (seen[x] >> j & 1) o[x][i][e] += to_f32<kBf16>(v);
-                        }
-                    }
-            }
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const uint32_t c = 64 * i + lane;
-                u32x4* v = reinterpret_cast<u32x4*>(vs + (c / kChunks) * kPitch + (c % kChunks) * 8);
-                *v = zero_nonfinite<kBf16>(*v);
-            }
-        }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < kOut; ++i) {
             // keys 4 quad + 0..3 and 16 + 4 quad + 0..3 of 16 columns
-            const uint16_t* v = vs + (4 * quad + (col >> 2)) * kPitch + 16 * i + 4 * (col & 3u);
-            const u32x2 v0 = read_tr(v), v1 = read_tr(v + 16 * kPitch);
+            const uint32_t v = vs_at + 2 * ((4 * quad + (col >> 2)) * kPitch + 16 * i + 4 * (col & 3u));
+            const u32x2 v0 = read_tr(v), v1 = read_tr(v + 32 * kPitch);
             const u32x4 vt{v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
             for (int x = 0; x < kBlocks; ++x) o[x][i] = mfma16<kBf16>(vt, pw[x], o[x][i]);
@@ -513,6 +613,20 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
         __builtin_amdgcn_wave_barrier();
     }
 
+    if (s.n_new > 1) {
+        const uint64_t any = __ballot((marks & 0x80008000u) != 0);
+        if (lane == 0) odd[wave] = any != 0;
+        __syncthreads();
+    }
+    if (s.n_new > 1 && (odd[0] | odd[1] | odd[2] | odd[3])) {
+        for (uint32_t x = wave; x < rows; x += kFewWaves) {
+            const uint32_t xt = x / a.group, xh = kvh * a.group + (x - xt * a.group);
+            const uint64_t row = (uint64_t(part) * a.seqs * a.kv_heads + uint64_t(b) * a.kv_heads + kvh) * a.few_rows + x;
+            plain_row<kBf16>(a, table, s.q0 + xt, xh, kvh, s.base + int32_t(xt), k_first, hi,
+                             cut.parts > 1, a.few_o + row * a.dim, a.few_ml + row);
+        }
+        return;
+    }
     // Join the waves, 16 rows at a time.
 #pragma unroll
     for (int x = 0; x < kBlocks; ++x) {
@@ -558,35 +672,70 @@ __global__ __launch_bounds__(64 * kFewWaves, kDim > 128 ? 1 : 2) void attend_few
 
 // One workgroup per (128 rows of a sequence and KV head, part of the keys):
 // each of the 4 waves holds 32 rows, all of them share the K and V of 64 keys
-// at a time, staged through registers into two LDS buffers (one barrier a
-// step).  Rows of LDS are 16-byte chunks in an order permuted by the row
-// (a power of two of them), so that the 8 rows of a read fall on different banks.
-template <bool kBf16, int kDim>
-__global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_tile_kernel(AttendArgs a)
+// at a time, which go from memory straight to one of two LDS buffers while the
+// other is used (one barrier a step).  Rows of LDS are 16-byte chunks in an order
+// permuted by the row (a power of two of them), so that the rows of a read
+// fall on different banks.
+template <int kDim>
+constexpr int tile_chunks()  // 16-byte chunks of an LDS row
 {
-    constexpr int kChunks = kDim <= 64 ? 8 : kDim <= 128 ? 16 : 32;  // chunks of an LDS row
-    constexpr int kPitch = kChunks * 8;
+    return kDim <= 64 ? 8 : kDim <= 128 ? 16 : 32;
+}
+// K lies in groups of the rows that one instruction of a wave fills (1 KiB),
+// with a gap after each.
+template <int kDim>
+constexpr int k_group_bytes()
+{
+    return 1024 + (tile_chunks<kDim>() == 32 ? 32 : 64);
+}
+template <int kDim>
+constexpr int k_bytes()
+{
+    return int(kTileKeys) * tile_chunks<kDim>() / 64 * k_group_bytes<kDim>();
+}
+template <int kDim>
+constexpr int tile_lds_bytes()  // two buffers of K and V
+{
+    return 2 * (k_bytes<kDim>() + int(kTileKeys) * tile_chunks<kDim>() * 16);
+}
+
+template <bool kBf16, int kDim>
+__device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, uint32_t group, uint32_t groups)
+{
+    constexpr int kChunks = tile_chunks<kDim>();
+    constexpr int kPitch = kChunks * 8;  // elements of a row
     constexpr int kThreads = 64 * int(kTileWaves);
     constexpr int kLoads = int(kTileKeys) * kChunks / kThreads;
     constexpr int kRowStep = kThreads / kChunks;
     constexpr int kSteps = kDim / 16;
     constexpr int kOut = kDim / 32;
-    __shared__ __attribute__((aligned(16))) uint16_t ks[2][kTileKeys * kPitch];
-    __shared__ __attribute__((aligned(16))) uint16_t vs[2][kTileKeys * kPitch];
-    __shared__ uint32_t odd_flag[2];
+    constexpr uint32_t kBufBytes = tile_lds_bytes<kDim>() / 2, kKBytes = k_bytes<kDim>();  // of a buffer: K, then V
+    constexpr uint32_t kGroup = k_group_bytes<kDim>(), kGroupRows = 64 / kChunks;
+    const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>((lds_void*)lds));
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = lane & 31u, half = lane >> 5;
-    if (a.q_starts && a.few_rows == 0 && blockIdx.x == 0) zero_unowned<kBf16>(a);
+    if (a.q_starts && a.few_rows == 0 && group == 0) zero_unowned<kBf16>(a);
 
-    // Workgroups in groups of one KV head's part; consecutive ones go to the
-    // same XCD (workgroup i runs on XCD i % 8), whose L2 then holds their K and V.
-    const uint32_t total = gridDim.x;
-    const uint32_t x8 = total / 8, r8 = total % 8;
-    const uint32_t xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
-    const uint32_t w = xcd * x8 + (xcd < r8 ? xcd : r8) + nth;
-    const uint32_t tile = a.tiles - 1 - w % a.tiles;  // the last tiles see most keys: first
-    const uint32_t rest = w / a.tiles;
-    const uint32_t part = rest % a.tile_split, kvh = rest / a.tile_split;
+    // A column is one KV head's part of the keys, over all tiles.  Workgroup i
+    // runs on XCD i % 8: whole columns go to one XCD, whose L2 then holds their
+    // K and V, dealt out back and forth, as the parts that only long sequences
+    // have come last; where the columns do not fill the XCDs evenly, each XCD
+    // takes an eighth of the list.
+    const uint32_t xcd = group % 8, nth = group / 8;
+    const uint32_t columns = groups / a.tiles;
+    uint32_t column, tile;
+    if (columns % 8 == 0) {
+        const uint32_t deal = nth / a.tiles;
+        column = 8 * deal + (deal % 2 ? 7 - xcd : xcd);
+        tile = nth % a.tiles;
+    } else {
+        const uint32_t x8 = groups / 8, r8 = groups % 8;
+        const uint32_t w = xcd * x8 + (xcd < r8 ? xcd : r8) + nth;
+        column = w / a.tiles;
+        tile = w % a.tiles;
+    }
+    tile = a.tiles - 1 - tile;  // the last tiles see most keys: first
+    const uint32_t kvh = column % a.kv_heads, part = column / a.kv_heads;
 
     // Sequence b's tiles start at floor(q_starts[b] * group / rows) + b, which
     // leaves it at least the tiles it needs.
@@ -617,6 +766,10 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
 
     const uint32_t r_last = (r0 + kTileRows < rows ? r0 + kTileRows : rows) - 1;
     const int32_t p_first = s.base + int32_t(r0 / a.group), p_last = s.base + int32_t(r_last / a.group);
+    // of this wave's rows (rows past the last repeat it)
+    const uint32_t w_first = r0 + wave * 32 < rows ? r0 + wave * 32 : r_last;
+    const uint32_t w_last = w_first + 31 < r_last ? w_first + 31 : r_last;
+    const int32_t pw_first = s.base + int32_t(w_first / a.group), pw_last = s.base + int32_t(w_last / a.group);
     const uint32_t r = r0 + wave * 32 + col;
     const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
     const int32_t pos = s.base + int32_t(tok);
@@ -641,98 +794,116 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    uint32_t marks = 0;  // of V that not every row sees
 
-    u32x4 kr[kLoads], vr[kLoads];
-    const uint32_t chunk = threadIdx.x % kChunks, row0 = threadIdx.x / kChunks;
+    // Chunk orders in LDS.  K is read a chunk of 32 rows at a time: x of a row
+    // permutes its lowest chunks so that the rows of a group, and the gaps so
+    // that the groups, fall on different banks; chunks 2k and 2k + 1 are read at
+    // one of two addresses plus a constant.  V is read four chunks of 4 rows at
+    // a time: the row's number permutes fours of chunks.  A thread fills the same
+    // place of every kRowStep-th row, which all have one order.
+    const auto k_order = [](uint32_t row) {
+        return kGroupRows == 8 ? (row >> 1) & 3u : row & (kGroupRows - 1);
+    };
+    const auto v_order = [](uint32_t row) { return (row << 2) & (kChunks - 1) & 12u; };
+    const auto k_place = [](uint32_t row, uint32_t c) {
+        return row / kGroupRows * kGroup + row % kGroupRows * (kChunks * 16) + c * 16;
+    };
+    const uint32_t place = threadIdx.x % kChunks, row0 = threadIdx.x / kChunks;
     const uint32_t kv_row = a.kv_heads * a.dim * 2u;
-    Keys<kTileKeys> keys;
-    const auto load = [&](int32_t kb) {
-        if ((1u << a.page_shift) >= kTileKeys) {
-            // one page holds the step's keys
-            const uint64_t at = uint64_t(keys.page_slot()) * a.slot_bytes +
-                                uint64_t(uint32_t(kb) & ((1u << a.page_shift) - 1u)) * kv_row + kvh * a.dim * 2u;
-            const uint8_t* kp = a.cache_k + at;
-            const uint8_t* vp = a.cache_v + at;
-            if (keys.ok == ~0ull && a.dim == kChunks * 8u) {
+    const bool in_page = (1u << a.page_shift) >= kTileKeys;
+    Window pages;
+    // The keys of [kb, kb + 64) that may be read: on held pages, in [lo, hi).
+    const auto readable = [&](int32_t kb) {
+        uint64_t ok = ~0ull;
+        if (kb < lo) ok <<= lo - kb;
+        if (hi - kb < 64) ok &= ~0ull >> (64 - (hi - kb));
+        if (in_page) return pages.slot(uint32_t(kb) >> a.page_shift) >= 0 ? ok : 0ull;
+        return ok & __ballot(pages.slot_of(uint32_t(kb + int32_t(lane)) >> a.page_shift) >= 0);
+    };
+    // K and V of keys [kb, kb + 64) into one buffer; the keys that may be read.
+    // Whole steps go from memory to LDS; a step with keys that may not be read
+    // comes through registers, which hold zeros for those.
+    const uint32_t k_chunk = place ^ k_order(row0), v_chunk = place ^ v_order(row0);
+    const auto fill = [&](int buf, int32_t kb) -> uint64_t {
+        if (kb >= hi) return 0;
+        pages.reach(a, table, kb, hi);
+        const uint64_t ok = readable(kb);
+        const uint32_t k_to = __builtin_amdgcn_readfirstlane(lds_at + buf * kBufBytes + wave * kGroup);
+        const uint32_t v_to = __builtin_amdgcn_readfirstlane(lds_at + buf * kBufBytes + kKBytes + wave * 1024);
+        const uint32_t in = uint32_t(kb) & ((1u << a.page_shift) - 1u);
+        if (ok == ~0ull && in_page && a.dim == kPitch) {
+            const uint64_t page = uint64_t(uint32_t(pages.slot(uint32_t(kb) >> a.page_shift))) * a.slot_bytes +
+                                  uint64_t(in) * kv_row + kvh * a.dim * 2u;
+            const uint8_t* const kp = uniform(a.cache_k + page);
+            const uint8_t* const vp = uniform(a.cache_v + page);
+            const uint32_t row = row0 * kv_row;
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    const uint32_t j = row0 + i * kRowStep;
-                    kr[i] = *reinterpret_cast<const u32x4*>(kp + j * kv_row + chunk * 16);
-                    vr[i] = *reinterpret_cast<const u32x4*>(vp + j * kv_row + chunk * 16);
-                }
-                return;
-            }
+            for (int i = 0; i < kLoads; ++i) to_lds(kp, i * kRowStep * kv_row + row + k_chunk * 16, k_to + i * 4 * kGroup);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const uint32_t j = row0 + i * kRowStep;
-                kr[i] = vr[i] = u32x4{0, 0, 0, 0};
-                if ((keys.ok >> j & 1) && chunk * 8 < a.dim) {
-                    kr[i] = *reinterpret_cast<const u32x4*>(kp + j * kv_row + chunk * 16);
-                    vr[i] = *reinterpret_cast<const u32x4*>(vp + j * kv_row + chunk * 16);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const uint32_t j = row0 + i * kRowStep;
-                const uint64_t off = keys.row(a, kb, j, kvh) + chunk * 16;
-                kr[i] = vr[i] = u32x4{0, 0, 0, 0};
-                if ((keys.ok >> j & 1) && chunk * 8 < a.dim) {
-                    kr[i] = *reinterpret_cast<const u32x4*>(a.cache_k + off);
-                    vr[i] = *reinterpret_cast<const u32x4*>(a.cache_v + off);
-                }
-            }
+            for (int i = 0; i < kLoads; ++i)
+                to_lds(vp, i * kRowStep * kv_row + row + v_chunk * 16, v_to + i * 4096);
+            return ok;
         }
-    };
-    // Chunk orders: K is read a chunk of 32 rows at a time (8 lanes a
-    // clock: rows of different r % 8), V two chunks of 4 rows.
-    const auto k_at = [](uint32_t row, uint32_t c) { return row * kPitch + ((c ^ (row & (kChunks - 1))) * 8); };
-    const auto v_at = [](uint32_t row, uint32_t c) {
-        return row * kPitch + ((c ^ ((row << 2) & (kChunks - 1) & 12)) * 8);
-    };
-    const auto stage = [&](int buf) {
+        const bool k_in = k_chunk * 8 < a.dim, v_in = v_chunk * 8 < a.dim;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const uint32_t j = row0 + i * kRowStep;
-            *reinterpret_cast<u32x4*>(&ks[buf][k_at(j, chunk)]) = kr[i];
-            *reinterpret_cast<u32x4*>(&vs[buf][v_at(j, chunk)]) = vr[i];
+            const uint32_t j = row0 + i * kRowStep, key = uint32_t(kb) + j;
+            const uint64_t at = uint64_t(uint32_t(pages.slot_of(key >> a.page_shift))) * a.slot_bytes +
+                                uint64_t(key & ((1u << a.page_shift) - 1u)) * kv_row + kvh * a.dim * 2u;
+            const uint8_t* const kp = a.cache_k + at + k_chunk * 16;
+            const uint8_t* const vp = a.cache_v + at + v_chunk * 16;
+            if (ok == ~0ull) {
+                if (k_in) to_lds(kp, k_to + i * 4 * kGroup);
+                if (v_in) to_lds(vp, v_to + i * 4096);
+            } else {
+                const bool mine = ok >> j & 1;
+                u32x4 k{0, 0, 0, 0}, v{0, 0, 0, 0};
+                if (mine && k_in) k = *reinterpret_cast<const u32x4*>(kp);
+                if (mine && v_in) v = *reinterpret_cast<const u32x4*>(vp);
+                uint8_t* const b2 = lds + buf * kBufBytes;
+                *reinterpret_cast<u32x4*>(b2 + k_place(j, place)) = k;
+                *reinterpret_cast<u32x4*>(b2 + kKBytes + (j * kChunks + place) * 16) = v;
+            }
         }
-    };
-    // Keys that some of the tile's rows see and others do not.
-    const auto is_partial = [&](int32_t kb) {
-        return (a.causal && kb + int32_t(kTileKeys) - 1 > p_first) || (a.window && kb <= p_last - int32_t(a.window));
-    };
-    // Before the barrier that makes a buffer visible: does it hold an infinity
-    // or NaN in V that not every row sees?
-    const auto flag_odd = [&](int buf, int32_t kb) {
-        if (!is_partial(kb)) return;
-        bool odd = false;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) odd |= any_nonfinite<kBf16>(vr[i]);
-        if (__ballot(odd) && lane == 0) odd_flag[buf] = 1;
+        return ok;
     };
 
-    if (threadIdx.x < 2) odd_flag[threadIdx.x] = 0;
-    uint64_t ok = 0;
-    if (k0 < hi) {
-        keys.fetch(a, table, k0, lo, hi);
-        keys.resolve(a);
-        keys.fetch(a, table, k0 + int32_t(kTileKeys), lo, hi);
-        load(k0);
-        ok = keys.ok;
+    // The chunks past the head dim stay zero.
+    if (a.dim < kPitch) {
+        for (uint32_t x = threadIdx.x; x < kTileKeys * kChunks; x += kThreads) {
+            const uint32_t j = x / kChunks, c = x % kChunks;
+            for (int b2 = 0; b2 < 2; ++b2) {
+                uint8_t* const b3 = lds + b2 * kBufBytes;
+                if ((c ^ k_order(j)) * 8 >= a.dim) *reinterpret_cast<u32x4*>(b3 + k_place(j, c)) = u32x4{0, 0, 0, 0};
+                if ((c ^ v_order(j)) * 8 >= a.dim) *reinterpret_cast<u32x4*>(b3 + kKBytes + x * 16) = u32x4{0, 0, 0, 0};
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    if (k0 < hi) {
-        stage(0);
-        flag_odd(0, k0);
-        keys.resolve(a);
-        keys.fetch(a, table, k0 + 2 * int32_t(kTileKeys), lo, hi);
-        if (k0 + int32_t(kTileKeys) < hi) load(k0 + int32_t(kTileKeys));
+    // Where this lane reads: row col of K at chunk `half` of each pair, even and
+    // odd k; the 4 rows of V at each 32 columns.
+    uint32_t k_read[2], v_read[kOut];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) k_read[x] = lds_at + k_place(col, (2 * x + half) ^ k_order(col));
+    const uint32_t v_row = 4 * half + ((lane & 15u) >> 2);
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+        const uint32_t d = 32 * i + (lane & 16u) + 4 * (lane & 3u);
+        v_read[i] = lds_at + kKBytes + v_row * (kChunks * 16) + (((d / 8) ^ v_order(v_row)) * 8 + d % 8) * 2;
     }
-    __syncthreads();
+    pages.start(a, table, k0, hi);
+    uint64_t ok_next = fill(0, k0);
     int buf = 0;
     for (; k0 < hi; k0 += int32_t(kTileKeys)) {
-        const int32_t next = k0 + int32_t(kTileKeys);
+        // This step's K and V are there, and every wave is done with the other
+        // buffer: the next step's go into it.
+        wait_loads();
+        __syncthreads();
+        const uint64_t ok = ok_next;
+        ok_next = fill(1 - buf, k0 + int32_t(kTileKeys));
+        const uint32_t in_buf = buf * kBufBytes;
+        const uint32_t k_even = k_read[0] + in_buf, k_odd = k_read[1] + in_buf;
         // The matrix instructions go first where two workgroups' waves meet on
         // a SIMD, so that one's weights are formed during the other's products.
         __builtin_amdgcn_s_setprio(1);
@@ -745,14 +916,16 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(&ks[buf][k_at(32 * y + col, 2 * k + half)]);
+                const u32x4 kf = read_lds((k % 2 ? k_odd : k_even) + k / 2 * 64 + y * (32 / kGroupRows * kGroup));
                 st[y] = mfma32<kBf16>(kf, q[k], st[y]);
             }
         __builtin_amdgcn_s_setprio(0);
-        const bool partial = is_partial(k0);
+        // Keys that some of the wave's rows see and others do not.
+        const bool partial = (a.causal && k0 + int32_t(kTileKeys) - 1 > pw_first) ||
+                             (a.window && k0 <= pw_last - int32_t(a.window));
         uint64_t seen = ok;
-        if (partial) seen = seen_bits(a, ok, k0, pos);
         if (partial || ok != ~0ull) {
+            if (partial) seen = seen_bits(a, ok, k0, pos);
             const uint64_t mine = seen >> (4 * half);
 #pragma unroll
             for (int y = 0; y < 2; ++y)
@@ -787,57 +960,52 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
                 sum[e % 4] += st[y][e];
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (partial && odd_flag[buf]) {
-            // Rows that see a key with an infinity or NaN take it itself (a
-            // weight is positive); then it is cleared for the product.
-            for (uint32_t j = 0; j < kTileKeys; ++j) {
-#pragma unroll
-                for (int i = 0; i < kOut; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const uint32_t d = 32 * i + 8 * (e / 4) + 4 * half + e % 4;
-                        const uint16_t v = vs[buf][v_at(j, d / 8) + d % 8];
-                        if (nonfinite<kBf16>(v) && (seen >> j & 1)) o[i][e] += to_f32<kBf16>(v);
-                    }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                u32x4* v = reinterpret_cast<u32x4*>(&vs[buf][v_at(row0 + i * kRowStep, chunk)]);
-                *v = zero_nonfinite<kBf16>(*v);
-            }
-            if (threadIdx.x == 0) odd_flag[buf] = 0;
-            __syncthreads();
-        }
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
+        const auto v_frag = [&](int y, int i) {
+            const uint32_t at = v_read[i] + in_buf + y * 16 * (kChunks * 16);
+            const u32x2 v0 = read_tr(at), v1 = read_tr(at + 8 * (kChunks * 16));
+            return u32x4{v0[0], v0[1], v1[0], v1[1]};
+        };
+        const auto weights = [&](int y) {
             f32x8 w;
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = st[y / 2][8 * (y % 2) + e];
-            const u32x4 pw = pack8<kBf16>(w);
-            const uint32_t row = 16 * y + 4 * half + ((lane & 15u) >> 2);
+            return pack8<kBf16>(w);
+        };
+        __builtin_amdgcn_s_setprio(1);
+        if (!partial) {
 #pragma unroll
-            for (int i = 0; i < kOut; ++i) {
-                const uint32_t d = 32 * i + (lane & 16u) + 4 * (lane & 3u);
-                const u32x2 v0 = read_tr(&vs[buf][v_at(row, d / 8) + d % 8]);
-                const u32x2 v1 = read_tr(&vs[buf][v_at(row + 8, d / 8) + d % 8]);
-                o[i] = mfma32<kBf16>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pw, o[i]);
+            for (int y = 0; y < 4; ++y) {
+                const u32x4 pw = weights(y);
+#pragma unroll
+                for (int i = 0; i < kOut; ++i) o[i] = mfma32<kBf16>(v_frag(y, i), pw, o[i]);
+            }
+        } else {
+            // Not every row sees these keys: an infinity or NaN in their V would
+            // meet a weight of 0.
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const u32x4 pw = weights(y);
+#pragma unroll
+                for (int i = 0; i < kOut; ++i) {
+                    const u32x4 v = v_frag(y, i);
+                    marks |= nonfinite_marks<kBf16>(v);
+                    o[i] = mfma32<kBf16>(v, pw, o[i]);
+                }
             }
         }
         __builtin_amdgcn_s_setprio(0);
-        buf ^= 1;
-        if (next < hi) {
-            stage(buf);
-            flag_odd(buf, next);
-            ok = keys.ok;
-            keys.resolve(a);
-            keys.fetch(a, table, next + 2 * int32_t(kTileKeys), lo, hi);
-            if (next + int32_t(kTileKeys) < hi) load(next + int32_t(kTileKeys));
-        }
-        __syncthreads();
+        buf = 1 - buf;
     }
 
+    if (__ballot((marks & 0x80008000u) != 0)) {
+        for (uint32_t x = r0 + wave * 32; x < r0 + wave * 32 + 32 && x < rows; ++x) {
+            const uint32_t xt = x / a.group, xh = kvh * a.group + (x - xt * a.group);
+            const uint64_t row = (uint64_t(part) * a.tokens + s.q0 + xt) * a.q_heads + xh;
+            plain_row<kBf16>(a, table, s.q0 + xt, xh, kvh, s.base + int32_t(xt), cut.lo + int32_t(part * a.tile_per), hi,
+                             cut.parts > 1, a.tile_o + row * a.dim, a.tile_ml + row);
+        }
+        return;
+    }
     l = across<false>(l, fadd2);
     if (r >= rows) return;
     const uint32_t t = s.q0 + tok;
@@ -866,57 +1034,166 @@ __global__ __launch_bounds__(64 * kTileWaves, kDim > 128 ? 1 : 2) void attend_ti
     }
 }
 
+// ---------------------------------------------------------------- kernels
+
+template <bool kBf16, int kDim, int kBlocks>
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_few_kernel(AttendArgs a)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds_bytes<kDim>()];
+    attend_few<kBf16, kDim, kBlocks>(a, lds, blockIdx.x, blockIdx.y);
+}
+
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim > 64 ? 2 : 3) void attend_tile_kernel(AttendArgs a)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t lds[tile_lds_bytes<kDim>()];
+    attend_tile<kBf16, kDim>(a, lds, blockIdx.x, gridDim.x);
+}
+
+// Both kinds of sequences in one launch: the tiles' workgroups first, which take
+// longest, and the few-row ones beside and after them.
+template <bool kBf16, int kDim, int kBlocks>
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(AttendArgs a)
+{
+    constexpr int kBytes = tile_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? tile_lds_bytes<kDim>() : few_lds_bytes<kDim>();
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
+    const uint32_t tiles = a.tiles * a.kv_heads * a.tile_split;
+    if (blockIdx.x < tiles) {
+        attend_tile<kBf16, kDim>(a, lds, blockIdx.x, tiles);
+    } else {
+        const uint32_t x = blockIdx.x - tiles, groups = a.seqs * a.kv_heads;
+        attend_few<kBf16, kDim, kBlocks>(a, lds, x % groups, x / groups);
+    }
+}
+
 // ---------------------------------------------------------------- parts joined
 
-// kWaves waves per (token, query head) of a split sequence: every wave reads
-// the parts' (m, l), one a lane; the numerators, 4 dims a lane, are summed by
-// groups of lanes that take every kStride-th part each, then over the groups in
-// their order.
-template <bool kBf16, int kDim, int kWaves>
+// Where a row's parts are, and how many.
+struct Parts {
+    const float2* ml;
+    const float* o;
+    uint64_t step;  // rows from one part to the next
+    uint32_t parts;
+};
+
+__device__ __forceinline__ Parts parts_of(const AttendArgs& a, const Seq& s, uint32_t t, uint32_t h)
+{
+    Parts p{nullptr, nullptr, 0, 0};
+    if (t < s.q0 || t >= s.q0 + s.n_new) return p;
+    const bool few = s.n_new * a.group <= a.few_rows;
+    p.parts = cut_of(a, s, few ? a.few_per : a.tile_per).parts;
+    const uint32_t kvh = h / a.group;
+    const uint64_t row = few ? (uint64_t(s.b) * a.kv_heads + kvh) * a.few_rows + (t - s.q0) * a.group + (h - kvh * a.group)
+                             : uint64_t(t) * a.q_heads + h;
+    p.step = few ? uint64_t(a.seqs) * a.kv_heads * a.few_rows : uint64_t(a.tokens) * a.q_heads;
+    p.ml = (few ? a.few_ml : a.tile_ml) + row;
+    p.o = (few ? a.few_o : a.tile_o) + row * a.dim;
+    return p;
+}
+
+// The last sequence that starts at or before row t (0 where there is none).
+__device__ __forceinline__ uint32_t seq_at(const AttendArgs& a, uint32_t t)
+{
+    if (!a.q_starts) return t;
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t n = 0;
+    for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64)
+        n += __popcll(__ballot(s0 + lane < a.seqs && start_of(a, s0 + lane) <= t));
+    return n ? n - 1 : 0;
+}
+
+// Lanes that hold one row, 4 dims a lane.
+template <int kDim>
+constexpr uint32_t row_lanes()
+{
+    return kDim <= 64 ? 16 : kDim <= 128 ? 32 : 64;
+}
+
+// Many rows: row_lanes lanes per (token, query head), the parts one after
+// another.
+template <bool kBf16, int kDim>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
 {
-    constexpr uint32_t kLanes = kDim / 4 > 64 ? 64 : kDim / 4 > 32 ? 64 : kDim / 4 > 16 ? 32 : 16;  // of one row
-    constexpr uint32_t kStride = 64 * kWaves / kLanes;
-    constexpr uint32_t kRows = 4 / kWaves;
-    __shared__ f32x4 sums[kWaves == 1 ? 1 : 4][64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t th = blockIdx.x * kRows + wave / kWaves;
-    if (th >= a.tokens * a.q_heads) return;
+    constexpr uint32_t kLanes = row_lanes<kDim>(), kRows = 64 / kLanes, kHeld = kMaxSplit / kLanes, kAhead = 4;
+    const uint32_t lane = threadIdx.x & 63u, sub = lane % kLanes, d = sub * 4;
+    const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows, rows = a.tokens * a.q_heads;
+    if (first >= rows) return;
+    const uint32_t th = first + lane / kLanes;
     const uint32_t t = th / a.q_heads, h = th - t * a.q_heads;
-    uint32_t b = t;
+    // (rows of a wave may belong to several sequences)
+    uint32_t b = seq_at(a, first / a.q_heads);
     if (a.q_starts) {
-        uint32_t at_or_before = 0;
-        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64)
-            at_or_before += __popcll(__ballot(s0 + lane < a.seqs && start_of(a, s0 + lane) <= t));
-        if (at_or_before == 0) return;
-        b = at_or_before - 1;
+        while (b + 1 < a.seqs && start_of(a, b + 1) <= t) ++b;
+    } else {
+        b = t < a.seqs ? t : a.seqs - 1;
     }
-    const Seq s = seq_of(a, b);
-    if (t < s.q0 || t >= s.q0 + s.n_new) return;
-    const bool few = s.n_new * a.group <= a.few_rows;
-    const Cut cut = cut_of(a, s, few ? a.few_per : a.tile_per);
-    if (cut.parts <= 1) return;
-    const uint32_t kvh = h / a.group;
-    const uint64_t row = few ? (uint64_t(b) * a.kv_heads + kvh) * a.few_rows + (t - s.q0) * a.group + (h - kvh * a.group)
-                             : uint64_t(t) * a.q_heads + h;
-    const uint64_t step = few ? uint64_t(a.seqs) * a.kv_heads * a.few_rows : uint64_t(a.tokens) * a.q_heads;
-    const float2* mls = (few ? a.few_ml : a.tile_ml) + row;
-    const float* os = (few ? a.few_o : a.tile_o) + row * a.dim;
-    float2 v{0.0f, 0.0f};
-    if (lane < cut.parts) v = mls[lane * step];
-    const uint32_t which = kWaves == 1 ? lane / kLanes : threadIdx.x / kLanes, d = lane % kLanes * 4;
-    f32x4 acc{0, 0, 0, 0};
-    constexpr uint32_t kAhead = kMaxSplit / kStride < 8 ? kMaxSplit / kStride : 8;
-    f32x4 part[kAhead];
-    const auto load = [&](uint32_t p0) {
+    Parts p{nullptr, nullptr, 0, 0};
+    if (th < rows) p = parts_of(a, seq_of(a, b), t, h);
+    const uint32_t parts = p.parts > 1 ? p.parts : 0;
+    if (__ballot(parts != 0) == 0) return;
+    float2 v[kHeld];
+    float top = -INFINITY;
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t p = p0 + which + i * kStride;
-            part[i] = f32x4{0, 0, 0, 0};
-            if (p < cut.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(os + p * step * a.dim + d);
+    for (uint32_t i = 0; i < kHeld; ++i) {
+        v[i] = float2{0.0f, 0.0f};
+        if (i * kLanes + sub < parts) v[i] = p.ml[(i * kLanes + sub) * p.step];
+        if (v[i].y != 0.0f) top = fmaxf(top, v[i].x);
+    }
+#pragma unroll
+    for (uint32_t x = kLanes / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, int(x)));
+    if (top == -INFINITY) top = 0.0f;
+    float f[kHeld], sum = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) {
+        f[i] = v[i].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v[i].x - top);
+        sum = __builtin_fmaf(v[i].y, f[i], sum);
+    }
+#pragma unroll
+    for (uint32_t x = kLanes / 2; x; x >>= 1) sum += __shfl_xor(sum, int(x));
+    f32x4 acc{0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) {
+        for (uint32_t p0 = 0; p0 < kLanes; p0 += kAhead) {
+            if (__ballot(i * kLanes + p0 < parts) == 0) break;
+            f32x4 part[kAhead];
+#pragma unroll
+            for (uint32_t x = 0; x < kAhead; ++x) {
+                const uint32_t n = i * kLanes + p0 + x;
+                part[x] = f32x4{0, 0, 0, 0};
+                if (n < parts && d < a.dim) part[x] = *reinterpret_cast<const f32x4*>(p.o + n * p.step * a.dim + d);
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < kAhead; ++x) {
+                const float fx = __shfl(f[i], int((lane & ~(kLanes - 1)) + p0 + x));
+                if (fx != 0.0f) acc += part[x] * fx;
+            }
         }
-    };
-    load(0);
+    }
+    if (parts && d < a.dim) store_out<kBf16>(a, t, h, d, acc, sum, top);
+}
+
+// Few rows: a workgroup per (token, query head), its groups of row_lanes lanes
+// taking every so-many-th part each, summed in their order at the end.
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(256) void attend_join_row_kernel(AttendArgs a)
+{
+    constexpr uint32_t kLanes = row_lanes<kDim>(), kStride = 256 / kLanes, kMost = kMaxSplit / kStride;
+    __shared__ f32x4 sums[4][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t t = blockIdx.x / a.q_heads, h = blockIdx.x - t * a.q_heads;
+    const uint32_t b = seq_at(a, t);
+    const Parts p = parts_of(a, seq_of(a, b), t, h);
+    if (p.parts <= 1) return;
+    float2 v{0.0f, 0.0f};
+    if (lane < p.parts) v = p.ml[lane * p.step];
+    const uint32_t which = threadIdx.x / kLanes, d = lane % kLanes * 4;
+    f32x4 part[kMost];
+#pragma unroll
+    for (uint32_t i = 0; i < kMost; ++i) {
+        const uint32_t n = which + i * kStride;
+        part[i] = f32x4{0, 0, 0, 0};
+        if (n < p.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(p.o + n * p.step * a.dim + d);
+    }
     float top = v.y == 0.0f ? -INFINITY : v.x;
 #pragma unroll
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
@@ -925,28 +1202,20 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
     float sum = v.y * f;
 #pragma unroll
     for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-    for (uint32_t p0 = 0;;) {
+    f32x4 acc{0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const float fp = __shfl(f, int((p0 + which + i * kStride) & 63u));
-            if (fp != 0.0f) acc += part[i] * fp;
-        }
-        p0 += kAhead * kStride;
-        if (p0 >= cut.parts) break;
-        load(p0);
+    for (uint32_t i = 0; i < kMost; ++i) {
+        const float fx = __shfl(f, int(which + i * kStride));
+        if (fx != 0.0f) acc += part[i] * fx;
     }
 #pragma unroll
     for (uint32_t x = kLanes; x < 64; x <<= 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], int(x));
-    if constexpr (kWaves > 1) {
-        sums[wave][lane] = acc;
-        __syncthreads();
-        if (wave != 0) return;
-        acc = sums[0][lane];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) acc += sums[w][lane];
-    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+    acc = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
     if (lane < kLanes && d < a.dim) store_out<kBf16>(a, t, h, d, acc, sum, top);
 }
 
@@ -1006,9 +1275,19 @@ Plan attend_plan(const si_paged_attention_desc& d)
     const uint64_t pairs = uint64_t(d.seqs) * d.kv_heads;
     if (p.few) p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &p.few_split);
     if (p.tile) {
-        p.tiles = uint32_t(d.q_starts ? rows / kTileRows + d.seqs
-                                      : uint64_t(d.seqs) * ((group + kTileRows - 1) / kTileRows));
-        p.tile_per = part_keys(uint64_t(p.tiles) * d.kv_heads, keys, kTileSplitMin, kTileKeys, kTileTarget, &p.tile_split);
+        const uint64_t tile_rows = kTileRows;
+        p.tiles = uint32_t(d.q_starts ? rows / tile_rows + d.seqs
+                                      : uint64_t(d.seqs) * ((group + tile_rows - 1) / tile_rows));
+        // Cut only where the tiles alone leave CUs idle; sequences of the
+        // few-row kernel have none.
+        const uint64_t groups = (rows / tile_rows + (p.few ? 1 : d.seqs)) * d.kv_heads;
+        p.tile_per = part_keys(groups, keys, groups < kTileFew ? kTileSplitMin : keys, kTileKeys, kTileTarget,
+                               &p.tile_split);
+        if (p.tile_split > 1) {
+            // whole columns for every XCD (see the kernel's order)
+            const uint32_t even = 8 / uint32_t(std::gcd(8u, d.kv_heads));
+            p.tile_split = (p.tile_split + even - 1) / even * even;
+        }
     }
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
@@ -1033,19 +1312,24 @@ uint64_t attend_workspace(const si_paged_attention_desc& d) { return attend_plan
 template <bool kBf16, int kDim>
 hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
 {
-    hipError_t e = hipSuccess;
-    if (p.few) {
-        const dim3 grid(a.seqs * a.kv_heads, p.few_split);
-        e = p.few_rows <= 16 ? launch(attend_few_kernel<kBf16, kDim, 1>, grid, dim3(64 * kFewWaves), stream, a)
-                             : launch(attend_few_kernel<kBf16, kDim, 2>, grid, dim3(64 * kFewWaves), stream, a);
+    const dim3 block(256);
+    const uint32_t tiles = p.tile ? p.tiles * a.kv_heads * p.tile_split : 0, few = p.few ? a.seqs * a.kv_heads : 0;
+    hipError_t e;
+    if (p.few && p.tile) {
+        const dim3 grid(tiles + few * p.few_split);
+        e = p.few_rows <= 16 ? launch(attend_mixed_kernel<kBf16, kDim, 1>, grid, block, stream, a)
+                             : launch(attend_mixed_kernel<kBf16, kDim, 2>, grid, block, stream, a);
+    } else if (p.few) {
+        const dim3 grid(few, p.few_split);
+        e = p.few_rows <= 16 ? launch(attend_few_kernel<kBf16, kDim, 1>, grid, block, stream, a)
+                             : launch(attend_few_kernel<kBf16, kDim, 2>, grid, block, stream, a);
+    } else {
+        e = launch(attend_tile_kernel<kBf16, kDim>, dim3(tiles), block, stream, a);
     }
-    if (e == hipSuccess && p.tile)
-        e = launch(attend_tile_kernel<kBf16, kDim>, dim3(p.tiles * a.kv_heads * p.tile_split), dim3(64 * kTileWaves),
-                   stream, a);
     if (e == hipSuccess && (p.few_split > 1 || p.tile_split > 1)) {
-        const uint32_t rows = a.tokens * a.q_heads;
-        e = rows <= kJoinWide ? launch(attend_join_kernel<kBf16, kDim, 4>, dim3(rows), dim3(256), stream, a)
-                              : launch(attend_join_kernel<kBf16, kDim, 1>, dim3((rows + 3) / 4), dim3(256), stream, a);
+        const uint32_t rows = a.tokens * a.q_heads, each = 256 / row_lanes<kDim>();
+        e = rows <= kJoinRows ? launch(attend_join_row_kernel<kBf16, kDim>, dim3(rows), block, stream, a)
+                              : launch(attend_join_kernel<kBf16, kDim>, dim3((rows + each - 1) / each), block, stream, a);
     }
     return e;
 }
