@@ -266,17 +266,17 @@ struct Keys {
     int32_t slot;
     uint64_t ok;    // bit j: key k0 + j
 
-    __device__ __forceinline__ void fetch(const AttendArgs& a, const int64_t* table, int32_t k0, int32_t lo, int32_t hi)
+    // (No bound but the row's: the sequence's length may still be on its way.)
+    __device__ __forceinline__ void fetch(const AttendArgs& a, const int64_t* table, int32_t k0)
+    {
+        const uint32_t page = (uint32_t(k0) + (threadIdx.x & (kKeys - 1))) >> a.page_shift;
+        entry = table[page < a.pages ? page : a.pages - 1];
+    }
+    __device__ __forceinline__ void resolve(const AttendArgs& a, int32_t k0, int32_t lo, int32_t hi)
     {
         const int32_t k = k0 + int32_t(threadIdx.x & (kKeys - 1));
-        entry = -1;
-        if (k >= lo && k < hi) entry = table[k >> a.page_shift];
-    }
-    __device__ __forceinline__ void resolve(const AttendArgs& a)
-    {
-        const bool h = held(entry, a.nslots);
         slot = int32_t(entry);
-        ok = __ballot(h);
+        ok = __ballot(held(entry, a.nslots) && k >= lo && k < hi);
         if constexpr (kKeys < 64) ok &= (1ull << kKeys) - 1ull;
     }
     // Byte offset of key k0 + j's row of KV head kvh in its cache (j: this
@@ -286,11 +286,6 @@ struct Keys {
         const uint32_t s = uint32_t(__shfl(slot, int(j)));
         return uint64_t(s) * a.slot_bytes +
                (uint64_t((uint32_t(k0) + j) & ((1u << a.page_shift) - 1u)) * a.kv_heads + kvh) * (a.dim * 2u);
-    }
-    // The one slot of a step that lies in one page (where any key is ok).
-    __device__ __forceinline__ uint32_t page_slot() const
-    {
-        return uint32_t(__builtin_amdgcn_readlane(slot, ok ? __builtin_ctzll(ok) : 0));
     }
 };
 
@@ -457,12 +452,17 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
     const uint32_t col = lane & 15u, quad = lane >> 4;
     if (a.q_starts && group == 0 && part == 0) zero_unowned<kBf16>(a);
     const uint32_t kvh = group % a.kv_heads, b = group / a.kv_heads;
+    const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
+    // Without a window the part's keys are known before the sequence's length:
+    // their pages are looked up while it is read.
+    Keys<kFewKeys> keys;
+    int32_t k0 = int32_t(part * a.few_per + wave * kFewKeys);
+    keys.fetch(a, table, k0);
     const Seq s = seq_of(a, b);
     const uint32_t rows = s.n_new * a.group;
     if (rows == 0 || rows > 16 * kBlocks) return;
     const Cut cut = cut_of(a, s, a.few_per);
     if (part > 0 && part >= cut.parts) return;
-    const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
 
     // Positions: row r is token r / group; the last row's token sees most.
     int32_t pos[kBlocks];
@@ -502,7 +502,6 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
 
     uint32_t marks = 0;  // of V that not every row sees
     u32x4 kr[2][kSteps], vr[kLoads];
-    Keys<kFewKeys> keys;
     const auto load_k = [&](int32_t k0) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
@@ -526,11 +525,13 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
             if ((keys.ok >> j & 1) && d < a.dim) vr[i] = *reinterpret_cast<const u32x4*>(a.cache_v + off + d * 2);
         }
     };
-    int32_t k0 = k_first + int32_t(wave * kFewKeys);
+    if (cut.lo > 0) {
+        k0 += cut.lo;
+        keys.fetch(a, table, k0);
+    }
     if (k0 < hi) {
-        keys.fetch(a, table, k0, lo, hi);
-        keys.resolve(a);
-        keys.fetch(a, table, k0 + int32_t(kFewStep), lo, hi);
+        keys.resolve(a, k0, lo, hi);
+        keys.fetch(a, table, k0 + int32_t(kFewStep));
         load_k(k0);
         load_v(k0);
     }
@@ -538,8 +539,8 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
         const uint64_t ok = keys.ok;
         const int32_t next = k0 + int32_t(kFewStep);
         if (next < hi) {
-            keys.resolve(a);
-            keys.fetch(a, table, next + int32_t(kFewStep), lo, hi);
+            keys.resolve(a, next, lo, hi);
+            keys.fetch(a, table, next + int32_t(kFewStep));
         }
         f32x4 st[kBlocks][2];
 #pragma unroll
@@ -1175,7 +1176,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
 // Few rows: a workgroup per (token, query head), its groups of row_lanes lanes
 // taking every so-many-th part each, summed in their order at the end.
 template <bool kBf16, int kDim>
-__global__ __launch_bounds__(256) void attend_join_row_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, 6) void attend_join_row_kernel(AttendArgs a)
 {
     constexpr uint32_t kLanes = row_lanes<kDim>(), kStride = 256 / kLanes, kMost = kMaxSplit / kStride;
     __shared__ f32x4 sums[4][64];
@@ -1187,12 +1188,14 @@ __global__ __launch_bounds__(256) void attend_join_row_kernel(AttendArgs a)
     float2 v{0.0f, 0.0f};
     if (lane < p.parts) v = p.ml[lane * p.step];
     const uint32_t which = threadIdx.x / kLanes, d = lane % kLanes * 4;
+    const uint64_t part_floats = p.step * a.dim;
+    const float* o = p.o + which * part_floats + d;
     f32x4 part[kMost];
 #pragma unroll
     for (uint32_t i = 0; i < kMost; ++i) {
-        const uint32_t n = which + i * kStride;
         part[i] = f32x4{0, 0, 0, 0};
-        if (n < p.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(p.o + n * p.step * a.dim + d);
+        if (which + i * kStride < p.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(o);
+        o += kStride * part_floats;
     }
     float top = v.y == 0.0f ? -INFINITY : v.x;
 #pragma unroll

@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes as ct
 import math
+from array import array
 
 import torch
 
@@ -280,25 +281,36 @@ def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causa
 
 # ------------------------------------------------------------------ pages
 
+class CacheSet:
+    """Caches of one shape, dtype, slot stride and device (every layer's K and V),
+    checked once: the page calls take it in the place of a list, which they
+    check on every call."""
+
+    def __init__(self, caches):
+        self.caches = list(caches)
+        self.geometry, addresses = _same_layout(self.caches)
+        self.addresses = (ct.c_void_p * len(addresses))(*addresses)
+
+
 def _same_layout(caches):
     """(device, dtype, slots, page tokens, heads, dim, slot stride) of caches
-    that share it, and their addresses.  (A set per property: a check of each tensor in
-    Python costs 1 us a tensor, which for 160 tensors is many times the copies.)"""
+    that share it, and their addresses (the library checks their alignment).
+    A property of all of them at a time: a check of each tensor in Python costs
+    1 us a tensor, which for 160 tensors is many times the copies."""
     if not caches:
         raise ValueError("no caches given")
     geometry = _paged_cache(caches[0], "a cache")
     T = torch.Tensor
     if len(caches) > 1:
-        if not all([isinstance(c, T) for c in caches]):
-            raise ValueError("a cache must be a device tensor")
-        if (len(set(map(T.size, caches))) > 1 or len({c.dtype for c in caches}) > 1
-                or len(set(map(T.get_device, caches))) > 1
-                or (len(set(map(T.stride, caches))) > 1 and any(_paged_cache(c, "a cache") != geometry for c in caches))):
+        try:
+            same = (len(set(map(T.size, caches))) == 1 and len(set(map(T.get_device, caches))) == 1
+                    and len({c.dtype for c in caches}) == 1)
+            dense = same and all(map(T.is_contiguous, caches))
+        except (TypeError, AttributeError) as e:
+            raise ValueError("a cache must be a device tensor") from e
+        if not same or (not dense and any([_paged_cache(c, "a cache") != geometry for c in caches])):
             raise ValueError("the caches must have one shape, dtype, slot stride and device")
-    addresses = list(map(T.data_ptr, caches))
-    if any([p & 15 for p in addresses]):
-        raise ValueError("a cache must start on a 16-byte boundary")
-    return geometry, addresses
+    return geometry, list(map(T.data_ptr, caches))
 
 
 def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, list_ndim, scrub, fail_count, out,
@@ -308,10 +320,16 @@ def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, 
     device = refs.get_device()
     _index(refs, "refs", 1, device, torch.int32)
     nslots = refs.shape[0]
-    addresses, slot_bytes, page_bytes = (), 0, 0
+    addresses, slot_bytes, page_bytes = None, 0, 0
     if caches is not None:
-        caches = list(caches)
-        (where, _, slots, page_tokens, heads, dim, step), addresses = _same_layout(caches)
+        if isinstance(caches, CacheSet):
+            geometry, addresses, caches = caches.geometry, caches.addresses, caches.caches
+        else:
+            caches = list(caches)
+            geometry, found = _same_layout(caches)
+            keep = array("Q", found)
+            addresses = (ct.c_void_p * len(found)).from_buffer(keep)
+        where, _, slots, page_tokens, heads, dim, step = geometry
         if where != device:
             raise ValueError("the caches must be on refs' device")
         if slots != nslots:
@@ -343,7 +361,7 @@ def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, 
             if o.shape != i.shape or o.dtype != i.dtype or o.get_device() != device or not o.is_contiguous():
                 raise ValueError("out must match the inputs in shape, dtype and device, and be contiguous")
     d = _lib.SiPagesDesc(
-        caches=(ct.c_void_p * max(1, len(addresses)))(*addresses), ncaches=len(addresses), page_tokens=page_tokens,
+        caches=addresses, ncaches=0 if addresses is None else len(addresses), page_tokens=page_tokens,
         slot_bytes=slot_bytes, page_bytes=page_bytes, nslots=nslots, tables=tables.data_ptr(), kv_lens=_ptr(kv_lens),
         refs=refs.data_ptr(), tables_out=out[0].data_ptr(), kv_lens_out=None if kv_lens is None else out[1].data_ptr(),
         refs_out=out[-1].data_ptr(), rows=rows, table_pages=pages, list=_ptr(rows_list),
@@ -360,7 +378,7 @@ def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, 
 def fork_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, pairs: torch.Tensor,
                fail_count: torch.Tensor | None = None, out=None, stream=None):
     """Each pair (parent row, child row) of ``pairs`` [n, 2] int64 makes the child
-    the parent's copy: whole pages are shared (refs + 1), a partly filled last page is
+    the parent's copy (``caches``: a list, or a CacheSet of it): whole pages are shared (refs + 1), a partly filled last page is
     copied in every tensor of ``caches`` into the lowest free slots, in the list's
     order.  A child must be an empty row named once; a pair that cannot be served (a
     row out of range, no free slot) leaves its child empty and is counted.
