@@ -632,7 +632,7 @@ typedef struct si_paged_attention_desc {
     const int64_t* kv_lens;
     const int64_t* q_starts;  /* seqs + 1, ascending; NULL: tokens == seqs     */
     uint32_t table_pages;     /* entries of a row; table_pages * page_tokens <= 2^30 */
-    uint32_t tokens;          /* rows of q: tokens * q_heads < 2^31            */
+    uint32_t tokens;          /* rows of q: tokens * q_heads < 2^26            */
     uint32_t seqs;
     uint32_t q_heads;         /* a multiple of kv_heads                        */
     uint32_t kv_heads;
@@ -672,7 +672,7 @@ typedef struct si_paged_append_desc {
     const int64_t* kv_lens;
     const int64_t* q_starts;
     uint32_t table_pages;
-    uint32_t tokens;
+    uint32_t tokens;          /* < 2^26                                        */
     uint32_t seqs;
     uint32_t kv_heads;
     uint32_t head_dim;        /* a multiple of 8                               */

@@ -62,15 +62,19 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr uint32_t kTileKeys = 64;
 constexpr uint32_t kTileWaves = 4;
 constexpr uint32_t kTileRows = 32 * kTileWaves;
-constexpr uint32_t kTileSplitMin = 256;
+constexpr uint32_t kTileSplitMin = 512;
 // The few-row kernel's keys per wave and step; a workgroup's step.
 constexpr uint32_t kFewKeys = 32;
 constexpr uint32_t kFewWaves = 4;
 constexpr uint32_t kFewStep = kFewKeys * kFewWaves;
+// Most rows of a sequence in the few-row kernel, one to a column of its matrix
+// instructions.  (Two columns blocks, for 32 rows: 32 sequences of 4 tokens x 8
+// heads over 4,096 keys 96 us, in tiles 64; 4 such sequences 22.5 and 22.8.)
+constexpr uint32_t kFewRows = 16;
 constexpr uint32_t kMaxSplit = 64;
 // Workgroups a launch is cut into, at the longest lengths the tables allow.
 constexpr uint64_t kFewTarget = 4096;
-constexpr uint64_t kTileTarget = 1280;
+constexpr uint64_t kTileTarget = 768;
 constexpr uint64_t kTileFew = 384;
 // Rows up to which a whole workgroup joins one row's parts.
 constexpr uint32_t kJoinRows = 2048;
@@ -135,15 +139,20 @@ __device__ __forceinline__ u32x4 read_lds(uint32_t at)
 // through registers.  Written as instructions because the compiler, which cannot tell the
 // two buffers apart, would wait for them at the next read of LDS; a wait_loads() and a
 // barrier stand before their data is read.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is named because it is written
 __device__ __forceinline__ void to_lds(const uint8_t* p, uint32_t to)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p)
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds(const uint8_t* base, uint32_t offset, uint32_t to)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
-                 : "memory");
+                 : "memory", "m0");
 }
+
+#pragma clang diagnostic pop
 
 // Everything this wave has asked memory for has arrived.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -419,7 +428,7 @@ __device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t,
 
 // ---------------------------------------------------------------- few rows
 
-// One workgroup per (sequence, KV head, part of the keys): at most 16 * kBlocks
+// One workgroup per (sequence, KV head, part of the keys): at most 16
 // rows.  Each wave takes every fourth step of 32 keys: K straight into the
 // registers of S^T = K Q^T, V through the wave's own LDS.  Memory bounds
 // it: the next step's K and V are in flight while a step is computed, with no
@@ -436,7 +445,7 @@ constexpr int few_lds_bytes()
     return int(kFewWaves) * (few_wave_bytes<kDim>() + 16 * 8 + 16);
 }
 
-template <bool kBf16, int kDim, int kBlocks>
+template <bool kBf16, int kDim>
 __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, uint32_t group, uint32_t part)
 {
     constexpr int kSteps = kDim / 32;       // contraction steps of K Q^T
@@ -460,26 +469,21 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
     keys.fetch(a, table, k0);
     const Seq s = seq_of(a, b);
     const uint32_t rows = s.n_new * a.group;
-    if (rows == 0 || rows > 16 * kBlocks) return;
+    if (rows == 0 || rows > kFewRows) return;
     const Cut cut = cut_of(a, s, a.few_per);
     if (part > 0 && part >= cut.parts) return;
 
     // Positions: row r is token r / group; the last row's token sees most.
-    int32_t pos[kBlocks];
-    u32x4 q[kBlocks][kSteps];
+    const uint32_t tok = col / a.group, h = kvh * a.group + (col - tok * a.group);
+    const int32_t pos = s.base + int32_t(tok);
+    u32x4 q[kSteps];
 #pragma unroll
-    for (int x = 0; x < kBlocks; ++x) {
-        const uint32_t r = 16 * x + col;
-        const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
-        pos[x] = s.base + int32_t(tok);
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const uint32_t d = 32 * k + 8 * quad;
-            u32x4 v{0, 0, 0, 0};
-            if (r < rows && d < a.dim)
-                v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
-            q[x][k] = v ^ (a.negate ? 0x80008000u : 0u);
-        }
+    for (int k = 0; k < kSteps; ++k) {
+        const uint32_t d = 32 * k + 8 * quad;
+        u32x4 v{0, 0, 0, 0};
+        if (col < rows && d < a.dim)
+            v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
+        q[k] = v ^ (a.negate ? 0x80008000u : 0u);
     }
     const int32_t p_last = s.base + int32_t(s.n_new) - 1;
     const int32_t hi0 = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
@@ -490,15 +494,10 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
 
     uint16_t* const vs = reinterpret_cast<uint16_t*>(lds + wave * kWaveBytes);
     const uint32_t vs_at = uint32_t(reinterpret_cast<uintptr_t>((lds_void*)lds)) + wave * kWaveBytes;
-    float m[kBlocks], l[kBlocks];
-    f32x4 o[kBlocks][kOut];
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[kOut];
 #pragma unroll
-    for (int x = 0; x < kBlocks; ++x) {
-        m[x] = -INFINITY;
-        l[x] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kOut; ++i) o[x][i] = f32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < kOut; ++i) o[i] = f32x4{0, 0, 0, 0};
 
     uint32_t marks = 0;  // of V that not every row sees
     u32x4 kr[2][kSteps], vr[kLoads];
@@ -542,15 +541,12 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
             keys.resolve(a, next, lo, hi);
             keys.fetch(a, table, next + int32_t(kFewStep));
         }
-        f32x4 st[kBlocks][2];
+        f32x4 st[2];
 #pragma unroll
-        for (int x = 0; x < kBlocks; ++x) {
+        for (int y = 0; y < 2; ++y) {
+            st[y] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                st[x][y] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) st[x][y] = mfma16<kBf16>(kr[y][k], q[x][k], st[x][y]);
-            }
+            for (int k = 0; k < kSteps; ++k) st[y] = mfma16<kBf16>(kr[y][k], q[k], st[y]);
         }
         if (next < hi) load_k(next);
 #pragma unroll
@@ -569,47 +565,41 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
         }
         if (next < hi) load_v(next);
 
-        u32x4 pw[kBlocks];
+        const uint32_t mine = uint32_t(partial ? seen_bits(a, ok, k0, pos) : ok) >> (4 * quad);
+        float top = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < kBlocks; ++x) {
-            const uint32_t mine = uint32_t(partial ? seen_bits(a, ok, k0, pos[x]) : ok) >> (4 * quad);
-            float top = -INFINITY;
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+            for (int i = 0; i < 4; ++i) {
+                if (!(mine >> (16 * y + i) & 1)) st[y][i] = -INFINITY;
+                top = fmaxf(top, st[y][i]);
+            }
+        top = across<true>(top, fmax2);
+        const float mn = fmaxf(m, top);
+        const float safe = mn == -INFINITY ? 0.0f : mn;
+        const float keep = __builtin_amdgcn_exp2f((m - safe) * a.scale_log2);
+        const float shift = safe * a.scale_log2;
+        m = mn;
+        f32x8 w;
+        float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!(mine >> (16 * y + i) & 1)) st[x][y][i] = -INFINITY;
-                    top = fmaxf(top, st[x][y][i]);
-                }
-            top = across<true>(top, fmax2);
-            const float mn = fmaxf(m[x], top);
-            const float safe = mn == -INFINITY ? 0.0f : mn;
-            const float keep = __builtin_amdgcn_exp2f((m[x] - safe) * a.scale_log2);
-            const float shift = safe * a.scale_log2;
-            m[x] = mn;
-            f32x8 w;
-            float sum = 0.0f;
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+            for (int i = 0; i < 4; ++i) {
+                w[4 * y + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][i], a.scale_log2, -shift));
+                sum += w[4 * y + i];
+            }
+        l = __builtin_fmaf(l, keep, sum);
+        const u32x4 pw = pack8<kBf16>(w);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[4 * y + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][y][i], a.scale_log2, -shift));
-                    sum += w[4 * y + i];
-                }
-            l[x] = __builtin_fmaf(l[x], keep, sum);
-            pw[x] = pack8<kBf16>(w);
-#pragma unroll
-            for (int i = 0; i < kOut; ++i) o[x][i] *= keep;
-        }
+        for (int i = 0; i < kOut; ++i) o[i] *= keep;
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < kOut; ++i) {
             // keys 4 quad + 0..3 and 16 + 4 quad + 0..3 of 16 columns
             const uint32_t v = vs_at + 2 * ((4 * quad + (col >> 2)) * kPitch + 16 * i + 4 * (col & 3u));
             const u32x2 v0 = read_tr(v), v1 = read_tr(v + 32 * kPitch);
-            const u32x4 vt{v0[0], v0[1], v1[0], v1[1]};
-#pragma unroll
-            for (int x = 0; x < kBlocks; ++x) o[x][i] = mfma16<kBf16>(vt, pw[x], o[x][i]);
+            o[i] = mfma16<kBf16>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pw, o[i]);
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -628,43 +618,37 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
         }
         return;
     }
-    // Join the waves, 16 rows at a time.
+    // Join the waves.
+    __syncthreads();
+    l = across<true>(l, fadd2);
+    if (quad == 0) ml[wave][col] = float2{m, l};
+    float* const ow = reinterpret_cast<float*>(lds + wave * kWaveBytes);
 #pragma unroll
-    for (int x = 0; x < kBlocks; ++x) {
-        if (16 * x >= int(rows)) break;
-        __syncthreads();
-        const float lw = across<true>(l[x], fadd2);
-        if (quad == 0) ml[wave][col] = float2{m[x], lw};
-        float* ow = reinterpret_cast<float*>(lds + wave * kWaveBytes);
+    for (int i = 0; i < kOut; ++i) *reinterpret_cast<f32x4*>(ow + col * kOPitch + 16 * i + 4 * quad) = o[i];
+    __syncthreads();
+    const uint32_t quads = a.dim / 4;
+    for (uint32_t e = threadIdx.x; e < rows * quads; e += 64 * kFewWaves) {
+        const uint32_t r = e / quads, d = (e - r * quads) * 4;
+        float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kOut; ++i)
-            *reinterpret_cast<f32x4*>(ow + col * kOPitch + 16 * i + 4 * quad) = o[x][i];
-        __syncthreads();
-        const uint32_t quads = a.dim / 4;
-        for (uint32_t e = threadIdx.x; e < 16 * quads; e += 64 * kFewWaves) {
-            const uint32_t rr = e / quads, d = (e - rr * quads) * 4, r = 16 * x + rr;
-            if (r >= rows) break;
-            float top = -INFINITY;
+        for (int w = 0; w < int(kFewWaves); ++w) top = fmaxf(top, ml[w][r].x);
+        const float safe = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        f32x4 acc{0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < int(kFewWaves); ++w) top = fmaxf(top, ml[w][rr].x);
-            const float safe = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
-            f32x4 acc{0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < int(kFewWaves); ++w) {
-                const float2 v = ml[w][rr];
-                const float f = __builtin_amdgcn_exp2f((v.x - safe) * a.scale_log2);
-                sum = __builtin_fmaf(v.y, f, sum);
-                acc += *reinterpret_cast<const f32x4*>(lds + w * kWaveBytes + (rr * kOPitch + d) * 4) * f;
-            }
-            const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group), t = s.q0 + tok;
-            if (cut.parts > 1) {
-                const uint64_t row = (uint64_t(part) * a.seqs * a.kv_heads + uint64_t(b) * a.kv_heads + kvh) * a.few_rows + r;
-                *reinterpret_cast<f32x4*>(a.few_o + row * a.dim + d) = acc;
-                if (d == 0) a.few_ml[row] = float2{safe * a.scale_log2, sum};
-            } else {
-                store_out<kBf16>(a, t, h, d, acc, sum, safe * a.scale_log2);
-            }
+        for (int w = 0; w < int(kFewWaves); ++w) {
+            const float2 v = ml[w][r];
+            const float f = __builtin_amdgcn_exp2f((v.x - safe) * a.scale_log2);
+            sum = __builtin_fmaf(v.y, f, sum);
+            acc += *reinterpret_cast<const f32x4*>(lds + w * kWaveBytes + (r * kOPitch + d) * 4) * f;
+        }
+        const uint32_t rt = r / a.group, rh = kvh * a.group + (r - rt * a.group);
+        if (cut.parts > 1) {
+            const uint64_t row = (uint64_t(part) * a.seqs * a.kv_heads + uint64_t(b) * a.kv_heads + kvh) * a.few_rows + r;
+            *reinterpret_cast<f32x4*>(a.few_o + row * a.dim + d) = acc;
+            if (d == 0) a.few_ml[row] = float2{safe * a.scale_log2, sum};
+        } else {
+            store_out<kBf16>(a, s.q0 + rt, rh, d, acc, sum, safe * a.scale_log2);
         }
     }
 }
@@ -1037,11 +1021,11 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
 
 // ---------------------------------------------------------------- kernels
 
-template <bool kBf16, int kDim, int kBlocks>
+template <bool kBf16, int kDim>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_few_kernel(AttendArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds_bytes<kDim>()];
-    attend_few<kBf16, kDim, kBlocks>(a, lds, blockIdx.x, blockIdx.y);
+    attend_few<kBf16, kDim>(a, lds, blockIdx.x, blockIdx.y);
 }
 
 template <bool kBf16, int kDim>
@@ -1053,7 +1037,7 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim > 64 ? 2 : 3) void atten
 
 // Both kinds of sequences in one launch: the tiles' workgroups first, which take
 // longest, and the few-row ones beside and after them.
-template <bool kBf16, int kDim, int kBlocks>
+template <bool kBf16, int kDim>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(AttendArgs a)
 {
     constexpr int kBytes = tile_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? tile_lds_bytes<kDim>() : few_lds_bytes<kDim>();
@@ -1063,7 +1047,7 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(A
         attend_tile<kBf16, kDim>(a, lds, blockIdx.x, tiles);
     } else {
         const uint32_t x = blockIdx.x - tiles, groups = a.seqs * a.kv_heads;
-        attend_few<kBf16, kDim, kBlocks>(a, lds, x % groups, x / groups);
+        attend_few<kBf16, kDim>(a, lds, x % groups, x / groups);
     }
 }
 
@@ -1229,7 +1213,7 @@ bool attend_ok(const si_paged_attention_desc& d)
     if (!d.q || !d.out || !d.cache_k || !d.cache_v || !d.tables || !d.kv_lens) return false;
     if (!d.tokens || !d.seqs || !d.q_heads || !d.kv_heads || d.q_heads % d.kv_heads || !d.table_pages) return false;
     if (!d.q_starts && d.tokens != d.seqs) return false;
-    if (uint64_t(d.tokens) * d.q_heads >= (1ull << 31) || d.seqs >= (1u << 31)) return false;
+    if (uint64_t(d.tokens) * d.q_heads >= (1ull << 26) || d.seqs >= (1u << 26)) return false;
     if (!d.head_dim || d.head_dim % 8 || d.head_dim > 256 || d.dtype > SI_DTYPE_FP16) return false;
     if (d.page_tokens < 8 || d.page_tokens > 32768 || (d.page_tokens & (d.page_tokens - 1))) return false;
     if (uint64_t(d.table_pages) * d.page_tokens > (1ull << 30)) return false;
@@ -1248,7 +1232,7 @@ bool attend_ok(const si_paged_attention_desc& d)
 // it is shorter.
 struct Plan {
     uint32_t few_rows = 0, few_per = 0, few_split = 1, tile_per = 0, tile_split = 1, tiles = 0;
-    bool few = false, tile = false;
+    bool few = false, tile = false, fits = true;
     uint64_t few_o = 0, few_ml = 0, tile_o = 0, tile_ml = 0, bytes = 0;
 };
 
@@ -1272,8 +1256,8 @@ Plan attend_plan(const si_paged_attention_desc& d)
     const uint64_t rows = d.tokens * group;
     // One token each: one kernel.  Any mix of lengths: both, unless no
     // sequence can be long or the only one is.
-    p.few = group <= 32 && (!d.q_starts || d.seqs > 1 || rows <= 32);
-    if (p.few) p.few_rows = group <= 16 ? 16 : 32;
+    p.few = group <= kFewRows && (!d.q_starts || d.seqs > 1 || rows <= kFewRows);
+    if (p.few) p.few_rows = kFewRows;
     p.tile = d.q_starts ? rows > p.few_rows : !p.few;
     const uint64_t pairs = uint64_t(d.seqs) * d.kv_heads;
     if (p.few) p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &p.few_split);
@@ -1292,6 +1276,10 @@ Plan attend_plan(const si_paged_attention_desc& d)
             p.tile_split = (p.tile_split + even - 1) / even * even;
         }
     }
+    // (threads of a launch dimension fit 32 bits)
+    const uint64_t most = (1ull << 32) / 256 - 1;
+    const uint64_t few_groups = p.few ? pairs * p.few_split : 0, tile_groups = uint64_t(p.tiles) * d.kv_heads * p.tile_split;
+    p.fits = few_groups + tile_groups <= most;
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
@@ -1310,8 +1298,6 @@ Plan attend_plan(const si_paged_attention_desc& d)
     return p;
 }
 
-uint64_t attend_workspace(const si_paged_attention_desc& d) { return attend_plan(d).bytes; }
-
 template <bool kBf16, int kDim>
 hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
 {
@@ -1320,12 +1306,10 @@ hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
     hipError_t e;
     if (p.few && p.tile) {
         const dim3 grid(tiles + few * p.few_split);
-        e = p.few_rows <= 16 ? launch(attend_mixed_kernel<kBf16, kDim, 1>, grid, block, stream, a)
-                             : launch(attend_mixed_kernel<kBf16, kDim, 2>, grid, block, stream, a);
+        e = launch(attend_mixed_kernel<kBf16, kDim>, grid, block, stream, a);
     } else if (p.few) {
         const dim3 grid(few, p.few_split);
-        e = p.few_rows <= 16 ? launch(attend_few_kernel<kBf16, kDim, 1>, grid, block, stream, a)
-                             : launch(attend_few_kernel<kBf16, kDim, 2>, grid, block, stream, a);
+        e = launch(attend_few_kernel<kBf16, kDim>, grid, block, stream, a);
     } else {
         e = launch(attend_tile_kernel<kBf16, kDim>, dim3(tiles), block, stream, a);
     }
@@ -1354,7 +1338,9 @@ extern "C" {
 
 uint64_t secure_infer_gpu_paged_attention_workspace(const si_paged_attention_desc* d)
 {
-    return d && si::attend_ok(*d) ? si::attend_workspace(*d) : UINT64_MAX;
+    if (!d || !si::attend_ok(*d)) return UINT64_MAX;
+    const si::Plan p = si::attend_plan(*d);
+    return p.fits ? p.bytes : UINT64_MAX;
 }
 
 int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attention_desc* d)
@@ -1362,6 +1348,7 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     using namespace si;
     if (!d || !attend_ok(*d)) return -1;
     const Plan p = attend_plan(*d);
+    if (!p.fits) return -1;
     if (p.bytes && (!d->workspace || d->workspace_bytes < p.bytes || !aligned(d->workspace, 16))) return -1;
     AttendArgs a{};
     a.q = static_cast<const uint16_t*>(d->q);
@@ -1387,7 +1374,7 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     a.dim = d->head_dim;
     a.page_shift = uint32_t(__builtin_ctz(d->page_tokens));
     a.causal = d->causal;
-    a.window = d->window;
+    a.window = d->window < (1u << 30) ? d->window : 0;  // no table is longer
     a.group = d->q_heads / d->kv_heads;
     a.negate = d->scale < 0.0f;
     // A scale of 0 (every seen key weighs the same) stays positive, so that a

@@ -586,7 +586,7 @@ int secure_infer_gpu_paged_append(hipStream_t stream, const si_paged_append_desc
 {
     using namespace si;
     if (!d || !d->k || !d->v || !d->cache_k || !d->cache_v || !d->tables || !d->kv_lens) return -1;
-    if (!d->tokens || d->tokens >= (1u << 31) || !d->seqs || !d->kv_heads || !d->head_dim || d->head_dim % 8 || !d->nslots ||
+    if (!d->tokens || d->tokens >= (1u << 26) || !d->seqs || !d->kv_heads || !d->head_dim || d->head_dim % 8 || !d->nslots ||
         d->nslots >= (1ull << 31) || !d->table_pages)
         return -1;
     if (!d->q_starts && d->tokens != d->seqs) return -1;

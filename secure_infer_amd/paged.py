@@ -39,6 +39,8 @@ def _ptr(t):
 def _stream_of(stream, device: int):
     """(raw handle, the torch stream if it is not the device's current one) of
     a call's stream: a torch stream, a raw handle, or None for the current."""
+    if torch.cuda.current_device() != device:
+        raise ValueError(f"the tensors are on cuda:{device}, which is not the current device")
     current = torch._C._cuda_getCurrentRawStream(device)
     if stream is None:
         return current, None
@@ -248,7 +250,7 @@ def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causa
         raise ValueError(f"q must be [tokens, query heads, {dim}] with a multiple of {heads} query heads")
     q_heads = q.shape[1]
     tokens, qt, qh = _rows(q, "q", q_heads, dim, dtype, device)
-    if tokens * q_heads >= 1 << 31:
+    if tokens * q_heads >= 1 << 26:
         raise ValueError("q has too many rows")
     seqs, pages, row = _sequences(tables, kv_lens, q_starts, tokens, ps, device)
     scale = dim ** -0.5 if scale is None else float(scale)
