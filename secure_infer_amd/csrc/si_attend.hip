@@ -118,7 +118,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
 }
 
 // Eight floats rounded to nearest even: the weights' one rounding, to the
-// type the matrix instruction takes (relative 2^-9 / 2^-12 a weight; the sum
+// type the matrix instruction takes (relative 2^-8 / 2^-11 a weight; the sum
 // they are divided by is that of the unrounded ones, in float).
 template <bool kBf16>
 __device__ __forceinline__ u32x4 pack8(f32x8 x)
@@ -1279,7 +1279,7 @@ Plan attend_plan(const si_paged_attention_desc& d)
     // (threads of a launch dimension fit 32 bits)
     const uint64_t most = (1ull << 32) / 256 - 1;
     const uint64_t few_groups = p.few ? pairs * p.few_split : 0, tile_groups = uint64_t(p.tiles) * d.kv_heads * p.tile_split;
-    p.fits = few_groups + tile_groups <= most;
+    p.fits = few_groups + tile_groups <= most && uint64_t(d.tokens) * d.q_heads / 4 < most;
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
