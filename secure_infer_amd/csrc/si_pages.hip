@@ -309,7 +309,8 @@ __device__ void plan_reserve(const PagesArgs& a, uint32_t* part)
             bad += !served;
             a.ws.row[b] = served && need > 0 ? int32_t(first) : -1;
             const int64_t add = a.list[b];
-            a.kv_lens_out[b] = a.kv_lens[b] + (add > 0 ? add : 0);
+            const int64_t had = a.kv_lens[b], room = had > 0 ? INT64_MAX - had : INT64_MAX;
+            a.kv_lens_out[b] = had + (add < 0 ? 0 : add > room ? room : add);
         }
     }
     fail(a, bad);

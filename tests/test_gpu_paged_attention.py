@@ -365,3 +365,23 @@ def test_append_counts_what_it_drops():
     # position 79 of sequence 2 lies on the table's last page, which it does not hold
     assert torch.equal(d["ck"].cpu(), want)
     assert int(fail) == 100 + 2 + 5 + 2
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 70]])
+def test_lengths_and_windows_past_the_table(new):
+    """Lengths beyond the table's pages end there, negative ones are empty, and a
+    window longer than any sequence is none."""
+    x = make(71, [256, 128, 192], new, 4, 2, 64, 64, torch.bfloat16, width=4)
+    x["tables"] = x["tables"][:, :4]
+    x["kv"][0] = (1 << 63) - 1
+    x["kv"][1] = -(1 << 63)
+    check(x)
+    out, lse = attend(x, lse=True)
+    for window in (1 << 20, (1 << 30) + 5, (1 << 31) - 1):
+        far = attend(x, lse=True, window=window)
+        assert torch.equal(far[0], out) and torch.equal(far[1], lse)
+
+
+@pytest.mark.parametrize("hq,hkv,new", [(40, 1, [33, 0, 2, 1]), (260, 2, [1, 3, 1, 1]), (17, 1, [1, 1, 1, 1])])
+def test_groups_wider_than_a_tile_of_columns(hq, hkv, new):
+    check(make(73 + hq, [300, 0, 65, 700], new, hq, hkv, 64, 32, torch.bfloat16))

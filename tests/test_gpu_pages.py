@@ -329,3 +329,39 @@ def test_on_another_stream_and_in_a_graph():
         want = py_free(x, [1 + shift, 4], True)
         same(got, want[:3])
         same_caches(caches, want[3])
+
+
+def test_a_cache_set_is_its_list():
+    x = make(35, 64, 12, 5, tensors=6)
+    rows = torch.tensor([1, 4, 7], device=DEV)
+    caches, *state = on_device(x)
+    kept = si.CacheSet(caches)
+    freed = si.free_pages(kept, *state, rows)
+    want = py_free(x, [1, 4, 7], True)
+    same(freed, want[:3])
+    same_caches(caches, want[3])
+    moved = si.compact_pages(kept, freed[0], freed[2])
+    again = [c.to(DEV) for c in x["caches"]]
+    freed2 = si.free_pages(again, *state, rows)
+    moved2 = si.compact_pages(again, freed2[0], freed2[2])
+    same(moved, [t.tolist() for t in moved2])
+    same_caches(caches, [c.cpu() for c in again])
+    for bad, what in (([], "no caches"), ([caches[0], caches[1].half()], "one shape"),
+                      ([caches[0], caches[1][:5]], "one shape"), ([caches[0].cpu()], "device tensor")):
+        with pytest.raises(ValueError, match=what):
+            si.CacheSet(bad)
+    with pytest.raises(ValueError, match="one entry per slot"):
+        si.compact_pages(kept, state[0], state[2][:-1])
+
+
+def test_reserve_bounds_its_lengths():
+    x = make(36, 40, 5, 4, held=0.3)
+    top = (1 << 63) - 1
+    counts = [top, 1 << 62, 3, -top, 0]
+    want = py_reserve(x, counts)
+    lens = [min(n, top) for n in want[1]]
+    _, *state = on_device(x)
+    fail = counter()
+    got = si.reserve_pages(*state, torch.tensor(counts, device=DEV), x["ps"], fail_count=fail)
+    same(got, (want[0], lens, want[2]))
+    assert int(fail) == want[3] >= 2
