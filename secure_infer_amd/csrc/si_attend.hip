@@ -1,4 +1,6 @@
-// Attention of new tokens over a paged KV cache.
+// Attention of new tokens over a paged KV cache:
+//   out = sum_j w_j V_j / sum_j w_j,  w_j = exp(scale q.K_j - m),  m >= max_j scale q.K_j
+// over the keys j a token sees, in one pass with a running m and sum, in float.
 //
 // Both kernels compute the transposed scores S^T = K Q^T with matrix
 // instructions, so a query is a column: a lane holds one query's scores of
@@ -8,6 +10,13 @@
 // come in the same order).  V^T comes out of LDS through transposing reads.
 // The rows of one KV head are (token, query head) pairs of its group, so K and V
 // are read once for all heads that share them.
+//
+// A sequence of at most 16 rows (a decoding step) is bound by the bytes of its K
+// and V and runs in the few-row kernel; longer ones are bound by the matrix
+// and vector instructions and run in tiles of 128 rows.  Keys are cut into parts where
+// there are too few rows for the chip, and the parts joined by a second launch (the join by the
+// workgroup that ends last was tried: its fences, which write back and drop
+// whole L2s, cost one token 38 us, stores past the L2 16.9, the launch 8 + 4).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -40,10 +49,11 @@ struct AttendArgs {
     float scale_log2;  // |scale| * log2(e): weights are powers of two
     // Sequences of at most few_rows rows (tokens * group) belong to the few-row
     // kernel, the others to the tile kernel.
-    uint32_t few_rows, few_per, tile_per, tile_split, tiles;
+    uint32_t few_rows, few_groups, few_least, few_per, tile_per, tile_split, tiles;
     // Parts of split sequences: numerators (dim floats a row) and (m, l).
     float* few_o;
     float2* few_ml;
+    uint2* few_parts;  // of each sequence and KV head: place of its first part, number of parts
     float* tile_o;
     float2* tile_ml;
 };
@@ -58,11 +68,14 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// The tile kernel's keys per step, and the fewest keys a split is made for.
+// The tile kernel's keys per step, and its rows: 32 a wave, whose scores of a step, numerators and
+// queries fill the registers that two waves a SIMD leave each other at head dim 128.  (64 rows a
+// wave, one wave a SIMD: 2,984 us where 32 rows take 2,430: the accumulators
+// move between the two halves of the registers.  8 waves on rings of 2 to 4
+// buffers: 2,385 and 2,400.)
 constexpr uint32_t kTileKeys = 64;
 constexpr uint32_t kTileWaves = 4;
 constexpr uint32_t kTileRows = 32 * kTileWaves;
-constexpr uint32_t kTileSplitMin = 512;
 // The few-row kernel's keys per wave and step; a workgroup's step.
 constexpr uint32_t kFewKeys = 32;
 constexpr uint32_t kFewWaves = 4;
@@ -72,11 +85,21 @@ constexpr uint32_t kFewStep = kFewKeys * kFewWaves;
 // heads over 4,096 keys 96 us, in tiles 64; 4 such sequences 22.5 and 22.8.)
 constexpr uint32_t kFewRows = 16;
 constexpr uint32_t kMaxSplit = 64;
-// Workgroups a launch is cut into, at the longest lengths the tables allow.
+// Workgroups that parts of a fixed length are made for, at the longest lengths the tables
+// allow.  Few-row parts, 64 ragged sequences to 8,192 keys of 4 heads: 4,096 62.2 us, 2,048
+// 64.4, 8,192 64.5.
 constexpr uint64_t kFewTarget = 4096;
+// Tiles are cut where there are fewer than kTileFew, into parts of at least kTileSplitMin keys.
+// Target and least 768 and 512, against 1,280 and 256, and 2,048 and 512: a chunk of 128 tokens over 8,192
+// keys, 32/8 heads, 43.7 us, 56, 55; 512 tokens over 32,768, 8/1 heads, 127, 131, 140.
+// 2,048 tokens over 8,192 keys, 32/8 heads (more than kTileFew): uncut 317, in 2 parts 393.
 constexpr uint64_t kTileTarget = 768;
 constexpr uint64_t kTileFew = 384;
-// Rows up to which a whole workgroup joins one row's parts.
+constexpr uint64_t kTileSplitMin = 512;
+// Rows up to which a whole workgroup joins one row's parts, all at once; above, groups of lanes
+// join a row each, the parts one after another.  Only the first: 27 sequences of 2,105 tokens x 12
+// heads 72 us in all, only the second 52; one token x 32 heads 20.0 and 20.3, 64 x 28 63.6
+// and 64.3.
 constexpr uint32_t kJoinRows = 2048;
 
 __device__ __forceinline__ bool held(int64_t e, int64_t nslots) { return e >= 0 && e < nslots; }
@@ -250,6 +273,59 @@ __device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Seq& s, uint32_
     c.parts = (span + per - 1) / per;
     return c;
 }
+
+// Sequences of at most this many units a KV head are left to the workgroup of
+// their first unit.
+constexpr uint32_t kFewWhole = kFewStep / kFewKeys;
+// Sums of x over the lanes up to and with this one.
+__device__ __forceinline__ uint32_t sums_up_to(uint32_t x)
+{
+    const auto add = [&](uint32_t y) { x += y; };
+    add(uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xf, 0xf, false)));  // lane - 1, of 16
+    add(uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xf, 0xf, false)));
+    add(uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xf, 0xf, false)));
+    add(uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xf, 0xf, false)));
+    add(uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xa, 0xf, false)));  // the last lane of the 16 before
+    add(uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xc, 0xf, false)));  // lane 31, to the upper half
+    return x;
+}
+
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
+{
+    return (a | b) >> 32 ? a / b : uint32_t(a) / uint32_t(b);
+}
+
+// Units of 32 keys of a KV head of a sequence for the few-row kernel.  (A
+// sequence without keys has outputs all the same: one.)
+__device__ __forceinline__ uint32_t few_units(const AttendArgs& a, const Seq& s)
+{
+    const uint32_t rows = s.n_new * a.group;
+    if (rows == 0 || rows > a.few_rows) return 0;
+    const uint32_t n = cut_of(a, s, kFewKeys).parts;
+    return n ? n : 1;
+}
+
+// Up to 64 sequences, one a lane: their units one sequence after another, each KV
+// head of it after the other.  Every workgroup takes `per` consecutive
+// ones, wherever sequences begin and end.
+struct Few {
+    uint32_t units, with;  // of a KV head; their sum up to and with the lane's (at most 64 * 2^25)
+    uint64_t total, per;
+
+    __device__ __forceinline__ void start(const AttendArgs& a)
+    {
+        const uint32_t b = threadIdx.x & 63u;
+        units = b < a.seqs ? few_units(a, seq_of(a, b)) : 0;
+        with = sums_up_to(units);
+        total = upto(a, 63);
+        const uint64_t even = quotient(total + a.few_groups - 1, a.few_groups);
+        per = even > a.few_least ? even : a.few_least;
+    }
+    __device__ __forceinline__ uint64_t upto(const AttendArgs& a, int x) const  // x: the same in every lane
+    {
+        return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(with), x))) * a.kv_heads;
+    }
+};
 
 // Rows of q before the first sequence and after the last: nothing to see.
 template <bool kBf16>
@@ -428,11 +504,21 @@ __device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t,
 
 // ---------------------------------------------------------------- few rows
 
-// One workgroup per (sequence, KV head, part of the keys): at most 16
-// rows.  Each wave takes every fourth step of 32 keys: K straight into the
-// registers of S^T = K Q^T, V through the wave's own LDS.  Memory bounds
-// it: the next step's K and V are in flight while a step is computed, with no
-// barrier until the waves' results are joined at the end.
+// A workgroup's work is a run of 32-key units of a (sequence, KV head): each wave
+// takes every fourth unit, K straight into the registers of S^T = K Q^T, V
+// through the wave's own LDS.  Memory bounds it: the next unit's K and V are in
+// flight while one is computed, with no barrier until the waves' results are
+// joined at the end.
+//
+// Up to 64 sequences whose (sequence, KV head) pairs number at most the workgroups that run at
+// a time are shared out evenly: each of those takes the same number of
+// consecutive units of the whole batch, wherever sequences begin and end.  More pairs fill
+// the chip by themselves and get parts of one length, a workgroup each.  64 sequences of 130
+// to 8,192 keys, 28/4 heads of 128 (261 MB), inputs in the caches and not: shared evenly 55
+// and 67 us, parts of one length 68 and 81; 64 of 8,192 keys (1.07 GB) 197 us, 5.5 TB/s, and 218;
+// 32 sequences of heads of 256 68 and 118.  But 1,000 sequences of 20 to 300 keys
+// 99 to 121 us and 59 (several short sequences one after another in a workgroup).
+// K through LDS as well took 61.4 us where this way took 62.2, for twice the LDS.
 template <int kDim>
 constexpr int few_wave_bytes()
 {
@@ -445,8 +531,11 @@ constexpr int few_lds_bytes()
     return int(kFewWaves) * (few_wave_bytes<kDim>() + 16 * 8 + 16);
 }
 
+// Units [first, first + n) of KV head kvh of a sequence whose keys start at `lo0`; not
+// `whole`: into part `slot`.
 template <bool kBf16, int kDim>
-__device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, uint32_t group, uint32_t part)
+__device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, const Seq& s, uint32_t kvh, int32_t lo0,
+                                           uint32_t first, uint32_t n, bool whole, uint32_t slot)
 {
     constexpr int kSteps = kDim / 32;       // contraction steps of K Q^T
     constexpr int kOut = kDim / 16;         // 16-wide blocks of the output
@@ -459,19 +548,12 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
     uint32_t* const odd = reinterpret_cast<uint32_t*>(lds + kFewWaves * (kWaveBytes + 16 * 8));
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = lane & 15u, quad = lane >> 4;
-    if (a.q_starts && group == 0 && part == 0) zero_unowned<kBf16>(a);
-    const uint32_t kvh = group % a.kv_heads, b = group / a.kv_heads;
-    const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
-    // Without a window the part's keys are known before the sequence's length:
-    // their pages are looked up while it is read.
+    const int64_t* table = a.tables + uint64_t(s.b) * a.table_stride;
+    const int32_t k_first = lo0 + int32_t(first * kFewKeys);
     Keys<kFewKeys> keys;
-    int32_t k0 = int32_t(part * a.few_per + wave * kFewKeys);
+    int32_t k0 = k_first + int32_t(wave * kFewKeys);
     keys.fetch(a, table, k0);
-    const Seq s = seq_of(a, b);
     const uint32_t rows = s.n_new * a.group;
-    if (rows == 0 || rows > kFewRows) return;
-    const Cut cut = cut_of(a, s, a.few_per);
-    if (part > 0 && part >= cut.parts) return;
 
     // Positions: row r is token r / group; the last row's token sees most.
     const uint32_t tok = col / a.group, h = kvh * a.group + (col - tok * a.group);
@@ -487,8 +569,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
     }
     const int32_t p_last = s.base + int32_t(s.n_new) - 1;
     const int32_t hi0 = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
-    const int32_t k_first = cut.lo + int32_t(part * a.few_per);
-    const int32_t hi = hi0 < k_first + int32_t(a.few_per) ? hi0 : k_first + int32_t(a.few_per);
+    const int32_t hi = hi0 < k_first + int32_t(n * kFewKeys) ? hi0 : k_first + int32_t(n * kFewKeys);
     // keys below lo are behind every row's window
     const int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
 
@@ -524,10 +605,6 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
             if ((keys.ok >> j & 1) && d < a.dim) vr[i] = *reinterpret_cast<const u32x4*>(a.cache_v + off + d * 2);
         }
     };
-    if (cut.lo > 0) {
-        k0 += cut.lo;
-        keys.fetch(a, table, k0);
-    }
     if (k0 < hi) {
         keys.resolve(a, k0, lo, hi);
         keys.fetch(a, table, k0 + int32_t(kFewStep));
@@ -612,9 +689,9 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
     if (s.n_new > 1 && (odd[0] | odd[1] | odd[2] | odd[3])) {
         for (uint32_t x = wave; x < rows; x += kFewWaves) {
             const uint32_t xt = x / a.group, xh = kvh * a.group + (x - xt * a.group);
-            const uint64_t row = (uint64_t(part) * a.seqs * a.kv_heads + uint64_t(b) * a.kv_heads + kvh) * a.few_rows + x;
-            plain_row<kBf16>(a, table, s.q0 + xt, xh, kvh, s.base + int32_t(xt), k_first, hi,
-                             cut.parts > 1, a.few_o + row * a.dim, a.few_ml + row);
+            const uint64_t row = uint64_t(slot) * kFewRows + x;
+            plain_row<kBf16>(a, table, s.q0 + xt, xh, kvh, s.base + int32_t(xt), k_first, hi, !whole,
+                             a.few_o + row * a.dim, a.few_ml + row);
         }
         return;
     }
@@ -643,13 +720,63 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
             acc += *reinterpret_cast<const f32x4*>(lds + w * kWaveBytes + (r * kOPitch + d) * 4) * f;
         }
         const uint32_t rt = r / a.group, rh = kvh * a.group + (r - rt * a.group);
-        if (cut.parts > 1) {
-            const uint64_t row = (uint64_t(part) * a.seqs * a.kv_heads + uint64_t(b) * a.kv_heads + kvh) * a.few_rows + r;
+        if (!whole) {
+            const uint64_t row = uint64_t(slot) * kFewRows + r;
             *reinterpret_cast<f32x4*>(a.few_o + row * a.dim + d) = acc;
             if (d == 0) a.few_ml[row] = float2{safe * a.scale_log2, sum};
         } else {
             store_out<kBf16>(a, s.q0 + rt, rh, d, acc, sum, safe * a.scale_log2);
         }
+    }
+}
+
+// Workgroup `group`'s work (see above).  With few_per it is a part of few_per units of one
+// sequence and KV head, in place `group`; without, consecutive units of all of them:
+// where a part begins in an earlier workgroup it is in this one's place
+// 2 group, where it goes on in the next in place 2 group + 1.
+template <bool kBf16, int kDim>
+__device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* lds, uint32_t group)
+{
+    if (a.q_starts && group == 0) zero_unowned<kBf16>(a);
+    Few w;
+    uint64_t at = 0, to = 1, per = a.few_per;
+    if (!per) {
+        w.start(a);
+        per = w.per;
+        at = group * per;
+        to = at + per < w.total ? at + per : w.total;
+    }
+    for (bool again = false; at < to; again = true) {
+        uint32_t b, kvh, first, n = 0, units = 0, place = group;
+        if (a.few_per) {
+            const uint32_t pairs = a.seqs * a.kv_heads, part = group / pairs, pair = group - part * pairs;
+            b = pair / a.kv_heads;
+            kvh = pair - b * a.kv_heads;
+            first = part * a.few_per;
+            at = to;
+        } else {
+            b = uint32_t(__ffsll(static_cast<unsigned long long>(__ballot(uint64_t(w.with) * a.kv_heads > at))) - 1);
+            units = uint32_t(__builtin_amdgcn_readlane(int(w.units), int(b)));
+            const uint64_t in = at + uint64_t(units) * a.kv_heads - w.upto(a, int(b));
+            kvh = uint32_t(quotient(in, units));
+            first = uint32_t(in - uint64_t(kvh) * units);
+            n = units - first;
+            const bool alone = units <= kFewWhole;
+            if (!alone && n > to - at) n = uint32_t(to - at);
+            at += n;
+            if (alone && first > 0) continue;
+            place = 2 * group + (first == 0);
+        }
+        const Seq s = seq_of(a, b);
+        if (a.few_per) {
+            units = few_units(a, s);
+            if (first >= units) return;
+            n = units - first < a.few_per ? units - first : a.few_per;
+        }
+        if (first == 0 && a.few_parts && threadIdx.x == 0)
+            a.few_parts[b * a.kv_heads + kvh] = uint2{place, 1 + uint32_t(quotient(units - n + per - 1, per))};
+        if (again) __syncthreads();  // the last ones' results in LDS have been read
+        attend_few<kBf16, kDim>(a, lds, s, kvh, cut_of(a, s, kFewKeys).lo, first, n, n == units, place);
     }
 }
 
@@ -661,6 +788,15 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, ui
 // other is used (one barrier a step).  Rows of LDS are 16-byte chunks in an order
 // permuted by the row (a power of two of them), so that the rows of a read
 // fall on different banks.
+//
+// 2,048 tokens over 32,768 keys, 64/8 heads of 128, bf16 (2.13 TFLOP): 2,040 to 2,220 us, about 1,000
+// TFLOP/s; a large library matrix product reaches 1,271 on this card.  The vector instructions
+// of the softmax bound it beside the matrix ones: of a step's 64 keys x 32 rows a wave spends 32 matrix
+// instructions (17.2 ns each) and some 64 exponentials and 200 other vector
+// instructions a lane, of which the two waves of a SIMD hide a part.  Rescaling
+// numerators only past 2^8, V's order in LDS, unpredicated whole pages and matrix instructions
+// first took it from 2,430 to 2,168, loads straight to LDS to 2,040.  Computing the next step's scores
+// beside this one's weights gained nothing (2,341 and 2,316 then).
 template <int kDim>
 constexpr int tile_chunks()  // 16-byte chunks of an LDS row
 {
@@ -1021,11 +1157,13 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
 
 // ---------------------------------------------------------------- kernels
 
+// (Three waves a SIMD for heads up to 64: tiles over 32,768 keys 365 us, two 442; for heads of 128 the
+// few-row kernel spills: 125 us where two take 54.)
 template <bool kBf16, int kDim>
-__global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_few_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim > 64 ? 2 : 3) void attend_few_kernel(AttendArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds_bytes<kDim>()];
-    attend_few<kBf16, kDim>(a, lds, blockIdx.x, blockIdx.y);
+    attend_few_units<kBf16, kDim>(a, lds, blockIdx.x);
 }
 
 template <bool kBf16, int kDim>
@@ -1046,8 +1184,7 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(A
     if (blockIdx.x < tiles) {
         attend_tile<kBf16, kDim>(a, lds, blockIdx.x, tiles);
     } else {
-        const uint32_t x = blockIdx.x - tiles, groups = a.seqs * a.kv_heads;
-        attend_few<kBf16, kDim>(a, lds, x % groups, x / groups);
+        attend_few_units<kBf16, kDim>(a, lds, blockIdx.x - tiles);
     }
 }
 
@@ -1058,21 +1195,35 @@ struct Parts {
     const float2* ml;
     const float* o;
     uint64_t step;  // rows from one part to the next
+    uint32_t back;  // rows that the parts after the first lie before that
     uint32_t parts;
+
+    __device__ __forceinline__ uint64_t row(uint32_t n) const { return n * step - (n == 0 ? 0 : back); }
 };
 
-__device__ __forceinline__ Parts parts_of(const AttendArgs& a, const Seq& s, uint32_t t, uint32_t h)
+__device__ __forceinline__ Parts parts_of(const AttendArgs& a, uint32_t b, uint32_t t, uint32_t h)
 {
-    Parts p{nullptr, nullptr, 0, 0};
-    if (t < s.q0 || t >= s.q0 + s.n_new) return p;
-    const bool few = s.n_new * a.group <= a.few_rows;
-    p.parts = cut_of(a, s, few ? a.few_per : a.tile_per).parts;
+    Parts p{nullptr, nullptr, 0, 0, 0};
     const uint32_t kvh = h / a.group;
-    const uint64_t row = few ? (uint64_t(s.b) * a.kv_heads + kvh) * a.few_rows + (t - s.q0) * a.group + (h - kvh * a.group)
-                             : uint64_t(t) * a.q_heads + h;
-    p.step = few ? uint64_t(a.seqs) * a.kv_heads * a.few_rows : uint64_t(a.tokens) * a.q_heads;
-    p.ml = (few ? a.few_ml : a.tile_ml) + row;
-    p.o = (few ? a.few_o : a.tile_o) + row * a.dim;
+    // (nothing the few-row kernel wrote where the sequence is not its)
+    const uint2 few_parts = a.few_parts ? a.few_parts[uint64_t(b) * a.kv_heads + kvh] : uint2{0, 0};
+    const Seq s = seq_of(a, b);
+    if (t < s.q0 || t >= s.q0 + s.n_new) return p;
+    if (s.n_new * a.group <= a.few_rows) {
+        const uint64_t row = uint64_t(few_parts.x) * kFewRows + (t - s.q0) * a.group + (h - kvh * a.group);
+        p.parts = few_parts.y;
+        // a place a workgroup apart: first ones with few_per; else see attend_few_units
+        p.step = a.few_per ? uint64_t(a.seqs) * a.kv_heads * kFewRows : 2 * kFewRows;
+        p.back = a.few_per ? 0 : kFewRows;
+        p.ml = a.few_ml + row;
+        p.o = a.few_o + row * a.dim;
+    } else {
+        const uint64_t row = uint64_t(t) * a.q_heads + h;
+        p.parts = cut_of(a, s, a.tile_per).parts;
+        p.step = uint64_t(a.tokens) * a.q_heads;
+        p.ml = a.tile_ml + row;
+        p.o = a.tile_o + row * a.dim;
+    }
     return p;
 }
 
@@ -1112,8 +1263,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
     } else {
         b = t < a.seqs ? t : a.seqs - 1;
     }
-    Parts p{nullptr, nullptr, 0, 0};
-    if (th < rows) p = parts_of(a, seq_of(a, b), t, h);
+    Parts p{nullptr, nullptr, 0, 0, 0};
+    if (th < rows) p = parts_of(a, b, t, h);
     const uint32_t parts = p.parts > 1 ? p.parts : 0;
     if (__ballot(parts != 0) == 0) return;
     float2 v[kHeld];
@@ -1121,7 +1272,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
 #pragma unroll
     for (uint32_t i = 0; i < kHeld; ++i) {
         v[i] = float2{0.0f, 0.0f};
-        if (i * kLanes + sub < parts) v[i] = p.ml[(i * kLanes + sub) * p.step];
+        if (i * kLanes + sub < parts) v[i] = p.ml[p.row(i * kLanes + sub)];
         if (v[i].y != 0.0f) top = fmaxf(top, v[i].x);
     }
 #pragma unroll
@@ -1145,7 +1296,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
             for (uint32_t x = 0; x < kAhead; ++x) {
                 const uint32_t n = i * kLanes + p0 + x;
                 part[x] = f32x4{0, 0, 0, 0};
-                if (n < parts && d < a.dim) part[x] = *reinterpret_cast<const f32x4*>(p.o + n * p.step * a.dim + d);
+                if (n < parts && d < a.dim) part[x] = *reinterpret_cast<const f32x4*>(p.o + p.row(n) * a.dim + d);
             }
 #pragma unroll
             for (uint32_t x = 0; x < kAhead; ++x) {
@@ -1167,19 +1318,17 @@ __global__ __launch_bounds__(256, 6) void attend_join_row_kernel(AttendArgs a)
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t t = blockIdx.x / a.q_heads, h = blockIdx.x - t * a.q_heads;
     const uint32_t b = seq_at(a, t);
-    const Parts p = parts_of(a, seq_of(a, b), t, h);
+    const Parts p = parts_of(a, b, t, h);
     if (p.parts <= 1) return;
     float2 v{0.0f, 0.0f};
-    if (lane < p.parts) v = p.ml[lane * p.step];
+    if (lane < p.parts) v = p.ml[p.row(lane)];
     const uint32_t which = threadIdx.x / kLanes, d = lane % kLanes * 4;
-    const uint64_t part_floats = p.step * a.dim;
-    const float* o = p.o + which * part_floats + d;
     f32x4 part[kMost];
 #pragma unroll
     for (uint32_t i = 0; i < kMost; ++i) {
         part[i] = f32x4{0, 0, 0, 0};
-        if (which + i * kStride < p.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(o);
-        o += kStride * part_floats;
+        const uint32_t n = which + i * kStride;
+        if (n < p.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(p.o + p.row(n) * a.dim + d);
     }
     float top = v.y == 0.0f ? -INFINITY : v.x;
 #pragma unroll
@@ -1231,9 +1380,9 @@ bool attend_ok(const si_paged_attention_desc& d)
 // width bounds them, and a sequence is cut into fewer parts on the device where
 // it is shorter.
 struct Plan {
-    uint32_t few_rows = 0, few_per = 0, few_split = 1, tile_per = 0, tile_split = 1, tiles = 0;
+    uint32_t few_rows = 0, few_groups = 0, few_least = 0, few_per = 0, tile_per = 0, tile_split = 1, tiles = 0;
     bool few = false, tile = false, fits = true;
-    uint64_t few_o = 0, few_ml = 0, tile_o = 0, tile_ml = 0, bytes = 0;
+    uint64_t few_o = 0, few_ml = 0, few_parts = 0, tile_o = 0, tile_ml = 0, bytes = 0;
 };
 
 // Keys of a part, so that `groups` sequences of `keys` keys make about `target`
@@ -1260,7 +1409,24 @@ Plan attend_plan(const si_paged_attention_desc& d)
     if (p.few) p.few_rows = kFewRows;
     p.tile = d.q_starts ? rows > p.few_rows : !p.few;
     const uint64_t pairs = uint64_t(d.seqs) * d.kv_heads;
-    if (p.few) p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &p.few_split);
+    uint64_t few_groups = 0, places = 0;
+    if (p.few) {
+        const uint64_t units = (keys + kFewKeys - 1) / kFewKeys, fewest = (units + kMaxSplit - 2) / (kMaxSplit - 1);
+        // workgroups that run at a time: 3 a CU for heads up to 64 (2 beside tiles), 2 up to 128, 1
+        // (768 or 1,536 for heads of 128: 64 sequences of 8,192 keys 229 and 209 us, 512 197)
+        const uint64_t at_once = d.head_dim <= 64 && !p.tile ? 768 : d.head_dim <= 128 ? 512 : 256;
+        p.few_least = uint32_t(fewest > kFewWhole ? fewest : kFewWhole);
+        if (d.seqs <= 64 && pairs <= at_once) {
+            const uint64_t most = (pairs * units + p.few_least - 1) / p.few_least;
+            few_groups = most < at_once ? most : at_once;
+            places = units > kFewWhole ? 2 * few_groups : 0;
+        } else {
+            uint32_t parts;
+            p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &parts) / kFewKeys;
+            few_groups = pairs * parts;
+            places = parts > 1 ? few_groups : 0;
+        }
+    }
     if (p.tile) {
         const uint64_t tile_rows = kTileRows;
         p.tiles = uint32_t(d.q_starts ? rows / tile_rows + d.seqs
@@ -1278,17 +1444,19 @@ Plan attend_plan(const si_paged_attention_desc& d)
     }
     // (threads of a launch dimension fit 32 bits)
     const uint64_t most = (1ull << 32) / 256 - 1;
-    const uint64_t few_groups = p.few ? pairs * p.few_split : 0, tile_groups = uint64_t(p.tiles) * d.kv_heads * p.tile_split;
+    const uint64_t tile_groups = uint64_t(p.tiles) * d.kv_heads * p.tile_split;
+    p.few_groups = uint32_t(few_groups);
     p.fits = few_groups + tile_groups <= most && uint64_t(d.tokens) * d.q_heads / 4 < most;
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
         return at;
     };
-    if (p.few_split > 1) {
-        const uint64_t n = p.few_split * pairs * p.few_rows;
+    if (places) {
+        const uint64_t n = places * kFewRows;
         p.few_o = take(n * d.head_dim * 4);
         p.few_ml = take(n * 8);
+        p.few_parts = take(pairs * 8);
     }
     if (p.tile_split > 1) {
         const uint64_t n = uint64_t(p.tile_split) * d.tokens * d.q_heads;
@@ -1302,18 +1470,16 @@ template <bool kBf16, int kDim>
 hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
 {
     const dim3 block(256);
-    const uint32_t tiles = p.tile ? p.tiles * a.kv_heads * p.tile_split : 0, few = p.few ? a.seqs * a.kv_heads : 0;
+    const uint32_t tiles = p.tile ? p.tiles * a.kv_heads * p.tile_split : 0;
     hipError_t e;
     if (p.few && p.tile) {
-        const dim3 grid(tiles + few * p.few_split);
-        e = launch(attend_mixed_kernel<kBf16, kDim>, grid, block, stream, a);
+        e = launch(attend_mixed_kernel<kBf16, kDim>, dim3(tiles + p.few_groups), block, stream, a);
     } else if (p.few) {
-        const dim3 grid(few, p.few_split);
-        e = launch(attend_few_kernel<kBf16, kDim>, grid, block, stream, a);
+        e = launch(attend_few_kernel<kBf16, kDim>, dim3(p.few_groups), block, stream, a);
     } else {
         e = launch(attend_tile_kernel<kBf16, kDim>, dim3(tiles), block, stream, a);
     }
-    if (e == hipSuccess && (p.few_split > 1 || p.tile_split > 1)) {
+    if (e == hipSuccess && p.bytes) {
         const uint32_t rows = a.tokens * a.q_heads, each = 256 / row_lanes<kDim>();
         e = rows <= kJoinRows ? launch(attend_join_row_kernel<kBf16, kDim>, dim3(rows), block, stream, a)
                               : launch(attend_join_kernel<kBf16, kDim>, dim3((rows + each - 1) / each), block, stream, a);
@@ -1381,13 +1547,16 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     // masked score's -inf times it is still -inf.
     a.scale_log2 = fmaxf(std::fabs(d->scale) * 1.44269504088896341f, 1e-30f);
     a.few_rows = p.few_rows;
+    a.few_groups = p.few_groups;
     a.few_per = p.few_per;
+    a.few_least = p.few_least;
     a.tile_per = p.tile_per;
     a.tile_split = p.tile_split;
     a.tiles = p.tiles;
     uint8_t* const ws = static_cast<uint8_t*>(d->workspace);
     a.few_o = reinterpret_cast<float*>(ws + p.few_o);
     a.few_ml = reinterpret_cast<float2*>(ws + p.few_ml);
+    a.few_parts = p.few_ml ? reinterpret_cast<uint2*>(ws + p.few_parts) : nullptr;
     a.tile_o = reinterpret_cast<float*>(ws + p.tile_o);
     a.tile_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
     const hipError_t e = d->dtype == SI_DTYPE_BF16 ? attend_by_dim<true>(stream, a, p)

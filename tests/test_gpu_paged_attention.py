@@ -385,3 +385,18 @@ def test_lengths_and_windows_past_the_table(new):
 @pytest.mark.parametrize("hq,hkv,new", [(40, 1, [33, 0, 2, 1]), (260, 2, [1, 3, 1, 1]), (17, 1, [1, 1, 1, 1])])
 def test_groups_wider_than_a_tile_of_columns(hq, hkv, new):
     check(make(73 + hq, [300, 0, 65, 700], new, hq, hkv, 64, 32, torch.bfloat16))
+
+
+@pytest.mark.parametrize("seqs,hkv,dim,window", [(64, 8, 64, 0), (64, 2, 128, 90), (65, 1, 64, 0), (130, 2, 96, 40),
+                                                 (33, 16, 128, 0), (90, 9, 64, 0)])
+def test_ragged_batches_over_both_ways_of_sharing_the_keys(seqs, hkv, dim, window):
+    """Lengths of nothing to many steps, one or two new tokens or none: sequences that begin
+    and end anywhere in a workgroup's share, and shares of one sequence."""
+    g = torch.Generator().manual_seed(seqs * hkv)
+    kv = [int(n) for n in torch.randint(0, 420, (seqs,), generator=g)]
+    kv[3], kv[seqs - 1] = 2500, 0
+    new = [int(n) for n in torch.randint(0, 3, (seqs,), generator=g)]
+    x = make(seqs, kv, new, 2 * hkv, hkv, dim, 32, torch.bfloat16)
+    check(x, window=window)
+    one = make(seqs + 1, kv, [1] * seqs, 2 * hkv, hkv, dim, 32, torch.bfloat16)
+    check(one, use_starts=False, window=window)
