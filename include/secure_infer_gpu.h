@@ -587,7 +587,7 @@ int secure_infer_d2h_swap(hipStream_t stream, si_session* session, const void* d
                           uint32_t heads, uint32_t head_dim);
 
 /* ------------------------------------------------------------------ */
-/* 4. Operators on the paged cache (no reference counterpart: the reference
+/* 5. Operators on the paged cache (no reference counterpart: the reference
  *    leaves attention and block management to vLLM).  They work on the caches
  *    the layer calls above fill and drain: `nslots` pages of `page_tokens`
  *    tokens per tensor, page s at base + s * slot_bytes, [page_tokens, kv

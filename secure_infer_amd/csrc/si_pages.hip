@@ -450,7 +450,7 @@ struct AppendArgs {
 
 // One wave per token: it finds the token's sequence by counting the starts at
 // or before it, 64 at a time, then copies the token's K and V rows, 16 bytes a
-// lane, four loads in flight.  The bytes bound it: 15,000 tokens of 8 x 128 heads, bf16,
+// lane, four loads in flight.  The bytes bound it: 14,668 tokens of 8 x 128 heads, bf16,
 // out of a fused projection (120 MB read and written) 25.5 us, 4.7 TB/s, 19.8 where
 // the caches still hold them.  One load at a time 30.8 and 19.9, two 29.6; with ordinary
 // stores 29.2 and 19.8; loads past the caches too 25.0 and 23.0.  64 tokens of 64 sequences:
