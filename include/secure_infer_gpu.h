@@ -687,7 +687,7 @@ int secure_infer_gpu_paged_append(hipStream_t stream, const si_paged_append_desc
  * refs and write tables_out, kv_lens_out and refs_out whole; each output may be
  * its input (in place), and must not overlap anything else. */
 typedef struct si_pages_desc {
-    void* const* caches;      /* host array: device base of each tensor        */
+    void* const* caches;      /* host array: device base of each tensor, distinct */
     uint32_t ncaches;
     uint32_t page_tokens;     /* a power of two                                */
     uint64_t slot_bytes;      /* from one page to the next, a multiple of 16   */

@@ -313,7 +313,10 @@ def _same_layout(caches):
             raise ValueError("a cache must be a device tensor") from e
         if not same or (not dense and any([_paged_cache(c, "a cache") != geometry for c in caches])):
             raise ValueError("the caches must have one shape, dtype, slot stride and device")
-    return geometry, list(map(T.data_ptr, caches))
+    addresses = list(map(T.data_ptr, caches))
+    if len(set(addresses)) != len(addresses):
+        raise ValueError("a cache is given twice")
+    return geometry, addresses
 
 
 def _pages_call(fn_name, caches, tables, kv_lens, refs, page_tokens, rows_list, list_ndim, scrub, fail_count, out,

@@ -365,3 +365,13 @@ def test_reserve_bounds_its_lengths():
     got = si.reserve_pages(*state, torch.tensor(counts, device=DEV), x["ps"], fail_count=fail)
     same(got, (want[0], lens, want[2]))
     assert int(fail) == want[3] >= 2
+
+
+def test_a_cache_given_twice_is_refused():
+    x = make(37, 8, 2, 2, tensors=2)
+    caches, tables, _, refs = on_device(x)
+    twice = [caches[0], caches[1], caches[0]]
+    for call in (lambda: si.CacheSet(twice), lambda: si.compact_pages(twice, tables, refs)):
+        with pytest.raises(ValueError, match="twice"):
+            call()
+    same_caches(caches, x["caches"])
