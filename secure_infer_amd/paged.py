@@ -286,7 +286,7 @@ def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causa
 class CacheSet:
     """Caches of one shape, dtype, slot stride and device (every layer's K and V),
     checked once: the page calls take it in the place of a list, which they
-    check on every call (160 tensors: 39 us).  It holds the tensors; they must keep the
+    check on every call (160 tensors: 43 us).  It holds the tensors; they must keep the
     memory they had, as in a captured graph."""
 
     def __init__(self, caches):
