@@ -1,0 +1,112 @@
+"""paged_attention and paged_append at the ends of what a call may be given: the
+longest tables, rows past 32-bit offsets, lengths past the table, NaN among the
+keys that are seen, outputs of any layout, keys joined from many parts.
+
+`definition` computes chosen rows in 64 bits on the CPU, a token standing at
+p = kv_len - n + i whatever its table holds.
+
+Bound on an output element: with u the unit roundoff of the 16-bit type, A = sum_j
+w_j |v_j| over the n keys seen, ds the rounding of a score ((dim + 4) 2^-24 scale sum_d
+|q_d k_d|: it moves a weight and the weights' sum by a factor exp(ds) each), one
+rounding of the weights to 16 bits, one of the output, and the float sums of the weights and of the
+values over n keys and at most 64 parts, (n + 64) 2^-24 each in any order,
+  |error| <= u |o| + (u + 4 ds + (n + 64) 2^-23) A + n 2^-25 max|v|,
+the last term for fp16 weights below its normal range.  The log-sum-exp moves
+by at most ds + (n + 64) 2^-24 + 2^-22 |lse|."""
+import math
+
+import pytest
+import torch
+
+import secure_infer_amd as si
+from tests.test_gpu_paged_attention import DEV, ROUND, attend, make, rand
+
+pytestmark = pytest.mark.gpu
+
+
+def definition(x, rows=None, scale=None, causal=True, window=0):
+    """{row: (out, lse, bound of out, bound of lse)} of the rows of q, [heads, dim] and
+    [heads] in float64."""
+    q, ck, cv, tables = x["q"], x["ck"], x["cv"], x["tables"]
+    hq, dim = q.shape[1:]
+    slots, ps, hkv, _ = ck.shape
+    scale = dim ** -0.5 if scale is None else scale
+    u = ROUND[q.dtype]
+    starts = x["starts"].tolist()
+    found = {}
+    for b in range(tables.shape[0]):
+        length = int(x["kv"][b])
+        for t in range(starts[b], starts[b + 1]):
+            if rows is not None and t not in rows:
+                continue
+            p = length - starts[b + 1] + t
+            pos = torch.arange(max(0, min(length, tables.shape[1] * ps)))
+            if causal:
+                pos = pos[pos <= p]
+            if window:
+                pos = pos[pos > p - window]
+            slot = tables[b][pos // ps]
+            keep = (slot >= 0) & (slot < slots)
+            pos, slot = pos[keep], slot[keep]
+            n = pos.numel()
+            if n == 0:
+                none = torch.zeros((hq, dim), dtype=torch.float64)
+                found[t] = none, torch.full((hq,), -math.inf, dtype=torch.float64), none, none[:, 0]
+                continue
+            k, v = (c[slot, pos % ps].double().repeat_interleave(hq // hkv, 1) for c in (ck, cv))
+            qq = q[t].double()
+            s = (k * qq).sum(2) * scale                                         # [keys, heads]
+            ds = (k * qq).abs().sum(2).amax(0) * abs(scale) * (dim + 4) * 2.0 ** -24  # [heads]
+            lse = torch.logsumexp(s, 0)
+            lse[torch.isnan(s).any(0)] = math.nan
+            w = torch.exp(s - lse)[:, :, None]
+            out, a = (w * v).sum(0), (w * v.abs()).sum(0)
+            tol = u * out.abs() + (u + 4 * ds[:, None] + (n + 64) * 2.0 ** -23) * a
+            if q.dtype == torch.float16:
+                tol += n * 2.0 ** -25 * v.abs().amax(0)
+            found[t] = out, lse, tol, ds + (n + 64) * 2.0 ** -24 + 2.0 ** -22 * lse.abs()
+    return found
+
+
+def agree(out, lse, found):
+    """Outputs within their bounds, NaN where the definition has NaN."""
+    for t, (want, want_lse, tol, lse_tol) in found.items():
+        for got, w, bound in ((out[t].cpu().double(), want, tol), (lse[t].cpu().double(), want_lse, lse_tol)):
+            assert torch.equal(torch.isnan(got), torch.isnan(w)), f"row {t}: NaN"
+            near = ((got - w).abs() <= bound) | (got == w) | torch.isnan(w)
+            assert near.all(), f"row {t}: off by {float((got - w).abs().nan_to_num(0).max())}"
+
+
+def check(x, use_starts=True, rows=None, **kw):
+    out, lse = attend(x, use_starts, lse=True, **kw)
+    agree(out, lse, definition(x, rows, **kw))
+
+
+def wide(x, pages):
+    """The batch with table rows of `pages` entries, no page past the ones it had."""
+    t = torch.full((x["tables"].shape[0], pages), -1, dtype=torch.int64)
+    t[:, :x["tables"].shape[1]] = x["tables"]
+    return {**x, "tables": t}
+
+
+def test_a_long_chunk_under_the_longest_table():
+    """Row tiles times the table's 2^30 positions pass 2^31 keys a part."""
+    x = wide(make(11, [13_100], [13_000], 16, 1, 8, 32768, torch.bfloat16, spare=0), 32768)
+    check(x, rows={0, 1, 6_500, 12_930, 12_999})
+
+
+def test_many_sequences_under_the_longest_table():
+    """2,048 sequences x 8 KV heads x 2^30 positions: every sequence has its outputs."""
+    x = make(12, [900], [1], 8, 8, 8, 32768, torch.bfloat16, spare=0)
+    g = torch.Generator().manual_seed(1)
+    seqs = 2048
+    x = dict(x, q=rand(g, seqs, 8, 8, dtype=torch.bfloat16), kv=torch.randint(0, 900, (seqs,), generator=g),
+             starts=torch.arange(seqs + 1))
+    x["kv"][-1] = 900
+    pages = 32768
+    row = wide(x, pages)["tables"].to(DEV)
+    d = {k: v.to(DEV) for k, v in x.items()}
+    lse = torch.full((seqs, 8), 7.0, device=DEV)
+    for starts in (None, d["starts"]):
+        out = si.paged_attention(d["q"], d["ck"], d["cv"], row.expand(seqs, pages), d["kv"], q_starts=starts, lse=lse)
+        agree(out, lse, definition({**x, "tables": x["tables"].expand(seqs, -1)}, {0, 1, 63, 64, 65, 1000, 2046, 2047}))
