@@ -606,11 +606,13 @@ enum {
 };
 
 /* Attention of new tokens over their sequences' pages.  Sequence b has
- * kv_lens[b] tokens in its pages (clamped to [0, table_pages * page_tokens]),
- * the last n_b of them the new ones: q rows [q_starts[b], q_starts[b + 1])
- * (clamped to [0, tokens]; NULL: row b alone).  New token i stands at p =
- * kv_lens[b] - n_b + i and sees key j iff j's page is held, j < kv_lens[b],
- * j <= p (causal) and j > p - window (window > 0).
+ * kv_lens[b] tokens (negative: none), the last n_b of them the new ones: q rows
+ * [q_starts[b], q_starts[b + 1]) (clamped to [0, tokens]; NULL: row b alone).
+ * New token i stands at p = kv_lens[b] - n_b + i and sees key j iff j's page is
+ * held, j < kv_lens[b], j <= p (causal) and j > p - window (window > 0).  A
+ * length may outgrow the table: its tokens past the table have no page, the
+ * others keep their positions.  (One over 3 * 2^29, half as long again as the
+ * longest table, ends at the table instead.)
  *   out = sum_j softmax_j(scale * q.k_j) v_j;  lse = log sum_j exp(scale * q.k_j)
  * over the seen keys; none: out = 0, lse = -inf.  Query head h reads KV head
  * h / (q_heads / kv_heads).  Keys that a token does not see have no influence

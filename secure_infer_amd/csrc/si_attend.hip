@@ -200,8 +200,8 @@ __device__ __forceinline__ uint32_t nonfinite_marks(u32x4 x)
 struct Seq {
     uint32_t b;
     uint32_t q0, n_new;  // rows [q0, q0 + n_new) of q
-    int32_t len;         // keys
-    int32_t base;        // position of its first new token (may be negative)
+    int32_t len;         // keys: its length, as far as the table goes
+    int32_t base;        // position of its first new token (may be negative, or past len)
 };
 
 __device__ __forceinline__ uint32_t start_of(const AttendArgs& a, uint32_t b)
@@ -221,16 +221,23 @@ __device__ __forceinline__ Seq seq_of(const AttendArgs& a, uint32_t b)
         const uint32_t end = start_of(a, b + 1);
         s.n_new = end > s.q0 ? end - s.q0 : 0;
     }
+    // New tokens stand where the append puts them, also where the length outgrows the table.
     const int64_t most = int64_t(a.pages) << a.page_shift;
     const int64_t n = a.kv_lens[b];
     s.len = int32_t(n < 0 ? 0 : n > most ? most : n);
-    s.base = s.len - int32_t(s.n_new);
+    s.base = (n > most && n <= int64_t(kMostLength) ? int32_t(n) : s.len) - int32_t(s.n_new);
     return s;
+}
+
+// Keys of a sequence at positions up to p.
+__device__ __forceinline__ int32_t keys_up_to(const Seq& s, int32_t p)
+{
+    return p < 0 ? 0 : p < s.len ? p + 1 : s.len;
 }
 
 // How a sequence's keys are cut: parts of `per` keys from `lo` (a multiple of
 // 64, behind every row's window).  All sequences' parts have one length, which
-// keeps workgroups of ragged batches alike.
+// keeps workgroups of ragged batches alike.  (Behind the last key: at most 63 keys, none seen.)
 struct Cut {
     int32_t lo;
     uint32_t parts;
@@ -240,7 +247,8 @@ __device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Seq& s, uint32_
 {
     Cut c;
     c.lo = 0;
-    if (a.window && s.base - int32_t(a.window) + 1 > 0) c.lo = (s.base - int32_t(a.window) + 1) & ~63;
+    if (a.window && s.base - int32_t(a.window) + 1 > 0) c.lo = s.base - int32_t(a.window) + 1;
+    c.lo = (c.lo < s.len ? c.lo : s.len) & ~63;
     const uint32_t span = s.len > c.lo ? uint32_t(s.len - c.lo) : 0;
     c.parts = (span + per - 1) / per;
     return c;
@@ -537,7 +545,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
         q[k] = v ^ (a.negate ? 0x80008000u : 0u);
     }
     const int32_t p_last = s.base + int32_t(s.n_new) - 1;
-    const int32_t hi0 = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
+    const int32_t hi0 = a.causal ? keys_up_to(s, p_last) : s.len;
     const int32_t hi = hi0 < k_first + int32_t(n * kFewKeys) ? hi0 : k_first + int32_t(n * kFewKeys);
     // keys below lo are behind every row's window
     const int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
@@ -872,7 +880,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
             v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
         q[k] = v ^ (a.negate ? 0x80008000u : 0u);
     }
-    int32_t hi = a.causal ? (p_last + 1 > 0 ? p_last + 1 : 0) : s.len;
+    int32_t hi = a.causal ? keys_up_to(s, p_last) : s.len;
     int32_t k0 = cut.lo + int32_t(part * a.tile_per);
     if (hi - k0 > int32_t(a.tile_per)) hi = k0 + int32_t(a.tile_per);
     const int32_t lo = a.window ? p_first - int32_t(a.window) + 1 : 0;  // behind every row's window below
@@ -1419,7 +1427,7 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     a.dim = d->head_dim;
     a.page_shift = uint32_t(__builtin_ctz(d->page_tokens));
     a.causal = d->causal;
-    a.window = d->window < (1u << 30) ? d->window : 0;  // no table is longer
+    a.window = d->window < kMostLength ? d->window : 0;  // no position is further
     a.group = d->q_heads / d->kv_heads;
     a.negate = d->scale < 0.0f;
     // A scale of 0 (every seen key weighs the same) stays positive, so that a

@@ -38,6 +38,9 @@ constexpr uint64_t kFewTarget = 4096;
 constexpr uint64_t kTileTarget = 768;
 constexpr uint64_t kTileFew = 384;
 constexpr uint64_t kTileSplitMin = 512;
+// Longest length that counts as it is: more than a table holds (2^30) by more than a call's
+// rows, so that a position, a window and their difference from a key fit 32 bits.
+constexpr uint32_t kMostLength = 3u << 29;
 // Sequences of at most this many units a KV head are left to the workgroup of
 // their first unit.
 constexpr uint32_t kFewWhole = kFewStep / kFewKeys;

@@ -203,8 +203,9 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     softmax(scale q k^T) v per token and query head (head h reads KV head
     h // (query heads / kv heads)).  Token i of a sequence with n new ones stands at p = kv_len
     - n + i; it sees the keys on held pages below kv_len, up to p
-    (``causal``) and after p - window (``window`` > 0).  Without a key to see
-    its output is 0.  ``scale`` defaults to head_dim ** -0.5.  ``lse`` [tokens, query heads]
+    (``causal``) and after p - window (``window`` > 0).  Where kv_len outgrows the table
+    the tokens keep the positions that paged_append gives them (one over 3 * 2**29
+    ends at the table instead).  Without a key to see its output is 0.  ``scale`` defaults to head_dim ** -0.5.  ``lse`` [tokens, query heads]
     float32, if given, receives the log-sum-exp of the scaled scores (-inf
     without a key), with which two parts' outputs can be joined.  ``workspace`` (uint8, at least
     ``paged_attention_workspace`` bytes) saves an allocation per call.  Returns ``out``."""

@@ -110,3 +110,45 @@ def test_many_sequences_under_the_longest_table():
     for starts in (None, d["starts"]):
         out = si.paged_attention(d["q"], d["ck"], d["cv"], row.expand(seqs, pages), d["kv"], q_starts=starts, lse=lse)
         agree(out, lse, definition({**x, "tables": x["tables"].expand(seqs, -1)}, {0, 1, 63, 64, 65, 1000, 2046, 2047}))
+
+
+@pytest.mark.parametrize("new,past", [(1, 1), (1, 40), (8, 4), (8, 8), (8, 9), (40, 3), (40, 39), (40, 200), (200, 130)])
+@pytest.mark.parametrize("window,causal", [(0, True), (7, True), (100, True), (7, False), (0, False)])
+def test_tokens_of_a_length_past_the_table_keep_their_places(new, past, window, causal):
+    """Lengths that outgrow a table of 512 positions by `past`: a token with a place in
+    the table stands there, one without sees what its position lets it see."""
+    kv = [512, 512, 300]
+    x = make(13, kv, [new, 2, new], 4, 2, 64, 64, torch.bfloat16, width=8)
+    x["kv"] = torch.tensor([512 + past, 512 + past, 300])
+    check(x, window=window, causal=causal)
+
+
+def test_a_row_that_outgrows_its_table_from_reserve_to_attention():
+    """60 of 64 positions are held and 8 tokens come: the first 4 are stored at 60 to 63,
+    see themselves and what is before them, and the other 4 are dropped."""
+    ps, width, hkv, dim = 16, 4, 2, 64
+    x = make(14, [60], [8], 4, hkv, dim, ps, torch.bfloat16, width=width)
+    d = {k: v.to(DEV) for k, v in x.items()}
+    refs = torch.zeros(x["ck"].shape[0], dtype=torch.int32)
+    refs[x["tables"][0]] = 1
+    fail = torch.zeros(1, dtype=torch.int32, device=DEV)
+    tables, kv, _ = si.reserve_pages(d["tables"], d["kv"], refs.to(DEV), torch.tensor([8], device=DEV), ps, fail)
+    assert int(fail) == 1 and kv.tolist() == [68]
+    k, v = torch.randn((2, 8, hkv, dim), device=DEV).to(torch.bfloat16)
+    si.paged_append(k, v, d["ck"], d["cv"], tables, kv, q_starts=d["starts"], fail_count=fail)
+    assert int(fail) == 5
+    assert torch.equal(d["ck"][tables[0, 3], 12:], k[:4]) and torch.equal(d["cv"][tables[0, 3], 12:], v[:4])
+    got = attend({**x, "ck": d["ck"].cpu(), "cv": d["cv"].cpu(), "kv": kv.cpu()}, lse=True)
+    agree(*got, definition({**x, "ck": d["ck"].cpu(), "cv": d["cv"].cpu(), "kv": kv.cpu()}))
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_lengths_at_the_last_position(new):
+    """Lengths up to 3 * 2^29 count as they are; a longer one ends at the table."""
+    last = 3 << 29
+    x = make(15, [256, 256], [new, 1], 4, 2, 64, 64, torch.bfloat16, width=4)
+    for length, counts_as in ((last, last), (last + 1, 256), (1 << 40, 256)):
+        for window in (0, last - 100, last - 300, (1 << 31) - 1):
+            x["kv"] = torch.tensor([length, 256])
+            got = attend(x, lse=True, window=window)
+            agree(*got, definition({**x, "kv": torch.tensor([counts_as, 256])}, window=window))
