@@ -445,10 +445,12 @@ __device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t,
         float top = s;
 #pragma unroll
         for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        const float mn = fmaxf(m, top);
-        if (mn == -INFINITY) continue;
-        const float w = seen ? __builtin_amdgcn_exp2f(s - mn) : 0.0f;
-        const float keep = __builtin_amdgcn_exp2f(m - mn);
+        const uint64_t mask = __ballot(seen);
+        if (!mask) continue;
+        // (a maximum passes over NaN: where every score is, they still reach the sums)
+        const float mn = fmaxf(m, top), safe = mn == -INFINITY ? 0.0f : mn;
+        const float w = seen ? __builtin_amdgcn_exp2f(s - safe) : 0.0f;
+        const float keep = __builtin_amdgcn_exp2f(m - safe);
         m = mn;
         float sum = w;
 #pragma unroll
@@ -456,7 +458,6 @@ __device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t,
         l = __builtin_fmaf(l, keep, sum);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] *= keep;
-        const uint64_t mask = __ballot(seen);
         for (int x = 0; x < 64; ++x) {
             if (!(mask >> x & 1)) continue;
             const float wx = __shfl(w, x);

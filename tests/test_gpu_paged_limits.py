@@ -152,3 +152,26 @@ def test_lengths_at_the_last_position(new):
             x["kv"] = torch.tensor([length, 256])
             got = attend(x, lse=True, window=window)
             agree(*got, definition({**x, "kv": torch.tensor([counts_as, 256])}, window=window))
+
+
+@pytest.mark.parametrize("kv,new,bad_k,bad_v", [
+    # keys whose K / V are NaN; every key of the first rows' first steps among them
+    (3, 3, [0], [0]), (20, 3, range(18), [17, 18]), (200, 5, range(64), [196]), (5000, 3, range(4000, 4500), [4998]),
+    (70, 70, [0], [0]), (200, 130, range(70), [70, 71]), (300, 40, range(128), [270]),
+    (5000, 70, range(4610, 4900), [4935]), (9000, 30, range(8000, 8990), [8990])])
+def test_what_a_token_sees_of_nan_is_nan(kv, new, bad_k, bad_v):
+    """Alone and in whole steps, with NaN or a sound V beside it, in one part of many."""
+    x = make(16, [kv], [new], 4, 2, 64, 64, torch.bfloat16)
+    for bad, cache in ((bad_k, x["ck"]), (bad_v, x["cv"])):
+        p = torch.tensor(list(bad))
+        cache[x["tables"][0, p // 64], p % 64] = math.nan
+    check(x)
+    check(x, window=66)
+
+
+@pytest.mark.parametrize("kv,new", [(20, 3), (200, 130), (4000, 4), (4000, 70)])
+def test_a_nan_query_has_nan_outputs_beside_nan_values(kv, new):
+    x = make(17, [kv], [new], 4, 2, 64, 64, torch.float16)
+    x["q"][new - 2, 1] = math.nan
+    x["cv"][x["tables"][0, (kv - 1) // 64], (kv - 1) % 64] = math.nan
+    check(x)
