@@ -237,7 +237,7 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
 def paged_attention_workspace(q, cache_k, cache_v, tables, kv_lens, q_starts=None, causal: bool = True,
                               window: int = 0) -> int:
     """Workspace bytes of a paged_attention call with these arguments."""
-    d, _ = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, None, causal, window, q, None)
+    d, _ = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, None, causal, window, None, None)
     return 0 if d is None else int(lib().secure_infer_gpu_paged_attention_workspace(ct.byref(d)))
 
 
@@ -264,8 +264,12 @@ def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causa
         if out.shape != q.shape:
             raise ValueError("out must have q's shape")
         _, ot, oh = _rows(out, "out", q_heads, dim, dtype, device)
-        if min(ot, oh) < dim or max(ot, oh) < min(ot, oh) * (q_heads if ot > oh else tokens):
-            raise ValueError("out's rows must not overlap")
+        # the larger stride steps over the smaller one's rows; that of a single token or head is never used
+        span = dim
+        for stride, n in sorted((stride, n) for stride, n in ((ot, tokens), (oh, q_heads)) if n > 1):
+            if stride < span:
+                raise ValueError("out's rows must not overlap")
+            span += stride * (n - 1)
     if lse is not None and (lse.get_device() != device or lse.dtype != torch.float32 or lse.shape != q.shape[:2]
                             or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous float32 [tokens, query heads] tensor on cuda:{device}")

@@ -175,3 +175,46 @@ def test_a_nan_query_has_nan_outputs_beside_nan_values(kv, new):
     x["q"][new - 2, 1] = math.nan
     x["cv"][x["tables"][0, (kv - 1) // 64], (kv - 1) % 64] = math.nan
     check(x)
+
+
+@pytest.mark.parametrize("shape,strides", [
+    ((4, 1, 64), (64, 64, 1)), ((4, 1, 64), (64, 8, 1)), ((4, 1, 64), (128, 64, 1)), ((1, 8, 64), (512, 128, 1)),
+    ((1, 8, 64), (8, 72, 1)), ((1, 1, 64), (8, 8, 1)), ((4, 8, 64), (64, 256, 1)), ((4, 8, 64), (640, 72, 1)),
+    ((4, 8, 64), (568, 72, 1))])
+def test_outputs_of_any_layout_without_overlaps(shape, strides):
+    """The stride of a single token or head is never used, so it overlaps nothing."""
+    tokens, heads, dim = shape
+    x = make(18, [50 + i for i in range(tokens)], [1] * tokens, heads, 1, dim, 16, torch.bfloat16)
+    d = {k: v.to(DEV) for k, v in x.items()}
+    base = torch.full((8192,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = base.as_strided(shape, strides)
+    assert si.paged_attention(d["q"], d["ck"], d["cv"], d["tables"], d["kv"], out=out) is out
+    assert torch.equal(out, attend(x, use_starts=False))
+    kept = torch.ones_like(base, dtype=torch.bool)
+    kept.as_strided(shape, strides)[:] = False
+    assert (base[kept] == 7).all()
+
+
+@pytest.mark.parametrize("shape,strides", [
+    ((4, 1, 64), (0, 64, 1)), ((4, 1, 64), (56, 64, 1)), ((1, 8, 64), (512, 0, 1)), ((1, 8, 64), (512, 56, 1)),
+    ((4, 8, 64), (64, 64, 1)), ((4, 8, 64), (0, 64, 1)), ((4, 8, 64), (504, 64, 1)), ((4, 8, 64), (64, 248, 1))])
+def test_outputs_that_overlap_are_refused(shape, strides):
+    tokens, heads, dim = shape
+    x = make(19, [50] * tokens, [1] * tokens, heads, 1, dim, 16, torch.bfloat16)
+    d = {k: v.to(DEV) for k, v in x.items()}
+    out = torch.zeros(8192, dtype=torch.bfloat16, device=DEV).as_strided(shape, strides)
+    with pytest.raises(ValueError, match="overlap"):
+        si.paged_attention(d["q"], d["ck"], d["cv"], d["tables"], d["kv"], out=out)
+
+
+@pytest.mark.parametrize("heads", [1, 8])
+def test_workspace_of_queries_of_any_layout(heads):
+    """The query is an input: its rows may be the same memory, and it is no output."""
+    x = make(20, [5000, 333, 40], [1, 1, 1], heads, 1, 64, 16, torch.bfloat16)
+    d = {k: v.to(DEV) for k, v in x.items()}
+    args = (d["ck"], d["cv"], d["tables"], d["kv"])
+    need = si.paged_attention_workspace(d["q"], *args)
+    one = d["q"][:1].expand(3, heads, 64)
+    assert si.paged_attention_workspace(one, *args) == need
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    assert torch.equal(si.paged_attention(one, *args, workspace=ws), si.paged_attention(one.contiguous(), *args))
