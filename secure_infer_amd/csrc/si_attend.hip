@@ -911,6 +911,9 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     const uint32_t place = threadIdx.x % kChunks, row0 = threadIdx.x / kChunks;
     const uint32_t kv_row = a.kv_heads * a.dim * 2u;
     const bool in_page = (1u << a.page_shift) >= kTileKeys;
+    // Steps of one page whose rows are read by 32-bit offsets from its first: below 2^32
+    // for rows below 2^26 bytes.
+    const bool by_offset = in_page && a.dim == kPitch && kv_row < (1u << 26);
     Window pages;
     // The keys of [kb, kb + 64) that may be read: on held pages, in [lo, hi).
     const auto readable = [&](int32_t kb) {
@@ -931,7 +934,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         const uint32_t k_to = __builtin_amdgcn_readfirstlane(lds_at + buf * kBufBytes + wave * kGroup);
         const uint32_t v_to = __builtin_amdgcn_readfirstlane(lds_at + buf * kBufBytes + kKBytes + wave * 1024);
         const uint32_t in = uint32_t(kb) & ((1u << a.page_shift) - 1u);
-        if (ok == ~0ull && in_page && a.dim == kPitch) {
+        if (ok == ~0ull && by_offset) {
             const uint64_t page = uint64_t(uint32_t(pages.slot(uint32_t(kb) >> a.page_shift))) * a.slot_bytes +
                                   uint64_t(in) * kv_row + kvh * a.dim * 2u;
             const uint8_t* const kp = uniform(a.cache_k + page);

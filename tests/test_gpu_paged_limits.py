@@ -218,3 +218,18 @@ def test_workspace_of_queries_of_any_layout(heads):
     assert si.paged_attention_workspace(one, *args) == need
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
     assert torch.equal(si.paged_attention(one, *args, workspace=ws), si.paged_attention(one.contiguous(), *args))
+
+
+def test_steps_of_keys_past_32_bit_offsets():
+    """64 keys of 270,336 KV heads x 128 lie 4.4 GB apart from first to last."""
+    heads, dim, ps, tokens = 270_336, 128, 64, 17
+    g = torch.Generator(device=DEV).manual_seed(3)
+    ck, cv, q = (torch.empty((n, heads, dim), dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+                 for n in (ps, ps, tokens))
+    lse = torch.empty((tokens, heads), device=DEV)
+    out = si.paged_attention(q, ck[None], cv[None], torch.zeros((1, 1), dtype=torch.int64, device=DEV),
+                             torch.tensor([ps], device=DEV), q_starts=torch.tensor([0, tokens], device=DEV), lse=lse)
+    some = torch.tensor([0, 1, 2, 100_000, 262_144, heads - 1], device=DEV)
+    x = dict(q=q[:, some].cpu(), ck=ck[None, :, some].cpu(), cv=cv[None, :, some].cpu(),
+             tables=torch.zeros((1, 1), dtype=torch.int64), kv=torch.tensor([ps]), starts=torch.tensor([0, tokens]))
+    agree(out[:, some], lse[:, some], definition(x))
