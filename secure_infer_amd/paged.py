@@ -14,7 +14,8 @@ tokens in a sequence's pages, the new ones included.  ``q_starts`` [sequences +
 sequence b's one new token).  What lives on the device is not read back: the
 kernels stay inside the tensors whatever it holds, and count what they cannot
 serve in ``fail_count`` (an int32 tensor they add to), as the reload calls
-do.  Every call is asynchronous on the given (default: current) stream, and
+do.  There is no backward pass: attention and append refuse tensors that
+require gradients where gradients are recorded.  Every call is asynchronous on the given (default: current) stream, and
 may be captured into a graph.
 """
 from __future__ import annotations
@@ -87,6 +88,12 @@ def _fail_count(t, device: int) -> None:
 def _aligned(t, name: str) -> None:
     if t.data_ptr() % 16:
         raise ValueError(f"{name} must start on a 16-byte boundary")
+
+
+def _tracked() -> None:
+    """A tensor requires gradients.  There is no backward pass: one is refused rather than lost."""
+    if torch.is_grad_enabled():
+        raise ValueError("no gradient passes through the paged cache: detach its tensors or use torch.no_grad()")
 
 
 def _paged_cache(t, name: str):
@@ -177,6 +184,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_
     v_tokens, vt, vh = _rows(v, "v", heads, dim, dtype, device)
     if tokens != v_tokens:
         raise ValueError("k and v must have the same tokens")
+    if k.requires_grad or v.requires_grad or cache_k.requires_grad or cache_v.requires_grad:
+        _tracked()
     seqs, pages, row = _sequences(tables, kv_lens, q_starts, tokens, ps, device)
     _fail_count(fail_count, device)
     if tokens == 0 or seqs == 0:
@@ -210,6 +219,8 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     without a key), with which two parts' outputs can be joined.  ``workspace`` (uint8, at least
     ``paged_attention_workspace`` bytes) saves an allocation per call.  Returns ``out``."""
     d, device = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse)
+    if q.requires_grad or cache_k.requires_grad or cache_v.requires_grad:
+        _tracked()
     if d is None:
         return torch.empty_like(q) if out is None else out
     raw, other = _stream_of(stream, device)

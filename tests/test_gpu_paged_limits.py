@@ -233,3 +233,26 @@ def test_steps_of_keys_past_32_bit_offsets():
     x = dict(q=q[:, some].cpu(), ck=ck[None, :, some].cpu(), cv=cv[None, :, some].cpu(),
              tables=torch.zeros((1, 1), dtype=torch.int64), kv=torch.tensor([ps]), starts=torch.tensor([0, tokens]))
     agree(out[:, some], lse[:, some], definition(x))
+
+
+def test_tensors_that_require_gradients_are_refused():
+    """There is no backward pass: a result without a history is not handed out unasked."""
+    x = make(21, [40, 20], [1, 1], 4, 2, 64, 16, torch.bfloat16)
+    d = {k: v.to(DEV) for k, v in x.items()}
+    args = dict(q=d["q"], cache_k=d["ck"], cache_v=d["cv"], tables=d["tables"], kv_lens=d["kv"])
+    want = si.paged_attention(**args)
+    for name in ("q", "cache_k", "cache_v"):
+        tracked = {**args, name: args[name].clone().requires_grad_()}
+        with pytest.raises(ValueError, match="gradient"):
+            si.paged_attention(**tracked)
+        with torch.no_grad():
+            assert torch.equal(si.paged_attention(**tracked), want)
+    k = torch.ones((2, 2, 64), dtype=torch.bfloat16, device=DEV)
+    rest = (d["ck"], d["cv"], d["tables"], d["kv"])
+    for kk, vv in ((k.clone().requires_grad_(), k), (k, k.clone().requires_grad_())):
+        before = d["ck"].clone()
+        with pytest.raises(ValueError, match="gradient"):
+            si.paged_append(kk, vv, *rest)
+        assert torch.equal(torch.nan_to_num(d["ck"]), torch.nan_to_num(before))
+        with torch.no_grad():
+            si.paged_append(kk, vv, *rest)
