@@ -188,8 +188,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_
         _tracked()
     seqs, pages, row = _sequences(tables, kv_lens, q_starts, tokens, ps, device)
     _fail_count(fail_count, device)
-    if tokens == 0 or seqs == 0:
+    if tokens == 0:
         return
+    if seqs == 0:
+        raise ValueError("there are new tokens but no sequences")
     if pages == 0:
         raise ValueError("tables has no pages")
     raw, other = _stream_of(stream, device)

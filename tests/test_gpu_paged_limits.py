@@ -256,3 +256,13 @@ def test_tensors_that_require_gradients_are_refused():
         assert torch.equal(torch.nan_to_num(d["ck"]), torch.nan_to_num(before))
         with torch.no_grad():
             si.paged_append(kk, vv, *rest)
+
+
+def test_tokens_without_any_sequence_are_refused():
+    x = make(22, [40], [1], 2, 2, 64, 16, torch.bfloat16)
+    d = {k: v.to(DEV) for k, v in x.items()}
+    none = (d["ck"], d["cv"], d["tables"][:0], d["kv"][:0])
+    start = torch.zeros(1, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError, match="no sequences"):
+        si.paged_append(d["q"], d["q"], *none, q_starts=start)
+    si.paged_append(d["q"][:0], d["q"][:0], *none, q_starts=start)
