@@ -45,7 +45,9 @@ struct AttendArgs {
     const int64_t* kv_lens;
     const int64_t* q_starts;
     uint32_t pages, tokens, seqs, q_heads, kv_heads, group, dim, page_shift, causal, window;
-    uint32_t negate;   // the scale is negative: q's sign is flipped instead
+    // A negative scale flips q's sign, one of 0 clears q (with a positive one here, so
+    // that a masked score's -inf times it is still -inf).
+    uint32_t q_keep, q_flip;
     float scale_log2;  // |scale| * log2(e): weights are powers of two
     // Sequences of at most few_rows rows (tokens * group) belong to the few-row
     // kernel, the others to the tile kernel.
@@ -425,7 +427,7 @@ __device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t,
     if (a.causal && to > pos + 1) to = pos + 1;
     if (a.window && from < pos - int32_t(a.window) + 1) from = pos - int32_t(a.window) + 1;
     const uint16_t* q = a.q + t * a.q_token + h * a.q_head;
-    const float c = a.negate ? -a.scale_log2 : a.scale_log2;
+    const float c = a.q_keep == 0 ? 0.0f : a.q_flip ? -a.scale_log2 : a.scale_log2;
     float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int32_t j0 = from; j0 < to; j0 += 64) {
         const int32_t j = j0 + int32_t(lane);
@@ -543,7 +545,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
         u32x4 v{0, 0, 0, 0};
         if (col < rows && d < a.dim)
             v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
-        q[k] = v ^ (a.negate ? 0x80008000u : 0u);
+        q[k] = (v & a.q_keep) ^ a.q_flip;
     }
     const int32_t p_last = s.base + int32_t(s.n_new) - 1;
     const int32_t hi0 = a.causal ? keys_up_to(s, p_last) : s.len;
@@ -879,7 +881,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         u32x4 v{0, 0, 0, 0};
         if (r < rows && d < a.dim)
             v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
-        q[k] = v ^ (a.negate ? 0x80008000u : 0u);
+        q[k] = (v & a.q_keep) ^ a.q_flip;
     }
     int32_t hi = a.causal ? keys_up_to(s, p_last) : s.len;
     int32_t k0 = cut.lo + int32_t(part * a.tile_per);
@@ -1433,10 +1435,10 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     a.causal = d->causal;
     a.window = d->window < kMostLength ? d->window : 0;  // no position is further
     a.group = d->q_heads / d->kv_heads;
-    a.negate = d->scale < 0.0f;
-    // A scale of 0 (every seen key weighs the same) stays positive, so that a
-    // masked score's -inf times it is still -inf.
-    a.scale_log2 = fmaxf(std::fabs(d->scale) * 1.44269504088896341f, 1e-30f);
+    a.scale_log2 = std::fabs(d->scale) * 1.44269504088896341f;
+    a.q_keep = a.scale_log2 > 0.0f ? ~0u : 0u;
+    a.q_flip = d->scale < 0.0f ? 0x80008000u : 0u;
+    if (!a.q_keep) a.scale_log2 = 1.0f;
     a.few_rows = p.few_rows;
     a.few_groups = p.few_groups;
     a.few_per = p.few_per;

@@ -266,3 +266,12 @@ def test_tokens_without_any_sequence_are_refused():
     with pytest.raises(ValueError, match="no sequences"):
         si.paged_append(d["q"], d["q"], *none, q_starts=start)
     si.paged_append(d["q"][:0], d["q"][:0], *none, q_starts=start)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-33, -1e-36])
+def test_scales_of_nothing_and_next_to_it(scale):
+    """Products of up to 1e35 under a scale of 0 weigh the same."""
+    x = make(23, [300, 70, 9], [40, 1, 3], 4, 2, 64, 32, torch.bfloat16)
+    x["q"] *= 1e17
+    x["ck"] *= 1e17
+    check(x, scale=scale)
