@@ -275,3 +275,23 @@ def test_scales_of_nothing_and_next_to_it(scale):
     x["q"] *= 1e17
     x["ck"] *= 1e17
     check(x, scale=scale)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,dtype", [(8, 2, 128, torch.bfloat16), (4, 1, 64, torch.float16),
+                                              (6, 2, 256, torch.bfloat16), (5, 1, 96, torch.float16)])
+def test_tiles_joined_from_many_parts(hq, hkv, dim, dtype):
+    """More than 2,048 (token, head) rows over keys cut into parts, beside next tokens."""
+    kv, new = [7001, 5003, 2111, 40, 3000], [501, 130, 1, 1, 77]
+    x = make(24, kv, new, hq, hkv, dim, 64, dtype)
+    check(x, rows={0, 250, 500, 501, 600, 630, 631, 632, 633, 680, 709})
+    check(x, window=1500, rows={0, 250, 500, 501, 600, 630, 631, 632, 633, 680, 709})
+
+
+def test_parts_beside_infinite_and_nan_values():
+    """Rows that do not see the bad keys near the diagonal of a sequence cut into parts."""
+    for bad in (math.nan, math.inf):
+        kv, new = [7001, 5003], [520, 130]
+        x = make(25, kv, new, 8, 2, 64, 64, torch.bfloat16)
+        for b, p in ((0, 6990), (0, 6700), (1, 4950)):
+            x["cv"][x["tables"][b, p // 64], p % 64] = bad
+        check(x, rows={0, 100, 218, 219, 400, 508, 509, 519, 520, 596, 597, 649})
