@@ -616,7 +616,8 @@ enum {
  *   out = sum_j softmax_j(scale * q.k_j) v_j;  lse = log sum_j exp(scale * q.k_j)
  * over the seen keys; none: out = 0, lse = -inf.  Query head h reads KV head
  * h / (q_heads / kv_heads).  Keys that a token does not see have no influence
- * on it, whatever bits they hold.  Scores, statistics and sums are float. */
+ * on it, whatever bits they hold.  Scores, statistics and sums are float; the
+ * weights are rounded once to `dtype` for their product with v. */
 typedef struct si_paged_attention_desc {
     const void* q;            /* rows of q_heads x head_dim, dim contiguous    */
     uint64_t q_token_stride;  /* in elements, as q_head_stride: multiples of 8 */
@@ -725,7 +726,8 @@ int secure_infer_gpu_pages_fork(hipStream_t stream, const si_pages_desc* desc);
  * beyond a slot's count, are counted. */
 int secure_infer_gpu_pages_free(hipStream_t stream, const si_pages_desc* desc);
 /* With L slots held, the held slots >= L move to the free slots < L, both
- * ascending, in every tensor; tables and refs follow. */
+ * ascending, in every tensor; tables and refs follow.  Without `scrub` the
+ * pages moved from keep their contents. */
 int secure_infer_gpu_pages_compact(hipStream_t stream, const si_pages_desc* desc);
 /* Row b grows by list[b] tokens: kv_lens_out = kv_lens + list[b], and the pages
  * it then lacks are taken from the free slots, the lowest first, rows in

@@ -216,7 +216,8 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     - n + i; it sees the keys on held pages below kv_len, up to p
     (``causal``) and after p - window (``window`` > 0).  Where kv_len outgrows the table
     the tokens keep the positions that paged_append gives them (one over 3 * 2**29
-    ends at the table instead).  Without a key to see its output is 0.  ``scale`` defaults to head_dim ** -0.5.  ``lse`` [tokens, query heads]
+    ends at the table instead).  Without a key to see its output is 0.  Scores
+    and sums are float; the weights are rounded to q's type once, for the product with v.  ``scale`` defaults to head_dim ** -0.5.  ``lse`` [tokens, query heads]
     float32, if given, receives the log-sum-exp of the scaled scores (-inf
     without a key), with which two parts' outputs can be joined.  ``workspace`` (uint8, at least
     ``paged_attention_workspace`` bytes) saves an allocation per call.  Returns ``out``."""
@@ -405,7 +406,7 @@ def fork_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
     the parent's copy: whole pages are shared (refs + 1), a partly filled last page is
     copied in every tensor of ``caches`` (a list, or a CacheSet of it) into the lowest
     free slots, in the list's order.  A child must be an empty row named once; a pair that cannot be served (a
-    row out of range, no free slot) leaves its child empty and is counted.
+    row out of range, no free slot) leaves its child as it was and is counted.
     Returns (tables, kv_lens, refs), new or written to ``out`` (which may be the
     inputs).  ``refs`` [slots] int32 counts the rows that hold a slot."""
     if not isinstance(pairs, torch.Tensor) or pairs.ndim != 2 or pairs.shape[1] != 2:
@@ -426,8 +427,8 @@ def free_pages(caches, tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
 
 def compact_pages(caches, tables: torch.Tensor, refs: torch.Tensor, scrub: bool = False, out=None, stream=None):
     """With L slots held, the held slots >= L move to the free slots < L (both
-    ascending) in every tensor of ``caches``; ``scrub`` zeroes the pages moved
-    from.  Returns (tables, refs), new or written to ``out``."""
+    ascending) in every tensor of ``caches``.  The pages moved from keep their contents,
+    plaintext in slots that are free, unless ``scrub`` zeroes them.  Returns (tables, refs), new or written to ``out``."""
     return _pages_call("secure_infer_gpu_pages_compact", caches, tables, None, refs, 0, None, 0,
                        scrub, None, out, stream)
 
@@ -436,8 +437,8 @@ def reserve_pages(tables: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tenso
                   page_tokens: int, fail_count: torch.Tensor | None = None, out=None, stream=None):
     """Row b grows by counts[b] tokens (negative: by none) and takes the pages it
     then lacks from the free slots, the lowest first, rows in order.  A row
-    that outgrows its table, or that needs more slots than are left, takes none
-    and is counted; its new length stands, so its tokens without a page are
+    that outgrows its table, or that needs more slots than the rows before it
+    that fit theirs leave (served or not), takes none and is counted; its new length stands, so its tokens without a page are
     dropped by paged_append and unseen by paged_attention.  Returns (tables,
     kv_lens, refs) as fork_pages does."""
     if not isinstance(counts, torch.Tensor) or not isinstance(tables, torch.Tensor) \
