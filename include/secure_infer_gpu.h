@@ -655,6 +655,29 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
  * refuse the descriptor. */
 uint64_t secure_infer_gpu_paged_attention_workspace(const si_paged_attention_desc* desc);
 
+/* What an attention call may have besides.
+ * sinks: with a window, a token also sees the keys j < sinks that it would see
+ *   without one.  (Without a window it changes nothing.)
+ * Shared prefixes: sequences group_starts[g] .. group_starts[g + 1] (clamped to
+ *   [0, seqs]) are group g.  Its tokens find the keys j < prefix_lens[g]
+ *   (clamped to the table) on the pages of its first sequence's row, whatever
+ *   their own rows hold there, and the others on their own rows' pages; which
+ *   of them a token sees does not change.  The prefix is read once for all
+ *   tokens of the group.  A group of one sequence, and sequences in no group,
+ *   are as without groups. */
+typedef struct si_paged_attention_more {
+    uint32_t sinks;               /* at most 2^30                              */
+    uint32_t groups;              /* 0: no shared prefixes; < 2^26             */
+    const int64_t* group_starts;  /* groups + 1, ascending                     */
+    const int64_t* prefix_lens;   /* groups                                    */
+} si_paged_attention_more;
+
+/* secure_infer_gpu_paged_attention with them; more == NULL: without. */
+int secure_infer_gpu_paged_attention_more(hipStream_t stream, const si_paged_attention_desc* desc,
+                                          const si_paged_attention_more* more);
+uint64_t secure_infer_gpu_paged_attention_more_workspace(const si_paged_attention_desc* desc,
+                                                         const si_paged_attention_more* more);
+
 /* New tokens' K and V rows into their pages: token i of sequence b (positions
  * and q_starts as above) goes to row p % page_tokens of page p /
  * page_tokens.  A token at p < 0, past the table or without a page is dropped
@@ -684,6 +707,33 @@ typedef struct si_paged_append_desc {
 } si_paged_append_desc;
 
 int secure_infer_gpu_paged_append(hipStream_t stream, const si_paged_append_desc* desc);
+
+/* The append with K (and the same tokens' queries) rotated by position on the
+ * way: with p a token's position and a_i = p * freqs[i] (the angle to float
+ * accuracy at any position), the pair (x, y) of dims (i, i + rot / 2), or (2 i, 2 i
+ * + 1) if adjacent, becomes magnitude * (x cos a_i - y sin a_i, y cos a_i + x sin
+ * a_i), computed in float and rounded once; dims from rot on, and V, go as they
+ * are.  q_out may be q itself; otherwise it must not overlap q, k or v.  Tokens
+ * dropped from the cache (as by paged_append) have their queries rotated all the
+ * same; a row of q that belongs to no sequence goes as it is. */
+typedef struct si_rotation {
+    const float* freqs;           /* rot / 2, radians a position               */
+    const int64_t* positions;     /* [tokens]; NULL: p as in paged_append      */
+    const void* q;                /* rows of q_heads x head_dim, dim contiguous */
+    void* q_out;
+    uint64_t q_token_stride;      /* in elements, multiples of 8               */
+    uint64_t q_head_stride;
+    uint64_t q_out_token_stride;
+    uint64_t q_out_head_stride;
+    uint32_t q_heads;             /* 0: no q                                   */
+    uint32_t rot;                 /* a multiple of 8, at most head_dim and 256 */
+    uint32_t adjacent;
+    uint32_t dtype;               /* SI_DTYPE_* of q, k, v and the caches      */
+    float magnitude;
+} si_rotation;
+
+int secure_infer_gpu_paged_append_rotated(hipStream_t stream, const si_paged_append_desc* desc,
+                                          const si_rotation* rotation);
 
 /* Page management over every layer's caches at once.  refs[s] counts the
  * sequences that hold slot s (0: free).  The calls read tables, kv_lens and

@@ -15,4 +15,5 @@ from .gcm import (  # noqa: F401
     set_chunk_rows, set_job_id, set_straddle_rows, transfer_prefetch_stats, wait_job_authentication,
     wire_stride, wire_tag_offset)
 from .paged import (  # noqa: F401
-    CacheSet, compact_pages, fork_pages, free_pages, paged_append, paged_attention, paged_attention_workspace, reserve_pages)
+    CacheSet, compact_pages, fork_pages, free_pages, paged_append, paged_append_rotated, paged_attention,
+    paged_attention_workspace, reserve_pages)

@@ -48,6 +48,11 @@ class SiPagedAttentionDesc(ct.Structure):
     ]
 
 
+class SiPagedAttentionMore(ct.Structure):
+    """si_paged_attention_more (include/secure_infer_gpu.h)."""
+    _fields_ = [("sinks", _u32), ("groups", _u32), ("group_starts", _v), ("prefix_lens", _v)]
+
+
 class SiPagedAppendDesc(ct.Structure):
     """si_paged_append_desc (include/secure_infer_gpu.h)."""
     _fields_ = [
@@ -56,6 +61,15 @@ class SiPagedAppendDesc(ct.Structure):
         ("tables", _v), ("table_stride", _u64), ("kv_lens", _v), ("q_starts", _v), ("table_pages", _u32),
         ("tokens", _u32), ("seqs", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("page_tokens", _u32),
         ("fail_count", _v),
+    ]
+
+
+class SiRotation(ct.Structure):
+    """si_rotation (include/secure_infer_gpu.h)."""
+    _fields_ = [
+        ("freqs", _v), ("positions", _v), ("q", _v), ("q_out", _v), ("q_token_stride", _u64), ("q_head_stride", _u64),
+        ("q_out_token_stride", _u64), ("q_out_head_stride", _u64), ("q_heads", _u32), ("rot", _u32),
+        ("adjacent", _u32), ("dtype", _u32), ("magnitude", ct.c_float),
     ]
 
 
@@ -97,7 +111,12 @@ SIGNATURES = {
     "secure_infer_gpu_writeback_layer": ([_v, _v, ct.POINTER(SiWritebackDesc)], _i),
     "secure_infer_gpu_paged_attention": ([_v, ct.POINTER(SiPagedAttentionDesc)], _i),
     "secure_infer_gpu_paged_attention_workspace": ([ct.POINTER(SiPagedAttentionDesc)], _u64),
+    "secure_infer_gpu_paged_attention_more": (
+        [_v, ct.POINTER(SiPagedAttentionDesc), ct.POINTER(SiPagedAttentionMore)], _i),
+    "secure_infer_gpu_paged_attention_more_workspace": (
+        [ct.POINTER(SiPagedAttentionDesc), ct.POINTER(SiPagedAttentionMore)], _u64),
     "secure_infer_gpu_paged_append": ([_v, ct.POINTER(SiPagedAppendDesc)], _i),
+    "secure_infer_gpu_paged_append_rotated": ([_v, ct.POINTER(SiPagedAppendDesc), ct.POINTER(SiRotation)], _i),
     "secure_infer_gpu_pages_fork": ([_v, ct.POINTER(SiPagesDesc)], _i),
     "secure_infer_gpu_pages_free": ([_v, ct.POINTER(SiPagesDesc)], _i),
     "secure_infer_gpu_pages_compact": ([_v, ct.POINTER(SiPagesDesc)], _i),

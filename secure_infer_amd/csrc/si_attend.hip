@@ -58,7 +58,19 @@ struct AttendArgs {
     uint2* few_parts;  // of each sequence and KV head: place of its first part, number of parts
     float* tile_o;
     float2* tile_ml;
+    // Sinks and shared prefixes (kMore and kShare).  Sequences that share one leave their own
+    // keys' whole parts in tile_o's first part.
+    uint32_t sinks;  // first keys seen in spite of the window (0 without one)
+    uint32_t groups, share_tiles, share_split;
+    const int64_t* group_starts;
+    const int64_t* prefix_lens;
+    float* share_o;
+    float2* share_ml;
 };
+
+// What a kernel's code knows of: a call without sinks and shared prefixes, one with them, and of the
+// latter the pass of the groups' tokens over their prefixes.
+enum Kind { kPlain = 0, kMore = 1, kShare = 2 };
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -75,6 +87,9 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // heads 72 us in all, only the second 52; one token x 32 heads 20.0 and 20.3, 64 x 28 63.6
 // and 64.3.
 constexpr uint32_t kJoinRows = 2048;
+
+// The last key of a query without one, behind every position.
+constexpr int32_t kNoLast = 0x7ffffffe;
 
 __device__ __forceinline__ bool held(int64_t e, int64_t nslots) { return e >= 0 && e < nslots; }
 
@@ -204,6 +219,7 @@ struct Seq {
     uint32_t q0, n_new;  // rows [q0, q0 + n_new) of q
     int32_t len;         // keys: its length, as far as the table goes
     int32_t base;        // position of its first new token (may be negative, or past len)
+    int32_t from;        // keys below are its group's (kMore)
 };
 
 __device__ __forceinline__ uint32_t start_of(const AttendArgs& a, uint32_t b)
@@ -212,10 +228,52 @@ __device__ __forceinline__ uint32_t start_of(const AttendArgs& a, uint32_t b)
     return uint32_t(s < 0 ? 0 : s > int64_t(a.tokens) ? int64_t(a.tokens) : s);
 }
 
+// Rows of q from sequence b's first on.
+__device__ __forceinline__ uint32_t rows_at(const AttendArgs& a, uint32_t b)
+{
+    return a.q_starts ? start_of(a, b) : b;
+}
+
+// Sequences [first, end) and the keys of the prefix they share, as far as the table goes: none for
+// fewer than two sequences.
+struct Group {
+    uint32_t first, end;
+    int32_t prefix;
+};
+
+__device__ __forceinline__ Group group_at(const AttendArgs& a, uint32_t g)
+{
+    const int64_t lo = a.group_starts[g], hi = a.group_starts[g + 1], seqs = a.seqs;
+    Group x;
+    x.first = uint32_t(lo < 0 ? 0 : lo > seqs ? seqs : lo);
+    x.end = uint32_t(hi < 0 ? 0 : hi > seqs ? seqs : hi);
+    const int64_t most = int64_t(a.pages) << a.page_shift, n = a.prefix_lens[g];
+    x.prefix = x.end < x.first + 2 || n < 0 ? 0 : int32_t(n > most ? most : n);
+    return x;
+}
+
+// Keys of the prefix that sequence b shares: that of the last group that starts at or before it.
+__device__ __forceinline__ int32_t prefix_of(const AttendArgs& a, uint32_t b)
+{
+    uint32_t at = 0;
+    for (uint32_t n = a.groups; n;) {
+        const uint32_t half = n / 2;
+        const bool up = a.group_starts[at + half] <= int64_t(b);
+        at = up ? at + half + 1 : at;
+        n = up ? n - half - 1 : half;
+    }
+    if (at == 0) return 0;
+    const Group g = group_at(a, at - 1);
+    return b < g.end ? g.prefix : 0;
+}
+
+template <int kKind = kPlain>
 __device__ __forceinline__ Seq seq_of(const AttendArgs& a, uint32_t b)
 {
     Seq s;
     s.b = b;
+    s.from = 0;
+    if constexpr (kKind == kMore) s.from = prefix_of(a, b);
     s.q0 = b;
     s.n_new = 1;
     if (a.q_starts) {
@@ -240,15 +298,44 @@ __device__ __forceinline__ int32_t keys_up_to(const Seq& s, int32_t p)
 // How a sequence's keys are cut: parts of `per` keys from `lo` (a multiple of
 // 64, behind every row's window).  All sequences' parts have one length, which
 // keeps workgroups of ragged batches alike.  (Behind the last key: at most 63 keys, none seen.)
+//
+// With sinks, or a prefix that the group attends to, the keys that are left are counted without the
+// gap: `head` keys from head_lo (the sinks), then those from lo on.  All three are multiples of `step`,
+// so that a step's keys follow one another.
 struct Cut {
     int32_t lo;
     uint32_t parts;
+    int32_t head_lo, head;
+
+    // The key in place x, and the first place with a key of at least k.
+    __device__ __forceinline__ int32_t key(int32_t x) const { return x < head ? head_lo + x : lo + (x - head); }
+    __device__ __forceinline__ int32_t place(int32_t k) const
+    {
+        return k <= head_lo ? 0 : k - head_lo < head ? k - head_lo : k <= lo ? head : k - lo + head;
+    }
 };
 
-__device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Seq& s, uint32_t per)
+template <int kKind = kPlain>
+__device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Seq& s, uint32_t per, uint32_t step = kTileKeys)
 {
     Cut c;
     c.lo = 0;
+    c.head_lo = c.head = 0;
+    if constexpr (kKind == kMore) {
+        const int32_t whole = -int32_t(step);  // & whole: down to a multiple
+        int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
+        lo = lo > s.from ? lo : s.from;
+        c.lo = (lo < s.len ? lo : s.len) & whole;
+        c.head_lo = s.from & whole;
+        if (int32_t(a.sinks) > s.from) {
+            const int32_t end = (int32_t(a.sinks) + int32_t(step) - 1) & whole;
+            c.head = (end < c.lo ? end : c.lo) - c.head_lo;
+            c.head = c.head > 0 ? c.head : 0;
+        }
+        const uint32_t span = uint32_t(c.head) + (s.len > c.lo ? uint32_t(s.len - c.lo) : 0);
+        c.parts = (span + per - 1) / per;
+        return c;
+    }
     if (a.window && s.base - int32_t(a.window) + 1 > 0) c.lo = s.base - int32_t(a.window) + 1;
     c.lo = (c.lo < s.len ? c.lo : s.len) & ~63;
     const uint32_t span = s.len > c.lo ? uint32_t(s.len - c.lo) : 0;
@@ -276,11 +363,12 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
 
 // Units of 32 keys of a KV head of a sequence for the few-row kernel.  (A
 // sequence without keys has outputs all the same: one.)
+template <int kKind>
 __device__ __forceinline__ uint32_t few_units(const AttendArgs& a, const Seq& s)
 {
     const uint32_t rows = s.n_new * a.group;
     if (rows == 0 || rows > a.few_rows) return 0;
-    const uint32_t n = cut_of(a, s, kFewKeys).parts;
+    const uint32_t n = cut_of<kKind>(a, s, kFewKeys, kFewKeys).parts;
     return n ? n : 1;
 }
 
@@ -291,10 +379,11 @@ struct Few {
     uint32_t units, with;  // of a KV head; their sum up to and with the lane's (at most 64 * 2^25)
     uint64_t total, per;
 
+    template <int kKind>
     __device__ __forceinline__ void start(const AttendArgs& a)
     {
         const uint32_t b = threadIdx.x & 63u;
-        units = b < a.seqs ? few_units(a, seq_of(a, b)) : 0;
+        units = b < a.seqs ? few_units<kKind>(a, seq_of<kKind>(a, b)) : 0;
         with = sums_up_to(units);
         total = upto(a, 63);
         const uint64_t even = quotient(total + a.few_groups - 1, a.few_groups);
@@ -336,11 +425,15 @@ struct Keys {
         const uint32_t page = (uint32_t(k0) + (threadIdx.x & (kKeys - 1))) >> a.page_shift;
         entry = table[page < a.pages ? page : a.pages - 1];
     }
-    __device__ __forceinline__ void resolve(const AttendArgs& a, int32_t k0, int32_t lo, int32_t hi)
+    template <int kKind>
+    __device__ __forceinline__ void resolve(const AttendArgs& a, int32_t k0, int32_t lo, int32_t hi, int32_t from)
     {
         const int32_t k = k0 + int32_t(threadIdx.x & (kKeys - 1));
         slot = int32_t(entry);
-        ok = __ballot(held(entry, a.nslots) && k >= lo && k < hi);
+        if constexpr (kKind == kPlain)
+            ok = __ballot(held(entry, a.nslots) && k >= lo && k < hi);
+        else
+            ok = __ballot(held(entry, a.nslots) && (k >= lo || k < int32_t(a.sinks)) && k >= from && k < hi);
         if constexpr (kKeys < 64) ok &= (1ull << kKeys) - 1ull;
     }
     // Byte offset of key k0 + j's row of KV head kvh in its cache (j: this
@@ -372,10 +465,13 @@ struct Window {
         now = held(e, a.nslots) ? int32_t(e) : -1;
         ahead = entry(a, table, base + 64, hi);
     }
-    // Moves on to the page of key k (at most 64 pages).
+    // Moves on to the page of key k (kPlain: by at most 64 pages).
+    template <int kKind>
     __device__ __forceinline__ void reach(const AttendArgs& a, const int64_t* table, int32_t k, int32_t hi)
     {
         if ((uint32_t(k) >> a.page_shift) - base < 64) return;
+        if constexpr (kKind != kPlain)
+            if ((uint32_t(k) >> a.page_shift) - base >= 128) return start(a, table, k, hi);
         base += 64;
         now = held(ahead, a.nslots) ? int32_t(ahead) : -1;
         ahead = entry(a, table, base + 64, hi);
@@ -396,6 +492,19 @@ __device__ __forceinline__ uint64_t seen_bits(const AttendArgs& a, uint64_t ok, 
         ok &= first <= 0 ? ~0ull : first > 63 ? 0ull : ~0ull << first;
     }
     return ok;
+}
+
+// Bits j of the keys k0 + j below `end`, at most 64.
+__device__ __forceinline__ uint64_t bits_below(int32_t k0, int32_t end)
+{
+    const int32_t n = end - k0;
+    return n <= 0 ? 0ull : n > 63 ? ~0ull : (1ull << n) - 1ull;
+}
+
+// The same beside sinks, for a query whose last key is `last` and whose window begins at `behind`.
+__device__ __forceinline__ uint64_t seen_bits(const AttendArgs& a, uint64_t ok, int32_t k0, int32_t last, int32_t behind)
+{
+    return ok & bits_below(k0, last + 1) & (~bits_below(k0, behind) | bits_below(k0, int32_t(a.sinks)));
 }
 
 // Four dims of one row: the numerators divided by the weights' sum.  l = 0: no
@@ -419,20 +528,30 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, uint32_t t, uint3
 // over the values.  No key that is not seen takes part in anything: the way
 // out where V holds an infinity or NaN among keys that not every row of a
 // workgroup sees, which the matrix product would multiply by 0.
-template <bool kBf16>
+// (kMore and kShare: [from, to) are places of `cut`; `first` the first key of the rows' own, `last` the last.)
+template <bool kBf16, int kKind>
 __device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t, uint32_t h, uint32_t kvh, int32_t pos,
-                          int32_t from, int32_t to, bool split, float* part_o, float2* part_ml)
+                          int32_t from, int32_t to, bool split, float* part_o, float2* part_ml, const Cut& cut,
+                          int32_t first, int32_t last)
 {
     const uint32_t lane = threadIdx.x & 63u;
-    if (a.causal && to > pos + 1) to = pos + 1;
-    if (a.window && from < pos - int32_t(a.window) + 1) from = pos - int32_t(a.window) + 1;
+    const int32_t behind = pos - int32_t(a.window) + 1;
+    if constexpr (kKind == kPlain) {
+        if (a.causal && to > pos + 1) to = pos + 1;
+        if (a.window && from < behind) from = behind;
+    }
     const uint16_t* q = a.q + t * a.q_token + h * a.q_head;
     const float c = a.q_keep == 0 ? 0.0f : a.q_flip ? -a.scale_log2 : a.scale_log2;
     float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int32_t j0 = from; j0 < to; j0 += 64) {
-        const int32_t j = j0 + int32_t(lane);
+        int32_t j = j0 + int32_t(lane);
+        bool in = j < to;
+        if constexpr (kKind != kPlain) {
+            j = cut.key(j);
+            in = in && j >= first && j <= last && (!a.window || j >= behind || j < int32_t(a.sinks));
+        }
         int64_t slot = -1;
-        if (j < to) slot = table[j >> a.page_shift];
+        if (in) slot = table[j >> a.page_shift];
         const bool seen = held(slot, a.nslots);
         const uint64_t at = seen ? uint64_t(slot) * a.slot_bytes +
                                        (uint64_t(uint32_t(j) & ((1u << a.page_shift) - 1u)) * a.kv_heads + kvh) * a.dim * 2
@@ -511,10 +630,30 @@ constexpr int few_lds_bytes()
     return int(kFewWaves) * (few_wave_bytes<kDim>() + 16 * 8 + 16);
 }
 
-// Units [first, first + n) of KV head kvh of a sequence whose keys start at `lo0`; not
+// Where row r (token s.q0 + tok, query head h) of a sequence leaves its numerators and (m, l): in part
+// `slot`, or, where it is the only one of a sequence that shares a prefix, in tile_o's first part.
+template <int kKind>
+__device__ __forceinline__ void few_place(const AttendArgs& a, const Seq& s, bool whole, uint32_t slot, uint32_t r,
+                                          uint32_t tok, uint32_t h, float*& o, float2*& ml)
+{
+    uint64_t row = uint64_t(slot) * kFewRows + r;
+    o = a.few_o;
+    ml = a.few_ml;
+    if constexpr (kKind == kMore) {
+        if (whole) {
+            row = uint64_t(s.q0 + tok) * a.q_heads + h;
+            o = a.tile_o;
+            ml = a.tile_ml;
+        }
+    }
+    o += row * a.dim;
+    ml += row;
+}
+
+// Units [first, first + n) of KV head kvh of a sequence whose keys are `cut`; not
 // `whole`: into part `slot`.
-template <bool kBf16, int kDim>
-__device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, const Seq& s, uint32_t kvh, int32_t lo0,
+template <bool kBf16, int kDim, int kKind>
+__device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, const Seq& s, uint32_t kvh, const Cut& cut,
                                            uint32_t first, uint32_t n, bool whole, uint32_t slot)
 {
     constexpr int kSteps = kDim / 32;       // contraction steps of K Q^T
@@ -529,11 +668,14 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = lane & 15u, quad = lane >> 4;
     const int64_t* table = a.tables + uint64_t(s.b) * a.table_stride;
-    const int32_t k_first = lo0 + int32_t(first * kFewKeys);
+    // (kMore: k0, next and hi are places of the cut)
+    const auto key = [&](int32_t x) { return kKind == kPlain ? x : cut.key(x); };
+    const int32_t k_first = (kKind == kPlain ? cut.lo : 0) + int32_t(first * kFewKeys);
     Keys<kFewKeys> keys;
     int32_t k0 = k_first + int32_t(wave * kFewKeys);
-    keys.fetch(a, table, k0);
+    keys.fetch(a, table, key(k0));
     const uint32_t rows = s.n_new * a.group;
+    const bool out = whole && (kKind == kPlain || s.from == 0);  // nothing to be joined
 
     // Positions: row r is token r / group; the last row's token sees most.
     const uint32_t tok = col / a.group, h = kvh * a.group + (col - tok * a.group);
@@ -548,7 +690,8 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
         q[k] = (v & a.q_keep) ^ a.q_flip;
     }
     const int32_t p_last = s.base + int32_t(s.n_new) - 1;
-    const int32_t hi0 = a.causal ? keys_up_to(s, p_last) : s.len;
+    const int32_t hi_key = a.causal ? keys_up_to(s, p_last) : s.len;
+    const int32_t hi0 = kKind == kPlain ? hi_key : cut.place(hi_key);
     const int32_t hi = hi0 < k_first + int32_t(n * kFewKeys) ? hi0 : k_first + int32_t(n * kFewKeys);
     // keys below lo are behind every row's window
     const int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
@@ -559,6 +702,9 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
     f32x4 o[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i) o[i] = f32x4{0, 0, 0, 0};
+
+    const int32_t last = a.causal ? pos : kNoLast;
+    const int32_t behind = a.window ? pos - int32_t(a.window) + 1 : 0;
 
     uint32_t marks = 0;  // of V that not every row sees
     u32x4 kr[2][kSteps], vr[kLoads];
@@ -585,18 +731,19 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
             if ((keys.ok >> j & 1) && d < a.dim) vr[i] = *reinterpret_cast<const u32x4*>(a.cache_v + off + d * 2);
         }
     };
+    const int32_t hi_seen = kKind == kPlain ? hi : hi_key;
     if (k0 < hi) {
-        keys.resolve(a, k0, lo, hi);
-        keys.fetch(a, table, k0 + int32_t(kFewStep));
-        load_k(k0);
-        load_v(k0);
+        keys.template resolve<kKind>(a, key(k0), lo, hi_seen, s.from);
+        keys.fetch(a, table, key(k0 + int32_t(kFewStep)));
+        load_k(key(k0));
+        load_v(key(k0));
     }
     for (; k0 < hi; k0 += int32_t(kFewStep)) {
         const uint64_t ok = keys.ok;
         const int32_t next = k0 + int32_t(kFewStep);
         if (next < hi) {
-            keys.resolve(a, next, lo, hi);
-            keys.fetch(a, table, next + int32_t(kFewStep));
+            keys.template resolve<kKind>(a, key(next), lo, hi_seen, s.from);
+            keys.fetch(a, table, key(next + int32_t(kFewStep)));
         }
         f32x4 st[2];
 #pragma unroll
@@ -605,7 +752,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) st[y] = mfma16<kBf16>(kr[y][k], q[k], st[y]);
         }
-        if (next < hi) load_k(next);
+        if (next < hi) load_k(key(next));
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t c = 64 * i + lane;
@@ -614,15 +761,17 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
         // Keys that some rows see and others do not: an infinity or NaN in their
         // V would meet a weight of 0.
         const bool partial =
-            s.n_new > 1 && ((a.causal && k0 + int32_t(kFewKeys) - 1 > s.base) ||
-                            (a.window && k0 <= p_last - int32_t(a.window)));
+            s.n_new > 1 && ((a.causal && key(k0) + int32_t(kFewKeys) - 1 > s.base) ||
+                            (a.window && key(k0) <= p_last - int32_t(a.window)));
         if (partial) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) marks |= nonfinite_marks<kBf16>(vr[i]);
         }
-        if (next < hi) load_v(next);
+        if (next < hi) load_v(key(next));
 
-        const uint32_t mine = uint32_t(partial ? seen_bits(a, ok, k0, pos) : ok) >> (4 * quad);
+        uint64_t seen = ok;
+        if (partial) seen = kKind == kPlain ? seen_bits(a, ok, k0, pos) : seen_bits(a, ok, key(k0), last, behind);
+        const uint32_t mine = uint32_t(seen) >> (4 * quad);
         float top = -INFINITY;
 #pragma unroll
         for (int y = 0; y < 2; ++y)
@@ -669,9 +818,12 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
     if (s.n_new > 1 && (odd[0] | odd[1] | odd[2] | odd[3])) {
         for (uint32_t x = wave; x < rows; x += kFewWaves) {
             const uint32_t xt = x / a.group, xh = kvh * a.group + (x - xt * a.group);
-            const uint64_t row = uint64_t(slot) * kFewRows + x;
-            plain_row<kBf16>(a, table, s.q0 + xt, xh, kvh, s.base + int32_t(xt), k_first, hi, !whole,
-                             a.few_o + row * a.dim, a.few_ml + row);
+            const int32_t xp = s.base + int32_t(xt);
+            float* o_at;
+            float2* ml_at;
+            few_place<kKind>(a, s, whole, slot, x, xt, xh, o_at, ml_at);
+            plain_row<kBf16, kKind>(a, table, s.q0 + xt, xh, kvh, xp, k_first, hi, !out, o_at, ml_at, cut, s.from,
+                                    a.causal ? xp : kNoLast);
         }
         return;
     }
@@ -700,10 +852,12 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
             acc += *reinterpret_cast<const f32x4*>(lds + w * kWaveBytes + (r * kOPitch + d) * 4) * f;
         }
         const uint32_t rt = r / a.group, rh = kvh * a.group + (r - rt * a.group);
-        if (!whole) {
-            const uint64_t row = uint64_t(slot) * kFewRows + r;
-            *reinterpret_cast<f32x4*>(a.few_o + row * a.dim + d) = acc;
-            if (d == 0) a.few_ml[row] = float2{safe * a.scale_log2, sum};
+        if (!out) {
+            float* o_at;
+            float2* ml_at;
+            few_place<kKind>(a, s, whole, slot, r, rt, rh, o_at, ml_at);
+            *reinterpret_cast<f32x4*>(o_at + d) = acc;
+            if (d == 0) *ml_at = float2{safe * a.scale_log2, sum};
         } else {
             store_out<kBf16>(a, s.q0 + rt, rh, d, acc, sum, safe * a.scale_log2);
         }
@@ -714,14 +868,14 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
 // sequence and KV head, in place `group`; without, consecutive units of all of them:
 // where a part begins in an earlier workgroup it is in this one's place
 // 2 group, where it goes on in the next in place 2 group + 1.
-template <bool kBf16, int kDim>
+template <bool kBf16, int kDim, int kKind>
 __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* lds, uint32_t group)
 {
     if (a.q_starts && group == 0) zero_unowned<kBf16>(a);
     Few w;
     uint64_t at = 0, to = 1, per = a.few_per;
     if (!per) {
-        w.start(a);
+        w.template start<kKind>(a);
         per = w.per;
         at = group * per;
         to = at + per < w.total ? at + per : w.total;
@@ -747,16 +901,16 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
             if (alone && first > 0) continue;
             place = 2 * group + (first == 0);
         }
-        const Seq s = seq_of(a, b);
+        const Seq s = seq_of<kKind>(a, b);
         if (a.few_per) {
-            units = few_units(a, s);
+            units = few_units<kKind>(a, s);
             if (first >= units) return;
             n = units - first < a.few_per ? units - first : a.few_per;
         }
         if (first == 0 && a.few_parts && threadIdx.x == 0)
             a.few_parts[b * a.kv_heads + kvh] = uint2{place, 1 + uint32_t(quotient(units - n + per - 1, per))};
         if (again) __syncthreads();  // the last ones' results in LDS have been read
-        attend_few<kBf16, kDim>(a, lds, s, kvh, cut_of(a, s, kFewKeys).lo, first, n, n == units, place);
+        attend_few<kBf16, kDim, kKind>(a, lds, s, kvh, cut_of<kKind>(a, s, kFewKeys, kFewKeys), first, n, n == units, place);
     }
 }
 
@@ -777,6 +931,48 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
 // numerators only past 2^8, V's order in LDS, unpredicated whole pages and matrix instructions
 // first took it from 2,430 to 2,168, loads straight to LDS to 2,040.  Computing the next step's scores
 // beside this one's weights gained nothing (2,341 and 2,316 then).
+// The sequence of the group that token t is of (every lane its own).
+__device__ __forceinline__ Seq owner_of(const AttendArgs& a, const Group& g, uint32_t t)
+{
+    uint32_t b = t;
+    if (a.q_starts) {
+        // the last one of [first, end) that starts at or before t
+        uint32_t at = g.first;
+        for (uint32_t n = g.end - g.first; n;) {
+            const uint32_t half = n / 2;
+            const bool up = start_of(a, at + half) <= t;
+            at = up ? at + half + 1 : at;
+            n = up ? n - half - 1 : half;
+        }
+        b = at > g.first ? at - 1 : g.first;
+    }
+    return seq_of(a, b);
+}
+
+// The least x of the wave, and of the workgroup's waves (which all call it before anything lies in LDS).
+__device__ __forceinline__ int32_t least_of(int32_t x)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const int32_t y = __shfl_xor(x, d);
+        x = y < x ? y : x;
+    }
+    return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int32_t tile_least(uint8_t* lds, uint32_t wave, int32_t x)
+{
+    volatile int32_t* const each = reinterpret_cast<volatile int32_t*>(lds);
+    if ((threadIdx.x & 63u) == 0) each[wave] = x;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kTileWaves; ++w) {
+        const int32_t y = each[w];
+        x = y < x ? y : x;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
 template <int kDim>
 constexpr int tile_chunks()  // 16-byte chunks of an LDS row
 {
@@ -800,7 +996,9 @@ constexpr int tile_lds_bytes()  // two buffers of K and V
     return 2 * (k_bytes<kDim>() + int(kTileKeys) * tile_chunks<kDim>() * 16);
 }
 
-template <bool kBf16, int kDim>
+// kShare: the same over (128 rows of all the tokens of a group of sequences, part of the prefix they share);
+// the rows differ in what they see of it.
+template <bool kBf16, int kDim, int kKind>
 __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, uint32_t group, uint32_t groups)
 {
     constexpr int kChunks = tile_chunks<kDim>();
@@ -815,7 +1013,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>((lds_void*)lds));
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = lane & 31u, half = lane >> 5;
-    if (a.q_starts && a.few_rows == 0 && group == 0) zero_unowned<kBf16>(a);
+    if (kKind != kShare && a.q_starts && a.few_rows == 0 && group == 0) zero_unowned<kBf16>(a);
 
     // A column is one KV head's part of the keys, over all tiles.  Workgroup i
     // runs on XCD i % 8: whole columns go to one XCD, whose L2 then holds their
@@ -823,31 +1021,37 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     // have come last; where the columns do not fill the XCDs evenly, each XCD
     // takes an eighth of the list.
     const uint32_t xcd = group % 8, nth = group / 8;
-    const uint32_t columns = groups / a.tiles;
+    const uint32_t tiles = kKind == kShare ? a.share_tiles : a.tiles;
+    const uint32_t columns = groups / tiles;
     uint32_t column, tile;
     if (columns % 8 == 0) {
-        const uint32_t deal = nth / a.tiles;
+        const uint32_t deal = nth / tiles;
         column = 8 * deal + (deal % 2 ? 7 - xcd : xcd);
-        tile = nth % a.tiles;
+        tile = nth % tiles;
     } else {
         const uint32_t x8 = groups / 8, r8 = groups % 8;
         const uint32_t w = xcd * x8 + (xcd < r8 ? xcd : r8) + nth;
-        column = w / a.tiles;
-        tile = w % a.tiles;
+        column = w / tiles;
+        tile = w % tiles;
     }
-    tile = a.tiles - 1 - tile;  // the last tiles see most keys: first
+    tile = tiles - 1 - tile;  // the last tiles see most keys: first
     const uint32_t kvh = column % a.kv_heads, part = column / a.kv_heads;
 
     // Sequence b's tiles start at floor(q_starts[b] * group / rows) + b, which
-    // leaves it at least the tiles it needs.
+    // leaves it at least the tiles it needs.  (kShare: b is a group.)
     uint32_t b = tile;
     uint32_t first_tile = tile;
-    if (a.q_starts) {
+    if (kKind == kShare || a.q_starts) {
+        const uint32_t n = kKind == kShare ? a.groups : a.seqs;
         uint32_t at_or_before = 0;
-        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
+        for (uint32_t s0 = 0; s0 < n; s0 += 64) {
             const uint32_t s = s0 + lane;
-            const uint32_t f = s < a.seqs ? uint32_t(uint64_t(start_of(a, s)) * a.group / kTileRows) + s : 0;
-            const uint64_t le = __ballot(s < a.seqs && f <= tile);
+            uint32_t f = 0;
+            if (s < n) {
+                const uint32_t row = kKind == kShare ? rows_at(a, group_at(a, s).first) : start_of(a, s);
+                f = uint32_t(uint64_t(row) * a.group / kTileRows) + s;
+            }
+            const uint64_t le = __ballot(s < n && f <= tile);
             at_or_before += __popcll(le);
             if (le) first_tile = __builtin_amdgcn_readfirstlane(__shfl(f, 63 - __clzll(le)));
         }
@@ -857,23 +1061,53 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         b = tile / ((a.group + kTileRows - 1) / kTileRows);
         first_tile = b * ((a.group + kTileRows - 1) / kTileRows);
     }
-    const Seq s = seq_of(a, b);
+    Group g{b, b + 1, 0};
+    Seq s;  // kShare: all the group's tokens, and its prefix
+    if constexpr (kKind == kShare) {
+        g = group_at(a, b);
+        if (g.prefix == 0) return;
+        s.b = g.first;
+        s.q0 = rows_at(a, g.first);
+        const uint32_t end = rows_at(a, g.end);
+        s.n_new = end > s.q0 ? end - s.q0 : 0;
+        s.len = g.prefix;
+        s.base = s.from = 0;
+    } else {
+        s = seq_of<kKind>(a, b);
+    }
     const uint32_t rows = s.n_new * a.group;
     const uint32_t r0 = (tile - first_tile) * kTileRows;
-    if (rows <= a.few_rows || r0 >= rows) return;
-    const Cut cut = cut_of(a, s, a.tile_per);
+    if ((kKind != kShare && rows <= a.few_rows) || r0 >= rows) return;
+    const uint32_t per = kKind == kShare ? share_part(s.len, a.share_split) : a.tile_per;
+    Cut cut;
+    if constexpr (kKind == kShare) {
+        cut.lo = cut.head_lo = cut.head = 0;
+        cut.parts = (uint32_t(s.len) + per - 1) / per;
+    } else {
+        cut = cut_of<kKind>(a, s, per);
+    }
     if (part > 0 && part >= cut.parts) return;
-    const int64_t* table = a.tables + uint64_t(b) * a.table_stride;
+    const int64_t* table = a.tables + uint64_t(s.b) * a.table_stride;
 
     const uint32_t r_last = (r0 + kTileRows < rows ? r0 + kTileRows : rows) - 1;
     const int32_t p_first = s.base + int32_t(r0 / a.group), p_last = s.base + int32_t(r_last / a.group);
     // of this wave's rows (rows past the last repeat it)
     const uint32_t w_first = r0 + wave * 32 < rows ? r0 + wave * 32 : r_last;
     const uint32_t w_last = w_first + 31 < r_last ? w_first + 31 : r_last;
-    const int32_t pw_first = s.base + int32_t(w_first / a.group), pw_last = s.base + int32_t(w_last / a.group);
+    int32_t pw_first = s.base + int32_t(w_first / a.group), pw_last = s.base + int32_t(w_last / a.group);
     const uint32_t r = r0 + wave * 32 + col;
     const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
-    const int32_t pos = s.base + int32_t(tok);
+    int32_t pos = s.base + int32_t(tok);
+    int32_t last = a.causal ? pos : kNoLast;  // the row's last key and its window's first
+    if constexpr (kKind == kShare) {
+        last = kNoLast;
+        if (r < rows) {
+            const Seq mine = owner_of(a, g, s.q0 + tok);
+            pos = mine.base + int32_t(s.q0 + tok - mine.q0);
+            last = a.causal && pos < mine.len ? pos : mine.len - 1;
+        }
+    }
+    const int32_t behind = a.window ? (pos < int32_t(a.window) ? 0 : pos - int32_t(a.window) + 1) : 0;
     u32x4 q[kSteps];
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
@@ -883,12 +1117,43 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
             v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
         q[k] = (v & a.q_keep) ^ a.q_flip;
     }
-    int32_t hi = a.causal ? keys_up_to(s, p_last) : s.len;
-    int32_t k0 = cut.lo + int32_t(part * a.tile_per);
-    if (hi - k0 > int32_t(a.tile_per)) hi = k0 + int32_t(a.tile_per);
-    const int32_t lo = a.window ? p_first - int32_t(a.window) + 1 : 0;  // behind every row's window below
-    if (a.window && lo > k0) k0 = lo & ~int32_t(kTileKeys - 1);
+    // The tile's keys: from k0 (behind every row's window below lo) to hi.  kMore and kShare: k0, k_first and
+    // k_end are places of the cut, from k_skip on those below k_lo are behind every window.
+    const int32_t hi_all = a.causal && kKind != kShare ? keys_up_to(s, p_last) : s.len;
+    int32_t hi = hi_all, lo, k_skip = 0, k_lo = 0;
+    const int32_t k_first = (kKind == kPlain ? cut.lo : 0) + int32_t(part * per);
+    int32_t k0 = k_first, k_end;
+    if constexpr (kKind == kPlain) {
+        if (hi - k0 > int32_t(per)) hi = k0 + int32_t(per);
+        lo = a.window ? p_first - int32_t(a.window) + 1 : 0;
+        if (a.window && lo > k0) k0 = lo & ~int32_t(kTileKeys - 1);
+        k_end = hi;
+    } else {
+        // what some rows of the wave, and all rows of the tile, do not see
+        if constexpr (kKind == kShare) {
+            const bool row = r < rows;
+            pw_first = least_of(last);
+            pw_last = a.window ? -least_of(row ? -behind : 0) + int32_t(a.window) - 1 : 0;
+            lo = a.window ? tile_least(lds, wave, least_of(row ? behind : kNoLast)) : 0;
+        } else {
+            lo = a.window && p_first >= int32_t(a.window) ? p_first - int32_t(a.window) + 1 : 0;
+        }
+        k_skip = cut.place((int32_t(a.sinks) + int32_t(kTileKeys) - 1) & ~int32_t(kTileKeys - 1));
+        k_lo = lo > cut.lo ? cut.head + ((lo - cut.lo) & ~int32_t(kTileKeys - 1)) : 0;
+        k_end = cut.place(hi);
+        if (k_end - k0 > int32_t(per)) k_end = k0 + int32_t(per);
+        if (k0 >= k_skip && k0 < k_lo) k0 = k_lo;
+    }
+    const auto key = [&](int32_t x) { return kKind == kPlain ? x : cut.key(x); };
+    const auto step_from = [&](int32_t x) {
+        x += int32_t(kTileKeys);
+        if (kKind != kPlain && x >= k_skip && x < k_lo) x = k_lo;
+        return x;
+    };
 
+    const bool out = kKind != kShare && cut.parts <= 1 && s.from == 0;  // nothing to be joined
+    float* const part_o = kKind == kShare ? a.share_o : a.tile_o;
+    float2* const part_ml = kKind == kShare ? a.share_ml : a.tile_ml;
     f32x16 o[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i)
@@ -920,7 +1185,12 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     // The keys of [kb, kb + 64) that may be read: on held pages, in [lo, hi).
     const auto readable = [&](int32_t kb) {
         uint64_t ok = ~0ull;
-        if (kb < lo) ok <<= lo - kb;
+        if constexpr (kKind == kPlain) {
+            if (kb < lo) ok <<= lo - kb;
+        } else {
+            if (kb < s.from) ok <<= s.from - kb;
+            if (kb < lo) ok &= ~bits_below(kb, lo) | bits_below(kb, int32_t(a.sinks));
+        }
         if (hi - kb < 64) ok &= ~0ull >> (64 - (hi - kb));
         if (in_page) return pages.slot(uint32_t(kb) >> a.page_shift) >= 0 ? ok : 0ull;
         return ok & __ballot(pages.slot_of(uint32_t(kb + int32_t(lane)) >> a.page_shift) >= 0);
@@ -929,9 +1199,10 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     // Whole steps go from memory to LDS; a step with keys that may not be read
     // comes through registers, which hold zeros for those.
     const uint32_t k_chunk = place ^ k_order(row0), v_chunk = place ^ v_order(row0);
-    const auto fill = [&](int buf, int32_t kb) -> uint64_t {
-        if (kb >= hi) return 0;
-        pages.reach(a, table, kb, hi);
+    const auto fill = [&](int buf, int32_t kx) -> uint64_t {
+        if (kx >= k_end) return 0;
+        const int32_t kb = key(kx);
+        pages.template reach<kKind>(a, table, kb, hi);
         const uint64_t ok = readable(kb);
         const uint32_t k_to = __builtin_amdgcn_readfirstlane(lds_at + buf * kBufBytes + wave * kGroup);
         const uint32_t v_to = __builtin_amdgcn_readfirstlane(lds_at + buf * kBufBytes + kKBytes + wave * 1024);
@@ -996,16 +1267,16 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         const uint32_t d = 32 * i + (lane & 16u) + 4 * (lane & 3u);
         v_read[i] = lds_at + kKBytes + v_row * (kChunks * 16) + (((d / 8) ^ v_order(v_row)) * 8 + d % 8) * 2;
     }
-    pages.start(a, table, k0, hi);
+    pages.start(a, table, key(k0), hi);
     uint64_t ok_next = fill(0, k0);
     int buf = 0;
-    for (; k0 < hi; k0 += int32_t(kTileKeys)) {
+    for (; k0 < k_end; k0 = step_from(k0)) {
         // This step's K and V are there, and every wave is done with the other
         // buffer: the next step's go into it.
         wait_loads();
         __syncthreads();
         const uint64_t ok = ok_next;
-        ok_next = fill(1 - buf, k0 + int32_t(kTileKeys));
+        ok_next = fill(1 - buf, step_from(k0));
         const uint32_t in_buf = buf * kBufBytes;
         const uint32_t k_even = k_read[0] + in_buf, k_odd = k_read[1] + in_buf;
         // The matrix instructions go first where two workgroups' waves meet on
@@ -1025,11 +1296,11 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
             }
         __builtin_amdgcn_s_setprio(0);
         // Keys that some of the wave's rows see and others do not.
-        const bool partial = (a.causal && k0 + int32_t(kTileKeys) - 1 > pw_first) ||
-                             (a.window && k0 <= pw_last - int32_t(a.window));
+        const bool partial = ((kKind == kShare || a.causal) && key(k0) + int32_t(kTileKeys) - 1 > pw_first) ||
+                             (a.window && key(k0) <= pw_last - int32_t(a.window));
         uint64_t seen = ok;
         if (partial || ok != ~0ull) {
-            if (partial) seen = seen_bits(a, ok, k0, pos);
+            if (partial) seen = kKind == kPlain ? seen_bits(a, ok, k0, pos) : seen_bits(a, ok, key(k0), last, behind);
             const uint64_t mine = seen >> (4 * half);
 #pragma unroll
             for (int y = 0; y < 2; ++y)
@@ -1105,8 +1376,14 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         for (uint32_t x = r0 + wave * 32; x < r0 + wave * 32 + 32 && x < rows; ++x) {
             const uint32_t xt = x / a.group, xh = kvh * a.group + (x - xt * a.group);
             const uint64_t row = (uint64_t(part) * a.tokens + s.q0 + xt) * a.q_heads + xh;
-            plain_row<kBf16>(a, table, s.q0 + xt, xh, kvh, s.base + int32_t(xt), cut.lo + int32_t(part * a.tile_per), hi,
-                             cut.parts > 1, a.tile_o + row * a.dim, a.tile_ml + row);
+            int32_t xp = s.base + int32_t(xt), x_last = a.causal ? xp : kNoLast;
+            if constexpr (kKind == kShare) {
+                const Seq mine = owner_of(a, g, s.q0 + xt);
+                xp = mine.base + int32_t(s.q0 + xt - mine.q0);
+                x_last = a.causal && xp < mine.len ? xp : mine.len - 1;
+            }
+            plain_row<kBf16, kKind>(a, table, s.q0 + xt, xh, kvh, xp, k_first, k_end, !out, part_o + row * a.dim,
+                                    part_ml + row, cut, s.from, x_last);
         }
         return;
     }
@@ -1114,16 +1391,16 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     if (r >= rows) return;
     const uint32_t t = s.q0 + tok;
     const float shift = m == -INFINITY ? 0.0f : m * a.scale_log2;
-    if (cut.parts > 1) {
+    if (!out) {
         const uint64_t row = (uint64_t(part) * a.tokens + t) * a.q_heads + h;
-        if (half == 0) a.tile_ml[row] = float2{shift, l};
+        if (half == 0) part_ml[row] = float2{shift, l};
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const uint32_t d = 32 * i + 2 * e + 4 * half;
                 if (d < a.dim)
-                    *reinterpret_cast<f32x4*>(a.tile_o + row * a.dim + d) =
+                    *reinterpret_cast<f32x4*>(part_o + row * a.dim + d) =
                         f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
             }
     } else {
@@ -1142,57 +1419,102 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
 
 // (Three waves a SIMD for heads up to 64: tiles over 32,768 keys 365 us, two 442; for heads of 128 the
 // few-row kernel spills: 125 us where two take 54.)
-template <bool kBf16, int kDim>
+template <bool kBf16, int kDim, int kKind>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim > 64 ? 2 : 3) void attend_few_kernel(AttendArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds_bytes<kDim>()];
-    attend_few_units<kBf16, kDim>(a, lds, blockIdx.x);
+    attend_few_units<kBf16, kDim, kKind>(a, lds, blockIdx.x);
 }
 
-template <bool kBf16, int kDim>
+template <bool kBf16, int kDim, int kKind>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim > 64 ? 2 : 3) void attend_tile_kernel(AttendArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[tile_lds_bytes<kDim>()];
-    attend_tile<kBf16, kDim>(a, lds, blockIdx.x, gridDim.x);
+    attend_tile<kBf16, kDim, kKind>(a, lds, blockIdx.x, gridDim.x);
 }
 
 // Both kinds of sequences in one launch: the tiles' workgroups first, which take
 // longest, and the few-row ones beside and after them.
-template <bool kBf16, int kDim>
+template <int kDim>
+constexpr int mixed_lds_bytes()
+{
+    return tile_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? tile_lds_bytes<kDim>() : few_lds_bytes<kDim>();
+}
+
+template <bool kBf16, int kDim, int kKind>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(AttendArgs a)
 {
-    constexpr int kBytes = tile_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? tile_lds_bytes<kDim>() : few_lds_bytes<kDim>();
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[mixed_lds_bytes<kDim>()];
     const uint32_t tiles = a.tiles * a.kv_heads * a.tile_split;
     if (blockIdx.x < tiles) {
-        attend_tile<kBf16, kDim>(a, lds, blockIdx.x, tiles);
+        attend_tile<kBf16, kDim, kKind>(a, lds, blockIdx.x, tiles);
     } else {
-        attend_few_units<kBf16, kDim>(a, lds, blockIdx.x - tiles);
+        attend_few_units<kBf16, kDim, kKind>(a, lds, blockIdx.x - tiles);
+    }
+}
+
+// The groups' prefixes first, then each sequence's own keys.
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_shared_kernel(AttendArgs a)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t lds[mixed_lds_bytes<kDim>()];
+    const uint32_t share = a.share_tiles * a.kv_heads * a.share_split, tiles = a.tiles * a.kv_heads * a.tile_split;
+    if (blockIdx.x < share) {
+        attend_tile<kBf16, kDim, kShare>(a, lds, blockIdx.x, share);
+    } else if (blockIdx.x - share < tiles) {
+        attend_tile<kBf16, kDim, kMore>(a, lds, blockIdx.x - share, tiles);
+    } else {
+        attend_few_units<kBf16, kDim, kMore>(a, lds, blockIdx.x - share - tiles);
     }
 }
 
 // ---------------------------------------------------------------- parts joined
 
-// Where a row's parts are, and how many.
+// Where a row's parts are, and how many: of its prefix (kMore: the first `share` ones), then of
+// its sequence's own keys.
 struct Parts {
     const float2* ml;
     const float* o;
     uint64_t step;  // rows from one part to the next
     uint32_t back;  // rows that the parts after the first lie before that
     uint32_t parts;
+    uint32_t share;
+    uint64_t row0;  // of the prefix's first part
 
     __device__ __forceinline__ uint64_t row(uint32_t n) const { return n * step - (n == 0 ? 0 : back); }
+    template <int kKind>
+    __device__ __forceinline__ float2 sums(const AttendArgs& a, uint32_t n) const
+    {
+        if (kKind == kMore && n < share) return a.share_ml[row0 + n * uint64_t(a.tokens) * a.q_heads];
+        return ml[row(n - share)];
+    }
+    template <int kKind>
+    __device__ __forceinline__ f32x4 four(const AttendArgs& a, uint32_t n, uint32_t d) const
+    {
+        if (kKind == kMore && n < share)
+            return *reinterpret_cast<const f32x4*>(a.share_o + (row0 + n * uint64_t(a.tokens) * a.q_heads) * a.dim + d);
+        return *reinterpret_cast<const f32x4*>(o + row(n - share) * a.dim + d);
+    }
 };
 
+template <int kKind>
 __device__ __forceinline__ Parts parts_of(const AttendArgs& a, uint32_t b, uint32_t t, uint32_t h)
 {
-    Parts p{nullptr, nullptr, 0, 0, 0};
+    Parts p{nullptr, nullptr, 0, 0, 0, 0, 0};
     const uint32_t kvh = h / a.group;
     // (nothing the few-row kernel wrote where the sequence is not its)
     const uint2 few_parts = a.few_parts ? a.few_parts[uint64_t(b) * a.kv_heads + kvh] : uint2{0, 0};
-    const Seq s = seq_of(a, b);
+    const Seq s = seq_of<kKind>(a, b);
     if (t < s.q0 || t >= s.q0 + s.n_new) return p;
-    if (s.n_new * a.group <= a.few_rows) {
+    if constexpr (kKind == kMore) {
+        if (s.from > 0) {
+            const uint32_t per = share_part(uint32_t(s.from), a.share_split);
+            p.share = (uint32_t(s.from) + per - 1) / per;
+            p.row0 = uint64_t(t) * a.q_heads + h;
+        }
+    }
+    const bool few = s.n_new * a.group <= a.few_rows;
+    if (few && (kKind == kPlain || (a.few_parts && few_parts.y > 1))) {
         const uint64_t row = uint64_t(few_parts.x) * kFewRows + (t - s.q0) * a.group + (h - kvh * a.group);
         p.parts = few_parts.y;
         // a place a workgroup apart: first ones with few_per; else see attend_few_units
@@ -1202,11 +1524,13 @@ __device__ __forceinline__ Parts parts_of(const AttendArgs& a, uint32_t b, uint3
         p.o = a.few_o + row * a.dim;
     } else {
         const uint64_t row = uint64_t(t) * a.q_heads + h;
-        p.parts = cut_of(a, s, a.tile_per).parts;
+        p.parts = few ? 1 : cut_of<kKind>(a, s, a.tile_per).parts;
+        if (kKind == kMore && p.parts == 0) p.parts = 1;
         p.step = uint64_t(a.tokens) * a.q_heads;
         p.ml = a.tile_ml + row;
         p.o = a.tile_o + row * a.dim;
     }
+    p.parts += p.share;
     return p;
 }
 
@@ -1230,7 +1554,7 @@ constexpr uint32_t row_lanes()
 
 // Many rows: row_lanes lanes per (token, query head), the parts one after
 // another.
-template <bool kBf16, int kDim>
+template <bool kBf16, int kDim, int kKind>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
 {
     constexpr uint32_t kLanes = row_lanes<kDim>(), kRows = 64 / kLanes, kHeld = kMaxSplit / kLanes, kAhead = 4;
@@ -1246,8 +1570,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
     } else {
         b = t < a.seqs ? t : a.seqs - 1;
     }
-    Parts p{nullptr, nullptr, 0, 0, 0};
-    if (th < rows) p = parts_of(a, b, t, h);
+    Parts p{nullptr, nullptr, 0, 0, 0, 0, 0};
+    if (th < rows) p = parts_of<kKind>(a, b, t, h);
     const uint32_t parts = p.parts > 1 ? p.parts : 0;
     if (__ballot(parts != 0) == 0) return;
     float2 v[kHeld];
@@ -1255,7 +1579,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
 #pragma unroll
     for (uint32_t i = 0; i < kHeld; ++i) {
         v[i] = float2{0.0f, 0.0f};
-        if (i * kLanes + sub < parts) v[i] = p.ml[p.row(i * kLanes + sub)];
+        if (i * kLanes + sub < parts) v[i] = p.template sums<kKind>(a, i * kLanes + sub);
         if (v[i].y != 0.0f) top = fmaxf(top, v[i].x);
     }
 #pragma unroll
@@ -1279,7 +1603,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
             for (uint32_t x = 0; x < kAhead; ++x) {
                 const uint32_t n = i * kLanes + p0 + x;
                 part[x] = f32x4{0, 0, 0, 0};
-                if (n < parts && d < a.dim) part[x] = *reinterpret_cast<const f32x4*>(p.o + p.row(n) * a.dim + d);
+                if (n < parts && d < a.dim) part[x] = p.template four<kKind>(a, n, d);
             }
 #pragma unroll
             for (uint32_t x = 0; x < kAhead; ++x) {
@@ -1293,7 +1617,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
 
 // Few rows: a workgroup per (token, query head), its groups of row_lanes lanes
 // taking every so-many-th part each, summed in their order at the end.
-template <bool kBf16, int kDim>
+template <bool kBf16, int kDim, int kKind>
 __global__ __launch_bounds__(256, 6) void attend_join_row_kernel(AttendArgs a)
 {
     constexpr uint32_t kLanes = row_lanes<kDim>(), kStride = 256 / kLanes, kMost = kMaxSplit / kStride;
@@ -1301,17 +1625,17 @@ __global__ __launch_bounds__(256, 6) void attend_join_row_kernel(AttendArgs a)
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t t = blockIdx.x / a.q_heads, h = blockIdx.x - t * a.q_heads;
     const uint32_t b = seq_at(a, t);
-    const Parts p = parts_of(a, b, t, h);
+    const Parts p = parts_of<kKind>(a, b, t, h);
     if (p.parts <= 1) return;
     float2 v{0.0f, 0.0f};
-    if (lane < p.parts) v = p.ml[p.row(lane)];
+    if (lane < p.parts) v = p.template sums<kKind>(a, lane);
     const uint32_t which = threadIdx.x / kLanes, d = lane % kLanes * 4;
     f32x4 part[kMost];
 #pragma unroll
     for (uint32_t i = 0; i < kMost; ++i) {
         part[i] = f32x4{0, 0, 0, 0};
         const uint32_t n = which + i * kStride;
-        if (n < p.parts && d < a.dim) part[i] = *reinterpret_cast<const f32x4*>(p.o + p.row(n) * a.dim + d);
+        if (n < p.parts && d < a.dim) part[i] = p.template four<kKind>(a, n, d);
     }
     float top = v.y == 0.0f ? -INFINITY : v.x;
 #pragma unroll
@@ -1359,34 +1683,44 @@ bool attend_ok(const si_paged_attention_desc& d)
     return true;
 }
 
-template <bool kBf16, int kDim>
+template <bool kBf16, int kDim, int kKind>
 hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
 {
     const dim3 block(256);
     const uint32_t tiles = p.tile ? p.tiles * a.kv_heads * p.tile_split : 0;
+    const uint32_t share = p.share_tiles * a.kv_heads * p.share_split;
     hipError_t e;
-    if (p.few && p.tile) {
-        e = launch(attend_mixed_kernel<kBf16, kDim>, dim3(tiles + p.few_groups), block, stream, a);
+    if (share) {
+        e = launch(attend_shared_kernel<kBf16, kDim>, dim3(share + tiles + (p.few ? p.few_groups : 0)), block, stream, a);
+    } else if (p.few && p.tile) {
+        e = launch(attend_mixed_kernel<kBf16, kDim, kKind>, dim3(tiles + p.few_groups), block, stream, a);
     } else if (p.few) {
-        e = launch(attend_few_kernel<kBf16, kDim>, dim3(p.few_groups), block, stream, a);
+        e = launch(attend_few_kernel<kBf16, kDim, kKind>, dim3(p.few_groups), block, stream, a);
     } else {
-        e = launch(attend_tile_kernel<kBf16, kDim>, dim3(tiles), block, stream, a);
+        e = launch(attend_tile_kernel<kBf16, kDim, kKind>, dim3(tiles), block, stream, a);
     }
     if (e == hipSuccess && p.bytes) {
         const uint32_t rows = a.tokens * a.q_heads, each = 256 / row_lanes<kDim>();
-        e = rows <= kJoinRows ? launch(attend_join_row_kernel<kBf16, kDim>, dim3(rows), block, stream, a)
-                              : launch(attend_join_kernel<kBf16, kDim>, dim3((rows + each - 1) / each), block, stream, a);
+        e = rows <= kJoinRows
+                ? launch(attend_join_row_kernel<kBf16, kDim, kKind>, dim3(rows), block, stream, a)
+                : launch(attend_join_kernel<kBf16, kDim, kKind>, dim3((rows + each - 1) / each), block, stream, a);
     }
     return e;
 }
 
-template <bool kBf16>
+template <bool kBf16, int kKind>
 hipError_t attend_by_dim(hipStream_t stream, const AttendArgs& a, const Plan& p)
 {
-    if (a.dim <= 64) return attend_launch<kBf16, 64>(stream, a, p);
-    if (a.dim <= 96) return attend_launch<kBf16, 96>(stream, a, p);
-    if (a.dim <= 128) return attend_launch<kBf16, 128>(stream, a, p);
-    return attend_launch<kBf16, 256>(stream, a, p);
+    if (a.dim <= 64) return attend_launch<kBf16, 64, kKind>(stream, a, p);
+    if (a.dim <= 96) return attend_launch<kBf16, 96, kKind>(stream, a, p);
+    if (a.dim <= 128) return attend_launch<kBf16, 128, kKind>(stream, a, p);
+    return attend_launch<kBf16, 256, kKind>(stream, a, p);
+}
+
+bool more_ok(const si_paged_attention_more* m)
+{
+    if (!m) return true;
+    return m->sinks <= (1u << 30) && m->groups < (1u << 26) && (!m->groups || (m->group_starts && m->prefix_lens));
 }
 
 }  // namespace
@@ -1395,18 +1729,30 @@ hipError_t attend_by_dim(hipStream_t stream, const AttendArgs& a, const Plan& p)
 
 extern "C" {
 
+uint64_t secure_infer_gpu_paged_attention_more_workspace(const si_paged_attention_desc* d,
+                                                         const si_paged_attention_more* more)
+{
+    if (!d || !si::attend_ok(*d) || !si::more_ok(more)) return UINT64_MAX;
+    const si::Plan p = si::attend_plan(*d, more);
+    return p.fits ? p.bytes : UINT64_MAX;
+}
+
 uint64_t secure_infer_gpu_paged_attention_workspace(const si_paged_attention_desc* d)
 {
-    if (!d || !si::attend_ok(*d)) return UINT64_MAX;
-    const si::Plan p = si::attend_plan(*d);
-    return p.fits ? p.bytes : UINT64_MAX;
+    return secure_infer_gpu_paged_attention_more_workspace(d, nullptr);
 }
 
 int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attention_desc* d)
 {
+    return secure_infer_gpu_paged_attention_more(stream, d, nullptr);
+}
+
+int secure_infer_gpu_paged_attention_more(hipStream_t stream, const si_paged_attention_desc* d,
+                                          const si_paged_attention_more* more)
+{
     using namespace si;
-    if (!d || !attend_ok(*d)) return -1;
-    const Plan p = attend_plan(*d);
+    if (!d || !attend_ok(*d) || !more_ok(more)) return -1;
+    const Plan p = attend_plan(*d, more);
     if (!p.fits) return -1;
     if (p.bytes && (!d->workspace || d->workspace_bytes < p.bytes || !aligned(d->workspace, 16))) return -1;
     AttendArgs a{};
@@ -1452,8 +1798,23 @@ int secure_infer_gpu_paged_attention(hipStream_t stream, const si_paged_attentio
     a.few_parts = p.few_ml ? reinterpret_cast<uint2*>(ws + p.few_parts) : nullptr;
     a.tile_o = reinterpret_cast<float*>(ws + p.tile_o);
     a.tile_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
-    const hipError_t e = d->dtype == SI_DTYPE_BF16 ? attend_by_dim<true>(stream, a, p)
-                                                   : attend_by_dim<false>(stream, a, p);
+    const bool bf16 = d->dtype == SI_DTYPE_BF16;
+    hipError_t e;
+    if (!p.sinks && !p.share_tiles) {
+        e = bf16 ? attend_by_dim<true, kPlain>(stream, a, p) : attend_by_dim<false, kPlain>(stream, a, p);
+    } else {
+        a.sinks = p.sinks;
+        if (p.share_tiles) {
+            a.groups = more->groups;
+            a.group_starts = more->group_starts;
+            a.prefix_lens = more->prefix_lens;
+        }
+        a.share_tiles = p.share_tiles;
+        a.share_split = p.share_split;
+        a.share_o = reinterpret_cast<float*>(ws + p.share_o);
+        a.share_ml = reinterpret_cast<float2*>(ws + p.share_ml);
+        e = bf16 ? attend_by_dim<true, kMore>(stream, a, p) : attend_by_dim<false, kMore>(stream, a, p);
+    }
     return e == hipSuccess ? 0 : -1;
 }
 

@@ -45,6 +45,17 @@ constexpr uint32_t kMostLength = 3u << 29;
 // their first unit.
 constexpr uint32_t kFewWhole = kFewStep / kFewKeys;
 
+// Prefixes that groups of sequences share: workgroups their tiles are cut for, and the least keys of a part.
+constexpr uint64_t kShareTarget = 512;
+constexpr uint32_t kShareMin = 256;
+
+// Keys of a part of a prefix that is cut into at most `split` parts.
+constexpr uint32_t share_part(uint32_t keys, uint32_t split)
+{
+    const uint32_t even = ((keys + split - 1) / split + kTileKeys - 1) / kTileKeys * kTileKeys;
+    return even > kShareMin ? even : kShareMin;
+}
+
 // How a call is launched.  The device's lengths are not known here: the table's
 // width bounds them, and a sequence is cut into fewer parts on the device where
 // it is shorter.
@@ -52,15 +63,18 @@ struct Plan {
     uint32_t few_rows = 0, few_groups = 0, few_least = 0, few_per = 0, tile_per = 0, tile_split = 1, tiles = 0;
     bool few = false, tile = false, fits = true;
     uint64_t few_o = 0, few_ml = 0, few_parts = 0, tile_o = 0, tile_ml = 0, bytes = 0;
+    uint32_t sinks = 0, share_tiles = 0, share_split = 1;
+    uint64_t share_o = 0, share_ml = 0;
 };
 
 // Keys of a part, so that `groups` sequences of `keys` keys make about `target`
 // workgroups, and the parts of the longest sequence.  A part is no longer than all the keys
 // (at most 2^30), whatever the number of groups: the kernels' positions have 32 bits.
-inline uint32_t part_keys(uint64_t groups, uint64_t keys, uint64_t least, uint64_t step, uint64_t target, uint32_t* parts)
+inline uint32_t part_keys(uint64_t groups, uint64_t keys, uint64_t least, uint64_t step, uint64_t target, uint32_t* parts,
+                          uint64_t most = kMaxSplit)
 {
     uint64_t per = groups * keys / target;
-    const uint64_t fewest = (keys + kMaxSplit - 1) / kMaxSplit;
+    const uint64_t fewest = (keys + most - 1) / most;
     per = per > least ? per : least;
     per = per > fewest ? per : fewest;
     per = per < keys ? per : keys;
@@ -69,11 +83,22 @@ inline uint32_t part_keys(uint64_t groups, uint64_t keys, uint64_t least, uint64
     return uint32_t(per);
 }
 
-inline Plan attend_plan(const si_paged_attention_desc& d)
+inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attention_more* more = nullptr)
 {
     Plan p;
     const uint64_t group = d.q_heads / d.kv_heads, keys = uint64_t(d.table_pages) * d.page_tokens;
     const uint64_t rows = d.tokens * group;
+    const uint64_t window = d.window < kMostLength ? d.window : 0;
+    p.sinks = more && window ? more->sinks : 0;
+    const uint32_t groups = more ? more->groups : 0;
+    // A row's parts of its prefix and of its own keys are joined together.
+    const uint64_t most_parts = groups ? kMaxSplit / 2 : kMaxSplit;
+    // Beside sinks a call is cut for the keys that its windows leave: a sequence's n new tokens see at most
+    // window + n - 1 keys, in whole steps, and the sinks.  (Without sinks by the table alone, as ever.)
+    const auto kept = [&](uint64_t n) {
+        const uint64_t left = window + n + p.sinks + 3 * kTileKeys;
+        return p.sinks && left < keys ? left : keys;
+    };
     // One token each: one kernel.  Any mix of lengths: both, unless no
     // sequence can be long or the only one is.
     p.few = group <= kFewRows && (!d.q_starts || d.seqs > 1 || rows <= kFewRows);
@@ -82,7 +107,8 @@ inline Plan attend_plan(const si_paged_attention_desc& d)
     const uint64_t pairs = uint64_t(d.seqs) * d.kv_heads;
     uint64_t few_groups = 0, places = 0;
     if (p.few) {
-        const uint64_t units = (keys + kFewKeys - 1) / kFewKeys, fewest = (units + kMaxSplit - 2) / (kMaxSplit - 1);
+        const uint64_t keys = kept(kFewRows);
+        const uint64_t units = (keys + kFewKeys - 1) / kFewKeys, fewest = (units + most_parts - 2) / (most_parts - 1);
         // workgroups that run at a time: 3 a CU for heads up to 64 (2 beside tiles), 2 up to 128, 1
         // (768 or 1,536 for heads of 128: 64 sequences of 8,192 keys 229 and 209 us, 512 197)
         const uint64_t at_once = d.head_dim <= 64 && !p.tile ? 768 : d.head_dim <= 128 ? 512 : 256;
@@ -93,31 +119,38 @@ inline Plan attend_plan(const si_paged_attention_desc& d)
             places = units > kFewWhole ? 2 * few_groups : 0;
         } else {
             uint32_t parts;
-            p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &parts) / kFewKeys;
+            p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &parts, most_parts) / kFewKeys;
             few_groups = pairs * parts;
             places = parts > 1 ? few_groups : 0;
         }
     }
     if (p.tile) {
-        const uint64_t tile_rows = kTileRows;
+        const uint64_t tile_rows = kTileRows, keys = kept(d.tokens);
         p.tiles = uint32_t(d.q_starts ? rows / tile_rows + d.seqs
                                       : uint64_t(d.seqs) * ((group + tile_rows - 1) / tile_rows));
         // Cut only where the tiles alone leave CUs idle; sequences of the
         // few-row kernel have none.
         const uint64_t groups = (rows / tile_rows + (p.few ? 1 : d.seqs)) * d.kv_heads;
         p.tile_per = part_keys(groups, keys, groups < kTileFew ? kTileSplitMin : keys, kTileKeys, kTileTarget,
-                               &p.tile_split);
+                               &p.tile_split, most_parts);
         if (p.tile_split > 1) {
             // whole columns for every XCD (see the kernel's order)
             const uint32_t even = 8 / uint32_t(std::gcd(8u, d.kv_heads));
             p.tile_split = (p.tile_split + even - 1) / even * even;
         }
     }
+    if (groups) {
+        p.share_tiles = uint32_t(rows / kTileRows + groups);
+        const uint64_t columns = (rows / kTileRows + 1) * d.kv_heads;
+        const uint64_t split = (kShareTarget + columns - 1) / columns;
+        p.share_split = uint32_t(split < most_parts ? split : most_parts);
+    }
     // (threads of a launch dimension fit 32 bits)
     const uint64_t most = (1ull << 32) / 256 - 1;
     const uint64_t tile_groups = uint64_t(p.tiles) * d.kv_heads * p.tile_split;
     p.few_groups = uint32_t(few_groups);
-    p.fits = few_groups + tile_groups <= most && uint64_t(d.tokens) * d.q_heads / 4 < most;
+    const uint64_t share_groups = uint64_t(p.share_tiles) * d.kv_heads * p.share_split;
+    p.fits = share_groups + few_groups + tile_groups <= most && uint64_t(d.tokens) * d.q_heads / 4 < most;
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
@@ -129,10 +162,15 @@ inline Plan attend_plan(const si_paged_attention_desc& d)
         p.few_ml = take(n * 8);
         p.few_parts = take(pairs * 8);
     }
-    if (p.tile_split > 1) {
+    if (p.tile_split > 1 || groups) {
         const uint64_t n = uint64_t(p.tile_split) * d.tokens * d.q_heads;
         p.tile_o = take(n * d.head_dim * 4);
         p.tile_ml = take(n * 8);
+    }
+    if (groups) {
+        const uint64_t n = uint64_t(p.share_split) * d.tokens * d.q_heads;
+        p.share_o = take(n * d.head_dim * 4);
+        p.share_ml = take(n * 8);
     }
     return p;
 }

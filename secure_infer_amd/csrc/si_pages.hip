@@ -13,6 +13,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <cmath>
+#include <cstring>
+
 #include "secure_infer_gpu.h"
 #include "si_launch.h"
 
@@ -511,6 +514,207 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
     }
 }
 
+// ---------------------------------------------------------------- append, rotated
+
+struct RotateArgs {
+    AppendArgs a;
+    const float* freqs;
+    const int64_t* positions;
+    const uint16_t* q;
+    uint16_t* q_out;
+    uint64_t q_token, q_head, q_out_token, q_out_head;
+    uint32_t q_heads, rot, dim, magnitude_bits;
+    uint32_t row_tasks, rot_tasks, tasks;  // of a K or query row, rotated ones among them; of a token
+    uint32_t split;                        // waves a token
+};
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// How a task's pairs lie: 8 adjacent dims; 8 dims of either half; 4 of either half (where halves are no
+// multiple of 8).
+enum Pairs { kAdjacent = 0, kHalves8 = 1, kHalves4 = 2 };
+
+template <bool kBf16>
+__device__ __forceinline__ float as_float(uint32_t x)  // of the low 16 bits
+{
+    if constexpr (kBf16) return __uint_as_float(x << 16);
+    else return float(__builtin_bit_cast(_Float16, uint16_t(x)));
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t as_16(float x)
+{
+    if constexpr (kBf16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+    else return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
+}
+
+// Pairs (x, y) turned by (cos, sin): float, rounded once.
+template <bool kBf16>
+__device__ __forceinline__ void turn(uint32_t x, uint32_t y, float2 cs, uint32_t& u, uint32_t& v)
+{
+    const float a = as_float<kBf16>(x), b = as_float<kBf16>(y);
+    u = as_16<kBf16>(__builtin_fmaf(a, cs.x, -(b * cs.y)));
+    v = as_16<kBf16>(__builtin_fmaf(b, cs.x, a * cs.y));
+}
+
+// One wave per token (or `split` waves, where tokens are few): its lanes form the cosines and sines of the
+// token's angles, a pair a lane, in the wave's LDS, and every head's rows are turned by them.
+constexpr uint32_t kRotateAhead = 4;
+constexpr uint32_t kRotatePairs = 128;
+
+template <bool kBf16, int kPairs>
+__global__ __launch_bounds__(256) void append_rotated_kernel(RotateArgs r)
+{
+    __shared__ __attribute__((aligned(16))) float2 turns[4][kRotatePairs];
+    const AppendArgs& a = r.a;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t w = blockIdx.x * 4 + wave;
+    const uint32_t t = w / r.split, share = w - t * r.split;
+    if (t >= a.tokens) return;
+    uint32_t b = t;
+    int64_t back = 1;
+    bool owned = true;
+    if (a.q_starts) {
+        uint32_t at_or_before = 0;
+        for (uint32_t s0 = 0; s0 <= a.seqs; s0 += 64) {
+            const bool le = s0 + lane <= a.seqs && a.q_starts[s0 + lane] <= int64_t(t);
+            at_or_before += __popcll(__ballot(le));
+        }
+        owned = at_or_before > 0 && at_or_before <= a.seqs;
+        b = owned ? at_or_before - 1 : 0;
+        const int64_t end = a.q_starts[b + 1];
+        back = (end < a.tokens ? end : a.tokens) - t;
+    }
+    const int64_t p = a.kv_lens[b] - back;
+    const int64_t page = p >> a.page_shift;
+    int64_t slot = -1;
+    if (owned && p >= 0 && page < a.pages) slot = a.tables[b * a.table_stride + uint64_t(page)];
+    const bool stored = held(slot, a.nslots);
+    if (!stored && share == 0 && lane == 0 && a.fail_count) atomicAdd(a.fail_count, 1u);
+    const uint64_t o = stored ? uint64_t(slot) * a.slot_bytes + uint64_t(p & ((1ll << a.page_shift) - 1)) * a.heads * r.dim * 2
+                              : 0;
+    // Angles in turns: the product with the position, and what is left of it without whole turns, in 64 bits
+    // (2^-52 of the angle: at position 2^30 2e-7 radians).
+    const double at = double(r.positions ? r.positions[t] : p);
+    const float magnitude = __uint_as_float(r.magnitude_bits);
+    for (uint32_t i = lane; i < r.rot / 2; i += 64) {
+        const double x = at * double(r.freqs[i]) * 0.15915494309189533577;
+        const float part = float(x - rint(x));
+        float s, c;
+        sincospif(2.0f * part, &s, &c);
+        turns[wave][i] = float2{c * magnitude, s * magnitude};
+    }
+    __builtin_amdgcn_wave_barrier();
+
+    // A token's tasks: K's rows, V's, q's.
+    const uint32_t k_tasks = a.heads * r.row_tasks, kv_tasks = k_tasks + a.heads * a.dim8;
+    const uint32_t half = r.rot / 2;
+    struct Task {
+        const uint16_t* src;
+        uint16_t* dst;
+        uint32_t c;   // which of the row's rotated tasks
+        bool turned, kept;
+    };
+    const auto task_of = [&](uint32_t x) {
+        Task k;
+        k.turned = false;
+        k.c = 0;
+        if (x >= k_tasks && x < kv_tasks) {
+            const uint32_t y = x - k_tasks, h = y / a.dim8, d = (y - h * a.dim8) * 8;
+            k.kept = stored;
+            k.src = a.v + t * a.v_token + h * a.v_head + d;
+            k.dst = reinterpret_cast<uint16_t*>(a.cache_v + o) + h * r.dim + d;
+            return k;
+        }
+        const bool is_q = x >= kv_tasks;
+        const uint32_t y = is_q ? x - kv_tasks : x, h = y / r.row_tasks, c = y - h * r.row_tasks;
+        const bool in_rot = c < r.rot_tasks;
+        k.turned = in_rot && owned;
+        k.c = c;
+        const uint32_t d = !in_rot ? r.rot + (c - r.rot_tasks) * 8 : kPairs == kHalves4 ? 4 * c : 8 * c;
+        k.kept = is_q || stored;
+        if (is_q) {
+            k.src = r.q + t * r.q_token + h * r.q_head + d;
+            k.dst = r.q_out + t * r.q_out_token + h * r.q_out_head + d;
+        } else {
+            k.src = a.k + t * a.k_token + h * a.k_head + d;
+            k.dst = reinterpret_cast<uint16_t*>(a.cache_k + o) + h * r.dim + d;
+        }
+        // (rows of q in no sequence: both halves are copied)
+        if (in_rot && !owned && kPairs != kAdjacent) k.c = c | 0x80000000u;
+        return k;
+    };
+    const auto pair = [&](const Task& k) { return kPairs != kAdjacent && (k.turned || k.c >> 31); };
+    for (uint32_t x0 = share * 64 + lane; x0 < r.tasks; x0 += 64 * r.split * kRotateAhead) {
+        u32x4 lo[kRotateAhead], hi[kRotateAhead];
+#pragma unroll
+        for (uint32_t i = 0; i < kRotateAhead; ++i) {
+            const uint32_t x = x0 + 64 * r.split * i;
+            if (x >= r.tasks) break;
+            const Task k = task_of(x);
+            if (!k.kept) continue;
+            if (kPairs == kHalves4 && pair(k)) {
+                const u32x2 u = *reinterpret_cast<const u32x2*>(k.src), v = *reinterpret_cast<const u32x2*>(k.src + half);
+                lo[i] = u32x4{u[0], u[1], v[0], v[1]};
+            } else {
+                lo[i] = *reinterpret_cast<const u32x4*>(k.src);
+                if (pair(k)) hi[i] = *reinterpret_cast<const u32x4*>(k.src + half);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kRotateAhead; ++i) {
+            const uint32_t x = x0 + 64 * r.split * i;
+            if (x >= r.tasks) break;
+            const Task k = task_of(x);
+            if (!k.kept) continue;
+            if (k.turned) {
+                constexpr uint32_t each = kPairs == kHalves8 ? 8 : 4;
+                float2 cs[each];
+                const float4* from = reinterpret_cast<const float4*>(&turns[wave][k.c * each]);
+#pragma unroll
+                for (uint32_t e = 0; e < each; e += 2) {
+                    const float4 f = from[e / 2];
+                    cs[e] = float2{f.x, f.y};
+                    cs[e + 1] = float2{f.z, f.w};
+                }
+                if constexpr (kPairs == kAdjacent) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        uint32_t u, v;
+                        turn<kBf16>(lo[i][e] & 0xffffu, lo[i][e] >> 16, cs[e], u, v);
+                        lo[i][e] = u | v << 16;
+                    }
+                } else if constexpr (kPairs == kHalves8) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        uint32_t u0, v0, u1, v1;
+                        turn<kBf16>(lo[i][e] & 0xffffu, hi[i][e] & 0xffffu, cs[2 * e], u0, v0);
+                        turn<kBf16>(lo[i][e] >> 16, hi[i][e] >> 16, cs[2 * e + 1], u1, v1);
+                        lo[i][e] = u0 | u1 << 16;
+                        hi[i][e] = v0 | v1 << 16;
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        uint32_t u0, v0, u1, v1;
+                        turn<kBf16>(lo[i][e] & 0xffffu, lo[i][e + 2] & 0xffffu, cs[2 * e], u0, v0);
+                        turn<kBf16>(lo[i][e] >> 16, lo[i][e + 2] >> 16, cs[2 * e + 1], u1, v1);
+                        lo[i][e] = u0 | u1 << 16;
+                        lo[i][e + 2] = v0 | v1 << 16;
+                    }
+                }
+            }
+            if (kPairs == kHalves4 && pair(k)) {
+                *reinterpret_cast<u32x2*>(k.dst) = u32x2{lo[i][0], lo[i][1]};
+                *reinterpret_cast<u32x2*>(k.dst + half) = u32x2{lo[i][2], lo[i][3]};
+            } else {
+                *reinterpret_cast<u32x4*>(k.dst) = lo[i];
+                if (pair(k)) *reinterpret_cast<u32x4*>(k.dst + half) = hi[i];
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------- host side
 
 bool aligned(const void* p, uint64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -592,6 +796,75 @@ int run_pages(hipStream_t stream, const si_pages_desc* d)
     return 0;
 }
 
+bool append_args(const si_paged_append_desc* d, AppendArgs& a)
+{
+    if (!d || !d->k || !d->v || !d->cache_k || !d->cache_v || !d->tables || !d->kv_lens) return false;
+    if (!d->tokens || d->tokens >= (1u << 26) || !d->seqs || !d->kv_heads || !d->head_dim || d->head_dim % 8 || !d->nslots ||
+        d->nslots >= (1ull << 31) || !d->table_pages)
+        return false;
+    if (!d->q_starts && d->tokens != d->seqs) return false;
+    if (!power_of_two(d->page_tokens) || d->page_tokens < 8 || d->page_tokens > 32768) return false;
+    const uint64_t row = 2ull * d->kv_heads * d->head_dim;
+    if (row >= (1ull << 30) || d->slot_bytes % 16 || d->slot_bytes < row * d->page_tokens) return false;
+    if ((d->k_token_stride | d->k_head_stride | d->v_token_stride | d->v_head_stride) % 8) return false;
+    for (const void* p : {d->k, d->v, static_cast<const void*>(d->cache_k), static_cast<const void*>(d->cache_v)})
+        if (!aligned(p, 16)) return false;
+    a = AppendArgs{};
+    a.k = static_cast<const uint16_t*>(d->k);
+    a.v = static_cast<const uint16_t*>(d->v);
+    a.k_token = d->k_token_stride;
+    a.k_head = d->k_head_stride;
+    a.v_token = d->v_token_stride;
+    a.v_head = d->v_head_stride;
+    a.cache_k = static_cast<uint8_t*>(d->cache_k);
+    a.cache_v = static_cast<uint8_t*>(d->cache_v);
+    a.slot_bytes = d->slot_bytes;
+    a.nslots = int64_t(d->nslots);
+    a.tables = d->tables;
+    a.table_stride = d->table_stride;
+    a.kv_lens = d->kv_lens;
+    a.q_starts = d->q_starts;
+    a.pages = d->table_pages;
+    a.tokens = d->tokens;
+    a.seqs = d->seqs;
+    a.heads = d->kv_heads;
+    a.dim8 = d->head_dim / 8;
+    a.page_shift = log2_of(d->page_tokens);
+    a.fail_count = d->fail_count;
+    return true;
+}
+
+bool rotate_args(const si_paged_append_desc& d, const si_rotation& x, RotateArgs& r)
+{
+    if (!x.freqs || !x.rot || x.rot % 8 || x.rot > d.head_dim || x.rot > 2 * kRotatePairs) return false;
+    if (x.dtype > SI_DTYPE_FP16 || !std::isfinite(x.magnitude)) return false;
+    if (x.q_heads) {
+        if (!x.q || !x.q_out || !aligned(x.q, 16) || !aligned(x.q_out, 16)) return false;
+        if ((x.q_token_stride | x.q_head_stride | x.q_out_token_stride | x.q_out_head_stride) % 8) return false;
+        if (2ull * x.q_heads * d.head_dim >= 1ull << 30) return false;
+    }
+    r.freqs = x.freqs;
+    r.positions = x.positions;
+    r.q = static_cast<const uint16_t*>(x.q);
+    r.q_out = static_cast<uint16_t*>(x.q_out);
+    r.q_token = x.q_token_stride;
+    r.q_head = x.q_head_stride;
+    r.q_out_token = x.q_out_token_stride;
+    r.q_out_head = x.q_out_head_stride;
+    r.q_heads = x.q_heads;
+    r.rot = x.rot;
+    r.dim = d.head_dim;
+    std::memcpy(&r.magnitude_bits, &x.magnitude, 4);
+    r.rot_tasks = !x.adjacent && x.rot % 16 == 0 ? x.rot / 16 : x.rot / 8;
+    r.row_tasks = r.rot_tasks + (d.head_dim - x.rot) / 8;
+    const uint64_t tasks = (uint64_t(d.kv_heads) + x.q_heads) * r.row_tasks + uint64_t(d.kv_heads) * (d.head_dim / 8);
+    r.tasks = uint32_t(tasks);
+    // Waves for the whole chip where tokens are few, one task a lane at most.
+    const uint64_t split = 4096 / d.tokens, most = (tasks + 63) / 64;
+    r.split = uint32_t(split < 1 ? 1 : split < most ? split : most);
+    return true;
+}
+
 }  // namespace
 
 }  // namespace si
@@ -623,40 +896,26 @@ int secure_infer_gpu_pages_reserve(hipStream_t stream, const si_pages_desc* d)
 int secure_infer_gpu_paged_append(hipStream_t stream, const si_paged_append_desc* d)
 {
     using namespace si;
-    if (!d || !d->k || !d->v || !d->cache_k || !d->cache_v || !d->tables || !d->kv_lens) return -1;
-    if (!d->tokens || d->tokens >= (1u << 26) || !d->seqs || !d->kv_heads || !d->head_dim || d->head_dim % 8 || !d->nslots ||
-        d->nslots >= (1ull << 31) || !d->table_pages)
-        return -1;
-    if (!d->q_starts && d->tokens != d->seqs) return -1;
-    if (!power_of_two(d->page_tokens) || d->page_tokens < 8 || d->page_tokens > 32768) return -1;
-    const uint64_t row = 2ull * d->kv_heads * d->head_dim;
-    if (row >= (1ull << 30) || d->slot_bytes % 16 || d->slot_bytes < row * d->page_tokens) return -1;
-    if ((d->k_token_stride | d->k_head_stride | d->v_token_stride | d->v_head_stride) % 8) return -1;
-    for (const void* p : {d->k, d->v, static_cast<const void*>(d->cache_k), static_cast<const void*>(d->cache_v)})
-        if (!aligned(p, 16)) return -1;
-    AppendArgs a{};
-    a.k = static_cast<const uint16_t*>(d->k);
-    a.v = static_cast<const uint16_t*>(d->v);
-    a.k_token = d->k_token_stride;
-    a.k_head = d->k_head_stride;
-    a.v_token = d->v_token_stride;
-    a.v_head = d->v_head_stride;
-    a.cache_k = static_cast<uint8_t*>(d->cache_k);
-    a.cache_v = static_cast<uint8_t*>(d->cache_v);
-    a.slot_bytes = d->slot_bytes;
-    a.nslots = int64_t(d->nslots);
-    a.tables = d->tables;
-    a.table_stride = d->table_stride;
-    a.kv_lens = d->kv_lens;
-    a.q_starts = d->q_starts;
-    a.pages = d->table_pages;
-    a.tokens = d->tokens;
-    a.seqs = d->seqs;
-    a.heads = d->kv_heads;
-    a.dim8 = d->head_dim / 8;
-    a.page_shift = log2_of(d->page_tokens);
-    a.fail_count = d->fail_count;
+    AppendArgs a;
+    if (!append_args(d, a)) return -1;
     return launch(append_kernel, dim3((d->tokens + 3) / 4), dim3(256), stream, a) == hipSuccess ? 0 : -1;
+}
+
+int secure_infer_gpu_paged_append_rotated(hipStream_t stream, const si_paged_append_desc* d, const si_rotation* rotation)
+{
+    using namespace si;
+    RotateArgs r{};
+    if (!append_args(d, r.a) || !rotation || !rotate_args(*d, *rotation, r)) return -1;
+    const uint32_t waves = d->tokens * r.split;
+    const auto go = [&](auto kernel) {
+        return launch(kernel, dim3((waves + 3) / 4), dim3(256), stream, r) == hipSuccess ? 0 : -1;
+    };
+    const bool bf16 = rotation->dtype == SI_DTYPE_BF16;
+    if (rotation->adjacent)
+        return go(bf16 ? append_rotated_kernel<true, kAdjacent> : append_rotated_kernel<false, kAdjacent>);
+    if (rotation->rot % 16 == 0)
+        return go(bf16 ? append_rotated_kernel<true, kHalves8> : append_rotated_kernel<false, kHalves8>);
+    return go(bf16 ? append_rotated_kernel<true, kHalves4> : append_rotated_kernel<false, kHalves4>);
 }
 
 }  // extern "C"

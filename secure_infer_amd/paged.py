@@ -1,6 +1,7 @@
 """Operators on the paged KV cache the transfers fill and drain.
 
-* ``paged_append`` writes new tokens' K and V rows into their pages.
+* ``paged_append`` writes new tokens' K and V rows into their pages;
+  ``paged_append_rotated`` rotates K by position on the way, and the tokens' queries.
 * ``paged_attention`` attends from new tokens (one per sequence, or a chunk
   of each) over their sequences' pages.
 * ``fork_pages`` / ``free_pages`` / ``compact_pages`` / ``reserve_pages`` manage
@@ -179,6 +180,16 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_
     head stride in multiples of 8) into their pages.  Token i of a sequence with n new
     ones goes to position kv_len - n + i; a token whose position is
     negative, past the table or on no page is dropped and counted."""
+    d, device = _append_desc(k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count)
+    if d is None:
+        return
+    raw, other = _stream_of(stream, device)
+    _check(lib().secure_infer_gpu_paged_append(raw, ct.byref(d)), "paged_append")
+    _kept_by(other, (k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count))
+
+
+def _append_desc(k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count):
+    """(the checked descriptor, or None without tokens; the device)."""
     device, dtype, slots, ps, heads, dim, step = _cache_pair(cache_k, cache_v)
     tokens, kt, kh = _rows(k, "k", heads, dim, dtype, device)
     v_tokens, vt, vh = _rows(v, "v", heads, dim, dtype, device)
@@ -189,27 +200,107 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_
     seqs, pages, row = _sequences(tables, kv_lens, q_starts, tokens, ps, device)
     _fail_count(fail_count, device)
     if tokens == 0:
-        return
+        return None, device
     if seqs == 0:
         raise ValueError("there are new tokens but no sequences")
     if pages == 0:
         raise ValueError("tables has no pages")
-    raw, other = _stream_of(stream, device)
-    d = _lib.SiPagedAppendDesc(
+    return _lib.SiPagedAppendDesc(
         k=k.data_ptr(), v=v.data_ptr(), k_token_stride=kt, k_head_stride=kh, v_token_stride=vt, v_head_stride=vh,
         cache_k=cache_k.data_ptr(), cache_v=cache_v.data_ptr(), slot_bytes=2 * step, nslots=slots,
         tables=tables.data_ptr(), table_stride=row, kv_lens=kv_lens.data_ptr(), q_starts=_ptr(q_starts),
         table_pages=pages, tokens=tokens, seqs=seqs, kv_heads=heads, head_dim=dim, page_tokens=ps,
-        fail_count=_ptr(fail_count))
-    _check(lib().secure_infer_gpu_paged_append(raw, ct.byref(d)), "paged_append")
-    _kept_by(other, (k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count))
+        fail_count=_ptr(fail_count)), device
+
+
+def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor,
+                         tables: torch.Tensor, kv_lens: torch.Tensor, freqs: torch.Tensor,
+                         q: torch.Tensor | None = None, q_starts: torch.Tensor | None = None,
+                         positions: torch.Tensor | None = None, adjacent: bool = False, magnitude: float = 1.0,
+                         q_out: torch.Tensor | None = None, fail_count: torch.Tensor | None = None,
+                         stream=None) -> torch.Tensor | None:
+    """paged_append with K, and the same tokens' queries ``q`` [tokens, query heads, head
+    dim], rotated by position on the way.  ``freqs`` [rot / 2] float32 are the angles a position;
+    with a = p * freqs[i] the dims (x, y) = (i, i + rot / 2), or (2 i, 2 i + 1) if ``adjacent``, become
+    ``magnitude`` * (x cos a - y sin a, y cos a + x sin a), in float from an angle that
+    is right to float accuracy at any position, rounded once; dims from rot on go as they are.  rot is a multiple of 8 up to the head
+    dim and 256.  p is the token's position in its sequence, or ``positions`` [tokens] int64
+    (for the rotation alone).  A token that the append drops has its query rotated all the
+    same; a row of q in no sequence goes as it is.  Returns ``q_out`` (new if it is not given; q itself rotates in
+    place), or None without q."""
+    d, device = _append_desc(k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count)
+    heads, dim, dtype, tokens = cache_k.shape[2], cache_k.shape[3], cache_k.dtype, k.shape[0]
+    _index(freqs, "freqs", 1, device, torch.float32)
+    rot = 2 * freqs.shape[0]
+    if rot == 0 or rot % 8 or rot > min(dim, 256):
+        raise ValueError(f"freqs must hold a multiple of 4 frequencies, at most {min(dim, 256) // 2}")
+    if not math.isfinite(magnitude):
+        raise ValueError("magnitude must be finite")
+    if positions is not None:
+        _index(positions, "positions", 1, device)
+        if positions.shape[0] != tokens:
+            raise ValueError("positions needs one entry per token")
+    r = _lib.SiRotation(freqs=freqs.data_ptr(), positions=_ptr(positions), rot=rot, adjacent=1 if adjacent else 0,
+                        dtype=_DTYPES[dtype], magnitude=magnitude)
+    other = None
+    if d is not None:
+        raw, other = _stream_of(stream, device)
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out goes with q")
+    else:
+        if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.shape[1] == 0:
+            raise ValueError(f"q must be [tokens, query heads, {dim}]")
+        q_heads = q.shape[1]
+        q_tokens, qt, qh = _rows(q, "q", q_heads, dim, dtype, device)
+        if q_tokens != tokens:
+            raise ValueError("q and k must have the same tokens")
+        if q.requires_grad or (q_out is not None and q_out.requires_grad):
+            _tracked()
+        if q_out is None:
+            q_out = _empty(other, q.shape, dtype, device)
+            ot, oh = q_heads * dim, dim
+        else:
+            if not isinstance(q_out, torch.Tensor) or q_out.shape != q.shape:
+                raise ValueError("q_out must have q's shape")
+            _, ot, oh = _rows(q_out, "q_out", q_heads, dim, dtype, device)
+            _apart(ot, oh, tokens, q_heads, dim, "q_out")
+            if q_out.data_ptr() != q.data_ptr() or (ot, oh) != (qt, qh):
+                for t, name in ((q, "q"), (k, "k"), (v, "v")):
+                    if _meet(q_out, t):
+                        raise ValueError(f"q_out must be q itself, or not overlap {name}")
+        r.q, r.q_out, r.q_heads = q.data_ptr(), q_out.data_ptr(), q_heads
+        r.q_token_stride, r.q_head_stride, r.q_out_token_stride, r.q_out_head_stride = qt, qh, ot, oh
+    if d is None:
+        return q_out
+    _check(lib().secure_infer_gpu_paged_append_rotated(raw, ct.byref(d), ct.byref(r)), "paged_append_rotated")
+    _kept_by(other, (k, v, cache_k, cache_v, tables, kv_lens, freqs, q, q_starts, positions, q_out, fail_count))
+    return q_out
+
+
+def _apart(token: int, head: int, tokens: int, heads: int, dim: int, name: str) -> None:
+    """The rows of an output do not overlap: the larger stride steps over the smaller
+    one's rows; that of a single token or head is never used."""
+    span = dim
+    for stride, n in sorted((stride, n) for stride, n in ((token, tokens), (head, heads)) if n > 1):
+        if stride < span:
+            raise ValueError(f"{name}'s rows must not overlap")
+        span += stride * (n - 1)
+
+
+def _meet(a, b) -> bool:
+    """The memory from a tensor's first element to its last overlaps the other's."""
+    def end(t):
+        return t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)))
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, tables: torch.Tensor,
                     kv_lens: torch.Tensor, q_starts: torch.Tensor | None = None, scale: float | None = None,
                     causal: bool = True, window: int = 0, out: torch.Tensor | None = None,
                     lse: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
-                    stream=None) -> torch.Tensor:
+                    stream=None, sinks: int = 0, prefix_groups: torch.Tensor | None = None,
+                    prefix_lens: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [tokens, query heads, head dim] over the pages:
     softmax(scale q k^T) v per token and query head (head h reads KV head
     h // (query heads / kv heads)).  Token i of a sequence with n new ones stands at p = kv_len
@@ -220,8 +311,19 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     and sums are float; the weights are rounded to q's type once, for the product with v.  ``scale`` defaults to head_dim ** -0.5.  ``lse`` [tokens, query heads]
     float32, if given, receives the log-sum-exp of the scaled scores (-inf
     without a key), with which two parts' outputs can be joined.  ``workspace`` (uint8, at least
-    ``paged_attention_workspace`` bytes) saves an allocation per call.  Returns ``out``."""
+    ``paged_attention_workspace`` bytes) saves an allocation per call.  Returns ``out``.
+
+    ``sinks``: a token also sees the first ``sinks`` keys that its window alone would hide.
+
+    ``prefix_groups`` [groups + 1] int64, ascending, and ``prefix_lens`` [groups] int64:
+    sequences prefix_groups[g] up to prefix_groups[g + 1] share their first prefix_lens[g] keys, which are
+    read once for all their tokens, from the pages of the group's first sequence (their own
+    rows' entries there do not count).  What a token sees does not change; a group of one
+    sequence, or a sequence in none, is as without groups."""
     d, device = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse)
+    more = None
+    if sinks or prefix_groups is not None or prefix_lens is not None:
+        more = _attention_more(sinks, prefix_groups, prefix_lens, device)
     if q.requires_grad or cache_k.requires_grad or cache_v.requires_grad:
         _tracked()
     if d is None:
@@ -231,7 +333,8 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
         out = _empty(other, q.shape, q.dtype, device)
         d.out, d.out_token_stride, d.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
     L = lib()
-    need = L.secure_infer_gpu_paged_attention_workspace(ct.byref(d))
+    need = (L.secure_infer_gpu_paged_attention_workspace(ct.byref(d)) if more is None else
+            L.secure_infer_gpu_paged_attention_more_workspace(ct.byref(d), ct.byref(more)))
     if need == _REFUSED:
         raise ValueError("paged_attention refuses these arguments")
     if need:
@@ -243,16 +346,40 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
             raise ValueError(f"workspace needs {need} bytes")
         _aligned(workspace, "workspace")
         d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _check(L.secure_infer_gpu_paged_attention(raw, ct.byref(d)), "paged_attention")
-    _kept_by(other, (q, cache_k, cache_v, tables, kv_lens, q_starts, out, lse, workspace))
+    if more is None:
+        _check(L.secure_infer_gpu_paged_attention(raw, ct.byref(d)), "paged_attention")
+    else:
+        _check(L.secure_infer_gpu_paged_attention_more(raw, ct.byref(d), ct.byref(more)), "paged_attention")
+    _kept_by(other, (q, cache_k, cache_v, tables, kv_lens, q_starts, out, lse, workspace, prefix_groups, prefix_lens))
     return out
 
 
 def paged_attention_workspace(q, cache_k, cache_v, tables, kv_lens, q_starts=None, causal: bool = True,
-                              window: int = 0) -> int:
+                              window: int = 0, sinks: int = 0, prefix_groups: torch.Tensor | None = None,
+                              prefix_lens: torch.Tensor | None = None) -> int:
     """Workspace bytes of a paged_attention call with these arguments."""
-    d, _ = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, None, causal, window, None, None)
-    return 0 if d is None else int(lib().secure_infer_gpu_paged_attention_workspace(ct.byref(d)))
+    d, device = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, None, causal, window, None, None)
+    more = _attention_more(sinks, prefix_groups, prefix_lens, device)
+    return 0 if d is None else int(lib().secure_infer_gpu_paged_attention_more_workspace(ct.byref(d), ct.byref(more)))
+
+
+def _attention_more(sinks, prefix_groups, prefix_lens, device: int):
+    """The checked sinks and shared prefixes."""
+    if not 0 <= int(sinks) <= 1 << 30:
+        raise ValueError("sinks must be 0 (none) or a number of keys up to 2**30")
+    if (prefix_groups is None) != (prefix_lens is None):
+        raise ValueError("prefix_groups and prefix_lens go together")
+    groups = 0
+    if prefix_groups is not None:
+        _index(prefix_groups, "prefix_groups", 1, device)
+        _index(prefix_lens, "prefix_lens", 1, device)
+        groups = prefix_lens.shape[0]
+        if prefix_groups.shape[0] != groups + 1:
+            raise ValueError("prefix_groups needs one entry more than prefix_lens")
+        if groups >= 1 << 26:
+            raise ValueError("there are too many groups")
+    return _lib.SiPagedAttentionMore(sinks=int(sinks), groups=groups, group_starts=_ptr(prefix_groups) if groups else None,
+                                     prefix_lens=_ptr(prefix_lens) if groups else None)
 
 
 def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse):
@@ -278,12 +405,7 @@ def _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causa
         if out.shape != q.shape:
             raise ValueError("out must have q's shape")
         _, ot, oh = _rows(out, "out", q_heads, dim, dtype, device)
-        # the larger stride steps over the smaller one's rows; that of a single token or head is never used
-        span = dim
-        for stride, n in sorted((stride, n) for stride, n in ((ot, tokens), (oh, q_heads)) if n > 1):
-            if stride < span:
-                raise ValueError("out's rows must not overlap")
-            span += stride * (n - 1)
+        _apart(ot, oh, tokens, q_heads, dim, "out")
     if lse is not None and (lse.get_device() != device or lse.dtype != torch.float32 or lse.shape != q.shape[:2]
                             or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous float32 [tokens, query heads] tensor on cuda:{device}")
