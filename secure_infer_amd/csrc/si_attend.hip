@@ -51,6 +51,7 @@ struct AttendArgs {
     float scale_log2;  // |scale| * log2(e): weights are powers of two
     // Sequences of at most few_rows rows (tokens * group) belong to the few-row
     // kernel, the others to the tile kernel.
+    // (few_least: kMore, the parts that a sequence may have.)
     uint32_t few_rows, few_groups, few_least, few_per, tile_per, tile_split, tiles;
     // Parts of split sequences: numerators (dim floats a row) and (m, l).
     float* few_o;
@@ -169,7 +170,8 @@ __device__ __forceinline__ void to_lds(const uint8_t* base, uint32_t offset, uin
 // Everything this wave has asked memory for has arrived.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// A pointer that is the same in every lane, as one.
+// A number, a pointer that is the same in every lane, as one.
+__device__ __forceinline__ uint32_t same(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p)
 {
     const uint64_t x = reinterpret_cast<uint64_t>(p);
@@ -361,14 +363,22 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
     return (a | b) >> 32 ? a / b : uint32_t(a) / uint32_t(b);
 }
 
-// Units of 32 keys of a KV head of a sequence for the few-row kernel.  (A
+// The few-row kernel's units of keys: a wave's step, or a workgroup's beside sinks and shared prefixes, whose
+// sequences are short: several in a workgroup follow one another, at about 4 us each.
+template <int kKind>
+constexpr uint32_t few_unit()
+{
+    return kKind == kPlain ? kFewKeys : kFewStep;
+}
+
+// Units of a KV head of a sequence for the few-row kernel.  (A
 // sequence without keys has outputs all the same: one.)
 template <int kKind>
 __device__ __forceinline__ uint32_t few_units(const AttendArgs& a, const Seq& s)
 {
     const uint32_t rows = s.n_new * a.group;
     if (rows == 0 || rows > a.few_rows) return 0;
-    const uint32_t n = cut_of<kKind>(a, s, kFewKeys, kFewKeys).parts;
+    const uint32_t n = cut_of<kKind>(a, s, few_unit<kKind>(), kFewKeys).parts;
     return n ? n : 1;
 }
 
@@ -387,7 +397,18 @@ struct Few {
         with = sums_up_to(units);
         total = upto(a, 63);
         const uint64_t even = quotient(total + a.few_groups - 1, a.few_groups);
-        per = even > a.few_least ? even : a.few_least;
+        uint32_t least = a.few_least;
+        if constexpr (kKind == kMore) {
+            // as many units a share as keep the longest sequence's parts to few_least
+            uint32_t most = units;
+#pragma unroll
+            for (int x = 32; x; x >>= 1) {
+                const uint32_t y = uint32_t(__shfl_xor(int(most), x));
+                most = y > most ? y : most;
+            }
+            least = (same(most) + a.few_least - 2) / (a.few_least - 1);
+        }
+        per = even > least ? even : least;
     }
     __device__ __forceinline__ uint64_t upto(const AttendArgs& a, int x) const  // x: the same in every lane
     {
@@ -670,7 +691,8 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
     const int64_t* table = a.tables + uint64_t(s.b) * a.table_stride;
     // (kMore: k0, next and hi are places of the cut)
     const auto key = [&](int32_t x) { return kKind == kPlain ? x : cut.key(x); };
-    const int32_t k_first = (kKind == kPlain ? cut.lo : 0) + int32_t(first * kFewKeys);
+    constexpr uint32_t kUnit = few_unit<kKind>();
+    const int32_t k_first = (kKind == kPlain ? cut.lo : 0) + int32_t(first * kUnit);
     Keys<kFewKeys> keys;
     int32_t k0 = k_first + int32_t(wave * kFewKeys);
     keys.fetch(a, table, key(k0));
@@ -692,7 +714,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
     const int32_t p_last = s.base + int32_t(s.n_new) - 1;
     const int32_t hi_key = a.causal ? keys_up_to(s, p_last) : s.len;
     const int32_t hi0 = kKind == kPlain ? hi_key : cut.place(hi_key);
-    const int32_t hi = hi0 < k_first + int32_t(n * kFewKeys) ? hi0 : k_first + int32_t(n * kFewKeys);
+    const int32_t hi = hi0 < k_first + int32_t(n * kUnit) ? hi0 : k_first + int32_t(n * kUnit);
     // keys below lo are behind every row's window
     const int32_t lo = a.window ? s.base - int32_t(a.window) + 1 : 0;
 
@@ -895,7 +917,7 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
             kvh = uint32_t(quotient(in, units));
             first = uint32_t(in - uint64_t(kvh) * units);
             n = units - first;
-            const bool alone = units <= kFewWhole;
+            const bool alone = units <= (kKind == kPlain ? kFewWhole : 1);
             if (!alone && n > to - at) n = uint32_t(to - at);
             at += n;
             if (alone && first > 0) continue;
@@ -910,7 +932,7 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
         if (first == 0 && a.few_parts && threadIdx.x == 0)
             a.few_parts[b * a.kv_heads + kvh] = uint2{place, 1 + uint32_t(quotient(units - n + per - 1, per))};
         if (again) __syncthreads();  // the last ones' results in LDS have been read
-        attend_few<kBf16, kDim, kKind>(a, lds, s, kvh, cut_of<kKind>(a, s, kFewKeys, kFewKeys), first, n, n == units, place);
+        attend_few<kBf16, kDim, kKind>(a, lds, s, kvh, cut_of<kKind>(a, s, few_unit<kKind>(), kFewKeys), first, n, n == units, place);
     }
 }
 
@@ -961,7 +983,7 @@ __device__ __forceinline__ int32_t least_of(int32_t x)
 }
 __device__ __forceinline__ int32_t tile_least(uint8_t* lds, uint32_t wave, int32_t x)
 {
-    volatile int32_t* const each = reinterpret_cast<volatile int32_t*>(lds);
+    int32_t* const each = reinterpret_cast<int32_t*>(lds);
     if ((threadIdx.x & 63u) == 0) each[wave] = x;
     __syncthreads();
 #pragma unroll
@@ -994,6 +1016,12 @@ template <int kDim>
 constexpr int tile_lds_bytes()  // two buffers of K and V
 {
     return 2 * (k_bytes<kDim>() + int(kTileKeys) * tile_chunks<kDim>() * 16);
+}
+// kShare: and each row's last key and window's first, which would cost the registers that the loop lacks.
+template <int kDim>
+constexpr int share_lds_bytes()
+{
+    return tile_lds_bytes<kDim>() + int(kTileRows) * 8;
 }
 
 // kShare: the same over (128 rows of all the tokens of a group of sequences, part of the prefix they share);
@@ -1065,10 +1093,11 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     Seq s;  // kShare: all the group's tokens, and its prefix
     if constexpr (kKind == kShare) {
         g = group_at(a, b);
+        g = Group{same(g.first), same(g.end), int32_t(same(uint32_t(g.prefix)))};
         if (g.prefix == 0) return;
         s.b = g.first;
-        s.q0 = rows_at(a, g.first);
-        const uint32_t end = rows_at(a, g.end);
+        s.q0 = same(rows_at(a, g.first));
+        const uint32_t end = same(rows_at(a, g.end));
         s.n_new = end > s.q0 ? end - s.q0 : 0;
         s.len = g.prefix;
         s.base = s.from = 0;
@@ -1096,18 +1125,31 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     const uint32_t w_last = w_first + 31 < r_last ? w_first + 31 : r_last;
     int32_t pw_first = s.base + int32_t(w_first / a.group), pw_last = s.base + int32_t(w_last / a.group);
     const uint32_t r = r0 + wave * 32 + col;
-    const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
-    int32_t pos = s.base + int32_t(tok);
-    int32_t last = a.causal ? pos : kNoLast;  // the row's last key and its window's first
+    const uint32_t tok = r / a.group;
+    uint32_t h = kvh * a.group + (r - tok * a.group);
+    const int32_t pos = s.base + int32_t(tok);
+    // The last key that a row sees, and its window's first.
+    const auto last_of = [&](int32_t p, int32_t len) { return a.causal ? (p < len ? p : len - 1) : len - 1; };
+    const auto behind_of = [&](int32_t p) {
+        return a.window && p >= int32_t(a.window) ? p - int32_t(a.window) + 1 : 0;
+    };
+    int2* const limits = reinterpret_cast<int2*>(lds + tile_lds_bytes<kDim>());
+    int32_t least_last = 0, most_behind = 0, least_behind = 0;  // of the wave's rows
     if constexpr (kKind == kShare) {
-        last = kNoLast;
-        if (r < rows) {
+        const bool row = r < rows;
+        int2 x{kNoLast, 0};
+        if (row) {
             const Seq mine = owner_of(a, g, s.q0 + tok);
-            pos = mine.base + int32_t(s.q0 + tok - mine.q0);
-            last = a.causal && pos < mine.len ? pos : mine.len - 1;
+            const int32_t p = mine.base + int32_t(s.q0 + tok - mine.q0);
+            x = int2{last_of(p, mine.len), behind_of(p)};
+        }
+        if (half == 0) limits[wave * 32 + col] = x;
+        least_last = least_of(x.x);
+        if (a.window) {
+            most_behind = -least_of(-x.y);
+            least_behind = tile_least(lds, wave, least_of(row ? x.y : kNoLast));
         }
     }
-    const int32_t behind = a.window ? (pos < int32_t(a.window) ? 0 : pos - int32_t(a.window) + 1) : 0;
     u32x4 q[kSteps];
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
@@ -1131,12 +1173,11 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     } else {
         // what some rows of the wave, and all rows of the tile, do not see
         if constexpr (kKind == kShare) {
-            const bool row = r < rows;
-            pw_first = least_of(last);
-            pw_last = a.window ? -least_of(row ? -behind : 0) + int32_t(a.window) - 1 : 0;
-            lo = a.window ? tile_least(lds, wave, least_of(row ? behind : kNoLast)) : 0;
+            pw_first = least_last;
+            pw_last = most_behind + int32_t(a.window) - 1;
+            lo = least_behind;
         } else {
-            lo = a.window && p_first >= int32_t(a.window) ? p_first - int32_t(a.window) + 1 : 0;
+            lo = behind_of(p_first);
         }
         k_skip = cut.place((int32_t(a.sinks) + int32_t(kTileKeys) - 1) & ~int32_t(kTileKeys - 1));
         k_lo = lo > cut.lo ? cut.head + ((lo - cut.lo) & ~int32_t(kTileKeys - 1)) : 0;
@@ -1213,6 +1254,15 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
             const uint8_t* const kp = uniform(a.cache_k + page);
             const uint8_t* const vp = uniform(a.cache_v + page);
             const uint32_t row = row0 * kv_row;
+            if constexpr (kKind != kPlain) {
+                // (the rows' distance in the uniform base: one offset a lane and not one a load)
+                const uint32_t k_at = row + k_chunk * 16, v_at = row + v_chunk * 16;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) to_lds(kp + uint64_t(i * kRowStep * kv_row), k_at, k_to + i * 4 * kGroup);
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) to_lds(vp + uint64_t(i * kRowStep * kv_row), v_at, v_to + i * 4096);
+                return ok;
+            }
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) to_lds(kp, i * kRowStep * kv_row + row + k_chunk * 16, k_to + i * 4 * kGroup);
 #pragma unroll
@@ -1300,7 +1350,16 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
                              (a.window && key(k0) <= pw_last - int32_t(a.window));
         uint64_t seen = ok;
         if (partial || ok != ~0ull) {
-            if (partial) seen = kKind == kPlain ? seen_bits(a, ok, k0, pos) : seen_bits(a, ok, key(k0), last, behind);
+            if (partial) {
+                if constexpr (kKind == kPlain) {
+                    seen = seen_bits(a, ok, k0, pos);
+                } else if constexpr (kKind == kMore) {
+                    seen = seen_bits(a, ok, key(k0), a.causal ? pos : kNoLast, behind_of(pos));
+                } else {
+                    const int2 x = limits[wave * 32 + col];
+                    seen = seen_bits(a, ok, key(k0), x.x, x.y);
+                }
+            }
             const uint64_t mine = seen >> (4 * half);
 #pragma unroll
             for (int y = 0; y < 2; ++y)
@@ -1380,7 +1439,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
             if constexpr (kKind == kShare) {
                 const Seq mine = owner_of(a, g, s.q0 + xt);
                 xp = mine.base + int32_t(s.q0 + xt - mine.q0);
-                x_last = a.causal && xp < mine.len ? xp : mine.len - 1;
+                x_last = last_of(xp, mine.len);
             }
             plain_row<kBf16, kKind>(a, table, s.q0 + xt, xh, kvh, xp, k_first, k_end, !out, part_o + row * a.dim,
                                     part_ml + row, cut, s.from, x_last);
@@ -1388,8 +1447,14 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         return;
     }
     l = across<false>(l, fadd2);
-    if (r >= rows) return;
-    const uint32_t t = s.q0 + tok;
+    // (kShare: worked out again, for the loop's registers)
+    uint32_t thread = threadIdx.x;
+    if constexpr (kKind == kShare) asm volatile("" : "+v"(thread));
+    const uint32_t r_out = kKind == kShare ? r0 + (thread >> 6) * 32 + (thread & 31u) : r;
+    if (r_out >= rows) return;
+    const uint32_t tok_out = kKind == kShare ? r_out / a.group : tok;
+    const uint32_t t = s.q0 + tok_out;
+    if constexpr (kKind == kShare) h = kvh * a.group + (r_out - tok_out * a.group);
     const float shift = m == -INFINITY ? 0.0f : m * a.scale_log2;
     if (!out) {
         const uint64_t row = (uint64_t(part) * a.tokens + t) * a.q_heads + h;
@@ -1457,7 +1522,8 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(A
 template <bool kBf16, int kDim>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_shared_kernel(AttendArgs a)
 {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[mixed_lds_bytes<kDim>()];
+    constexpr int kBytes = share_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? share_lds_bytes<kDim>() : few_lds_bytes<kDim>();
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
     const uint32_t share = a.share_tiles * a.kv_heads * a.share_split, tiles = a.tiles * a.kv_heads * a.tile_split;
     if (blockIdx.x < share) {
         attend_tile<kBf16, kDim, kShare>(a, lds, blockIdx.x, share);

@@ -89,6 +89,7 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
     const uint64_t group = d.q_heads / d.kv_heads, keys = uint64_t(d.table_pages) * d.page_tokens;
     const uint64_t rows = d.tokens * group;
     const uint64_t window = d.window < kMostLength ? d.window : 0;
+    if (more && !(window && more->sinks) && !more->groups) more = nullptr;
     p.sinks = more && window ? more->sinks : 0;
     const uint32_t groups = more ? more->groups : 0;
     // A row's parts of its prefix and of its own keys are joined together.
@@ -107,19 +108,20 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
     const uint64_t pairs = uint64_t(d.seqs) * d.kv_heads;
     uint64_t few_groups = 0, places = 0;
     if (p.few) {
-        const uint64_t keys = kept(kFewRows);
-        const uint64_t units = (keys + kFewKeys - 1) / kFewKeys, fewest = (units + most_parts - 2) / (most_parts - 1);
+        const uint64_t keys = kept(kFewRows), unit = more ? kFewStep : kFewKeys, whole = more ? 1 : kFewWhole;
+        const uint64_t units = (keys + unit - 1) / unit, fewest = (units + most_parts - 2) / (most_parts - 1);
         // workgroups that run at a time: 3 a CU for heads up to 64 (2 beside tiles), 2 up to 128, 1
         // (768 or 1,536 for heads of 128: 64 sequences of 8,192 keys 229 and 209 us, 512 197)
         const uint64_t at_once = d.head_dim <= 64 && !p.tile ? 768 : d.head_dim <= 128 ? 512 : 256;
-        p.few_least = uint32_t(fewest > kFewWhole ? fewest : kFewWhole);
+        p.few_least = uint32_t(more ? most_parts : fewest > whole ? fewest : whole);
         if (d.seqs <= 64 && pairs <= at_once) {
-            const uint64_t most = (pairs * units + p.few_least - 1) / p.few_least;
+            // (kMore: the device finds the least units of a share from the lengths)
+            const uint64_t least = more ? 1 : p.few_least, most = (pairs * units + least - 1) / least;
             few_groups = most < at_once ? most : at_once;
-            places = units > kFewWhole ? 2 * few_groups : 0;
+            places = units > whole ? 2 * few_groups : 0;
         } else {
             uint32_t parts;
-            p.few_per = part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &parts, most_parts) / kFewKeys;
+            p.few_per = uint32_t(part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &parts, most_parts) / unit);
             few_groups = pairs * parts;
             places = parts > 1 ? few_groups : 0;
         }

@@ -74,15 +74,18 @@ void check(const si_paged_attention_desc& d, const si_paged_attention_more& m, s
             const uint64_t len = i < 2 ? keys : g() % (keys + 1), group = d.q_heads / d.kv_heads;
             const uint64_t n = 1 + (d.q_starts ? g() % (kFewRows / group ? kFewRows / group : 1) : 0);
             const uint64_t from = m.groups && i % 2 ? g() % (keys + 1) : 0;
-            const uint64_t units = (left(d, p.sinks, len, n, from, kFewKeys) + kFewKeys - 1) / kFewKeys;
+            const uint64_t unit = p.sinks || m.groups ? kFewStep : kFewKeys;
+            const uint64_t units = (left(d, p.sinks, len, n, from, kFewKeys) + unit - 1) / unit;
             uint64_t parts = 1;
             if (p.few_per) {
                 parts = (units + p.few_per - 1) / p.few_per;
                 expect(parts * pairs <= p.few_groups || parts <= 1, "few-row parts", d, m);
             } else {
                 expect(d.seqs <= 64, "even shares", d, m);
-                // from anywhere in a share on; shares are of few_least units or more
-                if (units > kFewWhole) parts = (units + p.few_least - 2) / p.few_least + 1;
+                // from anywhere in a share on; shares are of `least` units or more
+                const bool more = p.sinks || m.groups;
+                const uint64_t least = more ? (units + p.few_least - 2) / (p.few_least - 1) : p.few_least;
+                if (units > (more ? 1 : kFewWhole)) parts = (units + least - 2) / least + 1;
             }
             expect(parts <= 1 || places, "few-row places", d, m);
             most = most > parts ? most : parts;
