@@ -62,11 +62,13 @@ struct AttendArgs {
     // Sinks and shared prefixes (kMore and kShare).  Sequences that share one leave their own
     // keys' whole parts in tile_o's first part.
     uint32_t sinks;  // first keys seen in spite of the window (0 without one)
-    uint32_t groups, share_tiles, share_split;
+    uint32_t groups, share_groups, share_split;  // share_groups: workgroups for the prefixes' tiles
     const int64_t* group_starts;
     const int64_t* prefix_lens;
     float* share_o;
     float2* share_ml;
+    uint4* few_joins;  // few_parts' place, and the parts of the prefix besides
+    uint32_t tile_groups;  // workgroups for the tiles
 };
 
 // What a kernel's code knows of: a call without sinks and shared prefixes, one with them, and of the
@@ -243,6 +245,8 @@ struct Group {
     int32_t prefix;
 };
 
+
+
 __device__ __forceinline__ Group group_at(const AttendArgs& a, uint32_t g)
 {
     const int64_t lo = a.group_starts[g], hi = a.group_starts[g + 1], seqs = a.seqs;
@@ -254,8 +258,8 @@ __device__ __forceinline__ Group group_at(const AttendArgs& a, uint32_t g)
     return x;
 }
 
-// Keys of the prefix that sequence b shares: that of the last group that starts at or before it.
-__device__ __forceinline__ int32_t prefix_of(const AttendArgs& a, uint32_t b)
+// The group of sequence b: the last one that starts at or before it; without a prefix where there is none.
+__device__ __forceinline__ Group group_of(const AttendArgs& a, uint32_t b)
 {
     uint32_t at = 0;
     for (uint32_t n = a.groups; n;) {
@@ -264,9 +268,20 @@ __device__ __forceinline__ int32_t prefix_of(const AttendArgs& a, uint32_t b)
         at = up ? at + half + 1 : at;
         n = up ? n - half - 1 : half;
     }
-    if (at == 0) return 0;
-    const Group g = group_at(a, at - 1);
-    return b < g.end ? g.prefix : 0;
+    Group g{0, 0, 0};
+    if (at > 0) g = group_at(a, at - 1);
+    if (b >= g.end) g.prefix = 0;
+    return g;
+}
+
+// Parts of the prefix, of `from` keys, that sequence b shares.
+__device__ __forceinline__ uint32_t share_parts(const AttendArgs& a, uint32_t b, int32_t from)
+{
+    if (from == 0) return 0;
+    const Group g = group_of(a, b);
+    const uint32_t row = rows_at(a, g.first), end = rows_at(a, g.end);
+    const uint32_t per = share_part(uint32_t(from), a.share_split, end > row ? uint64_t(end - row) * a.group : 0);
+    return (uint32_t(from) + per - 1) / per;
 }
 
 template <int kKind = kPlain>
@@ -275,7 +290,7 @@ __device__ __forceinline__ Seq seq_of(const AttendArgs& a, uint32_t b)
     Seq s;
     s.b = b;
     s.from = 0;
-    if constexpr (kKind == kMore) s.from = prefix_of(a, b);
+    if constexpr (kKind == kMore) s.from = group_of(a, b).prefix;
     s.q0 = b;
     s.n_new = 1;
     if (a.q_starts) {
@@ -388,12 +403,18 @@ __device__ __forceinline__ uint32_t few_units(const AttendArgs& a, const Seq& s)
 struct Few {
     uint32_t units, with;  // of a KV head; their sum up to and with the lane's (at most 64 * 2^25)
     uint64_t total, per;
+    Seq mine;
 
     template <int kKind>
     __device__ __forceinline__ void start(const AttendArgs& a)
     {
         const uint32_t b = threadIdx.x & 63u;
-        units = b < a.seqs ? few_units<kKind>(a, seq_of<kKind>(a, b)) : 0;
+        units = 0;
+        mine = Seq{b, 0, 0, 0, 0, 0};
+        if (b < a.seqs) {
+            mine = seq_of<kKind>(a, b);
+            units = few_units<kKind>(a, mine);
+        }
         with = sums_up_to(units);
         total = upto(a, 63);
         const uint64_t even = quotient(total + a.few_groups - 1, a.few_groups);
@@ -923,16 +944,27 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
             if (alone && first > 0) continue;
             place = 2 * group + (first == 0);
         }
-        const Seq s = seq_of<kKind>(a, b);
+        Seq s;
+        if (kKind == kMore && !a.few_per) {
+            const auto of_b = [&](uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), int(b))); };
+            s = Seq{b, of_b(w.mine.q0), of_b(w.mine.n_new), int32_t(of_b(uint32_t(w.mine.len))),
+                    int32_t(of_b(uint32_t(w.mine.base))), int32_t(of_b(uint32_t(w.mine.from)))};
+        } else {
+            s = seq_of<kKind>(a, b);
+        }
         if (a.few_per) {
             units = few_units<kKind>(a, s);
             if (first >= units) return;
             n = units - first < a.few_per ? units - first : a.few_per;
         }
-        if (first == 0 && a.few_parts && threadIdx.x == 0)
+        if (kKind == kPlain && first == 0 && a.few_parts && threadIdx.x == 0)
             a.few_parts[b * a.kv_heads + kvh] = uint2{place, 1 + uint32_t(quotient(units - n + per - 1, per))};
         if (again) __syncthreads();  // the last ones' results in LDS have been read
         attend_few<kBf16, kDim, kKind>(a, lds, s, kvh, cut_of<kKind>(a, s, few_unit<kKind>(), kFewKeys), first, n, n == units, place);
+        // (at the end: the join's kernel alone reads it)
+        if (kKind == kMore && first == 0 && a.few_joins && threadIdx.x == 0)
+            a.few_joins[b * a.kv_heads + kvh] =
+                uint4{place, 1 + uint32_t(quotient(units - n + per - 1, per)), share_parts(a, b, s.from), 0};
     }
 }
 
@@ -1025,9 +1057,10 @@ constexpr int share_lds_bytes()
 }
 
 // kShare: the same over (128 rows of all the tokens of a group of sequences, part of the prefix they share);
-// the rows differ in what they see of it.
+// the rows differ in what they see of it.  Rows from r0 on of sequence b (kShare: of group g).
 template <bool kBf16, int kDim, int kKind>
-__device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, uint32_t group, uint32_t groups)
+__device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uint32_t kvh, uint32_t part, uint32_t b,
+                                          uint32_t r0, const Group& g)
 {
     constexpr int kChunks = tile_chunks<kDim>();
     constexpr int kPitch = kChunks * 8;  // elements of a row
@@ -1041,59 +1074,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>((lds_void*)lds));
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = lane & 31u, half = lane >> 5;
-    if (kKind != kShare && a.q_starts && a.few_rows == 0 && group == 0) zero_unowned<kBf16>(a);
-
-    // A column is one KV head's part of the keys, over all tiles.  Workgroup i
-    // runs on XCD i % 8: whole columns go to one XCD, whose L2 then holds their
-    // K and V, dealt out back and forth, as the parts that only long sequences
-    // have come last; where the columns do not fill the XCDs evenly, each XCD
-    // takes an eighth of the list.
-    const uint32_t xcd = group % 8, nth = group / 8;
-    const uint32_t tiles = kKind == kShare ? a.share_tiles : a.tiles;
-    const uint32_t columns = groups / tiles;
-    uint32_t column, tile;
-    if (columns % 8 == 0) {
-        const uint32_t deal = nth / tiles;
-        column = 8 * deal + (deal % 2 ? 7 - xcd : xcd);
-        tile = nth % tiles;
-    } else {
-        const uint32_t x8 = groups / 8, r8 = groups % 8;
-        const uint32_t w = xcd * x8 + (xcd < r8 ? xcd : r8) + nth;
-        column = w / tiles;
-        tile = w % tiles;
-    }
-    tile = tiles - 1 - tile;  // the last tiles see most keys: first
-    const uint32_t kvh = column % a.kv_heads, part = column / a.kv_heads;
-
-    // Sequence b's tiles start at floor(q_starts[b] * group / rows) + b, which
-    // leaves it at least the tiles it needs.  (kShare: b is a group.)
-    uint32_t b = tile;
-    uint32_t first_tile = tile;
-    if (kKind == kShare || a.q_starts) {
-        const uint32_t n = kKind == kShare ? a.groups : a.seqs;
-        uint32_t at_or_before = 0;
-        for (uint32_t s0 = 0; s0 < n; s0 += 64) {
-            const uint32_t s = s0 + lane;
-            uint32_t f = 0;
-            if (s < n) {
-                const uint32_t row = kKind == kShare ? rows_at(a, group_at(a, s).first) : start_of(a, s);
-                f = uint32_t(uint64_t(row) * a.group / kTileRows) + s;
-            }
-            const uint64_t le = __ballot(s < n && f <= tile);
-            at_or_before += __popcll(le);
-            if (le) first_tile = __builtin_amdgcn_readfirstlane(__shfl(f, 63 - __clzll(le)));
-        }
-        if (at_or_before == 0) return;
-        b = at_or_before - 1;
-    } else {
-        b = tile / ((a.group + kTileRows - 1) / kTileRows);
-        first_tile = b * ((a.group + kTileRows - 1) / kTileRows);
-    }
-    Group g{b, b + 1, 0};
     Seq s;  // kShare: all the group's tokens, and its prefix
     if constexpr (kKind == kShare) {
-        g = group_at(a, b);
-        g = Group{same(g.first), same(g.end), int32_t(same(uint32_t(g.prefix)))};
         if (g.prefix == 0) return;
         s.b = g.first;
         s.q0 = same(rows_at(a, g.first));
@@ -1105,9 +1087,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         s = seq_of<kKind>(a, b);
     }
     const uint32_t rows = s.n_new * a.group;
-    const uint32_t r0 = (tile - first_tile) * kTileRows;
     if ((kKind != kShare && rows <= a.few_rows) || r0 >= rows) return;
-    const uint32_t per = kKind == kShare ? share_part(s.len, a.share_split) : a.tile_per;
+    const uint32_t per = kKind == kShare ? share_part(uint32_t(s.len), a.share_split, rows) : a.tile_per;
     Cut cut;
     if constexpr (kKind == kShare) {
         cut.lo = cut.head_lo = cut.head = 0;
@@ -1134,11 +1115,10 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         return a.window && p >= int32_t(a.window) ? p - int32_t(a.window) + 1 : 0;
     };
     int2* const limits = reinterpret_cast<int2*>(lds + tile_lds_bytes<kDim>());
-    int32_t least_last = 0, most_behind = 0, least_behind = 0;  // of the wave's rows
-    if constexpr (kKind == kShare) {
-        const bool row = r < rows;
+    int32_t least_last = 0, most_behind = 0, least_behind = 0;  // of the wave's rows, the last of the tile's
+    const auto find_limits = [&] {
         int2 x{kNoLast, 0};
-        if (row) {
+        if (r < rows) {
             const Seq mine = owner_of(a, g, s.q0 + tok);
             const int32_t p = mine.base + int32_t(s.q0 + tok - mine.q0);
             x = int2{last_of(p, mine.len), behind_of(p)};
@@ -1147,18 +1127,23 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         least_last = least_of(x.x);
         if (a.window) {
             most_behind = -least_of(-x.y);
-            least_behind = tile_least(lds, wave, least_of(row ? x.y : kNoLast));
+            least_behind = tile_least(lds, wave, least_of(r < rows ? x.y : kNoLast));
         }
-    }
+    };
+    // (kShare: the first keys' place does not wait for the rows' sequences, but where a window moves it)
+    if (kKind == kShare && a.window) find_limits();
     u32x4 q[kSteps];
+    const auto load_q = [&] {
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-        const uint32_t d = 16 * k + 8 * half;
-        u32x4 v{0, 0, 0, 0};
-        if (r < rows && d < a.dim)
-            v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
-        q[k] = (v & a.q_keep) ^ a.q_flip;
-    }
+        for (int k = 0; k < kSteps; ++k) {
+            const uint32_t d = 16 * k + 8 * half;
+            u32x4 v{0, 0, 0, 0};
+            if (r < rows && d < a.dim)
+                v = *reinterpret_cast<const u32x4*>(a.q + (s.q0 + tok) * a.q_token + h * a.q_head + d);
+            q[k] = (v & a.q_keep) ^ a.q_flip;
+        }
+    };
+    if constexpr (kKind != kShare) load_q();
     // The tile's keys: from k0 (behind every row's window below lo) to hi.  kMore and kShare: k0, k_first and
     // k_end are places of the cut, from k_skip on those below k_lo are behind every window.
     const int32_t hi_all = a.causal && kKind != kShare ? keys_up_to(s, p_last) : s.len;
@@ -1172,13 +1157,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         k_end = hi;
     } else {
         // what some rows of the wave, and all rows of the tile, do not see
-        if constexpr (kKind == kShare) {
-            pw_first = least_last;
-            pw_last = most_behind + int32_t(a.window) - 1;
-            lo = least_behind;
-        } else {
-            lo = behind_of(p_first);
-        }
+        lo = kKind == kShare ? least_behind : behind_of(p_first);
         k_skip = cut.place((int32_t(a.sinks) + int32_t(kTileKeys) - 1) & ~int32_t(kTileKeys - 1));
         k_lo = lo > cut.lo ? cut.head + ((lo - cut.lo) & ~int32_t(kTileKeys - 1)) : 0;
         k_end = cut.place(hi);
@@ -1319,6 +1298,12 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     }
     pages.start(a, table, key(k0), hi);
     uint64_t ok_next = fill(0, k0);
+    if constexpr (kKind == kShare) {
+        load_q();
+        if (!a.window) find_limits();
+        pw_first = least_last;
+        pw_last = most_behind + int32_t(a.window) - 1;
+    }
     int buf = 0;
     for (; k0 < k_end; k0 = step_from(k0)) {
         // This step's K and V are there, and every wave is done with the other
@@ -1480,6 +1465,113 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
     }
 }
 
+// Which (column, tile) workgroup `group` of `groups` takes.  A column is one KV head's part of the keys, over all
+// tiles.  Workgroup i runs on XCD i % 8: whole columns go to one XCD, whose L2 then holds their
+// K and V, dealt out back and forth, as the parts that only long sequences
+// have come last; where the columns do not fill the XCDs evenly, each XCD
+// takes an eighth of the list.
+__device__ __forceinline__ void deal_tile(uint32_t group, uint32_t groups, uint32_t tiles, uint32_t& column, uint32_t& tile)
+{
+    const uint32_t xcd = group % 8, nth = group / 8;
+    const uint32_t columns = groups / tiles;
+    if (columns % 8 == 0) {
+        const uint32_t deal = nth / tiles;
+        column = 8 * deal + (deal % 2 ? 7 - xcd : xcd);
+        tile = nth % tiles;
+    } else {
+        const uint32_t x8 = groups / 8, r8 = groups % 8;
+        const uint32_t w = xcd * x8 + (xcd < r8 ? xcd : r8) + nth;
+        column = w / tiles;
+        tile = w % tiles;
+    }
+    tile = tiles - 1 - tile;  // the last tiles see most keys: first
+}
+
+template <bool kBf16, int kDim>
+__device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, uint32_t group, uint32_t groups)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    if (a.q_starts && a.few_rows == 0 && group == 0) zero_unowned<kBf16>(a);
+    uint32_t column, tile;
+    deal_tile(group, groups, a.tiles, column, tile);
+    const uint32_t kvh = column % a.kv_heads, part = column / a.kv_heads;
+
+    // Sequence b's tiles start at floor(q_starts[b] * group / rows) + b, which
+    // leaves it at least the tiles it needs.
+    uint32_t b = tile;
+    uint32_t first_tile = tile;
+    if (a.q_starts) {
+        uint32_t at_or_before = 0;
+        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
+            const uint32_t s = s0 + lane;
+            const uint32_t f = s < a.seqs ? uint32_t(uint64_t(start_of(a, s)) * a.group / kTileRows) + s : 0;
+            const uint64_t le = __ballot(s < a.seqs && f <= tile);
+            at_or_before += __popcll(le);
+            if (le) first_tile = __builtin_amdgcn_readfirstlane(__shfl(f, 63 - __clzll(le)));
+        }
+        if (at_or_before == 0) return;
+        b = at_or_before - 1;
+    } else {
+        b = tile / ((a.group + kTileRows - 1) / kTileRows);
+        first_tile = b * ((a.group + kTileRows - 1) / kTileRows);
+    }
+    tile_rows<kBf16, kDim, kPlain>(a, lds, kvh, part, b, (tile - first_tile) * kTileRows, Group{b, b + 1, 0});
+}
+
+// kMore and kShare: the tiles that there are, counted, one to a workgroup; the workgroups behind them leave.
+template <bool kBf16, int kDim, int kKind>
+__device__ __forceinline__ void attend_tiles(const AttendArgs& a, uint8_t* lds, uint32_t group)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    if (kKind == kMore && a.q_starts && a.few_rows == 0 && group == 0) zero_unowned<kBf16>(a);
+    const uint32_t n = kKind == kShare ? a.groups : a.seqs;
+    // of the lane's sequence or group of 64: its tiles, their sum up to and with it
+    Group mine{0, 0, 0};
+    uint32_t tiles = 0, with = 0;
+    const auto count = [&](uint32_t s0) {
+        const uint32_t s = s0 + lane;
+        uint32_t from = 0, end = 0, least = 0;
+        if (s < n) {
+            if constexpr (kKind == kShare) {
+                mine = group_at(a, s);
+                if (mine.prefix > 0) {
+                    from = rows_at(a, mine.first);
+                    end = rows_at(a, mine.end);
+                }
+            } else {
+                from = rows_at(a, s);
+                end = rows_at(a, s + 1);
+                least = a.few_rows;
+            }
+        }
+        const uint32_t rows = end > from ? (end - from) * a.group : 0;
+        tiles = rows > least ? (rows + kTileRows - 1) / kTileRows : 0;
+        with = sums_up_to(tiles);
+        return uint32_t(__builtin_amdgcn_readlane(int(with), 63));
+    };
+    uint32_t total = count(0);
+    for (uint32_t s0 = 64; s0 < n; s0 += 64) total += count(s0);
+    // (tiles of a call fit 32 bits with their columns: the host's count of them does)
+    const uint32_t groups = total * a.kv_heads * (kKind == kShare ? a.share_split : a.tile_split);
+    if (group >= groups) return;
+    uint32_t column, tile;
+    deal_tile(group, groups, total, column, tile);
+    uint32_t sum = 0, s0 = 0;
+    uint64_t past = 0;
+    for (; s0 < n; s0 += 64) {
+        const uint32_t here = n > 64 ? count(s0) : total;
+        past = __ballot(sum + with > tile);
+        if (past) break;
+        sum += here;
+    }
+    if (!past) return;  // (there is one, unless the starts are written meanwhile)
+    const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+    const uint32_t before = sum + uint32_t(__builtin_amdgcn_readlane(int(with - tiles), at));
+    const Group g{same(__shfl(mine.first, at)), same(__shfl(mine.end, at)), int32_t(same(uint32_t(__shfl(mine.prefix, at))))};
+    tile_rows<kBf16, kDim, kKind>(a, lds, column % a.kv_heads, column / a.kv_heads, s0 + uint32_t(at),
+                                  (tile - before) * kTileRows, g);
+}
+
 // ---------------------------------------------------------------- kernels
 
 // (Three waves a SIMD for heads up to 64: tiles over 32,768 keys 365 us, two 442; for heads of 128 the
@@ -1495,7 +1587,8 @@ template <bool kBf16, int kDim, int kKind>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim > 64 ? 2 : 3) void attend_tile_kernel(AttendArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[tile_lds_bytes<kDim>()];
-    attend_tile<kBf16, kDim, kKind>(a, lds, blockIdx.x, gridDim.x);
+    if constexpr (kKind == kPlain) attend_tile<kBf16, kDim>(a, lds, blockIdx.x, gridDim.x);
+    else attend_tiles<kBf16, kDim, kKind>(a, lds, blockIdx.x);
 }
 
 // Both kinds of sequences in one launch: the tiles' workgroups first, which take
@@ -1510,9 +1603,10 @@ template <bool kBf16, int kDim, int kKind>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(AttendArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[mixed_lds_bytes<kDim>()];
-    const uint32_t tiles = a.tiles * a.kv_heads * a.tile_split;
+    const uint32_t tiles = kKind == kPlain ? a.tiles * a.kv_heads * a.tile_split : a.tile_groups;
     if (blockIdx.x < tiles) {
-        attend_tile<kBf16, kDim, kKind>(a, lds, blockIdx.x, tiles);
+        if constexpr (kKind == kPlain) attend_tile<kBf16, kDim>(a, lds, blockIdx.x, tiles);
+        else attend_tiles<kBf16, kDim, kKind>(a, lds, blockIdx.x);
     } else {
         attend_few_units<kBf16, kDim, kKind>(a, lds, blockIdx.x - tiles);
     }
@@ -1524,13 +1618,12 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_shared_kernel(
 {
     constexpr int kBytes = share_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? share_lds_bytes<kDim>() : few_lds_bytes<kDim>();
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
-    const uint32_t share = a.share_tiles * a.kv_heads * a.share_split, tiles = a.tiles * a.kv_heads * a.tile_split;
-    if (blockIdx.x < share) {
-        attend_tile<kBf16, kDim, kShare>(a, lds, blockIdx.x, share);
-    } else if (blockIdx.x - share < tiles) {
-        attend_tile<kBf16, kDim, kMore>(a, lds, blockIdx.x - share, tiles);
+    if (blockIdx.x < a.share_groups) {
+        attend_tiles<kBf16, kDim, kShare>(a, lds, blockIdx.x);
+    } else if (blockIdx.x - a.share_groups < a.tile_groups) {
+        attend_tiles<kBf16, kDim, kMore>(a, lds, blockIdx.x - a.share_groups);
     } else {
-        attend_few_units<kBf16, kDim, kMore>(a, lds, blockIdx.x - share - tiles);
+        attend_few_units<kBf16, kDim, kMore>(a, lds, blockIdx.x - a.share_groups - a.tile_groups);
     }
 }
 
@@ -1563,39 +1656,56 @@ struct Parts {
     }
 };
 
+// The parts of a few-row sequence's row: `place` and `parts` as its first workgroup left them.
+__device__ __forceinline__ void few_rows_of(const AttendArgs& a, Parts& p, uint32_t place, uint32_t parts, uint32_t r)
+{
+    const uint64_t row = uint64_t(place) * kFewRows + r;
+    p.parts = parts;
+    // a place a workgroup apart: first ones with few_per; else see attend_few_units
+    p.step = a.few_per ? uint64_t(a.seqs) * a.kv_heads * kFewRows : 2 * kFewRows;
+    p.back = a.few_per ? 0 : kFewRows;
+    p.ml = a.few_ml + row;
+    p.o = a.few_o + row * a.dim;
+}
+
+__device__ __forceinline__ void tile_rows_of(const AttendArgs& a, Parts& p, uint32_t parts, uint32_t t, uint32_t h)
+{
+    const uint64_t row = uint64_t(t) * a.q_heads + h;
+    p.parts = parts;
+    p.step = uint64_t(a.tokens) * a.q_heads;
+    p.ml = a.tile_ml + row;
+    p.o = a.tile_o + row * a.dim;
+}
+
 template <int kKind>
 __device__ __forceinline__ Parts parts_of(const AttendArgs& a, uint32_t b, uint32_t t, uint32_t h)
 {
     Parts p{nullptr, nullptr, 0, 0, 0, 0, 0};
     const uint32_t kvh = h / a.group;
-    // (nothing the few-row kernel wrote where the sequence is not its)
-    const uint2 few_parts = a.few_parts ? a.few_parts[uint64_t(b) * a.kv_heads + kvh] : uint2{0, 0};
-    const Seq s = seq_of<kKind>(a, b);
-    if (t < s.q0 || t >= s.q0 + s.n_new) return p;
-    if constexpr (kKind == kMore) {
-        if (s.from > 0) {
-            const uint32_t per = share_part(uint32_t(s.from), a.share_split);
-            p.share = (uint32_t(s.from) + per - 1) / per;
-            p.row0 = uint64_t(t) * a.q_heads + h;
-        }
+    if constexpr (kKind == kPlain) {
+        // (nothing the few-row kernel wrote where the sequence is not its)
+        const uint2 few_parts = a.few_parts ? a.few_parts[uint64_t(b) * a.kv_heads + kvh] : uint2{0, 0};
+        const Seq s = seq_of(a, b);
+        if (t < s.q0 || t >= s.q0 + s.n_new) return p;
+        if (s.n_new * a.group <= a.few_rows) few_rows_of(a, p, few_parts.x, few_parts.y, (t - s.q0) * a.group + (h - kvh * a.group));
+        else tile_rows_of(a, p, cut_of(a, s, a.tile_per).parts, t, h);
+        return p;
     }
-    const bool few = s.n_new * a.group <= a.few_rows;
-    if (few && (kKind == kPlain || (a.few_parts && few_parts.y > 1))) {
-        const uint64_t row = uint64_t(few_parts.x) * kFewRows + (t - s.q0) * a.group + (h - kvh * a.group);
-        p.parts = few_parts.y;
-        // a place a workgroup apart: first ones with few_per; else see attend_few_units
-        p.step = a.few_per ? uint64_t(a.seqs) * a.kv_heads * kFewRows : 2 * kFewRows;
-        p.back = a.few_per ? 0 : kFewRows;
-        p.ml = a.few_ml + row;
-        p.o = a.few_o + row * a.dim;
+    // A few-row sequence's parts are in few_joins: nothing else is waited for.
+    const uint4 joins = a.few_joins[uint64_t(b) * a.kv_heads + kvh];
+    const uint32_t q0 = rows_at(a, b), end = rows_at(a, b + 1);
+    if (t < q0 || t >= end) return p;
+    if ((end - q0) * a.group <= a.few_rows) {
+        if (joins.y > 1) few_rows_of(a, p, joins.x, joins.y, (t - q0) * a.group + (h - kvh * a.group));
+        else tile_rows_of(a, p, 1, t, h);
+        p.share = joins.z;
     } else {
-        const uint64_t row = uint64_t(t) * a.q_heads + h;
-        p.parts = few ? 1 : cut_of<kKind>(a, s, a.tile_per).parts;
-        if (kKind == kMore && p.parts == 0) p.parts = 1;
-        p.step = uint64_t(a.tokens) * a.q_heads;
-        p.ml = a.tile_ml + row;
-        p.o = a.tile_o + row * a.dim;
+        const Seq s = seq_of<kKind>(a, b);
+        const uint32_t parts = cut_of<kKind>(a, s, a.tile_per).parts;
+        tile_rows_of(a, p, parts ? parts : 1, t, h);
+        p.share = share_parts(a, b, s.from);
     }
+    p.row0 = uint64_t(t) * a.q_heads + h;
     p.parts += p.share;
     return p;
 }
@@ -1753,11 +1863,11 @@ template <bool kBf16, int kDim, int kKind>
 hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
 {
     const dim3 block(256);
-    const uint32_t tiles = p.tile ? p.tiles * a.kv_heads * p.tile_split : 0;
-    const uint32_t share = p.share_tiles * a.kv_heads * p.share_split;
+    const uint32_t tiles = p.tile_groups;
     hipError_t e;
-    if (share) {
-        e = launch(attend_shared_kernel<kBf16, kDim>, dim3(share + tiles + (p.few ? p.few_groups : 0)), block, stream, a);
+    if (p.share_groups) {
+        e = launch(attend_shared_kernel<kBf16, kDim>, dim3(p.share_groups + tiles + (p.few ? p.few_groups : 0)), block,
+                   stream, a);
     } else if (p.few && p.tile) {
         e = launch(attend_mixed_kernel<kBf16, kDim, kKind>, dim3(tiles + p.few_groups), block, stream, a);
     } else if (p.few) {
@@ -1861,24 +1971,26 @@ int secure_infer_gpu_paged_attention_more(hipStream_t stream, const si_paged_att
     uint8_t* const ws = static_cast<uint8_t*>(d->workspace);
     a.few_o = reinterpret_cast<float*>(ws + p.few_o);
     a.few_ml = reinterpret_cast<float2*>(ws + p.few_ml);
-    a.few_parts = p.few_ml ? reinterpret_cast<uint2*>(ws + p.few_parts) : nullptr;
+    a.few_parts = p.few_parts ? reinterpret_cast<uint2*>(ws + p.few_parts) : nullptr;
     a.tile_o = reinterpret_cast<float*>(ws + p.tile_o);
     a.tile_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
     const bool bf16 = d->dtype == SI_DTYPE_BF16;
     hipError_t e;
-    if (!p.sinks && !p.share_tiles) {
+    if (!p.sinks && !p.share_groups) {
         e = bf16 ? attend_by_dim<true, kPlain>(stream, a, p) : attend_by_dim<false, kPlain>(stream, a, p);
     } else {
         a.sinks = p.sinks;
-        if (p.share_tiles) {
+        if (p.share_groups) {
             a.groups = more->groups;
             a.group_starts = more->group_starts;
             a.prefix_lens = more->prefix_lens;
         }
-        a.share_tiles = p.share_tiles;
+        a.share_groups = p.share_groups;
         a.share_split = p.share_split;
         a.share_o = reinterpret_cast<float*>(ws + p.share_o);
         a.share_ml = reinterpret_cast<float2*>(ws + p.share_ml);
+        a.few_joins = p.few_joins ? reinterpret_cast<uint4*>(ws + p.few_joins) : nullptr;
+        a.tile_groups = p.tile_groups;
         e = bf16 ? attend_by_dim<true, kMore>(stream, a, p) : attend_by_dim<false, kMore>(stream, a, p);
     }
     return e == hipSuccess ? 0 : -1;

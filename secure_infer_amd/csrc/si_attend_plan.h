@@ -46,14 +46,20 @@ constexpr uint32_t kMostLength = 3u << 29;
 constexpr uint32_t kFewWhole = kFewStep / kFewKeys;
 
 // Prefixes that groups of sequences share: workgroups their tiles are cut for, and the least keys of a part.
+// A part's numerators (rows x dim floats, written and read again) weigh against its K and V (keys x dim x
+// 4 bytes): four keys a row, of a tile's 128.  64 next tokens x 7 heads behind 8,192 keys: least 512 33.3 us, 256
+// 38.5; 8 x 4 heads behind 6,144: 25.5 and 18.6.
 constexpr uint64_t kShareTarget = 512;
 constexpr uint32_t kShareMin = 256;
+constexpr uint32_t kShareMost = 4 * kTileRows;
 
-// Keys of a part of a prefix that is cut into at most `split` parts.
-constexpr uint32_t share_part(uint32_t keys, uint32_t split)
+// Keys of a part of a prefix that is cut into at most `split` parts, of a group of `rows` rows a KV head.
+constexpr uint32_t share_part(uint32_t keys, uint32_t split, uint64_t rows)
 {
     const uint32_t even = ((keys + split - 1) / split + kTileKeys - 1) / kTileKeys * kTileKeys;
-    return even > kShareMin ? even : kShareMin;
+    const uint64_t four = (4 * rows + kTileKeys - 1) / kTileKeys * kTileKeys;
+    const uint32_t least = four < kShareMin ? kShareMin : four < kShareMost ? uint32_t(four) : kShareMost;
+    return even > least ? even : least;
 }
 
 // How a call is launched.  The device's lengths are not known here: the table's
@@ -63,8 +69,8 @@ struct Plan {
     uint32_t few_rows = 0, few_groups = 0, few_least = 0, few_per = 0, tile_per = 0, tile_split = 1, tiles = 0;
     bool few = false, tile = false, fits = true;
     uint64_t few_o = 0, few_ml = 0, few_parts = 0, tile_o = 0, tile_ml = 0, bytes = 0;
-    uint32_t sinks = 0, share_tiles = 0, share_split = 1;
-    uint64_t share_o = 0, share_ml = 0;
+    uint32_t sinks = 0, share_groups = 0, share_split = 1, tile_groups = 0;
+    uint64_t share_o = 0, share_ml = 0, few_joins = 0;
 };
 
 // Keys of a part, so that `groups` sequences of `keys` keys make about `target`
@@ -141,18 +147,26 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
             p.tile_split = (p.tile_split + even - 1) / even * even;
         }
     }
+    // Workgroups: a place for each tile and column that the call's sizes allow.  Beside sinks and shared prefixes the
+    // device counts the tiles there are: all rows' full ones and one more of each sequence that is long enough, or
+    // of each group of two or more.  (A multiple of the XCDs.)
+    uint64_t tile_groups = uint64_t(p.tiles) * d.kv_heads * p.tile_split, share_groups = 0;
+    const auto least = [](uint64_t x, uint64_t y) { return x < y ? x : y; };
+    if (more && p.tile && d.q_starts)
+        tile_groups = (rows / kTileRows + least(d.seqs, rows / (p.few_rows + 1))) * d.kv_heads * p.tile_split;
+    if (more && p.tile) tile_groups = (tile_groups + 7) / 8 * 8;
     if (groups) {
-        p.share_tiles = uint32_t(rows / kTileRows + groups);
-        const uint64_t columns = (rows / kTileRows + 1) * d.kv_heads;
-        const uint64_t split = (kShareTarget + columns - 1) / columns;
+        const uint64_t columns = (rows / kTileRows + 1) * d.kv_heads, split = (kShareTarget + columns - 1) / columns;
         p.share_split = uint32_t(split < most_parts ? split : most_parts);
+        share_groups = (rows / kTileRows + least(groups, d.seqs / 2)) * d.kv_heads * p.share_split;
+        share_groups = (share_groups + 8) / 8 * 8;
     }
     // (threads of a launch dimension fit 32 bits)
     const uint64_t most = (1ull << 32) / 256 - 1;
-    const uint64_t tile_groups = uint64_t(p.tiles) * d.kv_heads * p.tile_split;
     p.few_groups = uint32_t(few_groups);
-    const uint64_t share_groups = uint64_t(p.share_tiles) * d.kv_heads * p.share_split;
     p.fits = share_groups + few_groups + tile_groups <= most && uint64_t(d.tokens) * d.q_heads / 4 < most;
+    p.tile_groups = uint32_t(tile_groups);
+    p.share_groups = uint32_t(share_groups);
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
@@ -162,7 +176,7 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
         const uint64_t n = places * kFewRows;
         p.few_o = take(n * d.head_dim * 4);
         p.few_ml = take(n * 8);
-        p.few_parts = take(pairs * 8);
+        if (!more) p.few_parts = take(pairs * 8);
     }
     if (p.tile_split > 1 || groups) {
         const uint64_t n = uint64_t(p.tile_split) * d.tokens * d.q_heads;
@@ -174,6 +188,7 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
         p.share_o = take(n * d.head_dim * 4);
         p.share_ml = take(n * 8);
     }
+    if (more && p.bytes) p.few_joins = take(pairs * 16);
     return p;
 }
 

@@ -52,7 +52,7 @@ void check(const si_paged_attention_desc& d, const si_paged_attention_more& m, s
     if (!p.sinks && !m.groups) {
         const Plan q = attend_plan(d);
         expect(p.bytes == q.bytes && p.few_groups == q.few_groups && p.few_per == q.few_per && p.tile_per == q.tile_per &&
-                   p.tile_split == q.tile_split && p.tiles == q.tiles && p.fits == q.fits && p.share_tiles == 0,
+                   p.tile_split == q.tile_split && p.tiles == q.tiles && p.fits == q.fits && p.share_groups == 0,
                "plain", d, m);
     }
     if (!p.fits) return;
@@ -68,7 +68,7 @@ void check(const si_paged_attention_desc& d, const si_paged_attention_more& m, s
             const uint64_t n = p.few_per ? p.few_groups : 2ull * p.few_groups;
             region(p.few_o, n * kFewRows * d.head_dim * 4);
             region(p.few_ml, n * kFewRows * 8);
-            region(p.few_parts, pairs * 8);
+            if (!p.sinks && !m.groups) region(p.few_parts, pairs * 8);
         }
         for (int i = 0; i < 6; ++i) {
             const uint64_t len = i < 2 ? keys : g() % (keys + 1), group = d.q_heads / d.kv_heads;
@@ -111,13 +111,35 @@ void check(const si_paged_attention_desc& d, const si_paged_attention_more& m, s
         region(p.share_o, n * d.head_dim * 4);
         region(p.share_ml, n * 8);
         expect(p.share_split >= 1 && p.share_split <= kMaxSplit / 2, "prefix parts' number", d, m);
-        // (a group's tiles begin at floor(row / 128) + its number)
-        expect(p.share_tiles >= uint64_t(d.tokens) * (d.q_heads / d.kv_heads) / kTileRows + m.groups, "prefix tiles", d, m);
+        expect(p.share_groups > 0 && p.share_groups % 8 == 0, "prefix tiles", d, m);
         for (uint64_t len : {uint64_t(1), keys, 1 + g() % keys}) {
-            const uint64_t per = share_part(uint32_t(len), p.share_split);
+            const uint64_t per = share_part(uint32_t(len), p.share_split, g() % (1 + uint64_t(d.tokens) * d.q_heads));
             expect(per % kTileKeys == 0 && per >= kTileKeys && (len + per - 1) / per <= p.share_split, "prefix part", d, m);
         }
         most += p.share_split;
+    }
+    if (p.few_joins) region(p.few_joins, pairs * 16);
+    expect(p.few_joins || p.bytes == 0 || !(p.sinks || m.groups), "joins", d, m);
+    if (p.sinks || m.groups) {
+        // workgroups for every tile that lengths can make: n sequences, or groups, of rows that add up
+        const uint64_t group = d.q_heads / d.kv_heads, tokens = d.tokens;
+        for (int i = 0; i < 4; ++i) {
+            // sequences of n tokens each, and the tokens that are left to one more
+            const uint64_t n = i ? 1 + g() % (i == 1 ? 2 * kTileRows / group + 1 : tokens) : kFewRows / group + 1;
+            uint64_t seqs = tokens / n < d.seqs ? tokens / n : d.seqs, rest = seqs < d.seqs ? tokens - seqs * n : 0;
+            const auto tiles = [&](uint64_t t) { return t * group > p.few_rows ? (t * group + kTileRows - 1) / kTileRows : 0; };
+            if (!d.q_starts) seqs = tokens, rest = 0;
+            const uint64_t there = seqs * tiles(d.q_starts ? n : 1) + tiles(rest);
+            if (p.tile) expect(there * d.kv_heads * p.tile_split <= p.tile_groups, "tiles", d, m);
+            else expect(there == 0, "tiles without a kernel", d, m);
+            // groups of at least two sequences, of n tokens each
+            if (m.groups) {
+                const uint64_t most_groups = m.groups < d.seqs / 2 ? m.groups : d.seqs / 2;
+                const uint64_t k = tokens / n < most_groups ? tokens / n : most_groups;
+                const uint64_t t = k * ((n * group + kTileRows - 1) / kTileRows);
+                expect(t * d.kv_heads * p.share_split <= p.share_groups, "prefix tiles", d, m);
+            }
+        }
     }
     expect(most <= kMaxSplit, "parts of a row", d, m);
 }
