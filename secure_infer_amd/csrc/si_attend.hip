@@ -1600,7 +1600,7 @@ constexpr int mixed_lds_bytes()
 }
 
 template <bool kBf16, int kDim, int kKind>
-__global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim <= 64 && kKind == kMore ? 3 : 2) void attend_mixed_kernel(AttendArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[mixed_lds_bytes<kDim>()];
     const uint32_t tiles = kKind == kPlain ? a.tiles * a.kv_heads * a.tile_split : a.tile_groups;
@@ -1612,9 +1612,10 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_mixed_kernel(A
     }
 }
 
-// The groups' prefixes first, then each sequence's own keys.
+// The groups' prefixes first, then each sequence's own keys.  (Three waves a SIMD for heads up to 64, here and in
+// kMore's mixed kernel: 45 sequences of 4 tokens, 12/4 heads, behind seven prefixes 27.2 us, two 31.5.)
 template <bool kBf16, int kDim>
-__global__ __launch_bounds__(256, kDim > 128 ? 1 : 2) void attend_shared_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim <= 64 ? 3 : 2) void attend_shared_kernel(AttendArgs a)
 {
     constexpr int kBytes = share_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? share_lds_bytes<kDim>() : few_lds_bytes<kDim>();
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];

@@ -118,7 +118,7 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
         const uint64_t units = (keys + unit - 1) / unit, fewest = (units + most_parts - 2) / (most_parts - 1);
         // workgroups that run at a time: 3 a CU for heads up to 64 (2 beside tiles), 2 up to 128, 1
         // (768 or 1,536 for heads of 128: 64 sequences of 8,192 keys 229 and 209 us, 512 197)
-        const uint64_t at_once = d.head_dim <= 64 && !p.tile ? 768 : d.head_dim <= 128 ? 512 : 256;
+        const uint64_t at_once = d.head_dim <= 64 && (more || !p.tile) ? 768 : d.head_dim <= 128 ? 512 : 256;
         p.few_least = uint32_t(more ? most_parts : fewest > whole ? fewest : whole);
         if (d.seqs <= 64 && pairs <= at_once) {
             // (kMore: the device finds the least units of a share from the lengths)
@@ -127,7 +127,10 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
             places = units > whole ? 2 * few_groups : 0;
         } else {
             uint32_t parts;
-            p.few_per = uint32_t(part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &parts, most_parts) / unit);
+            // (own keys behind a shared prefix are mostly few, and parts that are not there cost a workgroup each:
+            // 256 of 1 to 256 keys x 8 heads behind 32,768 343 us, with kFewTarget 348)
+            const uint64_t target = groups ? kFewTarget / 4 : kFewTarget;
+            p.few_per = uint32_t(part_keys(pairs, keys, kFewStep, kFewStep, target, &parts, most_parts) / unit);
             few_groups = pairs * parts;
             places = parts > 1 ? few_groups : 0;
         }

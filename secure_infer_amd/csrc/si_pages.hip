@@ -557,9 +557,17 @@ __device__ __forceinline__ void turn(uint32_t x, uint32_t y, float2 cs, uint32_t
     v = as_16<kBf16>(__builtin_fmaf(b, cs.x, a * cs.y));
 }
 
-// One wave per token (or `split` waves, where tokens are few): its lanes form the cosines and sines of the
-// token's angles, a pair a lane, in the wave's LDS, and every head's rows are turned by them.
-constexpr uint32_t kRotateAhead = 4;
+// The append with rotation: y = m (x cos a - x' sin a), y' = m (x' cos a + x sin a), a = p f_i, of K's and q's
+// rows; V as it is.  `split` waves a token: a wave's lanes form the cosines and sines of the token's angles, a
+// pair a lane, in the wave's LDS, and turn their share of its heads' rows by them.  A task is 16 bytes of
+// V, or a pair of them of K or q: one lane reads and writes both of a pair, so that q can turn in place.  The bytes
+// bound it: 14,668 tokens of 32 + 8 + 8 heads of 128, bf16, out of a fused projection (360 MB) 66.7 us, 5.4 TB/s (some
+// of it in the Infinity Cache).  Eight loads in flight and at most four tasks a lane: four in flight 66.8, and 6.4 us
+// where eight take 5.8 for 1,944 tokens of 12 + 4 + 4 heads of 80; all tasks of a token to one wave 74, two a lane 80.
+// Stores past the caches, q's too (the next kernel runs on other XCDs): 70.8 where ordinary ones took 74.9.  64 tokens:
+// 3.4 us, the latency of finding the place.
+constexpr uint32_t kRotateAhead = 8;
+constexpr uint32_t kRotateTasks = 4 * 64;
 constexpr uint32_t kRotatePairs = 128;
 
 template <bool kBf16, int kPairs>
@@ -705,11 +713,11 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(RotateArgs r)
                 }
             }
             if (kPairs == kHalves4 && pair(k)) {
-                *reinterpret_cast<u32x2*>(k.dst) = u32x2{lo[i][0], lo[i][1]};
-                *reinterpret_cast<u32x2*>(k.dst + half) = u32x2{lo[i][2], lo[i][3]};
+                __builtin_nontemporal_store(u32x2{lo[i][0], lo[i][1]}, reinterpret_cast<u32x2*>(k.dst));
+                __builtin_nontemporal_store(u32x2{lo[i][2], lo[i][3]}, reinterpret_cast<u32x2*>(k.dst + half));
             } else {
-                *reinterpret_cast<u32x4*>(k.dst) = lo[i];
-                if (pair(k)) *reinterpret_cast<u32x4*>(k.dst + half) = hi[i];
+                __builtin_nontemporal_store(lo[i], reinterpret_cast<u32x4*>(k.dst));
+                if (pair(k)) __builtin_nontemporal_store(hi[i], reinterpret_cast<u32x4*>(k.dst + half));
             }
         }
     }
@@ -859,9 +867,11 @@ bool rotate_args(const si_paged_append_desc& d, const si_rotation& x, RotateArgs
     r.row_tasks = r.rot_tasks + (d.head_dim - x.rot) / 8;
     const uint64_t tasks = (uint64_t(d.kv_heads) + x.q_heads) * r.row_tasks + uint64_t(d.kv_heads) * (d.head_dim / 8);
     r.tasks = uint32_t(tasks);
-    // Waves for the whole chip where tokens are few, one task a lane at most.
-    const uint64_t split = 4096 / d.tokens, most = (tasks + 63) / 64;
-    r.split = uint32_t(split < 1 ? 1 : split < most ? split : most);
+    // At most kRotateTasks tasks a wave; waves for the whole chip where tokens are few, of a task a lane at least.
+    // (4,096 waves: 2,048 tokens 11.3 us; 16,384 15.0, the angles formed once a wave.)
+    const uint64_t least = (tasks + kRotateTasks - 1) / kRotateTasks, most = (tasks + 63) / 64;
+    const uint64_t split = 4096 / d.tokens > least ? 4096 / d.tokens : least;
+    r.split = uint32_t(split < most ? split : most);
     return true;
 }
 
@@ -906,9 +916,10 @@ int secure_infer_gpu_paged_append_rotated(hipStream_t stream, const si_paged_app
     using namespace si;
     RotateArgs r{};
     if (!append_args(d, r.a) || !rotation || !rotate_args(*d, *rotation, r)) return -1;
-    const uint32_t waves = d->tokens * r.split;
+    const uint64_t waves = uint64_t(d->tokens) * r.split;
+    if (waves / 4 >= (1ull << 32) / 256 - 1) return -1;  // (threads of a launch dimension fit 32 bits)
     const auto go = [&](auto kernel) {
-        return launch(kernel, dim3((waves + 3) / 4), dim3(256), stream, r) == hipSuccess ? 0 : -1;
+        return launch(kernel, dim3(uint32_t((waves + 3) / 4)), dim3(256), stream, r) == hipSuccess ? 0 : -1;
     };
     const bool bf16 = rotation->dtype == SI_DTYPE_BF16;
     if (rotation->adjacent)
