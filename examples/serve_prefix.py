@@ -3,7 +3,7 @@
 The prefix's K and V come back from host memory through the authenticated
 reload into pages taken from the free slots; a prompt chunk is appended and
 attended to over them; the sequence is forked into samples that share the
-prefix's pages and decode a token a step; one sample ends, its pages are
+prefix's pages, which their tokens' attention reads once for all, and decode a token a step; one sample ends, its pages are
 cleared, and the cache is compacted; the kept sequence's pages go back to host
 memory sealed.  The model is a stand-in: random q, k and v per token.
 
@@ -54,15 +54,18 @@ class Server:
     def compact(self) -> None:
         self.tables, self.refs = si.compact_pages(self.caches, self.tables, self.refs, scrub=True)
 
-    def attend(self, layer: int, q, k, v, rows, counts):
+    def attend(self, layer: int, q, k, v, rows, counts, shared=0):
         """New tokens of `rows` (counts[i] of row rows[i], already reserved): their K
-        and V into the pages, and their attention."""
+        and V into the pages, and their attention.  The rows' first `shared` tokens are the same."""
         k_cache, v_cache = self.layers[layer]
         r = torch.tensor(rows, device="cuda")
         starts = torch.tensor([0, *counts], device="cuda").cumsum(0)
         tables, kv_lens = self.tables[r], self.kv_lens[r]
         si.paged_append(k, v, k_cache, v_cache, tables, kv_lens, q_starts=starts, fail_count=self.unserved)
-        return si.paged_attention(q, k_cache, v_cache, tables, kv_lens, q_starts=starts)
+        groups = torch.tensor([0, len(rows)], device="cuda") if shared else None
+        lens = torch.tensor([shared], device="cuda") if shared else None
+        return si.paged_attention(q, k_cache, v_cache, tables, kv_lens, q_starts=starts, prefix_groups=groups,
+                                  prefix_lens=lens)
 
     def slots_of(self, row: int) -> torch.Tensor:
         """The row's slots on the host, as the transfers' mappings want them."""
@@ -99,14 +102,14 @@ def serve(layers=4, q_heads=8, heads=2, dim=128, prefix=700, chunk=45, samples=3
         if transfer.wait_layer(layer) != 0:
             raise RuntimeError(f"layer {layer}: the stored prefix did not authenticate")
 
-    def step(rows, counts):
+    def step(rows, counts, shared=0):
         add = [0] * (samples + 1)
         for r, n in zip(rows, counts):
             add[r] = n
         srv.reserve(add)
         for layer in range(layers):
             k, v, q = rand(sum(counts), heads, dim), rand(sum(counts), heads, dim), rand(sum(counts), q_heads, dim)
-            out = srv.attend(layer, q, k, v, rows, counts)
+            out = srv.attend(layer, q, k, v, rows, counts, shared)
             at = 0
             for r, n in zip(rows, counts):
                 log.append((layer, r, k[at:at + n], v[at:at + n], q[at:at + n], out[at:at + n]))
@@ -117,7 +120,7 @@ def serve(layers=4, q_heads=8, heads=2, dim=128, prefix=700, chunk=45, samples=3
     log.append(("fork", 0, list(range(1, samples + 1))))
     rows = list(range(samples + 1))
     for i in range(steps):
-        step(rows, [1] * len(rows))
+        step(rows, [1] * len(rows), (prefix + chunk) // TOKENS * TOKENS)  # a fork shares whole pages
         if i == steps // 2 and samples:        # one sample ends
             srv.free([rows.pop()])
             srv.compact()

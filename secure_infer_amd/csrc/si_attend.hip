@@ -1693,7 +1693,7 @@ __device__ __forceinline__ Parts parts_of(const AttendArgs& a, uint32_t b, uint3
         return p;
     }
     // A few-row sequence's parts are in few_joins: nothing else is waited for.
-    const uint4 joins = a.few_joins[uint64_t(b) * a.kv_heads + kvh];
+    const uint4 joins = a.few_joins ? a.few_joins[uint64_t(b) * a.kv_heads + kvh] : uint4{0, 0, 0, 0};
     const uint32_t q0 = rows_at(a, b), end = rows_at(a, b + 1);
     if (t < q0 || t >= end) return p;
     if ((end - q0) * a.group <= a.few_rows) {

@@ -191,7 +191,7 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
         p.share_o = take(n * d.head_dim * 4);
         p.share_ml = take(n * 8);
     }
-    if (more && p.bytes) p.few_joins = take(pairs * 16);
+    if (more && p.few && p.bytes) p.few_joins = take(pairs * 16);
     return p;
 }
 

@@ -234,6 +234,8 @@ def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor
     rot = 2 * freqs.shape[0]
     if rot == 0 or rot % 8 or rot > min(dim, 256):
         raise ValueError(f"freqs must hold a multiple of 4 frequencies, at most {min(dim, 256) // 2}")
+    if freqs.requires_grad:
+        _tracked()
     if not math.isfinite(magnitude):
         raise ValueError("magnitude must be finite")
     if positions is not None:
@@ -258,16 +260,20 @@ def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor
         if q.requires_grad or (q_out is not None and q_out.requires_grad):
             _tracked()
         if q_out is None:
-            q_out = _empty(other, q.shape, dtype, device)
+            q_out = q.new_empty(q.shape) if other is None else _empty(other, q.shape, dtype, device)
             ot, oh = q_heads * dim, dim
         else:
             if not isinstance(q_out, torch.Tensor) or q_out.shape != q.shape:
                 raise ValueError("q_out must have q's shape")
             _, ot, oh = _rows(q_out, "q_out", q_heads, dim, dtype, device)
             _apart(ot, oh, tokens, q_heads, dim, "q_out")
-            if q_out.data_ptr() != q.data_ptr() or (ot, oh) != (qt, qh):
-                for t, name in ((q, "q"), (k, "k"), (v, "v")):
-                    if _meet(q_out, t):
+            if d is not None and (q_out.data_ptr() != q.data_ptr() or (ot, oh) != (qt, qh)):
+                # the memory from an input's first element to its last
+                lo, hi = _extent(q_out.data_ptr(), ot, oh, tokens, q_heads, dim)
+                for name, at in (("q", _extent(q.data_ptr(), qt, qh, tokens, q_heads, dim)),
+                                 ("k", _extent(d.k, d.k_token_stride, d.k_head_stride, tokens, heads, dim)),
+                                 ("v", _extent(d.v, d.v_token_stride, d.v_head_stride, tokens, heads, dim))):
+                    if lo < at[1] and at[0] < hi:
                         raise ValueError(f"q_out must be q itself, or not overlap {name}")
         r.q, r.q_out, r.q_heads = q.data_ptr(), q_out.data_ptr(), q_heads
         r.q_token_stride, r.q_head_stride, r.q_out_token_stride, r.q_out_head_stride = qt, qh, ot, oh
@@ -288,11 +294,9 @@ def _apart(token: int, head: int, tokens: int, heads: int, dim: int, name: str) 
         span += stride * (n - 1)
 
 
-def _meet(a, b) -> bool:
-    """The memory from a tensor's first element to its last overlaps the other's."""
-    def end(t):
-        return t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)))
-    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+def _extent(start: int, token: int, head: int, tokens: int, heads: int, dim: int) -> tuple[int, int]:
+    """First byte, and the one after the last, of 16-bit rows."""
+    return start, start + 2 * ((tokens - 1) * token + (heads - 1) * head + dim)
 
 
 def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, tables: torch.Tensor,
@@ -330,7 +334,7 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
         return torch.empty_like(q) if out is None else out
     raw, other = _stream_of(stream, device)
     if out is None:
-        out = _empty(other, q.shape, q.dtype, device)
+        out = q.new_empty(q.shape) if other is None else _empty(other, q.shape, q.dtype, device)
         d.out, d.out_token_stride, d.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
     L = lib()
     need = (L.secure_infer_gpu_paged_attention_workspace(ct.byref(d)) if more is None else

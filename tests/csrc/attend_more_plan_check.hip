@@ -119,7 +119,7 @@ void check(const si_paged_attention_desc& d, const si_paged_attention_more& m, s
         most += p.share_split;
     }
     if (p.few_joins) region(p.few_joins, pairs * 16);
-    expect(p.few_joins || p.bytes == 0 || !(p.sinks || m.groups), "joins", d, m);
+    expect(p.few_joins || !p.few || p.bytes == 0 || !(p.sinks || m.groups), "joins", d, m);
     if (p.sinks || m.groups) {
         // workgroups for every tile that lengths can make: n sequences, or groups, of rows that add up
         const uint64_t group = d.q_heads / d.kv_heads, tokens = d.tokens;

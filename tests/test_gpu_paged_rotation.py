@@ -207,7 +207,7 @@ def test_refusals():
             (dict(cache_v=d["cv"].half()), "cache_v"), (dict(kv_lens=d["kv"].int()), "kv_lens")):
         with pytest.raises(ValueError, match=what):
             si.paged_append_rotated(**{**good, **change})
-    for name in ("q", "k", "v"):
+    for name in ("q", "k", "v", "freqs"):
         with pytest.raises(ValueError, match="gradient"):
             si.paged_append_rotated(**{**good, name: good[name].clone().requires_grad_()})
     none = dict(k=d["k"][:0], v=d["v"][:0], q=d["q"][:0], tables=d["tables"][:0], kv_lens=d["kv"][:0])

@@ -448,3 +448,56 @@ def test_in_a_graph_and_pages_past_32_bit_offsets():
             got = out.clone()
             assert torch.equal(got, step())
             torch.cuda.synchronize()
+
+
+def wide(x, pages):
+    """The batch with table rows of `pages` entries, no page past the ones it had."""
+    t = torch.full((x["tables"].shape[0], pages), -1, dtype=torch.int64)
+    t[:, :x["tables"].shape[1]] = x["tables"]
+    return {**x, "tables": t}
+
+
+@pytest.mark.parametrize("new", [1, 9, 700])
+def test_under_the_longest_table(new):
+    """Tables of 2^30 positions: windows with sinks, and prefixes, of sequences that end long before."""
+    x = share(18, [(900, [(new, new), (new + 40, new)]), (33, [(new, new), (new, new)])], 16, 1, 8, 32768, torch.bfloat16)
+    x = wide(x, 32768)
+    rows = {0, 1, new - 1, new, 2 * new - 1, 2 * new, 4 * new - 1}
+    check(x, rows=rows)
+    check(x, rows=rows, window=200, sinks=5)
+    plain = {k: v for k, v in x.items() if k not in ("groups", "prefix")}
+    plain["tables"][1, 0], plain["tables"][3, 0] = plain["tables"][0, 0], plain["tables"][2, 0]
+    check(plain, rows=rows, window=200, sinks=5)
+    check(plain, rows=rows, window=(1 << 31) - 1, sinks=1 << 30)
+
+
+def test_positions_at_their_last_place():
+    """Lengths up to 3 * 2^29 count as they are; the keys there are, sinks among them, end with the table."""
+    last = 3 << 29
+    x = share(19, [(200, [(56, 1), (60, 1)])], 4, 2, 64, 64, torch.bfloat16)
+    x["tables"] = x["tables"][:, :4]
+    for window, sinks in ((0, 0), (last - 100, 3), (last - 300, 70), (5, 9)):
+        x["kv"] = torch.tensor([last, 256])
+        check(x, window=window, sinks=sinks)
+        plain = {k: v for k, v in x.items() if k not in ("groups", "prefix")}
+        check(plain, window=window, sinks=sinks)
+
+
+def test_many_sequences_of_one_prefix_and_one_long_tail():
+    """More pairs than the even shares take, most of them short, one of many parts."""
+    g = torch.Generator().manual_seed(5)
+    tails = [int(n) for n in torch.randint(1, 200, (140,), generator=g)]
+    tails[77] = 6000
+    x = share(20, [(300, [(n, 1) for n in tails])], 8, 4, 64, 64, torch.bfloat16)
+    check(x, use_starts=False, rows={0, 1, 76, 77, 78, 139})
+    check(x, rows={0, 1, 76, 77, 78, 139}, window=2500, sinks=40)
+
+
+@pytest.mark.parametrize("new", [[300, 1, 1], [700, 40, 3]])
+def test_long_chunks_behind_a_prefix(new):
+    """Sequences of a group that run in tiles of their own, their keys in several parts."""
+    x = share(21, [(777, [(n + 3000 * (i == 0), n) for i, n in enumerate(new)])], 8, 2, 128, 64, torch.bfloat16)
+    rows = {0, 1, 150, new[0] - 1, new[0], sum(new) - 1}
+    check(x, rows=rows)
+    check(x, rows=rows, causal=False)
+    check(x, rows=rows, window=1000, sinks=10)
