@@ -284,6 +284,15 @@ __device__ __forceinline__ uint32_t share_parts(const AttendArgs& a, uint32_t b,
     return (uint32_t(from) + per - 1) / per;
 }
 
+// Where a sequence of n tokens, s.n_new of them new, stands: these stand where the append puts them,
+// also where the length outgrows the table.
+__device__ __forceinline__ void place_seq(const AttendArgs& a, Seq& s, int64_t n)
+{
+    const int64_t most = int64_t(a.pages) << a.page_shift;
+    s.len = int32_t(n < 0 ? 0 : n > most ? most : n);
+    s.base = (n > most && n <= int64_t(kMostLength) ? int32_t(n) : s.len) - int32_t(s.n_new);
+}
+
 template <int kKind = kPlain>
 __device__ __forceinline__ Seq seq_of(const AttendArgs& a, uint32_t b)
 {
@@ -298,11 +307,7 @@ __device__ __forceinline__ Seq seq_of(const AttendArgs& a, uint32_t b)
         const uint32_t end = start_of(a, b + 1);
         s.n_new = end > s.q0 ? end - s.q0 : 0;
     }
-    // New tokens stand where the append puts them, also where the length outgrows the table.
-    const int64_t most = int64_t(a.pages) << a.page_shift;
-    const int64_t n = a.kv_lens[b];
-    s.len = int32_t(n < 0 ? 0 : n > most ? most : n);
-    s.base = (n > most && n <= int64_t(kMostLength) ? int32_t(n) : s.len) - int32_t(s.n_new);
+    place_seq(a, s, a.kv_lens[b]);
     return s;
 }
 
@@ -1057,9 +1062,10 @@ constexpr int share_lds_bytes()
 }
 
 // kShare: the same over (128 rows of all the tokens of a group of sequences, part of the prefix they share);
-// the rows differ in what they see of it.  Rows from r0 on of sequence b (kShare: of group g).
+// the rows differ in what they see of it.  Rows from r0 on of sequence s (kShare: all the tokens of group g, and
+// its prefix).
 template <bool kBf16, int kDim, int kKind>
-__device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uint32_t kvh, uint32_t part, uint32_t b,
+__device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uint32_t kvh, uint32_t part, const Seq& s,
                                           uint32_t r0, const Group& g)
 {
     constexpr int kChunks = tile_chunks<kDim>();
@@ -1074,18 +1080,6 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
     const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>((lds_void*)lds));
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = lane & 31u, half = lane >> 5;
-    Seq s;  // kShare: all the group's tokens, and its prefix
-    if constexpr (kKind == kShare) {
-        if (g.prefix == 0) return;
-        s.b = g.first;
-        s.q0 = same(rows_at(a, g.first));
-        const uint32_t end = same(rows_at(a, g.end));
-        s.n_new = end > s.q0 ? end - s.q0 : 0;
-        s.len = g.prefix;
-        s.base = s.from = 0;
-    } else {
-        s = seq_of<kKind>(a, b);
-    }
     const uint32_t rows = s.n_new * a.group;
     if ((kKind != kShare && rows <= a.few_rows) || r0 >= rows) return;
     const uint32_t per = kKind == kShare ? share_part(uint32_t(s.len), a.share_split, rows) : a.tile_per;
@@ -1143,7 +1137,7 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
             q[k] = (v & a.q_keep) ^ a.q_flip;
         }
     };
-    if constexpr (kKind != kShare) load_q();
+    if constexpr (kKind == kPlain) load_q();  // (else behind the first keys, which do not wait for it)
     // The tile's keys: from k0 (behind every row's window below lo) to hi.  kMore and kShare: k0, k_first and
     // k_end are places of the cut, from k_skip on those below k_lo are behind every window.
     const int32_t hi_all = a.causal && kKind != kShare ? keys_up_to(s, p_last) : s.len;
@@ -1298,8 +1292,8 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
     }
     pages.start(a, table, key(k0), hi);
     uint64_t ok_next = fill(0, k0);
+    if constexpr (kKind != kPlain) load_q();
     if constexpr (kKind == kShare) {
-        load_q();
         if (!a.window) find_limits();
         pw_first = least_last;
         pw_last = most_behind + int32_t(a.window) - 1;
@@ -1444,6 +1438,8 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
     if (!out) {
         const uint64_t row = (uint64_t(part) * a.tokens + t) * a.q_heads + h;
         if (half == 0) part_ml[row] = float2{shift, l};
+        // (numerators without a weight are not read)
+        if (kKind != kPlain && l == 0.0f) return;
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
 #pragma unroll
@@ -1515,7 +1511,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, uint8_t* lds, u
         b = tile / ((a.group + kTileRows - 1) / kTileRows);
         first_tile = b * ((a.group + kTileRows - 1) / kTileRows);
     }
-    tile_rows<kBf16, kDim, kPlain>(a, lds, kvh, part, b, (tile - first_tile) * kTileRows, Group{b, b + 1, 0});
+    tile_rows<kBf16, kDim, kPlain>(a, lds, kvh, part, seq_of(a, b), (tile - first_tile) * kTileRows, Group{b, b + 1, 0});
 }
 
 // kMore and kShare: the tiles that there are, counted, one to a workgroup; the workgroups behind them leave.
@@ -1527,10 +1523,12 @@ __device__ __forceinline__ void attend_tiles(const AttendArgs& a, uint8_t* lds, 
     const uint32_t n = kKind == kShare ? a.groups : a.seqs;
     // of the lane's sequence or group of 64: its tiles, their sum up to and with it
     Group mine{0, 0, 0};
-    uint32_t tiles = 0, with = 0;
+    uint32_t tiles = 0, with = 0, from = 0, end = 0;
+    int64_t length = 0;
     const auto count = [&](uint32_t s0) {
         const uint32_t s = s0 + lane;
-        uint32_t from = 0, end = 0, least = 0;
+        uint32_t least = 0;
+        from = end = 0;
         if (s < n) {
             if constexpr (kKind == kShare) {
                 mine = group_at(a, s);
@@ -1541,6 +1539,7 @@ __device__ __forceinline__ void attend_tiles(const AttendArgs& a, uint8_t* lds, 
             } else {
                 from = rows_at(a, s);
                 end = rows_at(a, s + 1);
+                length = a.kv_lens[s];
                 least = a.few_rows;
             }
         }
@@ -1567,9 +1566,23 @@ __device__ __forceinline__ void attend_tiles(const AttendArgs& a, uint8_t* lds, 
     if (!past) return;  // (there is one, unless the starts are written meanwhile)
     const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
     const uint32_t before = sum + uint32_t(__builtin_amdgcn_readlane(int(with - tiles), at));
-    const Group g{same(__shfl(mine.first, at)), same(__shfl(mine.end, at)), int32_t(same(uint32_t(__shfl(mine.prefix, at))))};
-    tile_rows<kBf16, kDim, kKind>(a, lds, column % a.kv_heads, column / a.kv_heads, s0 + uint32_t(at),
-                                  (tile - before) * kTileRows, g);
+    // (the lane's own, without another look at memory)
+    const auto of_at = [&](uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), at)); };
+    Group g{0, 0, 0};
+    Seq seq;
+    seq.q0 = of_at(from);
+    seq.n_new = of_at(end) > seq.q0 ? of_at(end) - seq.q0 : 0;
+    if constexpr (kKind == kShare) {
+        g = Group{of_at(mine.first), of_at(mine.end), int32_t(of_at(uint32_t(mine.prefix)))};
+        seq.b = g.first;
+        seq.len = g.prefix;
+        seq.base = seq.from = 0;
+    } else {
+        seq.b = s0 + uint32_t(at);
+        seq.from = a.groups ? group_of(a, seq.b).prefix : 0;
+        place_seq(a, seq, int64_t(uint64_t(of_at(uint32_t(uint64_t(length) >> 32))) << 32 | of_at(uint32_t(length))));
+    }
+    tile_rows<kBf16, kDim, kKind>(a, lds, column % a.kv_heads, column / a.kv_heads, seq, (tile - before) * kTileRows, g);
 }
 
 // ---------------------------------------------------------------- kernels
@@ -1780,7 +1793,12 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a)
             for (uint32_t x = 0; x < kAhead; ++x) {
                 const uint32_t n = i * kLanes + p0 + x;
                 part[x] = f32x4{0, 0, 0, 0};
-                if (n < parts && d < a.dim) part[x] = p.template four<kKind>(a, n, d);
+                bool weighs = n < parts;
+                if constexpr (kKind == kMore) {
+                    const float fx = __shfl(f[i], int((lane & ~(kLanes - 1)) + p0 + x));
+                    weighs = weighs && fx != 0.0f;
+                }
+                if (weighs && d < a.dim) part[x] = p.template four<kKind>(a, n, d);
             }
 #pragma unroll
             for (uint32_t x = 0; x < kAhead; ++x) {
