@@ -69,6 +69,7 @@ struct AttendArgs {
     float2* share_ml;
     uint4* few_joins;  // few_parts' place, and the parts of the prefix besides
     uint32_t tile_groups;  // workgroups for the tiles
+    uint32_t alone_groups;  // workgroups whose waves take a short sequence's KV head each (0: none do)
 };
 
 // What a kernel's code knows of: a call without sinks and shared prefixes, one with them, and of the
@@ -399,6 +400,7 @@ __device__ __forceinline__ uint32_t few_units(const AttendArgs& a, const Seq& s)
     const uint32_t rows = s.n_new * a.group;
     if (rows == 0 || rows > a.few_rows) return 0;
     const uint32_t n = cut_of<kKind>(a, s, few_unit<kKind>(), kFewKeys).parts;
+    if (kKind == kMore && a.alone_groups && n <= 1) return 0;  // a wave's alone
     return n ? n : 1;
 }
 
@@ -698,8 +700,8 @@ __device__ __forceinline__ void few_place(const AttendArgs& a, const Seq& s, boo
 }
 
 // Units [first, first + n) of KV head kvh of a sequence whose keys are `cut`; not
-// `whole`: into part `slot`.
-template <bool kBf16, int kDim, int kKind>
+// `whole`: into part `slot`.  kAlone: by this wave alone, which waits for no other.
+template <bool kBf16, int kDim, int kKind, bool kAlone = false>
 __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, const Seq& s, uint32_t kvh, const Cut& cut,
                                            uint32_t first, uint32_t n, bool whole, uint32_t slot)
 {
@@ -720,7 +722,8 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
     constexpr uint32_t kUnit = few_unit<kKind>();
     const int32_t k_first = (kKind == kPlain ? cut.lo : 0) + int32_t(first * kUnit);
     Keys<kFewKeys> keys;
-    int32_t k0 = k_first + int32_t(wave * kFewKeys);
+    constexpr uint32_t kStep = kAlone ? kFewKeys : kFewStep;
+    int32_t k0 = k_first + (kAlone ? 0 : int32_t(wave * kFewKeys));
     keys.fetch(a, table, key(k0));
     const uint32_t rows = s.n_new * a.group;
     const bool out = whole && (kKind == kPlain || s.from == 0);  // nothing to be joined
@@ -782,16 +785,16 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
     const int32_t hi_seen = kKind == kPlain ? hi : hi_key;
     if (k0 < hi) {
         keys.template resolve<kKind>(a, key(k0), lo, hi_seen, s.from);
-        keys.fetch(a, table, key(k0 + int32_t(kFewStep)));
+        keys.fetch(a, table, key(k0 + int32_t(kStep)));
         load_k(key(k0));
         load_v(key(k0));
     }
-    for (; k0 < hi; k0 += int32_t(kFewStep)) {
+    for (; k0 < hi; k0 += int32_t(kStep)) {
         const uint64_t ok = keys.ok;
-        const int32_t next = k0 + int32_t(kFewStep);
+        const int32_t next = k0 + int32_t(kStep);
         if (next < hi) {
             keys.template resolve<kKind>(a, key(next), lo, hi_seen, s.from);
-            keys.fetch(a, table, key(next + int32_t(kFewStep)));
+            keys.fetch(a, table, key(next + int32_t(kStep)));
         }
         f32x4 st[2];
 #pragma unroll
@@ -858,13 +861,19 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
         __builtin_amdgcn_wave_barrier();
     }
 
+    bool any_odd = false;
     if (s.n_new > 1) {
         const uint64_t any = __ballot((marks & 0x80008000u) != 0);
-        if (lane == 0) odd[wave] = any != 0;
-        __syncthreads();
+        if constexpr (kAlone) {
+            any_odd = any != 0;
+        } else {
+            if (lane == 0) odd[wave] = any != 0;
+            __syncthreads();
+            any_odd = odd[0] | odd[1] | odd[2] | odd[3];
+        }
     }
-    if (s.n_new > 1 && (odd[0] | odd[1] | odd[2] | odd[3])) {
-        for (uint32_t x = wave; x < rows; x += kFewWaves) {
+    if (any_odd) {
+        for (uint32_t x = kAlone ? 0 : wave; x < rows; x += kAlone ? 1 : kFewWaves) {
             const uint32_t xt = x / a.group, xh = kvh * a.group + (x - xt * a.group);
             const int32_t xp = s.base + int32_t(xt);
             float* o_at;
@@ -876,24 +885,29 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
         return;
     }
     // Join the waves.
-    __syncthreads();
+    const auto all_there = [] {
+        if constexpr (kAlone) __builtin_amdgcn_wave_barrier();
+        else __syncthreads();
+    };
+    all_there();
     l = across<true>(l, fadd2);
     if (quad == 0) ml[wave][col] = float2{m, l};
     float* const ow = reinterpret_cast<float*>(lds + wave * kWaveBytes);
 #pragma unroll
     for (int i = 0; i < kOut; ++i) *reinterpret_cast<f32x4*>(ow + col * kOPitch + 16 * i + 4 * quad) = o[i];
-    __syncthreads();
+    all_there();
     const uint32_t quads = a.dim / 4;
-    for (uint32_t e = threadIdx.x; e < rows * quads; e += 64 * kFewWaves) {
+    const int w_first = kAlone ? int(same(wave)) : 0, w_end = kAlone ? w_first + 1 : int(kFewWaves);
+    for (uint32_t e = kAlone ? lane : threadIdx.x; e < rows * quads; e += kAlone ? 64 : 64 * kFewWaves) {
         const uint32_t r = e / quads, d = (e - r * quads) * 4;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < int(kFewWaves); ++w) top = fmaxf(top, ml[w][r].x);
+        for (int w = w_first; w < w_end; ++w) top = fmaxf(top, ml[w][r].x);
         const float safe = top == -INFINITY ? 0.0f : top;
         float sum = 0.0f;
         f32x4 acc{0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < int(kFewWaves); ++w) {
+        for (int w = w_first; w < w_end; ++w) {
             const float2 v = ml[w][r];
             const float f = __builtin_amdgcn_exp2f((v.x - safe) * a.scale_log2);
             sum = __builtin_fmaf(v.y, f, sum);
@@ -916,12 +930,15 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
 // sequence and KV head, in place `group`; without, consecutive units of all of them:
 // where a part begins in an earlier workgroup it is in this one's place
 // 2 group, where it goes on in the next in place 2 group + 1.
-template <bool kBf16, int kDim, int kKind>
+// (kParts: with few_per; else the kernel looks.)
+template <bool kBf16, int kDim, int kKind, bool kParts = false>
 __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* lds, uint32_t group)
 {
+    const uint32_t few_per = a.few_per;
+    if constexpr (kParts) __builtin_assume(few_per != 0);
     if (a.q_starts && group == 0) zero_unowned<kBf16>(a);
     Few w;
-    uint64_t at = 0, to = 1, per = a.few_per;
+    uint64_t at = 0, to = 1, per = few_per;
     if (!per) {
         w.template start<kKind>(a);
         per = w.per;
@@ -930,11 +947,11 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
     }
     for (bool again = false; at < to; again = true) {
         uint32_t b, kvh, first, n = 0, units = 0, place = group;
-        if (a.few_per) {
+        if (few_per) {
             const uint32_t pairs = a.seqs * a.kv_heads, part = group / pairs, pair = group - part * pairs;
             b = pair / a.kv_heads;
             kvh = pair - b * a.kv_heads;
-            first = part * a.few_per;
+            first = part * few_per;
             at = to;
         } else {
             b = uint32_t(__ffsll(static_cast<unsigned long long>(__ballot(uint64_t(w.with) * a.kv_heads > at))) - 1);
@@ -950,17 +967,17 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
             place = 2 * group + (first == 0);
         }
         Seq s;
-        if (kKind == kMore && !a.few_per) {
+        if (kKind == kMore && !few_per) {
             const auto of_b = [&](uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), int(b))); };
             s = Seq{b, of_b(w.mine.q0), of_b(w.mine.n_new), int32_t(of_b(uint32_t(w.mine.len))),
                     int32_t(of_b(uint32_t(w.mine.base))), int32_t(of_b(uint32_t(w.mine.from)))};
         } else {
             s = seq_of<kKind>(a, b);
         }
-        if (a.few_per) {
+        if (few_per) {
             units = few_units<kKind>(a, s);
             if (first >= units) return;
-            n = units - first < a.few_per ? units - first : a.few_per;
+            n = units - first < few_per ? units - first : few_per;
         }
         if (kKind == kPlain && first == 0 && a.few_parts && threadIdx.x == 0)
             a.few_parts[b * a.kv_heads + kvh] = uint2{place, 1 + uint32_t(quotient(units - n + per - 1, per))};
@@ -971,6 +988,23 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
             a.few_joins[b * a.kv_heads + kvh] =
                 uint4{place, 1 + uint32_t(quotient(units - n + per - 1, per)), share_parts(a, b, s.from), 0};
     }
+}
+
+// With few_per and groups: sequences whose own keys are at most one step of a workgroup's, a wave for each KV head of
+// them, where a workgroup would wait for as long.
+template <bool kBf16, int kDim>
+__device__ __forceinline__ void attend_alone(const AttendArgs& a, uint8_t* lds, uint32_t group)
+{
+    const uint32_t pair = same(group * kFewWaves + (threadIdx.x >> 6));
+    if (pair >= a.seqs * a.kv_heads) return;
+    const uint32_t b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+    const Seq s = seq_of<kMore>(a, b);
+    const uint32_t rows = s.n_new * a.group;
+    if (rows == 0 || rows > a.few_rows) return;
+    const Cut cut = cut_of<kMore>(a, s, kFewStep, kFewKeys);
+    if (cut.parts > 1) return;
+    attend_few<kBf16, kDim, kMore, true>(a, lds, s, kvh, cut, 0, 1, true, 0);
+    if ((threadIdx.x & 63u) == 0) a.few_joins[pair] = uint4{0, 1, share_parts(a, b, s.from), 0};
 }
 
 // ---------------------------------------------------------------- tiles of rows
@@ -1627,18 +1661,23 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim <= 64 && kKind == kMore 
 
 // The groups' prefixes first, then each sequence's own keys.  (Three waves a SIMD for heads up to 64, here and in
 // kMore's mixed kernel: 45 sequences of 4 tokens, 12/4 heads, behind seven prefixes 27.2 us, two 31.5.)
-template <bool kBf16, int kDim>
+//
+// Own tiles, of which there may be none, come last.  kParts: with few_per, and short sequences by a wave each; a kernel
+// of its own, as more code makes the others slower to start (20.4 us where this takes 18.2, eight samples).
+template <bool kBf16, int kDim, bool kParts>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim <= 64 ? 3 : 2) void attend_shared_kernel(AttendArgs a)
 {
     constexpr int kBytes = share_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? share_lds_bytes<kDim>() : few_lds_bytes<kDim>();
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
-    if (blockIdx.x < a.share_groups) {
-        attend_tiles<kBf16, kDim, kShare>(a, lds, blockIdx.x);
-    } else if (blockIdx.x - a.share_groups < a.tile_groups) {
-        attend_tiles<kBf16, kDim, kMore>(a, lds, blockIdx.x - a.share_groups);
-    } else {
-        attend_few_units<kBf16, kDim, kMore>(a, lds, blockIdx.x - a.share_groups - a.tile_groups);
+    uint32_t group = blockIdx.x;
+    if (group < a.share_groups) return attend_tiles<kBf16, kDim, kShare>(a, lds, group);
+    group -= a.share_groups;
+    if constexpr (kParts) {
+        if (group < a.alone_groups) return attend_alone<kBf16, kDim>(a, lds, group);
+        group -= a.alone_groups;
     }
+    if (group < a.few_groups) return attend_few_units<kBf16, kDim, kMore, kParts>(a, lds, group);
+    attend_tiles<kBf16, kDim, kMore>(a, lds, group - a.few_groups);
 }
 
 // ---------------------------------------------------------------- parts joined
@@ -1885,8 +1924,9 @@ hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
     const uint32_t tiles = p.tile_groups;
     hipError_t e;
     if (p.share_groups) {
-        e = launch(attend_shared_kernel<kBf16, kDim>, dim3(p.share_groups + tiles + (p.few ? p.few_groups : 0)), block,
-                   stream, a);
+        const dim3 grid(p.share_groups + p.alone_groups + p.few_groups + tiles);
+        e = p.few_per ? launch(attend_shared_kernel<kBf16, kDim, true>, grid, block, stream, a)
+                      : launch(attend_shared_kernel<kBf16, kDim, false>, grid, block, stream, a);
     } else if (p.few && p.tile) {
         e = launch(attend_mixed_kernel<kBf16, kDim, kKind>, dim3(tiles + p.few_groups), block, stream, a);
     } else if (p.few) {
@@ -2010,6 +2050,7 @@ int secure_infer_gpu_paged_attention_more(hipStream_t stream, const si_paged_att
         a.share_ml = reinterpret_cast<float2*>(ws + p.share_ml);
         a.few_joins = p.few_joins ? reinterpret_cast<uint4*>(ws + p.few_joins) : nullptr;
         a.tile_groups = p.tile_groups;
+        a.alone_groups = p.alone_groups;
         e = bf16 ? attend_by_dim<true, kMore>(stream, a, p) : attend_by_dim<false, kMore>(stream, a, p);
     }
     return e == hipSuccess ? 0 : -1;

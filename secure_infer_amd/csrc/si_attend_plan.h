@@ -69,7 +69,7 @@ struct Plan {
     uint32_t few_rows = 0, few_groups = 0, few_least = 0, few_per = 0, tile_per = 0, tile_split = 1, tiles = 0;
     bool few = false, tile = false, fits = true;
     uint64_t few_o = 0, few_ml = 0, few_parts = 0, tile_o = 0, tile_ml = 0, bytes = 0;
-    uint32_t sinks = 0, share_groups = 0, share_split = 1, tile_groups = 0;
+    uint32_t sinks = 0, share_groups = 0, share_split = 1, tile_groups = 0, alone_groups = 0;
     uint64_t share_o = 0, share_ml = 0, few_joins = 0;
 };
 
@@ -98,8 +98,8 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
     if (more && !(window && more->sinks) && !more->groups) more = nullptr;
     p.sinks = more && window ? more->sinks : 0;
     const uint32_t groups = more ? more->groups : 0;
-    // A row's parts of its prefix and of its own keys are joined together.
-    const uint64_t most_parts = groups ? kMaxSplit / 2 : kMaxSplit;
+    // A row's parts of its prefix and of its own keys are joined together; the prefix is the longer, mostly.
+    const uint64_t most_share = kMaxSplit / 4 * 3, most_parts = groups ? kMaxSplit - most_share : kMaxSplit;
     // Beside sinks a call is cut for the keys that its windows leave: a sequence's n new tokens see at most
     // window + n - 1 keys, in whole steps, and the sinks.  (Without sinks by the table alone, as ever.)
     const auto kept = [&](uint64_t n) {
@@ -142,8 +142,11 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
         // Cut only where the tiles alone leave CUs idle; sequences of the
         // few-row kernel have none.
         const uint64_t groups = (rows / tile_rows + (p.few ? 1 : d.seqs)) * d.kv_heads;
-        p.tile_per = part_keys(groups, keys, groups < kTileFew ? kTileSplitMin : keys, kTileKeys, kTileTarget,
-                               &p.tile_split, most_parts);
+        // (beside sinks and prefixes shorter parts where they all run at a time)
+        const uint64_t shortest = more && groups * ((keys + kTileKeys * 4 - 1) / (kTileKeys * 4)) <= 512 ? kTileKeys * 4
+                                                                                                        : kTileSplitMin;
+        p.tile_per = part_keys(groups, keys, groups < kTileFew ? shortest : keys, kTileKeys, kTileTarget, &p.tile_split,
+                               most_parts);
         if (p.tile_split > 1) {
             // whole columns for every XCD (see the kernel's order)
             const uint32_t even = 8 / uint32_t(std::gcd(8u, d.kv_heads));
@@ -160,16 +163,20 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
     if (more && p.tile) tile_groups = (tile_groups + 7) / 8 * 8;
     if (groups) {
         const uint64_t columns = (rows / kTileRows + 1) * d.kv_heads, split = (kShareTarget + columns - 1) / columns;
-        p.share_split = uint32_t(split < most_parts ? split : most_parts);
+        p.share_split = uint32_t(split < most_share ? split : most_share);
         share_groups = (rows / kTileRows + least(groups, d.seqs / 2)) * d.kv_heads * p.share_split;
         share_groups = (share_groups + 8) / 8 * 8;
     }
+    // With few_per short sequences go by a wave each (256 of 1 to 256 own keys x 8 KV heads behind 32,768: 336 us
+    // without, 332).
+    const uint64_t alone = groups && p.few_per ? (pairs + kFewWaves - 1) / kFewWaves : 0;
     // (threads of a launch dimension fit 32 bits)
     const uint64_t most = (1ull << 32) / 256 - 1;
     p.few_groups = uint32_t(few_groups);
-    p.fits = share_groups + few_groups + tile_groups <= most && uint64_t(d.tokens) * d.q_heads / 4 < most;
+    p.fits = share_groups + few_groups + tile_groups + alone <= most && uint64_t(d.tokens) * d.q_heads / 4 < most;
     p.tile_groups = uint32_t(tile_groups);
     p.share_groups = uint32_t(share_groups);
+    p.alone_groups = uint32_t(alone);
     const auto take = [&](uint64_t n) {
         const uint64_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;

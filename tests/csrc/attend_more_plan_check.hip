@@ -110,7 +110,7 @@ void check(const si_paged_attention_desc& d, const si_paged_attention_more& m, s
         const uint64_t n = uint64_t(p.share_split) * d.tokens * d.q_heads;
         region(p.share_o, n * d.head_dim * 4);
         region(p.share_ml, n * 8);
-        expect(p.share_split >= 1 && p.share_split <= kMaxSplit / 2, "prefix parts' number", d, m);
+        expect(p.share_split >= 1 && p.share_split <= kMaxSplit / 4 * 3, "prefix parts' number", d, m);
         expect(p.share_groups > 0 && p.share_groups % 8 == 0, "prefix tiles", d, m);
         for (uint64_t len : {uint64_t(1), keys, 1 + g() % keys}) {
             const uint64_t per = share_part(uint32_t(len), p.share_split, g() % (1 + uint64_t(d.tokens) * d.q_heads));
