@@ -53,6 +53,9 @@ constexpr uint64_t kShareTarget = 512;
 constexpr uint32_t kShareMin = 256;
 constexpr uint32_t kShareMost = 4 * kTileRows;
 
+// Keys of a prefix for each row (of a KV head, on average) of the sequences that share it, from which on they do.
+constexpr uint64_t kShareKeys = 16;
+
 // Keys of a part of a prefix that is cut into at most `split` parts, of a group of `rows` rows a KV head.
 constexpr uint32_t share_part(uint32_t keys, uint32_t split, uint64_t rows)
 {

@@ -212,9 +212,9 @@ def test_the_largest_windows_and_sinks(new):
 
 # ------------------------------------------------------------------ shared prefixes
 
-def share(seed, groups, hq, hkv, dim, ps, dtype, before=(), after=(), stale=math.nan, junk=-1):
+def share(seed, groups, hq, hkv, dim, ps, dtype, before=(), after=(), stale=math.nan):
     """A batch whose groups are (prefix, [(own keys, new tokens), ...]): the rows' pages wholly below the prefix
-    are the first row's (the other rows hold `junk` there); sequences `before` and `after`
+    are the first row's, the one at its end a copy, as a fork leaves them; sequences `before` and `after`
     them, (keys, new), are in no group.  A negative number of own keys ends the sequence inside the prefix."""
     lens, news, starts, prefix = [n for n, _ in before], [m for _, m in before], [len(before)], []
     for p, members in groups:
@@ -232,7 +232,10 @@ def share(seed, groups, hq, hkv, dim, ps, dtype, before=(), after=(), stale=math
     x["kv"] = torch.tensor(lens)
     for g, (p, members) in enumerate(groups):
         for b in range(starts[g] + 1, starts[g + 1]):
-            x["tables"][b, :p // ps] = junk
+            x["tables"][b, :p // ps] = x["tables"][starts[g], :p // ps]
+            if p % ps and x["tables"][b, p // ps] >= 0:
+                for c in ("ck", "cv"):
+                    x[c][x["tables"][b, p // ps], :p % ps] = x[c][x["tables"][starts[g], p // ps], :p % ps]
     x["groups"], x["prefix"] = torch.tensor(starts), torch.tensor(prefix, dtype=torch.int64)
     return x
 
@@ -251,7 +254,7 @@ def test_next_tokens_of_groups(hq, hkv, dim, ps, dtype):
 def test_chunks_of_groups(hq, hkv, dim, ps, dtype, causal):
     groups = [(257, [(1, 1), (140, 130), (3, 3)]), (300, [(70, 33), (17, 16), (0, 0), (5, 5), (2, 40), (-60, 30)]),
               (64, [(64, 64)]), (31, [(n, min(n, 4)) for n in range(1, 60, 5)])]
-    x = share(hq + dim, groups, hq, hkv, dim, ps, dtype, before=[(70, 20)], after=[(140, 3), (3, 3)], junk=1 << 50)
+    x = share(hq + dim, groups, hq, hkv, dim, ps, dtype, before=[(70, 20)], after=[(140, 3), (3, 3)])
     check(x, causal=causal)
 
 
@@ -264,6 +267,28 @@ def test_groups_with_windows_and_sinks(window, sinks, causal, new):
     check(x, window=window, sinks=sinks, causal=causal)
     if new == 1:
         check(x, use_starts=False, window=window, sinks=sinks, causal=causal)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,ps,dtype", GEOMETRIES[:6])
+@pytest.mark.parametrize("kw", [dict(), dict(causal=False), dict(window=300, sinks=5), dict(window=3000, sinks=70)])
+def test_chunks_behind_long_prefixes(hq, hkv, dim, ps, dtype, kw):
+    """Groups whose tokens attend to their prefix together: a few tokens a sequence, and chunks beside single ones."""
+    rows = 40 * hkv // hq  # of a chunk: about 40 rows a KV head
+    groups = [(3333, [(1, 1), (rows + 70, rows), (3, 3), (-2000, 2), (0, 1)]), (2050, [(n, min(n, 2)) for n in range(1, 60, 5)]),
+              (700, [(n, 1) for n in (1, 40, 200)])]
+    x = share(hq + dim, groups, hq, hkv, dim, ps, dtype, before=[(70, 20)], after=[(140, 3), (3, 3)])
+    tokens = x["q"].shape[0]
+    check(x, rows=set(range(18, tokens, 5)) | {20, 21, tokens - 1}, **kw)
+
+
+def test_groups_together_and_alone():
+    """Sequences of many rows for the prefix's keys go by themselves, whether they share it or not: the same bits as
+    without groups where all of a batch's do."""
+    x = share(31, [(64, [(64, 64), (40, 33)]), (100, [(90, 70), (50, 50), (77, 77)])], 8, 2, 64, 32, torch.bfloat16)
+    plain = {k: v for k, v in x.items() if k not in ("groups", "prefix")}
+    got, want = attend(x), definition(plain)
+    agree(*got, want)
+    agree(*attend(plain), want)
 
 
 def test_a_long_prefix_in_many_parts():
@@ -295,10 +320,14 @@ def test_many_groups():
 def test_what_lies_behind_a_sequence_has_no_influence(bad):
     """Sequences that end inside the prefix, or see it through a window, beside infinite and NaN K and V there."""
     groups = [(300, [(-250, 1), (-100, 3), (40, 2), (1, 1)])]
+    def spoil(x, caches):
+        for p in (60, 299):
+            for b in range(4):  # every row's copy
+                if x["tables"][b, p // 64] >= 0:
+                    for c in caches:
+                        x[c][x["tables"][b, p // 64], p % 64] = bad
     x = share(8, groups, 4, 2, 64, 64, torch.bfloat16)
-    for p in (60, 299):
-        x["ck"][x["tables"][0, p // 64], p % 64] = bad
-        x["cv"][x["tables"][0, p // 64], p % 64] = bad
+    spoil(x, ("ck", "cv"))
     out, lse = attend(x)
     clean = {k: v.clone() for k, v in x.items()}
     for c in ("ck", "cv"):
@@ -309,8 +338,7 @@ def test_what_lies_behind_a_sequence_has_no_influence(bad):
         check(x)
         check(x, window=30, sinks=3)
     x = share(9, groups, 4, 2, 64, 64, torch.bfloat16)  # an infinite or NaN V alone
-    for p in (60, 299):
-        x["cv"][x["tables"][0, p // 64], p % 64] = bad
+    spoil(x, ("cv",))
     check(x)
     check(x, window=45, sinks=3)
 
@@ -320,7 +348,7 @@ def test_groups_and_prefixes_out_of_bounds_are_clamped():
     x["groups"] = torch.tensor([-(1 << 62), 2, 1 << 62])
     check(x)
     x["prefix"] = torch.tensor([-5, 1 << 62])
-    x["tables"][1] = x["tables"][0]
+    x["tables"][3:] = x["tables"][2]
     check(x)
 
 
