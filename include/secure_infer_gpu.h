@@ -659,12 +659,13 @@ uint64_t secure_infer_gpu_paged_attention_workspace(const si_paged_attention_des
  * sinks: with a window, a token also sees the keys j < sinks that it would see
  *   without one.  (Without a window it changes nothing.)
  * Shared prefixes: sequences group_starts[g] .. group_starts[g + 1] (clamped to
- *   [0, seqs]) are group g.  Their rows hold the same K and V for the keys j <
- *   prefix_lens[g] (clamped to the table; on one page, as a fork leaves them, or
- *   on copies), which the call may read from the pages of any of them: once for
- *   all the group's tokens from its first row's, where that is the faster way.
- *   What a token sees, and the result but for rounding, does not change.  A
- *   group of one sequence, and sequences in no group, are as without groups. */
+ *   [0, seqs]) are group g.  As far as their lengths go their rows hold the same
+ *   K and V for the keys j < prefix_lens[g] (clamped to the table; on one page,
+ *   as a fork leaves them, or on copies), which the call may read from the pages
+ *   of any row that is long enough: once for all the group's tokens, where that
+ *   is the faster way.  What a token sees, and the result but for rounding, does
+ *   not change.  A group of one sequence, and sequences in no group, are as
+ *   without groups. */
 typedef struct si_paged_attention_more {
     uint32_t sinks;               /* at most 2^30                              */
     uint32_t groups;              /* 0: no shared prefixes; < 2^26             */

@@ -14,7 +14,9 @@
 // A sequence of at most 16 rows (a decoding step) is bound by the bytes of its K
 // and V and runs in the few-row kernel; longer ones are bound by the matrix
 // and vector instructions and run in tiles of 128 rows.  Keys are cut into parts where
-// there are too few rows for the chip, and the parts joined by a second launch (the join by the
+// there are too few rows for the chip.  Beside a window and sinks the keys that are left are walked over
+// without the gap between them (kMore); a prefix that a group of sequences shares is attended to in tiles of all
+// the group's rows (kShare), beside each sequence's own keys.  Parts are joined by a second launch (the join by the
 // workgroup that ends last was tried: its fences, which write back and drop
 // whole L2s, cost one token 38 us, stores past the L2 16.9, the launch 8 + 4).
 #include <hip/hip_runtime.h>
@@ -1048,6 +1050,34 @@ __device__ __forceinline__ Seq owner_of(const AttendArgs& a, const Group& g, uin
     return seq_of(a, b);
 }
 
+// The first sequence of the group that is as long as the prefix, or else the longest: it holds every key of the
+// prefix that any of them sees (the others may have ended).  The same in every wave.
+__device__ __forceinline__ uint32_t longest_of(const AttendArgs& a, const Group& g)
+{
+    uint32_t row = g.first;
+    int32_t best = -1;
+    for (uint32_t s0 = g.first; s0 < g.end && best < g.prefix; s0 += 64) {
+        const uint32_t s = s0 + (threadIdx.x & 63u);
+        int32_t held = -1;
+        if (s < g.end) {
+            const int64_t n = a.kv_lens[s];
+            held = int32_t(n < 0 ? 0 : n > g.prefix ? g.prefix : n);
+        }
+        int32_t most = held;
+#pragma unroll
+        for (int x = 32; x; x >>= 1) {
+            const int32_t y = __shfl_xor(most, x);
+            most = y > most ? y : most;
+        }
+        most = int32_t(same(uint32_t(most)));
+        if (most > best) {
+            best = most;
+            row = s0 + uint32_t(__ffsll(static_cast<unsigned long long>(__ballot(held == most)))) - 1;
+        }
+    }
+    return same(row);
+}
+
 // The least x of the wave, and of the workgroup's waves (which all call it before anything lies in LDS).
 __device__ __forceinline__ int32_t least_of(int32_t x)
 {
@@ -1614,7 +1644,7 @@ __device__ __forceinline__ void attend_tiles(const AttendArgs& a, uint8_t* lds, 
     seq.n_new = of_at(end) > seq.q0 ? of_at(end) - seq.q0 : 0;
     if constexpr (kKind == kShare) {
         g = Group{of_at(mine.first), of_at(mine.end), int32_t(of_at(uint32_t(mine.prefix)))};
-        seq.b = g.first;
+        seq.b = longest_of(a, g);
         seq.len = g.prefix;
         seq.base = seq.from = 0;
     } else {

@@ -22,8 +22,8 @@ pytestmark = pytest.mark.gpu
 
 
 def definition(x, rows=None, scale=None, causal=True, window=0, sinks=0):
-    """{row: (out, lse, bound of out, bound of lse)} of the rows of q.  x["groups"] and x["prefix"], where they
-    are, say which sequences find their first keys on another's pages."""
+    """{row: (out, lse, bound of out, bound of lse)} of the rows of q, each sequence over its own row's pages,
+    whichever it shares."""
     q, ck, cv, tables = x["q"], x["ck"], x["cv"], x["tables"]
     hq, dim = q.shape[1:]
     slots, ps, hkv, _ = ck.shape
@@ -31,11 +31,6 @@ def definition(x, rows=None, scale=None, causal=True, window=0, sinks=0):
     u = ROUND[q.dtype]
     seqs, most = tables.shape[0], tables.shape[1] * ps
     starts = x["starts"].clamp(0, q.shape[0]).tolist()
-    first, below = list(range(seqs)), [0] * seqs
-    for g in range(len(x.get("prefix", ()))):
-        lo, hi = (min(max(int(x["groups"][g + i]), 0), seqs) for i in range(2))
-        for b in range(lo, hi):
-            first[b], below[b] = lo, min(max(int(x["prefix"][g]), 0), most)
     found = {}
     for b in range(seqs):
         length = int(x["kv"][b])
@@ -48,7 +43,7 @@ def definition(x, rows=None, scale=None, causal=True, window=0, sinks=0):
                 pos = pos[pos <= p]
             if window:
                 pos = pos[(pos > p - window) | (pos < sinks)]
-            slot = torch.where(pos < below[b], tables[first[b]][pos // ps], tables[b][pos // ps])
+            slot = tables[b][pos // ps]
             keep = (slot >= 0) & (slot < slots)
             pos, slot = pos[keep], slot[keep]
             n = pos.numel()
@@ -529,3 +524,22 @@ def test_long_chunks_behind_a_prefix(new):
     check(x, rows=rows)
     check(x, rows=rows, causal=False)
     check(x, rows=rows, window=1000, sinks=10)
+
+
+@pytest.mark.parametrize("members", [3, 90])
+@pytest.mark.parametrize("use_starts", [True, False])
+def test_rows_of_a_group_that_have_ended(members, use_starts):
+    """Ended rows hold no page, shorter ones the first pages: the prefix is read from a row that holds it."""
+    x = share(22, [(777, [(n % 50, 1) for n in range(1, members + 1)])], 4, 2, 64, 32, torch.bfloat16, after=[(100, 1)])
+    whole = {k: v.clone() for k, v in x.items()}
+
+    def cut(b, n):
+        x["kv"][b] = n
+        x["tables"][b, -(-n // 32):] = -1
+    for kept in ([members - 1], [1], []):
+        x.update({k: v.clone() for k, v in whole.items()})
+        for b in range(members):
+            if b not in kept:
+                cut(b, 0 if b % 2 == 0 else 37 * b % 500)
+        check(x, use_starts=use_starts)
+        check(x, use_starts=use_starts, window=300, sinks=9)
