@@ -419,11 +419,15 @@ struct Few {
     uint32_t units, with;  // of a KV head; their sum up to and with the lane's (at most 64 * 2^25)
     uint64_t total, per;
     Seq mine;
+    // kMany: 64 sequences at a time, from s0 on; the units of those before.  (In the other kernels this
+    // would spill 8 registers: 64 next tokens under a window 30.1 us, 33.0 with it.)
+    uint32_t s0;
+    uint64_t before;
 
-    template <int kKind>
-    __device__ __forceinline__ void start(const AttendArgs& a)
+    template <int kKind, bool kMany>
+    __device__ __forceinline__ void load(const AttendArgs& a)
     {
-        const uint32_t b = threadIdx.x & 63u;
+        const uint32_t b = (threadIdx.x & 63u) + (kMany ? s0 : 0);
         units = 0;
         mine = Seq{b, 0, 0, 0, 0, 0};
         if (b < a.seqs) {
@@ -431,12 +435,38 @@ struct Few {
             units = few_units<kKind>(a, mine);
         }
         with = sums_up_to(units);
+    }
+    // On to the sequences that unit `at` belongs to.
+    __device__ __forceinline__ void reach(const AttendArgs& a, uint64_t at)
+    {
+        while (at - before >= upto(a, 63) && s0 + 64 < a.seqs) {
+            before += upto(a, 63);
+            s0 += 64;
+            load<kMore, true>(a);
+        }
+    }
+    template <int kKind, bool kMany>
+    __device__ __forceinline__ void start(const AttendArgs& a)
+    {
+        s0 = 0;
+        before = 0;
+        load<kKind, kMany>(a);
         total = upto(a, 63);
+        uint32_t longest = units;
+        if (kMany && a.seqs > 64) {
+            for (s0 = 64; s0 < a.seqs; s0 += 64) {
+                load<kKind, kMany>(a);
+                total += upto(a, 63);
+                longest = units > longest ? units : longest;
+            }
+            s0 = 0;
+            load<kKind, kMany>(a);
+        }
         const uint64_t even = quotient(total + a.few_groups - 1, a.few_groups);
         uint32_t least = a.few_least;
         if constexpr (kKind == kMore) {
             // as many units a share as keep the longest sequence's parts to few_least
-            uint32_t most = units;
+            uint32_t most = longest;
 #pragma unroll
             for (int x = 32; x; x >>= 1) {
                 const uint32_t y = uint32_t(__shfl_xor(int(most), x));
@@ -938,17 +968,15 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, uint8_t* lds, co
 // sequence and KV head, in place `group`; without, consecutive units of all of them:
 // where a part begins in an earlier workgroup it is in this one's place
 // 2 group, where it goes on in the next in place 2 group + 1.
-// (kParts: with few_per; else the kernel looks.)
-template <bool kBf16, int kDim, int kKind, bool kParts = false>
+template <bool kBf16, int kDim, int kKind, bool kMany = false>
 __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* lds, uint32_t group)
 {
     const uint32_t few_per = a.few_per;
-    if constexpr (kParts) __builtin_assume(few_per != 0);
     if (a.q_starts && group == 0) zero_unowned<kBf16>(a);
     Few w;
     uint64_t at = 0, to = 1, per = few_per;
     if (!per) {
-        w.template start<kKind>(a);
+        w.template start<kKind, kMany>(a);
         per = w.per;
         at = group * per;
         to = at + per < w.total ? at + per : w.total;
@@ -962,9 +990,14 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
             first = part * few_per;
             at = to;
         } else {
-            b = uint32_t(__ffsll(static_cast<unsigned long long>(__ballot(uint64_t(w.with) * a.kv_heads > at))) - 1);
+            uint64_t here = at;
+            if constexpr (kMany) {
+                w.reach(a, at);
+                here -= w.before;
+            }
+            b = uint32_t(__ffsll(static_cast<unsigned long long>(__ballot(uint64_t(w.with) * a.kv_heads > here))) - 1);
             units = uint32_t(__builtin_amdgcn_readlane(int(w.units), int(b)));
-            const uint64_t in = at + uint64_t(units) * a.kv_heads - w.upto(a, int(b));
+            const uint64_t in = here + uint64_t(units) * a.kv_heads - w.upto(a, int(b));
             kvh = uint32_t(quotient(in, units));
             first = uint32_t(in - uint64_t(kvh) * units);
             n = units - first;
@@ -977,8 +1010,9 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
         Seq s;
         if (kKind == kMore && !few_per) {
             const auto of_b = [&](uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), int(b))); };
-            s = Seq{b, of_b(w.mine.q0), of_b(w.mine.n_new), int32_t(of_b(uint32_t(w.mine.len))),
+            s = Seq{kMany ? w.s0 + b : b, of_b(w.mine.q0), of_b(w.mine.n_new), int32_t(of_b(uint32_t(w.mine.len))),
                     int32_t(of_b(uint32_t(w.mine.base))), int32_t(of_b(uint32_t(w.mine.from)))};
+            b = s.b;
         } else {
             s = seq_of<kKind>(a, b);
         }
@@ -998,7 +1032,7 @@ __device__ __forceinline__ void attend_few_units(const AttendArgs& a, uint8_t* l
     }
 }
 
-// With few_per and groups: sequences whose own keys are at most one step of a workgroup's, a wave for each KV head of
+// Many sequences of groups: those whose own keys are at most one step of a workgroup's, a wave for each KV head of
 // them, where a workgroup would wait for as long.
 template <bool kBf16, int kDim>
 __device__ __forceinline__ void attend_alone(const AttendArgs& a, uint8_t* lds, uint32_t group)
@@ -1698,9 +1732,9 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim <= 64 && kKind == kMore 
 // The groups' prefixes first, then each sequence's own keys.  (Three waves a SIMD for heads up to 64, here and in
 // kMore's mixed kernel: 45 sequences of 4 tokens, 12/4 heads, behind seven prefixes 27.2 us, two 31.5.)
 //
-// Own tiles, of which there may be none, come last.  kParts: with few_per, and short sequences by a wave each; a kernel
+// Own tiles, of which there may be none, come last.  kMany: short sequences by a wave each; a kernel
 // of its own, as more code makes the others slower to start (20.4 us where this takes 18.2, eight samples).
-template <bool kBf16, int kDim, bool kParts>
+template <bool kBf16, int kDim, bool kMany>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim <= 64 ? 3 : 2) void attend_shared_kernel(AttendArgs a)
 {
     constexpr int kBytes = share_lds_bytes<kDim>() > few_lds_bytes<kDim>() ? share_lds_bytes<kDim>() : few_lds_bytes<kDim>();
@@ -1708,11 +1742,11 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim <= 64 ? 3 : 2) void atte
     uint32_t group = blockIdx.x;
     if (group < a.share_groups) return attend_tiles<kBf16, kDim, kShare>(a, lds, group);
     group -= a.share_groups;
-    if constexpr (kParts) {
+    if constexpr (kMany) {
         if (group < a.alone_groups) return attend_alone<kBf16, kDim>(a, lds, group);
         group -= a.alone_groups;
     }
-    if (group < a.few_groups) return attend_few_units<kBf16, kDim, kMore, kParts>(a, lds, group);
+    if (group < a.few_groups) return attend_few_units<kBf16, kDim, kMore, kMany>(a, lds, group);
     attend_tiles<kBf16, kDim, kMore>(a, lds, group - a.few_groups);
 }
 
@@ -1961,7 +1995,7 @@ hipError_t attend_launch(hipStream_t stream, const AttendArgs& a, const Plan& p)
     hipError_t e;
     if (p.share_groups) {
         const dim3 grid(p.share_groups + p.alone_groups + p.few_groups + tiles);
-        e = p.few_per ? launch(attend_shared_kernel<kBf16, kDim, true>, grid, block, stream, a)
+        e = p.alone_groups ? launch(attend_shared_kernel<kBf16, kDim, true>, grid, block, stream, a)
                       : launch(attend_shared_kernel<kBf16, kDim, false>, grid, block, stream, a);
     } else if (p.few && p.tile) {
         e = launch(attend_mixed_kernel<kBf16, kDim, kKind>, dim3(tiles + p.few_groups), block, stream, a);

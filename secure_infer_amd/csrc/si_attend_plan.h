@@ -53,6 +53,11 @@ constexpr uint64_t kShareTarget = 512;
 constexpr uint32_t kShareMin = 256;
 constexpr uint32_t kShareMost = 4 * kTileRows;
 
+// Sequences of groups whose own keys are shared out evenly, 64 looked at at a time: short ones are not among them
+// beyond 64, so that what is left may be few, and long (137 next tokens x 32/8 heads, one of them in a group of its
+// own with 7,605 keys: 208 us in one part, 90 shared out).
+constexpr uint32_t kShareSeqs = 256;
+
 // Keys of a prefix for each row (of a KV head, on average) of the sequences that share it, from which on they do.
 constexpr uint64_t kShareKeys = 16;
 
@@ -124,7 +129,7 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
         // (768 or 1,536 for heads of 128: 64 sequences of 8,192 keys 229 and 209 us, 512 197)
         const uint64_t at_once = d.head_dim <= 64 && (more || !p.tile) ? 768 : d.head_dim <= 128 ? 512 : 256;
         p.few_least = uint32_t(more ? most_parts : fewest > whole ? fewest : whole);
-        if (d.seqs <= 64 && pairs <= at_once) {
+        if (d.seqs <= 64 ? pairs <= at_once || groups : groups && d.seqs <= kShareSeqs) {
             // (kMore: the device finds the least units of a share from the lengths)
             const uint64_t least = more ? 1 : p.few_least, most = (pairs * units + least - 1) / least;
             few_groups = most < at_once ? most : at_once;
@@ -173,9 +178,9 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
         share_groups = (rows / kTileRows + least(groups, d.seqs / 2)) * d.kv_heads * p.share_split;
         share_groups = (share_groups + 8) / 8 * 8;
     }
-    // With few_per short sequences go by a wave each (256 of 1 to 256 own keys x 8 KV heads behind 32,768: 336 us
+    // Of many sequences the short ones go by a wave each (256 of 1 to 256 own keys x 8 KV heads behind 32,768: 336 us
     // without, 332).
-    const uint64_t alone = groups && p.few_per ? (pairs + kFewWaves - 1) / kFewWaves : 0;
+    const uint64_t alone = groups && p.few && (d.seqs > 64 || p.few_per) ? (pairs + kFewWaves - 1) / kFewWaves : 0;
     // (threads of a launch dimension fit 32 bits)
     const uint64_t most = (1ull << 32) / 256 - 1;
     p.few_groups = uint32_t(few_groups);

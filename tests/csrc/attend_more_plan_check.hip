@@ -81,7 +81,7 @@ void check(const si_paged_attention_desc& d, const si_paged_attention_more& m, s
                 parts = (units + p.few_per - 1) / p.few_per;
                 expect(parts * pairs <= p.few_groups || parts <= 1, "few-row parts", d, m);
             } else {
-                expect(d.seqs <= 64, "even shares", d, m);
+                expect(d.seqs <= (m.groups ? kShareSeqs : 64), "even shares", d, m);
                 // from anywhere in a share on; shares are of `least` units or more
                 const bool more = p.sinks || m.groups;
                 const uint64_t least = more ? (units + p.few_least - 2) / (p.few_least - 1) : p.few_least;
