@@ -663,7 +663,9 @@ uint64_t secure_infer_gpu_paged_attention_workspace(const si_paged_attention_des
  *   K and V for the keys j < prefix_lens[g] (clamped to the table; on one page,
  *   as a fork leaves them, or on copies), which the call may read from the pages
  *   of any row that is long enough: once for all the group's tokens, where that
- *   is the faster way.  What a token sees, and the result but for rounding, does
+ *   is the faster way.  Beside a window each row may have given up pages (no
+ *   slot in its table) that none of its own new tokens, nor any later one, sees.
+ *   What a token sees, and the result but for rounding, does
  *   not change.  A group of one sequence, and sequences in no group, are as
  *   without groups. */
 typedef struct si_paged_attention_more {

@@ -299,6 +299,8 @@ __device__ __forceinline__ void place_seq(const AttendArgs& a, Seq& s, int64_t n
 {
     const int64_t most = int64_t(a.pages) << a.page_shift;
     s.len = int32_t(n < 0 ? 0 : n > most ? most : n);
+    // (see source_of)
+    if (a.window && s.len < s.from) s.from = 0;
     s.base = (n > most && n <= int64_t(kMostLength) ? int32_t(n) : s.len) - int32_t(s.n_new);
 }
 
@@ -1084,20 +1086,28 @@ __device__ __forceinline__ Seq owner_of(const AttendArgs& a, const Group& g, uin
     return seq_of(a, b);
 }
 
-// The first sequence of the group that is as long as the prefix, or else the longest: it holds every key of the
-// prefix that any of them sees (the others may have ended).  The same in every wave.
-__device__ __forceinline__ uint32_t longest_of(const AttendArgs& a, const Group& g)
+// The sequence of the group whose row the prefix is read from: the first that is as long as the prefix, or else the
+// longest, which holds every key of the prefix that any of them sees (the others may have ended).  Beside a window
+// a row may have given up the pages that none of its tokens sees any more: of those as long as the prefix the one whose
+// new tokens stand first, whose window holds what the others' do of the prefix.  The ones that have ended inside
+// it may see keys that no such row still has, and attend to them by themselves.  The same in every wave.
+__device__ __forceinline__ uint32_t source_of(const AttendArgs& a, const Group& g)
 {
     uint32_t row = g.first;
     int32_t best = -1;
-    for (uint32_t s0 = g.first; s0 < g.end && best < g.prefix; s0 += 64) {
+    for (uint32_t s0 = g.first; s0 < g.end && (a.window || best < g.prefix); s0 += 64) {
         const uint32_t s = s0 + (threadIdx.x & 63u);
-        int32_t held = -1;
+        int32_t good = -1;
         if (s < g.end) {
-            const int64_t n = a.kv_lens[s];
-            held = int32_t(n < 0 ? 0 : n > g.prefix ? g.prefix : n);
+            if (a.window) {
+                const Seq x = seq_of(a, s);
+                good = x.len < g.prefix ? -1 : int32_t(kMostLength) - x.base;
+            } else {
+                const int64_t n = a.kv_lens[s];
+                good = int32_t(n < 0 ? 0 : n > g.prefix ? g.prefix : n);
+            }
         }
-        int32_t most = held;
+        int32_t most = good;
 #pragma unroll
         for (int x = 32; x; x >>= 1) {
             const int32_t y = __shfl_xor(most, x);
@@ -1106,7 +1116,7 @@ __device__ __forceinline__ uint32_t longest_of(const AttendArgs& a, const Group&
         most = int32_t(same(uint32_t(most)));
         if (most > best) {
             best = most;
-            row = s0 + uint32_t(__ffsll(static_cast<unsigned long long>(__ballot(held == most)))) - 1;
+            row = s0 + uint32_t(__ffsll(static_cast<unsigned long long>(__ballot(good == most)))) - 1;
         }
     }
     return same(row);
@@ -1212,6 +1222,8 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
     const auto behind_of = [&](int32_t p) {
         return a.window && p >= int32_t(a.window) ? p - int32_t(a.window) + 1 : 0;
     };
+    // (kShare: whether the sequence attends to the prefix here, see source_of)
+    const auto shares = [&](const Seq& x) { return !a.window || x.len >= g.prefix; };
     int2* const limits = reinterpret_cast<int2*>(lds + tile_lds_bytes<kDim>());
     int32_t least_last = 0, most_behind = 0, least_behind = 0;  // of the wave's rows, the last of the tile's
     const auto find_limits = [&] {
@@ -1219,13 +1231,13 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
         if (r < rows) {
             const Seq mine = owner_of(a, g, s.q0 + tok);
             const int32_t p = mine.base + int32_t(s.q0 + tok - mine.q0);
-            x = int2{last_of(p, mine.len), behind_of(p)};
+            x = int2{shares(mine) ? last_of(p, mine.len) : -1, behind_of(p)};
         }
         if (half == 0) limits[wave * 32 + col] = x;
         least_last = least_of(x.x);
         if (a.window) {
             most_behind = -least_of(-x.y);
-            least_behind = tile_least(lds, wave, least_of(r < rows ? x.y : kNoLast));
+            least_behind = tile_least(lds, wave, least_of(r < rows && x.x >= 0 ? x.y : kNoLast));
         }
     };
     // (kShare: the first keys' place does not wait for the rows' sequences, but where a window moves it)
@@ -1522,7 +1534,7 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
             if constexpr (kKind == kShare) {
                 const Seq mine = owner_of(a, g, s.q0 + xt);
                 xp = mine.base + int32_t(s.q0 + xt - mine.q0);
-                x_last = last_of(xp, mine.len);
+                x_last = shares(mine) ? last_of(xp, mine.len) : -1;
             }
             plain_row<kBf16, kKind>(a, table, s.q0 + xt, xh, kvh, xp, k_first, k_end, !out, part_o + row * a.dim,
                                     part_ml + row, cut, s.from, x_last);
@@ -1678,7 +1690,7 @@ __device__ __forceinline__ void attend_tiles(const AttendArgs& a, uint8_t* lds, 
     seq.n_new = of_at(end) > seq.q0 ? of_at(end) - seq.q0 : 0;
     if constexpr (kKind == kShare) {
         g = Group{of_at(mine.first), of_at(mine.end), int32_t(of_at(uint32_t(mine.prefix)))};
-        seq.b = longest_of(a, g);
+        seq.b = source_of(a, g);
         seq.len = g.prefix;
         seq.base = seq.from = 0;
     } else {
