@@ -268,12 +268,11 @@ def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor
             _, ot, oh = _rows(q_out, "q_out", q_heads, dim, dtype, device)
             _apart(ot, oh, tokens, q_heads, dim, "q_out")
             if d is not None and (q_out.data_ptr() != q.data_ptr() or (ot, oh) != (qt, qh)):
-                # the memory from an input's first element to its last
-                lo, hi = _extent(q_out.data_ptr(), ot, oh, tokens, q_heads, dim)
-                for name, at in (("q", _extent(q.data_ptr(), qt, qh, tokens, q_heads, dim)),
-                                 ("k", _extent(d.k, d.k_token_stride, d.k_head_stride, tokens, heads, dim)),
-                                 ("v", _extent(d.v, d.v_token_stride, d.v_head_stride, tokens, heads, dim))):
-                    if lo < at[1] and at[0] < hi:
+                to = q_out.data_ptr(), ot, oh, q_heads
+                for name, rows in (("q", (q.data_ptr(), qt, qh, q_heads)),
+                                   ("k", (d.k, d.k_token_stride, d.k_head_stride, heads)),
+                                   ("v", (d.v, d.v_token_stride, d.v_head_stride, heads))):
+                    if _meet(to, rows, tokens, dim):
                         raise ValueError(f"q_out must be q itself, or not overlap {name}")
         r.q, r.q_out, r.q_heads = q.data_ptr(), q_out.data_ptr(), q_heads
         r.q_token_stride, r.q_head_stride, r.q_out_token_stride, r.q_out_head_stride = qt, qh, ot, oh
@@ -294,9 +293,28 @@ def _apart(token: int, head: int, tokens: int, heads: int, dim: int, name: str) 
         span += stride * (n - 1)
 
 
-def _extent(start: int, token: int, head: int, tokens: int, heads: int, dim: int) -> tuple[int, int]:
-    """First byte, and the one after the last, of 16-bit rows."""
-    return start, start + 2 * ((tokens - 1) * token + (heads - 1) * head + dim)
+def _meet(a, b, tokens: int, dim: int) -> bool:
+    """Whether 16-bit rows of the same tokens, (address, token stride, head stride, heads) each,
+    have an element in common: exactly where the token strides are one, as in a fused buffer;
+    otherwise whether the memory from the first element to the last does."""
+    (at, step, a_head, a_heads), (other, b_step, b_head, b_heads) = a, b
+    gap, last = (other - at) // 2, tokens - 1
+    a_span, b_span = (a_heads - 1) * a_head + dim, (b_heads - 1) * b_head + dim
+    if gap >= last * step + a_span or -gap >= last * b_step + b_span:
+        return False
+    if last and (step != b_step or step == 0):
+        return True
+    if last:
+        # all of a token's rows beside each other, or head by head with the others'
+        if a_span <= gap % step <= step - b_span:
+            return False
+        if a_head == b_head and a_head and step % a_head == 0 and dim <= gap % a_head <= a_head - dim:
+            return False
+    for x in {gap + j * b_head - i * a_head for i in range(a_heads) for j in range(b_heads)}:
+        # some b token less an a token, from -last to last, brings the heads' rows within dim
+        if abs(x) < dim or last and max((1 - dim - x + step - 1) // step, -last) <= min((dim - 1 - x) // step, last):
+            return True
+    return False
 
 
 def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, tables: torch.Tensor,
