@@ -716,9 +716,9 @@ int secure_infer_gpu_paged_append(hipStream_t stream, const si_paged_append_desc
  * accuracy at any position), the pair (x, y) of dims (i, i + rot / 2), or (2 i, 2 i
  * + 1) if adjacent, becomes magnitude * (x cos a_i - y sin a_i, y cos a_i + x sin
  * a_i), computed in float and rounded once; dims from rot on, and V, go as they
- * are.  q_out may be q itself; otherwise it must not overlap q, k or v.  Tokens
- * dropped from the cache (as by paged_append) have their queries rotated all the
- * same; a row of q that belongs to no sequence goes as it is. */
+ * are.  q_out may be q itself, and must not overlap q otherwise, nor k or v at
+ * all.  Tokens dropped from the cache (as by paged_append) have their queries
+ * rotated all the same; a row of q that belongs to no sequence goes as it is. */
 typedef struct si_rotation {
     const float* freqs;           /* rot / 2, radians a position               */
     const int64_t* positions;     /* [tokens]; NULL: p as in paged_append      */

@@ -226,8 +226,8 @@ def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor
     is right to float accuracy at any position, rounded once; dims from rot on go as they are.  rot is a multiple of 8 up to the head
     dim and 256.  p is the token's position in its sequence, or ``positions`` [tokens] int64
     (for the rotation alone).  A token that the append drops has its query rotated all the
-    same; a row of q in no sequence goes as it is.  Returns ``q_out`` (new if it is not given; q itself rotates in
-    place), or None without q."""
+    same; a row of q in no sequence goes as it is.  Returns ``q_out`` (new if it is not given; q itself, if it shares no memory
+    with k and v, rotates in place), or None without q."""
     d, device = _append_desc(k, v, cache_k, cache_v, tables, kv_lens, q_starts, fail_count)
     heads, dim, dtype, tokens = cache_k.shape[2], cache_k.shape[3], cache_k.dtype, k.shape[0]
     _index(freqs, "freqs", 1, device, torch.float32)
@@ -267,13 +267,15 @@ def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor
                 raise ValueError("q_out must have q's shape")
             _, ot, oh = _rows(q_out, "q_out", q_heads, dim, dtype, device)
             _apart(ot, oh, tokens, q_heads, dim, "q_out")
-            if d is not None and (q_out.data_ptr() != q.data_ptr() or (ot, oh) != (qt, qh)):
-                to = q_out.data_ptr(), ot, oh, q_heads
-                for name, rows in (("q", (q.data_ptr(), qt, qh, q_heads)),
-                                   ("k", (d.k, d.k_token_stride, d.k_head_stride, heads)),
+            if d is not None:
+                to, own = (q_out.data_ptr(), ot, oh, q_heads), (q.data_ptr(), qt, qh, q_heads)
+                if to != own and _meet(to, own, tokens, dim):
+                    raise ValueError("q_out must be q itself, or not overlap q")
+                # (q too, where it turns in place: other waves may not have read K and V yet)
+                for name, rows in (("k", (d.k, d.k_token_stride, d.k_head_stride, heads)),
                                    ("v", (d.v, d.v_token_stride, d.v_head_stride, heads))):
                     if _meet(to, rows, tokens, dim):
-                        raise ValueError(f"q_out must be q itself, or not overlap {name}")
+                        raise ValueError(f"q_out must not overlap {name}")
         r.q, r.q_out, r.q_heads = q.data_ptr(), q_out.data_ptr(), q_heads
         r.q_token_stride, r.q_head_stride, r.q_out_token_stride, r.q_out_head_stride = qt, qh, ot, oh
     if d is None:
