@@ -713,7 +713,7 @@ int secure_infer_gpu_paged_append(hipStream_t stream, const si_paged_append_desc
 
 /* The append with K (and the same tokens' queries) rotated by position on the
  * way: with p a token's position and a_i = p * freqs[i] (the angle to float
- * accuracy at any position), the pair (x, y) of dims (i, i + rot / 2), or (2 i, 2 i
+ * accuracy at any position, for frequencies up to 2^16), the pair (x, y) of dims (i, i + rot / 2), or (2 i, 2 i
  * + 1) if adjacent, becomes magnitude * (x cos a_i - y sin a_i, y cos a_i + x sin
  * a_i), computed in float and rounded once; dims from rot on, and V, go as they
  * are.  q_out may be q itself, and must not overlap q otherwise, nor k or v at

@@ -601,12 +601,22 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(RotateArgs r)
     if (!stored && share == 0 && lane == 0 && a.fail_count) atomicAdd(a.fail_count, 1u);
     const uint64_t o = stored ? uint64_t(slot) * a.slot_bytes + uint64_t(p & ((1ll << a.page_shift) - 1)) * a.heads * r.dim * 2
                               : 0;
-    // Angles in turns: the product with the position, and what is left of it without whole turns, in 64 bits
-    // (2^-52 of the angle: at position 2^30 2e-7 radians).
-    const double at = double(r.positions ? r.positions[t] : p);
+    // Angles in turns, without the whole ones.  The frequency's turns a position are a sum of two doubles (1 / 2 pi to 2^-108),
+    // the position's upper and lower 32 bits a double each, and the products' rounding is kept: 2^-44 of a turn at
+    // any position, for frequencies up to 1, 2^-29 up to 2^16.  (One double for each: 2^-52 of the angle, 1e-4 radians
+    // at 2^40.)
+    const int64_t at = r.positions ? r.positions[t] : p;
+    const double near = double(uint32_t(at)), far = double(at >> 32) * 4294967296.0;
     const float magnitude = __uint_as_float(r.magnitude_bits);
     for (uint32_t i = lane; i < r.rot / 2; i += 64) {
-        const double x = at * double(r.freqs[i]) * 0.15915494309189533577;
+        const double f = double(r.freqs[i]), turn = 0.15915494309189535, turn_rest = -9.839338337591243e-18;
+        const double g = f * turn, g_rest = fma(f, turn, -g) + f * turn_rest;
+        const auto turns_of = [&](double n) {
+            const double h = n * g;
+            return (h - rint(h)) + (fma(n, g, -h) + n * g_rest);
+        };
+        double x = turns_of(near);
+        if (far != 0.0) x += turns_of(far);
         const float part = float(x - rint(x));
         float s, c;
         sincospif(2.0f * part, &s, &c);

@@ -223,7 +223,7 @@ def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor
     dim], rotated by position on the way.  ``freqs`` [rot / 2] float32 are the angles a position;
     with a = p * freqs[i] the dims (x, y) = (i, i + rot / 2), or (2 i, 2 i + 1) if ``adjacent``, become
     ``magnitude`` * (x cos a - y sin a, y cos a + x sin a), in float from an angle that
-    is right to float accuracy at any position, rounded once; dims from rot on go as they are.  rot is a multiple of 8 up to the head
+    is right to float accuracy at any position (for frequencies up to 2**16), rounded once; dims from rot on go as they are.  rot is a multiple of 8 up to the head
     dim and 256.  p is the token's position in its sequence, or ``positions`` [tokens] int64
     (for the rotation alone).  A token that the append drops has its query rotated all the
     same; a row of q in no sequence goes as it is.  Returns ``q_out`` (new if it is not given; q itself, if it shares no memory
