@@ -32,6 +32,7 @@ from .gcm import _check, lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _REFUSED = (1 << 64) - 1
+_FLOAT_MAX = torch.finfo(torch.float32).max
 
 
 def _ptr(t):
@@ -236,8 +237,8 @@ def paged_append_rotated(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor
         raise ValueError(f"freqs must hold a multiple of 4 frequencies, at most {min(dim, 256) // 2}")
     if freqs.requires_grad:
         _tracked()
-    if not math.isfinite(magnitude):
-        raise ValueError("magnitude must be finite")
+    if not abs(magnitude) <= _FLOAT_MAX:
+        raise ValueError("magnitude must be finite in float32")
     if positions is not None:
         _index(positions, "positions", 1, device)
         if positions.shape[0] != tokens:

@@ -63,3 +63,15 @@ def test_far_positions(at, fast):
                                       magnitude=magnitude).cpu().double()
         want, tol = rotated(x["q"], positions, freqs, adjacent, magnitude)
         assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("magnitude", [1e39, -1e300, 3.5e38, math.inf, math.nan])
+def test_magnitudes_past_float_are_refused(magnitude):
+    x = batch(63, [30, 40], [1, 1], 4, 2, 64, 16, torch.bfloat16)
+    d = {n: t.to(DEV) for n, t in x.items()}
+    args = d["k"], d["v"], d["ck"], d["cv"], d["tables"], d["kv"], frequencies(64).to(DEV)
+    with pytest.raises(ValueError, match="magnitude"):
+        si.paged_append_rotated(*args, q=d["q"], magnitude=magnitude)
+    with pytest.raises(ValueError, match="magnitude"):
+        si.paged_append_rotated(*args, magnitude=magnitude)
+    si.paged_append_rotated(*args, q=d["q"], magnitude=torch.finfo(torch.float32).max)
