@@ -55,8 +55,11 @@ constexpr uint32_t kShareMost = 4 * kTileRows;
 
 // Sequences of groups whose own keys are shared out evenly, 64 looked at at a time: short ones are not among them
 // beyond 64, so that what is left may be few, and long (137 next tokens x 32/8 heads, one of them in a group of its
-// own with 7,605 keys: 208 us in one part, 90 shared out).
-constexpr uint32_t kShareSeqs = 256;
+// own with 7,605 keys: 208 us in one part, 90 shared out).  More than these get parts of one length, as without groups.
+// Next tokens behind 2,048 keys, with up to 100 own ones, and with one of 30,000 among up to 256, shared out and
+// not: 300 x 32/8 heads 49 and 66 us, 132 and 415; 2,000 252 and 296, 471 and 811; 2,000 x 8/1 92 and 91, 179 and
+// 300; but 4,000 x 8/1, whose every workgroup looks at all of them, 106 and 80, 281 and 622.
+constexpr uint32_t kShareSeqs = 2048;
 
 // Keys of a prefix for each row (of a KV head, on average) of the sequences that share it, from which on they do.
 constexpr uint64_t kShareKeys = 16;
@@ -136,10 +139,7 @@ inline Plan attend_plan(const si_paged_attention_desc& d, const si_paged_attenti
             places = units > whole ? 2 * few_groups : 0;
         } else {
             uint32_t parts;
-            // (own keys behind a shared prefix are mostly few, and parts that are not there cost a workgroup each:
-            // 256 of 1 to 256 keys x 8 heads behind 32,768 343 us, with kFewTarget 348)
-            const uint64_t target = groups ? kFewTarget / 4 : kFewTarget;
-            p.few_per = uint32_t(part_keys(pairs, keys, kFewStep, kFewStep, target, &parts, most_parts) / unit);
+            p.few_per = uint32_t(part_keys(pairs, keys, kFewStep, kFewStep, kFewTarget, &parts, most_parts) / unit);
             few_groups = pairs * parts;
             places = parts > 1 ? few_groups : 0;
         }
