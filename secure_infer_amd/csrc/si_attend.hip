@@ -1318,7 +1318,7 @@ __device__ __forceinline__ void tile_rows(const AttendArgs& a, uint8_t* lds, uin
         if constexpr (kKind == kPlain) {
             if (kb < lo) ok <<= lo - kb;
         } else {
-            if (kb < s.from) ok <<= s.from - kb;
+            ok &= ~bits_below(kb, s.from);
             if (kb < lo) ok &= ~bits_below(kb, lo) | bits_below(kb, int32_t(a.sinks));
         }
         if (hi - kb < 64) ok &= ~0ull >> (64 - (hi - kb));
