@@ -662,12 +662,17 @@ uint64_t secure_infer_gpu_paged_attention_workspace(const si_paged_attention_des
  *   [0, seqs]) are group g.  As far as their lengths go their rows hold the same
  *   K and V for the keys j < prefix_lens[g] (clamped to the table; on one page,
  *   as a fork leaves them, or on copies), which the call may read from the pages
- *   of any row that is long enough: once for all the group's tokens, where that
- *   is the faster way.  Beside a window each row may have given up pages (no
- *   slot in its table) that none of its own new tokens, nor any later one, sees.
- *   What a token sees, and the result but for rounding, does
- *   not change.  A group of one sequence, and sequences in no group, are as
- *   without groups. */
+ *   of any row that is long enough: once for all the group's tokens, where the
+ *   prefix has at least 16 keys for each row (new token and query head of a KV
+ *   head) that a sequence of the group has on average; else the sequences attend
+ *   by themselves.  Beside a window each row may have given up pages (no slot in
+ *   its table) that none of its own new tokens, nor any later one, sees.  What a
+ *   token sees, and the result but for rounding, does not change.  A group of
+ *   one sequence, and sequences in no group, are as without groups.
+ *   The rule does not weigh what is saved: a few sequences behind a short
+ *   prefix are faster without groups.  The workspace holds numerators and sums
+ *   (4 head_dim + 8 bytes) of every token and query head at least twice,
+ *   whether the groups then share or not. */
 typedef struct si_paged_attention_more {
     uint32_t sinks;               /* at most 2^30                              */
     uint32_t groups;              /* 0: no shared prefixes; < 2^26             */

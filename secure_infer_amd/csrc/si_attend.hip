@@ -699,7 +699,7 @@ __device__ void plain_row(const AttendArgs& a, const int64_t* table, uint32_t t,
 // joined at the end.
 //
 // Up to 64 sequences whose (sequence, KV head) pairs number at most the workgroups that run at
-// a time are shared out evenly: each of those takes the same number of
+// a time (beside groups any number of pairs, and up to kShareSeqs sequences) are shared out evenly: each of those takes the same number of
 // consecutive units of the whole batch, wherever sequences begin and end.  More pairs fill
 // the chip by themselves and get parts of one length, a workgroup each.  64 sequences of 130
 // to 8,192 keys, 28/4 heads of 128 (261 MB), inputs in the caches and not: shared evenly 55

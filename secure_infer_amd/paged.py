@@ -343,9 +343,12 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     ``prefix_groups`` [groups + 1] int64, ascending, and ``prefix_lens`` [groups] int64:
     sequences prefix_groups[g] up to prefix_groups[g + 1] share their first prefix_lens[g] keys: as far as their lengths go their
     rows hold the same K and V there, on the same pages, as fork_pages leaves them, or on copies, and the call may read them
-    from any row that is long enough: once for all their tokens, where that is the faster way.  Beside a window each
-    row may have given up pages (an entry that is no slot) that none of its own new tokens, nor any later one, sees.
-    What a token sees, and the result but for rounding, does not change; a group of one sequence, or a sequence in none, is as without groups."""
+    from any row that is long enough: once for all their tokens, where the prefix has at least 16 keys for each row (new
+    token and query head of a KV head) that a sequence of the group has on average.  Beside a window each row may have given
+    up pages (an entry that is no slot) that none of its own new tokens, nor any later one, sees.  What a token sees, and the
+    result but for rounding, does not change; a group of one sequence, or a sequence in none, is as without groups.  A few
+    sequences behind a short prefix are faster without groups, and the workspace of a call with groups holds float
+    numerators of all its tokens at least twice: name them for next tokens and short chunks."""
     d, device = _attention_desc(q, cache_k, cache_v, tables, kv_lens, q_starts, scale, causal, window, out, lse)
     more = None
     if sinks or prefix_groups is not None or prefix_lens is not None:
