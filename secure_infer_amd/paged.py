@@ -307,11 +307,12 @@ def _meet(a, b, tokens: int, dim: int) -> bool:
         return False
     if last and (step != b_step or step == 0):
         return True
-    if last:
-        # all of a token's rows beside each other, or head by head with the others'
-        if a_span <= gap % step <= step - b_span:
-            return False
-        if a_head == b_head and a_head and step % a_head == 0 and dim <= gap % a_head <= a_head - dim:
+    # a token's rows beside the other's, or a head's
+    if last and a_span <= gap % step <= step - b_span:
+        return False
+    if a_head == b_head and a_head:
+        head_span = dim if step % a_head == 0 else last * step + dim
+        if head_span <= gap % a_head <= a_head - head_span:
             return False
     for x in {gap + j * b_head - i * a_head for i in range(a_heads) for j in range(b_heads)}:
         # some b token less an a token, from -last to last, brings the heads' rows within dim

@@ -51,3 +51,7 @@ def test_fused_projections(tokens):
     q, k, v = three.unbind(2)
     assert not _meet(rows(q), rows(k), tokens, dim) and not _meet(rows(q), rows(v), tokens, dim)
     assert _meet(rows(q), rows(three[:, 2:4, 0]), tokens, dim)
+    heads = torch.empty((hq, 3, tokens, dim), dtype=torch.bfloat16)
+    q, k, v = (t.transpose(0, 1) for t in heads.unbind(1))
+    assert not _meet(rows(q), rows(k), tokens, dim) and not _meet(rows(v), rows(q), tokens, dim)
+    assert _meet(rows(q), rows(heads[1:3, 0].transpose(0, 1)), tokens, dim)
